@@ -12,6 +12,10 @@ Public surface (mirrors the reference's call surface):
                                 exchange of the rows' bests inside the kernel)
   PagedKVCache                  paged target cache with the accepted-branch commit
   PagedKVPool                   many sequences in one page pool, batched commit
+  PagedAttentionPlan, paged_attention
+                                the target's own attention over the paged cache
+                                (prompt chunks, single tokens; 16- and 8-bit pages)
+  rope_tables                   cos and sin tables for ``ops.append_kv``
   cascade_verify_forward        generation/verification.py:cascade_verify_forward
                                 on these kernels
   PeerExchange                  KV-head-sharded output all-gather done by kernel (b)'s
@@ -24,6 +28,7 @@ from .accept import BatchVerifier, ShardedVerifier, Verifier, verify
 from .cascade import CascadePlan, Request, cascade_attention, shared_trunk_map
 from .flashinfer_compat import merge_state_in_place, single_prefill_with_kv_cache
 from .kv_cache import PagedKVCache, PagedKVPool
+from .paged import PagedAttentionPlan, paged_attention, rope_tables
 from .runner import CascadeGraphRunner
 from .sharding import PeerExchange, RecordExchange
 
@@ -31,6 +36,7 @@ __all__ = [
     "BatchVerifier",
     "CascadeGraphRunner",
     "CascadePlan",
+    "PagedAttentionPlan",
     "PagedKVCache",
     "PagedKVPool",
     "PeerExchange",
@@ -40,6 +46,8 @@ __all__ = [
     "Verifier",
     "cascade_attention",
     "merge_state_in_place",
+    "paged_attention",
+    "rope_tables",
     "shared_trunk_map",
     "single_prefill_with_kv_cache",
     "verify",

@@ -1,0 +1,623 @@
+// Attention of a ragged batch's new tokens over the paged cache (causal, window,
+// sinks; 16-bit and e4m3 pages), for few rows per kv head: single tokens and
+// drafted blocks.
+//
+// Row (token, g) of a kv head sees the keys j of its request with
+// pos - window < j <= pos. With s_j = scale * log2e * (q . k_j):
+//   m = max s_j, l = sum 2^(s_j - m), o = sum 2^(s_j - m) v_j / l, lse2 = m + log2 l
+// in one pass over the keys (running maximum and sum). A row without a key gets
+// o = 0 and lse2 = -inf.
+//
+// rows_kernel: a CTA takes 16 query rows of one kv head against a span of keys
+// (paged_plan.h); its eight warps take the span's 16-key pages in turn, each with
+// a ring of pages of its own in shared memory, so the loop has no CTA barrier and
+// about 190 KB of loads are in flight per SM -- the bound is HBM. The products
+// are m16n8k16 matrix instructions: one 16-row tile is all the rows there are,
+// and a 128-row tensor-core tile would be mostly padding. A page is stored as
+// 8-row x 16-byte core matrices, exactly what ldmatrix fetches, without bank
+// conflicts and without a swizzle; pages of plain rows are put into that order by
+// the copy. At the end the warps' states are joined in shared memory, and for a
+// unit of several spans the last CTA joins the spans.
+//
+// e4m3 pages: the fragments are widened to bf16 in registers (sign and the seven
+// magnitude bits moved into place, then a product with 2^120, all exact). A
+// 16-byte row of a core matrix holds 16 elements of d; ldmatrix hands a lane four
+// neighbouring ones, and since the order of the summed index is free, q's
+// fragment takes the same four (K), or two neighbouring output columns (V). The
+// key's scale multiplies the score, the value's scale the weight, in fp32.
+//
+// Weights are rounded to the value type (bf16: 2^-8 relative, f16: 2^-11) for the
+// second product; maximum, sum and output stay in fp32.
+#include <atomic>
+#include <string>
+
+#include "paged.cuh"
+#include "paged_plan.h"
+
+namespace d2sd {
+namespace {
+
+using namespace paged;
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+
+struct AttnArgs {
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_st, q_sh, o_st, o_sh, lse_st;  // element strides
+  const uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
+  const int32_t* page_table;
+  int64_t page_table_len;
+  const int32_t* plan;
+  float* slots;      // partial states: [slot][rows * (D + 2)]
+  uint32_t* tickets;
+  const float* sinks;
+  int32_t* status;
+  PageGeom g;
+  float scale_log2;
+  int32_t sink_mode;
+};
+
+template <int D, int ELEM>
+struct RowsCfg {
+  static constexpr int kPageBytes = 16 * D * ELEM;        // one of K, V
+  static constexpr int kStageBytes = 2 * kPageBytes + (ELEM == 1 ? 32 : 0);  // + 16 + 16 scale bytes
+  static constexpr int kRing = 24576;                     // bytes of a warp's ring
+  static constexpr int kStages = (kRing / kStageBytes) < 8 ? (kRing / kStageBytes) : 8;
+  static constexpr int kState = 16 * D * 4;               // a warp's O, over its ring at the end
+  static constexpr int kSmemMl = kWarps * kRing;          // [warps][16] m, then l
+  static constexpr int kSmemBars = kSmemMl + 2 * kWarps * 16 * 4;
+  static constexpr int kSmemFlags = kSmemBars + kWarps * 8 * 8;
+  static constexpr int kSmemBytes = kSmemFlags + 16 + 128;
+  static_assert(kState <= kRing, "the state fits the ring");
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                 uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) { return pack_bf16x2(lo, hi); }
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// Bytes 0 and 2 (even) or 1 and 3 (odd) of x, e4m3, to two bf16. Moving sign and
+// magnitude into a bf16's places gives value * 2^-120 (the exponent biases differ
+// by 120; subnormals likewise), so a product with 2^120 ends it. NaN (0x7f) is
+// not one after this; the writer marks such rows in their scale byte.
+__device__ __forceinline__ uint32_t mul_2p120(uint32_t x) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7b807b80u));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_even(uint32_t x) {
+  return mul_2p120(((x & 0x00800080u) << 8) | ((x & 0x007f007fu) << 4));
+}
+__device__ __forceinline__ uint32_t e4m3_odd(uint32_t x) {
+  return mul_2p120((x & 0x80008000u) | ((x & 0x7f007f00u) >> 4));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Factor of the attention sink: o *= sigmoid(lse - sink) (include/d2sd.h).
+__device__ __forceinline__ float sink_factor(float lse2, float sink, int mode) {
+  const float x = (mode == D2SD_SINK_EXACT ? lse2 * kLn2 : lse2) - sink;
+  return 1.f / (1.f + expf(-x));
+}
+
+// One 16-byte chunk of zeros is written over rows [r0, r1) of a page in smem.
+template <int D, int ELEM>
+__device__ __forceinline__ void zero_rows(uint8_t* page, int r0, int r1) {
+  constexpr int C = D * ELEM / 16;
+  const int lane = threadIdx.x & 31;
+  for (int i = lane; i < 16 * C; i += 32) {
+    const int r = i & 15, c = i >> 4;
+    if (r >= r0 && r < r1)
+      *reinterpret_cast<uint4*>(page + ((r >> 3) * C + c) * 128 + (r & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ELEM: bytes of a cached value (2: T, 1: e4m3); UMMA: pages in core-matrix order,
+// fetched with one bulk copy each (else rows, 16-byte cp.async).
+template <typename T, int D, int ELEM, bool UMMA>
+__global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
+  using C = RowsCfg<D, ELEM>;
+  constexpr int kChunks = D * ELEM / 16;  // 16-byte chunks of a row
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) &
+                                             ~static_cast<uintptr_t>(127));
+  float* sm_m = reinterpret_cast<float*>(smem + C::kSmemMl);
+  float* sm_l = sm_m + kWarps * 16;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kSmemBars);
+  volatile int* flags = reinterpret_cast<volatile int*>(smem + C::kSmemFlags);  // abort, last
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  uint8_t* ring = smem + warp * C::kRing;
+  uint64_t* full = bars + warp * 8;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWarps * 8; ++i) mbar_init(&bars[i], 1);
+    flags[0] = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  grid_dep_wait();
+
+  const int32_t* sec = a.plan + H_SECTION;
+  const int G = a.plan[H_GROUP];
+  if (static_cast<int>(blockIdx.x) >= sec[S_CTAS]) return;  // a fixed grid's spare CTA
+  const int item0 = a.plan[sec[S_OFF_CTA] + blockIdx.x], item1 = a.plan[sec[S_OFF_CTA] + blockIdx.x + 1];
+  const int qr = lane >> 2, qc = lane & 3;
+  uint32_t uses = 0;  // stages this warp has consumed so far (ring position and parity)
+
+  for (int it = item0; it < item1; ++it) {
+    const int32_t* I = a.plan + sec[S_OFF_ITEMS] + it * kItemInts;
+    const int head = I[P_HEAD], tok0 = I[P_TOK0], row0 = I[P_ROW0], nrows = I[P_NROWS];
+    const int key0 = I[P_KEY0], key1 = I[P_KEY1], pos0 = I[P_POS0], window = I[P_WINDOW];
+    const int kv_len = I[P_KV_LEN];
+    const int64_t page_off = I[P_PAGE_OFF];
+    // keys a row sees: [lo, hi)
+    auto row_hi = [&](int r) { return r < nrows ? max(0, min(kv_len, pos0 + (row0 + r) / G + 1)) : 0; };
+    auto row_lo = [&](int r) { return window ? max(0, pos0 + (row0 + r) / G + 1 - window) : 0; };
+    const int hi0 = row_hi(qr), hi1 = row_hi(qr + 8), lo0 = row_lo(qr), lo1 = row_lo(qr + 8);
+    const int hi_min = row_hi(0), hi_max = row_hi(nrows - 1);
+    const int lo_min = row_lo(0), lo_max = row_lo(nrows - 1);
+
+    // ---- q fragments (A operand, 16 rows x 16 of d per step) ----
+    uint32_t qf[D / 16][4];
+    {
+      const T* qb = static_cast<const T*>(a.q);
+      const T* q0 = nullptr;
+      const T* q1 = nullptr;
+      if (qr < nrows)
+        q0 = qb + (tok0 + static_cast<int64_t>((row0 + qr) / G)) * a.q_st + (head * G + (row0 + qr) % G) * a.q_sh;
+      if (qr + 8 < nrows)
+        q1 = qb + (tok0 + static_cast<int64_t>((row0 + qr + 8) / G)) * a.q_st +
+             (head * G + (row0 + qr + 8) % G) * a.q_sh;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        if (ELEM == 2) {
+          const int d = ks * 16 + qc * 2;
+          qf[ks][0] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + d) : 0u;
+          qf[ks][1] = q1 ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
+          qf[ks][2] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + d + 8) : 0u;
+          qf[ks][3] = q1 ? *reinterpret_cast<const uint32_t*>(q1 + d + 8) : 0u;
+        } else {  // the four elements this lane's K bytes belong to: even ones, then odd ones
+          const int d = ks * 16 + qc * 4;
+          const uint2 x = q0 ? *reinterpret_cast<const uint2*>(q0 + d) : make_uint2(0u, 0u);
+          const uint2 y = q1 ? *reinterpret_cast<const uint2*>(q1 + d) : make_uint2(0u, 0u);
+          qf[ks][0] = __byte_perm(x.x, x.y, 0x5410);
+          qf[ks][2] = __byte_perm(x.x, x.y, 0x7632);
+          qf[ks][1] = __byte_perm(y.x, y.y, 0x5410);
+          qf[ks][3] = __byte_perm(y.x, y.y, 0x7632);
+        }
+      }
+    }
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+    // ---- this warp's pages of 16 keys: b0 + warp, b0 + warp + 8, ... ----
+    const int b0 = key0 / 16, nb = (key1 - key0 + 15) / 16;
+    const int mine = nb > warp ? (nb - warp + kWarps - 1) / kWarps : 0;
+    int ids = 0;  // lane j: the page of block `base + j` of mine
+    auto fetch_ids = [&](int base) {
+      const int64_t pos = static_cast<int64_t>(b0 + warp + (base + lane) * kWarps) * 16;
+      const int64_t e = page_off + pos / a.g.page_size;
+      ids = 0;
+      if (base + lane < mine && e < a.page_table_len) {
+        const int64_t id = a.page_table[e];
+        ids = static_cast<int>(id < 0 ? 0 : (id >= a.g.num_pages ? a.g.num_pages - 1 : id));
+      }
+    };
+    auto issue = [&](int j) {  // fetch block j of mine into its stage
+      if ((j & 31) == 0) fetch_ids(j);
+      const int64_t page = __shfl_sync(0xffffffffu, ids, j & 31);
+      const uint32_t st = (uses + j) % C::kStages;
+      uint8_t* dst = ring + st * C::kStageBytes;
+      const int64_t off = page * a.g.stride_page + head * a.g.stride_head;
+      if (UMMA) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full[st], C::kStageBytes);
+          bulk_load(dst, a.k_pool + off, C::kPageBytes, &full[st]);
+          bulk_load(dst + C::kPageBytes, a.v_pool + off, C::kPageBytes, &full[st]);
+          if (ELEM == 1) {
+            const int64_t so = page * a.g.scale_page + head * a.g.scale_head;
+            bulk_load(dst + 2 * C::kPageBytes, a.k_scale + so, 16, &full[st]);
+            bulk_load(dst + 2 * C::kPageBytes + 16, a.v_scale + so, 16, &full[st]);
+          }
+        }
+      } else {
+        const int slot0 = (b0 + warp + j * kWarps) * 16 % a.g.page_size;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint8_t* src = (kv ? a.v_pool : a.k_pool) + off;
+          const uint32_t d = smem_u32(dst + kv * C::kPageBytes);
+#pragma unroll
+          for (int i = 0; i < kChunks / 2; ++i) {  // 8 rows x 4 chunks at a time
+            const int r = (lane & 7) + 8 * (i & 1), c = (i >> 1) * 4 + (lane >> 3);
+            cp_async16(d + ((r >> 3) * kChunks + c) * 128 + (r & 7) * 16,
+                       src + static_cast<int64_t>(slot0 + r) * a.g.stride_slot + c * 16);
+          }
+        }
+      }
+    };
+    auto commit = [&] {
+      if (!UMMA) asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int j = 0; j < C::kStages - 1; ++j) {
+      if (j < mine) issue(j);
+      commit();
+    }
+    bool alive = true;
+    int j = 0;
+    for (; j < mine; ++j) {
+      // the stage freed by block j - 1 takes block j + kStages - 1
+      if (j + C::kStages - 1 < mine) issue(j + C::kStages - 1);
+      commit();
+      const uint32_t st = (uses + j) % C::kStages;
+      if (UMMA) {
+        const bool ok = mbar_wait(&full[st], ((uses + j) / C::kStages) & 1, flags);
+        if (!__all_sync(0xffffffffu, ok)) {
+          alive = false;
+          break;
+        }
+      } else {
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+        __syncwarp();
+      }
+      uint8_t* kp = ring + st * C::kStageBytes;
+      uint8_t* vp = kp + C::kPageBytes;
+      const int key = (b0 + warp + j * kWarps) * 16;
+      const bool edge = key + 16 > hi_min || key < lo_max;
+      if (edge && (key + 16 > hi_max || key < lo_min)) {
+        // values no row of the unit sees may be anything; a weight of 0 would
+        // still turn a NaN or an infinity there into NaN
+        zero_rows<D, ELEM>(vp, max(0, hi_max - key), 16);
+        zero_rows<D, ELEM>(vp, 0, min(16, lo_min - key));
+        if (UMMA) fence_proxy_async_smem();  // before the next bulk copy into this stage
+        __syncwarp();
+      }
+      // ---- scores ----
+      float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      const uint32_t ka = smem_u32(kp) + (lane & 7) * 16;
+      const int mt = lane >> 3;  // matrix of an x4 this lane addresses
+      if (ELEM == 2) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t b[4];  // (keys 0-7, d lo), (0-7, hi), (8-15, lo), (8-15, hi)
+          ldsm4(ka + ((mt >> 1) * kChunks + ks * 2 + (mt & 1)) * 128, b);
+          mma16816<T>(c[0], qf[ks], b[0], b[1]);
+          mma16816<T>(c[1], qf[ks], b[2], b[3]);
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ks += 2) {
+          uint32_t b[4];  // (keys 0-7, chunk ks), (8-15, ks), (0-7, ks + 1), (8-15, ks + 1)
+          ldsm4(ka + ((mt & 1) * kChunks + ks + (mt >> 1)) * 128, b);
+          mma16816<T>(c[0], qf[ks], e4m3_even(b[0]), e4m3_odd(b[0]));
+          mma16816<T>(c[1], qf[ks], e4m3_even(b[1]), e4m3_odd(b[1]));
+          mma16816<T>(c[0], qf[ks + 1], e4m3_even(b[2]), e4m3_odd(b[2]));
+          mma16816<T>(c[1], qf[ks + 1], e4m3_even(b[3]), e4m3_odd(b[3]));
+        }
+      }
+      float vs[2][2] = {{1.f, 1.f}, {1.f, 1.f}};  // value scales of this lane's four keys
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float s0 = a.scale_log2, s1 = a.scale_log2;
+        if (ELEM == 1) {
+          const uint8_t* sp = kp + 2 * C::kPageBytes + n * 8 + qc * 2;
+          const uint32_t kb = *reinterpret_cast<const uint16_t*>(sp);
+          const uint32_t vb = *reinterpret_cast<const uint16_t*>(sp + 16);
+          s0 *= e4m3_scale(kb & 255u);
+          s1 *= e4m3_scale(kb >> 8);
+          vs[n][0] = e4m3_scale(vb & 255u);
+          vs[n][1] = e4m3_scale(vb >> 8);
+        }
+        c[n][0] *= s0;
+        c[n][1] *= s1;
+        c[n][2] *= s0;
+        c[n][3] *= s1;
+      }
+      if (edge) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int x = key + n * 8 + qc * 2 + e;
+            if (x >= hi0 || x < lo0) c[n][e] = -INFINITY;
+            if (x >= hi1 || x < lo1) c[n][2 + e] = -INFINITY;
+            if (x >= hi_max || x < lo_min) vs[n][e] = 0.f;  // a scale byte no row sees
+          }
+      }
+      // ---- running maximum and sum; o is rescaled only when a maximum grew ----
+      float x0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
+      float x1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        const float f0 = m0 == n0 ? 1.f : fast_exp2(m0 - n0), f1 = m1 == n1 ? 1.f : fast_exp2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][0] *= f0;
+          o[i][1] *= f0;
+          o[i][2] *= f1;
+          o[i][3] *= f1;
+        }
+      }
+      const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+      uint32_t p[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float p0 = fast_exp2(c[n][0] - r0), p1 = fast_exp2(c[n][1] - r0);
+        const float p2 = fast_exp2(c[n][2] - r1), p3 = fast_exp2(c[n][3] - r1);
+        l0 += p0 + p1;
+        l1 += p2 + p3;
+        p[2 * n] = pack2(p0 * vs[n][0], p1 * vs[n][1], T());
+        p[2 * n + 1] = pack2(p2 * vs[n][0], p3 * vs[n][1], T());
+      }
+      // ---- o += p v ----
+      const uint32_t va = smem_u32(vp) + (lane & 7) * 16;
+      if (ELEM == 2) {
+#pragma unroll
+        for (int i = 0; i < D / 8; i += 2) {
+          uint32_t b[4];  // (keys 0-7, chunk i), (8-15, i), (0-7, i + 1), (8-15, i + 1), transposed
+          ldsm4_t(va + ((mt & 1) * kChunks + i + (mt >> 1)) * 128, b);
+          mma16816<T>(o[i], p, b[0], b[1]);
+          mma16816<T>(o[i + 1], p, b[2], b[3]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 2) {
+          uint32_t b[4];  // pairs of neighbouring d, transposed
+          ldsm4_t(va + ((mt & 1) * kChunks + i + (mt >> 1)) * 128, b);
+          mma16816<T>(o[2 * i], p, e4m3_even(b[0]), e4m3_even(b[1]));
+          mma16816<T>(o[2 * i + 1], p, e4m3_odd(b[0]), e4m3_odd(b[1]));
+          mma16816<T>(o[2 * i + 2], p, e4m3_even(b[2]), e4m3_even(b[3]));
+          mma16816<T>(o[2 * i + 3], p, e4m3_odd(b[2]), e4m3_odd(b[3]));
+        }
+      }
+      __syncwarp();  // the stage is free for block j + kStages
+    }
+    if (!alive) {
+      // give up: wait (bounded) for the copies in flight, so that none lands in
+      // another block's shared memory
+      flags[0] = 1;
+      for (int x = j; x < min(j + C::kStages, mine); ++x) {
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(&full[(uses + x) % C::kStages], ((uses + x) / C::kStages) & 1) &&
+               global_timer_ns() - t0 < kWaitTimeoutNs) {
+        }
+      }
+    }
+    uses += mine;
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+
+    // ---- join the warps: O over the warp's own ring, m and l beside it ----
+    __syncwarp();
+    float* os = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      // 16-bit: columns of tile i are d = 8 i + n. 8-bit: tiles 2 j, 2 j + 1 hold
+      // the even and the odd d of chunk j
+      const int d0 = ELEM == 2 ? i * 8 + qc * 2 : (i >> 1) * 16 + qc * 4 + (i & 1);
+      const int d1 = ELEM == 2 ? d0 + 1 : d0 + 2;
+      os[qr * D + d0] = o[i][0];
+      os[qr * D + d1] = o[i][1];
+      os[(qr + 8) * D + d0] = o[i][2];
+      os[(qr + 8) * D + d1] = o[i][3];
+    }
+    if (qc == 0) {
+      sm_m[warp * 16 + qr] = m0;
+      sm_m[warp * 16 + qr + 8] = m1;
+      sm_l[warp * 16 + qr] = l0;
+      sm_l[warp * 16 + qr + 8] = l1;
+    }
+    if (UMMA) fence_proxy_async_smem();  // before the next item's bulk copies into the ring
+    __syncthreads();
+    constexpr int kPer = 16 * D / kThreads;  // outputs of a thread, neighbours in a row
+    const int row = threadIdx.x / (kThreads / 16), dcol = (threadIdx.x % (kThreads / 16)) * kPer;
+    float M = -INFINITY, L = 0.f, acc[kPer];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w * 16 + row]);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+    const float Mr = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = fast_exp2(sm_m[w * 16 + row] - Mr);
+      L += sm_l[w * 16 + row] * f;
+      const float* ow = reinterpret_cast<const float*>(smem + w * C::kRing) + row * D + dcol;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = fmaf(ow[e], f, acc[e]);
+    }
+    const int parts = I[P_PARTS];
+    bool write = true;
+    if (parts > 1) {
+      constexpr int kSlot = 16 * (D + 2);
+      float* mine_s = a.slots + static_cast<int64_t>(I[P_SLOT]) * kSlot;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) mine_s[row * D + dcol + e] = acc[e];
+      if (dcol == 0) {
+        mine_s[16 * D + row] = M;
+        mine_s[16 * D + 16 + row] = L;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0)
+        flags[1] = atom_add_acq_rel_gpu(&a.tickets[I[P_TICKET]], 1u) == static_cast<uint32_t>(parts - 1);
+      __syncthreads();
+      write = flags[1] != 0;
+      if (write) {  // the last span: join all of them, in slot order
+        if (threadIdx.x == 0) a.tickets[I[P_TICKET]] = 0;
+        const float* s0 = a.slots + static_cast<int64_t>(I[P_FIRST_SLOT]) * kSlot;
+        M = -INFINITY;
+        for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(s0 + p * kSlot + 16 * D + row));
+        const float mr = M == -INFINITY ? 0.f : M;
+        L = 0.f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+        for (int p = 0; p < parts; ++p) {
+          const float* sp = s0 + p * kSlot;
+          const float f = fast_exp2(__ldcg(sp + 16 * D + row) - mr);
+          L += __ldcg(sp + 16 * D + 16 + row) * f;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) acc[e] = fmaf(__ldcg(sp + row * D + dcol + e), f, acc[e]);
+        }
+      }
+    }
+    if (write && row < nrows) {
+      const int64_t tok = tok0 + static_cast<int64_t>((row0 + row) / G);
+      const int hq = head * G + (row0 + row) % G;
+      const float lse2 = L > 0.f ? M + log2f(L) : (L == 0.f ? -INFINITY : L);
+      float f = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+      if (a.sinks) f *= sink_factor(lse2, a.sinks[hq], a.sink_mode);
+      T* op = static_cast<T*>(a.out) + tok * a.o_st + hq * a.o_sh + dcol;
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2)
+        *reinterpret_cast<uint32_t*>(op + e) = pack2(acc[e] * f, acc[e + 1] * f, T());
+      if (a.lse && dcol == 0) a.lse[tok * a.lse_st + hq] = lse2;
+    }
+    __syncthreads();  // the rings are read; the next item's copies may land
+    if (flags[0]) break;
+  }
+  if (threadIdx.x == 0 && flags[0] && a.status) atomicExch(a.status, 1);
+}
+
+template <typename T, int D, int ELEM, bool UMMA>
+int launch_rows(const AttnArgs& a, int ctas, cudaStream_t stream) {
+  using C = RowsCfg<D, ELEM>;
+  static std::atomic<uint64_t> configured{0};  // bit per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !((configured.load() >> dev) & 1)) {
+    cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, D, ELEM, UMMA>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+    if (e != cudaSuccess)
+      return fail(D2SD_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+    if (dev < 64) configured.fetch_or(1ull << dev);
+  }
+  return launch_pdl(rows_kernel<T, D, ELEM, UMMA>, dim3(ctas), dim3(kThreads), C::kSmemBytes, stream,
+                    "rows_kernel", a);
+}
+
+}  // namespace
+}  // namespace d2sd
+
+// Tickets first, then the slots: a CTA's first and last item can be spans of split
+// units, so 2 per CTA bounds both.
+extern "C" int64_t d2sd_paged_workspace_bytes(int32_t num_ctas, int32_t head_dim) {
+  using namespace d2sd::paged;
+  if (num_ctas <= 0 || (head_dim != 64 && head_dim != 128)) return -1;
+  return ticket_bytes(num_ctas) + 2 * static_cast<int64_t>(num_ctas) * kRowsTile * (head_dim + 2) * 4;
+}
+
+extern "C" int d2sd_paged_attention(
+    const void* q, int64_t q_stride_token, int64_t q_stride_head, int32_t dtype, const void* k_pool,
+    const void* v_pool, int64_t cache_stride_page, int64_t cache_stride_slot, int64_t cache_stride_head,
+    int32_t page_size, int64_t num_pages, int32_t cache_format, const void* k_scale, const void* v_scale,
+    int64_t scale_stride_page, int64_t scale_stride_head, const int32_t* page_table,
+    int64_t page_table_len, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, float sm_scale,
+    const int32_t* plan, const int32_t* sections, int32_t num_ctas, int32_t fixed_grid, void* workspace, int64_t workspace_bytes,
+    const float* sinks, int32_t sink_mode, void* out, int64_t out_stride_token, int64_t out_stride_head,
+    float* lse, int64_t lse_stride_token, int32_t* status, void* stream) {
+  using namespace d2sd;
+  using namespace d2sd::paged;
+  const char* const w = "d2sd_paged_attention";
+  if (!plan || !sections || num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
+  if (sections[S_ITEMS] == 0 && !fixed_grid) return D2SD_OK;  // no query rows
+  if (!q || !out || !k_pool || !v_pool || !page_table || page_table_len < 0)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": head_dim must be 64 or 128");
+  if (dtype != D2SD_DTYPE_BF16 && dtype != D2SD_DTYPE_F16)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": q must be bf16 or fp16");
+  const bool scaled = k_scale != nullptr;
+  if (scaled != (v_scale != nullptr))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": k_scale and v_scale go together");
+  if (scaled && dtype != D2SD_DTYPE_BF16)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": 8-bit pages take bf16 queries");
+  if (sinks && sink_mode != D2SD_SINK_REFERENCE && sink_mode != D2SD_SINK_EXACT)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": unknown sink_mode");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(k_pool) || !aligned16(v_pool) ||
+      !aligned16(k_scale) || !aligned16(v_scale) || q_stride_token % 8 || q_stride_head % 8 ||
+      out_stride_token % 8 || out_stride_head % 8 || scale_stride_page % 16 || scale_stride_head % 16)
+    return fail(D2SD_ERR_INVALID_ARGUMENT,
+                std::string(w) + ": rows must be 16-byte aligned, strides multiples of 8");
+  if (num_ctas <= 0 || sections[S_CTAS] > num_ctas || sections[S_TICKETS] > 2 * num_ctas ||
+      sections[S_SLOTS] > 2 * num_ctas)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": the plan is for another grid");
+  if (workspace_bytes < d2sd_paged_workspace_bytes(num_ctas, head_dim) || !workspace ||
+      !aligned16(workspace))
+    return fail(D2SD_ERR_WORKSPACE, std::string(w) + ": workspace too small or unaligned");
+  AttnArgs a{};
+  int rc = make_page_geom(&a.g, w, head_dim, scaled ? 1 : 2, cache_stride_page, cache_stride_slot,
+                          cache_stride_head, page_size, num_pages, cache_format, scaled,
+                          scale_stride_page, scale_stride_head);
+  if (rc) return rc;
+  if (page_size % 16)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": page_size must be a multiple of 16");
+  a.q = q, a.out = out, a.lse = lse;
+  a.q_st = q_stride_token, a.q_sh = q_stride_head, a.o_st = out_stride_token, a.o_sh = out_stride_head,
+  a.lse_st = lse_stride_token;
+  a.k_pool = static_cast<const uint8_t*>(k_pool), a.v_pool = static_cast<const uint8_t*>(v_pool);
+  a.k_scale = static_cast<const uint8_t*>(k_scale), a.v_scale = static_cast<const uint8_t*>(v_scale);
+  a.page_table = page_table, a.page_table_len = page_table_len;
+  a.plan = plan;
+  a.tickets = static_cast<uint32_t*>(workspace);
+  a.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ticket_bytes(num_ctas));
+  a.sinks = sinks, a.sink_mode = sink_mode;
+  a.status = status;
+  a.scale_log2 = sm_scale * kLog2e;
+  const int ctas = fixed_grid ? num_ctas : sections[S_CTAS];
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool d128 = head_dim == 128, umma = a.g.umma != 0;
+  if (scaled) return d128 ? launch_rows<__nv_bfloat16, 128, 1, true>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 1, true>(a, ctas, st);
+  if (dtype == D2SD_DTYPE_BF16) {
+    if (umma) return d128 ? launch_rows<__nv_bfloat16, 128, 2, true>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 2, true>(a, ctas, st);
+    return d128 ? launch_rows<__nv_bfloat16, 128, 2, false>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 2, false>(a, ctas, st);
+  }
+  if (umma) return d128 ? launch_rows<__half, 128, 2, true>(a, ctas, st) : launch_rows<__half, 64, 2, true>(a, ctas, st);
+  return d128 ? launch_rows<__half, 128, 2, false>(a, ctas, st) : launch_rows<__half, 64, 2, false>(a, ctas, st);
+}

@@ -1,0 +1,547 @@
+// Writing new tokens into the paged cache and reading rows back out of it.
+//
+// append_kernel: the step between a layer's projections and its attention, for a
+// ragged batch of new tokens, in one pass: per-head RMSNorm of q and k
+// (optional), the rotary position of q and k (optional), and the write of k and v
+// into the cache's pages, in their own type or as e4m3 rows with a scale byte
+// (paged.cuh). With c, s = cos, sin of the token's position (fp32 tables, so any
+// scaling of the angles for long contexts is the table's):
+//   y = x * rsqrt(mean(x^2) + eps) * w
+//   (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s)
+// with pairs (i, i + rotary/2) or (2i, 2i + 1), i < rotary/2; the rest of the head
+// stays. All of it in fp32 and rounded once, into q_out and into the cache.
+// read_kernel: rows back out of the pages, 8-bit values times their scale.
+// commit_e4m3_kernel: the accepted branch's rows (commit.cu) into an 8-bit cache.
+//
+// head_dim / 8 lanes hold one (token, head) row, 8 elements each: the norm's sum
+// and the row's largest magnitude are shuffles inside that group, and the rotary
+// partner is either in the lane (interleaved) or rotary/16 lanes away.
+#include <string>
+
+#include "paged.cuh"
+
+namespace d2sd {
+
+int make_page_geom(PageGeom* g, const char* what, int32_t head_dim, int32_t elem, int64_t stride_page,
+                   int64_t stride_slot, int64_t stride_head, int32_t page_size, int64_t num_pages,
+                   int32_t cache_format, bool scaled, int64_t scale_stride_page,
+                   int64_t scale_stride_head) {
+  const std::string w(what);
+  if (page_size <= 0 || num_pages <= 0)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, w + ": invalid page size or pool size");
+  if (cache_format != D2SD_KV_ROWS && cache_format != D2SD_KV_UMMA_PAGES)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, w + ": unknown cache_format");
+  const bool umma = cache_format == D2SD_KV_UMMA_PAGES;
+  if (umma && (page_size != 16 || elem > 2))
+    return fail(D2SD_ERR_UNSUPPORTED, w + ": UMMA pages hold 16 rows of 8- or 16-bit values");
+  if (scaled && !umma)
+    return fail(D2SD_ERR_UNSUPPORTED, w + ": 8-bit rows are kept in UMMA pages");
+  const int64_t ve = 16 / elem;
+  if (stride_page % ve || stride_head % ve || (!umma && stride_slot % ve))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, w + ": cache strides must keep rows 16-byte aligned");
+  g->stride_page = stride_page * elem;
+  g->stride_slot = stride_slot * elem;
+  g->stride_head = stride_head * elem;
+  g->scale_page = scale_stride_page;
+  g->scale_head = scale_stride_head;
+  g->num_pages = num_pages;
+  g->page_size = page_size;
+  g->umma = umma ? 1 : 0;
+  return D2SD_OK;
+}
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int W>  // sum / max over the W lanes of a row's group
+__device__ __forceinline__ float group_sum(float x) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+template <int W>
+__device__ __forceinline__ float group_max(float x) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+// Lane `part` of the row's group holds elements 8 part .. 8 part + 7. Writes the
+// row's 8-bit form to slot s of (page, head) of a pool and its scale pool. The
+// whole group calls it; rows with store == false only take part in the shuffles.
+template <int D>
+__device__ __forceinline__ void store_e4m3(const float (&f)[8], int part, uint8_t* pool, uint8_t* scale,
+                                           const PageGeom& g, int64_t page, int head, int s,
+                                           bool store) {
+  float m = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    m = fmaxf(m, fabsf(f[i]));
+    bad |= !(fabsf(f[i]) <= 3.402823466e38f);
+  }
+  m = group_max<D / 8>(bad ? INFINITY : m);
+  const bool finite = m <= 3.402823466e38f;
+  const uint32_t byte = finite ? e4m3_scale_byte(m) : 255u;
+  const float inv = finite ? e4m3_inv_scale(byte) : 0.f;
+  uint2 q;
+  q.x = e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
+  q.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
+  if (!finite) q.x = q.y = 0x7f7f7f7fu;
+  if (!store) return;
+  *reinterpret_cast<uint2*>(pool + page_chunk(g, page, head, s, part >> 1, D / 16) + (part & 1) * 8) = q;
+  if (part == 0) scale[page * g.scale_page + head * g.scale_head + s] = static_cast<uint8_t>(byte);
+}
+
+struct AppendArgs {
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_st, q_sh, o_st, o_sh, k_st, k_sh, v_st, v_sh;  // element strides
+  const void *q_weight, *k_weight;
+  const float *cos, *sin;
+  int64_t table_stride, table_rows;
+  const int32_t *token_start, *first_pos;
+  const int32_t *page_table, *page_bounds;
+  uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
+  int32_t* status;
+  int64_t tokens;
+  PageGeom g;
+  float eps;
+  int32_t R, Hq, Hk, half, interleaved;  // half: rotary_dim / 2, 0 without rotation
+};
+
+// A CTA takes one token at a time; its groups take the token's q, k and v heads
+// in turn, so the position, the page and the lane's cos and sin are found once.
+template <typename T, int D, bool Q8>
+__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
+  constexpr int W = D / 8;               // lanes of a row
+  constexpr int kGroups = kThreads / W;  // rows a CTA holds at once
+  const int group = threadIdx.x / W, part = threadIdx.x % W;
+  grid_dep_wait();
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    const int r = find_request(a.token_start, a.R, t);
+    if (r >= a.R || t < a.token_start[r]) continue;  // behind the last sequence
+    const int64_t pos = static_cast<int64_t>(a.first_pos[r]) + (t - a.token_start[r]);
+    const int64_t lo = a.page_bounds[r], n = a.page_bounds[r + 1] - lo;
+    int err = 0;
+    int64_t page = 0;
+    int slot = 0;
+    if (pos < 0 || pos / a.g.page_size >= n) {
+      err = kStatusPosition;
+    } else {
+      page = a.page_table[lo + pos / a.g.page_size];
+      slot = static_cast<int>(pos % a.g.page_size);
+      if (page < 0 || page >= a.g.num_pages) err = kStatusPage;
+      else if (a.half && pos >= a.table_rows) err = kStatusTable;
+    }
+    if (err) {  // the token's rows are not written at all
+      if (threadIdx.x == 0 && a.status) atomicExch(a.status, err);
+      continue;
+    }
+    // this lane's cos and sin: columns of its 8 elements' pairs
+    float c[8], s[8];
+    const int rot_lanes = a.half / 4;  // lanes that hold rotated elements
+    const bool rotated = part < rot_lanes;
+    if (rotated) {
+      const float* cr = a.cos + pos * a.table_stride;
+      const float* sr = a.sin + pos * a.table_stride;
+      if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          c[2 * i] = c[2 * i + 1] = __ldg(cr + part * 4 + i);
+          s[2 * i] = s[2 * i + 1] = __ldg(sr + part * 4 + i);
+        }
+      } else {
+        const int col = part * 8 - (part >= rot_lanes / 2 ? a.half : 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          c[i] = __ldg(cr + col + i);
+          s[i] = __ldg(sr + col + i);
+        }
+      }
+    }
+    const int rows = a.Hq + 2 * a.Hk;
+    for (int r0 = 0; r0 < rows; r0 += kGroups) {
+      const int row = r0 + group;
+      const bool live = row < rows;
+      const bool is_q = row < a.Hq, is_k = !is_q && row < a.Hq + a.Hk;
+      const int head = is_q ? row : (is_k ? row - a.Hq : row - a.Hq - a.Hk);
+      const T* src = static_cast<const T*>(is_q ? a.q : (is_k ? a.k : a.v));
+      const int64_t off = t * (is_q ? a.q_st : (is_k ? a.k_st : a.v_st)) +
+                          head * (is_q ? a.q_sh : (is_k ? a.k_sh : a.v_sh)) + part * 8;
+      Vec8<T> x;
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (live) {
+        x.load(src + off);
+        x.get(f);
+      }
+      if (a.q_weight) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
+        const float inv = rsqrtf(group_sum<W>(ss) * (1.f / D) + a.eps);
+        if (is_q || is_k) {
+          Vec8<T> wv;
+          float w[8];
+          wv.load(static_cast<const T*>(is_q ? a.q_weight : a.k_weight) + part * 8);
+          wv.get(w);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
+        }
+      }
+      if (a.half) {
+        float p[8];  // the partners
+        if (a.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[i] = (i & 1) ? f[i - 1] : -f[i + 1];
+        } else {
+          const bool first = part < rot_lanes / 2;
+          const int lane = threadIdx.x & 31;
+          const int from = rotated ? (first ? lane + rot_lanes / 2 : lane - rot_lanes / 2) : lane;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            p[i] = __shfl_sync(0xffffffffu, f[i], from);
+            if (first) p[i] = -p[i];
+          }
+        }
+        if (rotated && (is_q || is_k)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + p[i] * s[i];
+        }
+      }
+      if (Q8) {
+        const bool kv = live && !is_q;
+        store_e4m3<D>(f, part, is_k ? a.k_pool : a.v_pool, is_k ? a.k_scale : a.v_scale, a.g, page,
+                      kv ? head : 0, slot, kv);
+      }
+      if (live && (is_q || !Q8)) {
+        x.set(f);
+        if (is_q) {
+          x.store(static_cast<T*>(a.q_out) + t * a.o_st + head * a.o_sh + part * 8);
+        } else {
+          uint8_t* pool = is_k ? a.k_pool : a.v_pool;
+          if (sizeof(T) == 2)
+            x.store(pool + page_chunk(a.g, page, head, slot, part, D / 8));
+          else
+            x.store(pool + page_chunk(a.g, page, head, slot, part * 2, D / 4));
+        }
+      }
+    }
+  }
+}
+
+struct ReadArgs {
+  const uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
+  void *k_out, *v_out;
+  int64_t ko_st, ko_sh, vo_st, vo_sh;  // element strides
+  const int32_t *token_start, *first_pos, *page_table, *page_bounds;
+  int32_t* status;
+  int64_t tokens;
+  PageGeom g;
+  int32_t R, Hk;
+};
+
+template <typename T, int D, bool Q8>
+__global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
+  constexpr int W = D / 8;
+  constexpr int kGroups = kThreads / W;
+  const int group = threadIdx.x / W, part = threadIdx.x % W;
+  grid_dep_wait();
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    const int r = find_request(a.token_start, a.R, t);
+    if (r >= a.R || t < a.token_start[r]) continue;
+    const int64_t pos = static_cast<int64_t>(a.first_pos[r]) + (t - a.token_start[r]);
+    const int64_t lo = a.page_bounds[r], n = a.page_bounds[r + 1] - lo;
+    int64_t page = -1;
+    int err = 0;
+    if (pos < 0 || pos / a.g.page_size >= n) {
+      err = kStatusPosition;
+    } else {
+      page = a.page_table[lo + pos / a.g.page_size];
+      if (page < 0 || page >= a.g.num_pages) err = kStatusPage;
+    }
+    if (err) {
+      if (threadIdx.x == 0 && a.status) atomicExch(a.status, err);
+      continue;
+    }
+    const int slot = static_cast<int>(pos % a.g.page_size);
+    for (int row = group; row < 2 * a.Hk; row += kGroups) {
+      const bool is_k = row < a.Hk;
+      const int head = is_k ? row : row - a.Hk;
+      const uint8_t* pool = is_k ? a.k_pool : a.v_pool;
+      Vec8<T> x;
+      if (Q8) {
+        const uint2 q = *reinterpret_cast<const uint2*>(
+            pool + page_chunk(a.g, page, head, slot, part >> 1, D / 16) + (part & 1) * 8);
+        const float sc = e4m3_scale(
+            (is_k ? a.k_scale : a.v_scale)[page * a.g.scale_page + head * a.g.scale_head + slot]);
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 p = e4m3x2_to_f((i < 2 ? q.x : q.y) >> ((i & 1) * 16));
+          f[2 * i] = p.x * sc;
+          f[2 * i + 1] = p.y * sc;
+        }
+        x.set(f);
+      } else {
+        x.load(pool + (sizeof(T) == 2 ? page_chunk(a.g, page, head, slot, part, D / 8)
+                                      : page_chunk(a.g, page, head, slot, part * 2, D / 4)));
+      }
+      T* out = static_cast<T*>(is_k ? a.k_out : a.v_out) + t * (is_k ? a.ko_st : a.vo_st) +
+               head * (is_k ? a.ko_sh : a.vo_sh) + part * 8;
+      x.store(out);
+    }
+  }
+}
+
+struct CommitArgs8 {
+  const void* const* layer_ptrs;  // [L][6] {new_k, new_v, cache_k, cache_v, k_scale, v_scale}
+  int64_t n_sr, n_sb, n_sh, n_st;
+  const int32_t *page_table, *page_bounds, *accept_results, *cache_lens;
+  int32_t* status;
+  PageGeom g;
+  int32_t R, L, Hk, TB;
+};
+
+// One group per (request, layer, K | V, head): the accepted rows one after another.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) commit_e4m3_kernel(const CommitArgs8 a) {
+  constexpr int W = D / 8;
+  const int part = threadIdx.x % W;
+  grid_dep_wait();
+  const int64_t total = static_cast<int64_t>(a.R) * a.L * 2 * a.Hk;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / W);
+  const int64_t first = blockIdx.x * static_cast<int64_t>(kThreads / W) + threadIdx.x / W;
+  // every group of a warp runs the same number of rounds (the shuffles are the whole warp's)
+  for (int64_t i0 = 0; i0 < total; i0 += step) {
+    const int64_t id = i0 + first;
+    const bool live = id < total;
+    const int64_t x = live ? id : 0;
+    const int h = static_cast<int>(x % a.Hk);
+    const int kv = static_cast<int>(x / a.Hk % 2);
+    const int l = static_cast<int>(x / a.Hk / 2 % a.L);
+    const int r = static_cast<int>(x / a.Hk / 2 / a.L);
+    const int acc = live ? min(max(a.accept_results[2 * r], 0), a.TB) : 0;
+    const int branch = a.accept_results[2 * r + 1];
+    const int64_t len = a.cache_lens[r];
+    const int64_t lo = a.page_bounds[r], n = a.page_bounds[r + 1] - lo;
+    const T* src = static_cast<const T*>(a.layer_ptrs[6 * l + kv]) + r * a.n_sr + branch * a.n_sb +
+                   h * a.n_sh + part * 8;
+    uint8_t* pool = static_cast<uint8_t*>(const_cast<void*>(a.layer_ptrs[6 * l + 2 + kv]));
+    uint8_t* scale = static_cast<uint8_t*>(const_cast<void*>(a.layer_ptrs[6 * l + 4 + kv]));
+    int most = acc;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    for (int t = 0; t < most; ++t) {
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      bool ok = t < acc;
+      int64_t page = 0;
+      const int64_t pos = len + t;
+      if (ok) {
+        int err = 0;
+        if (pos < 0 || pos / 16 >= n) {
+          err = kStatusPosition;
+        } else {
+          page = a.page_table[lo + pos / 16];
+          if (page < 0 || page >= a.g.num_pages) err = kStatusPage;
+        }
+        if (err) {
+          ok = false;
+          if (part == 0 && a.status) atomicExch(a.status, err);
+        } else {
+          Vec8<T> v;
+          v.load(src + t * a.n_st);
+          v.get(f);
+        }
+      }
+      store_e4m3<D>(f, part, pool, scale, a.g, ok ? page : 0, h, static_cast<int>(pos & 15), ok);
+    }
+  }
+}
+
+bool aligned_rows(int64_t a, int64_t b) { return a % 8 == 0 && b % 8 == 0; }
+
+}  // namespace
+}  // namespace d2sd
+
+extern "C" int d2sd_append_kv(
+    const void* q, int64_t q_stride_token, int64_t q_stride_head, void* q_out,
+    int64_t q_out_stride_token, int64_t q_out_stride_head, int32_t num_qo_heads, const void* k,
+    int64_t k_stride_token, int64_t k_stride_head, const void* v, int64_t v_stride_token,
+    int64_t v_stride_head, int32_t num_kv_heads, int64_t num_tokens, int32_t head_dim, int32_t dtype,
+    const void* q_weight, const void* k_weight, float eps, const float* cos_table,
+    const float* sin_table, int64_t table_stride, int64_t table_rows, int32_t rotary_dim,
+    int32_t interleaved, const int32_t* token_start, const int32_t* first_pos, int32_t num_requests,
+    void* k_pool, void* v_pool, int64_t cache_stride_page, int64_t cache_stride_slot,
+    int64_t cache_stride_head, int32_t page_size, int64_t num_pages, int32_t cache_format,
+    void* k_scale, void* v_scale, int64_t scale_stride_page, int64_t scale_stride_head,
+    const int32_t* page_table, const int32_t* page_bounds, int32_t* status, void* stream) {
+  using namespace d2sd;
+  const char* const w = "d2sd_append_kv";
+  if (num_tokens < 0 || num_requests < 0 || num_kv_heads <= 0 || num_qo_heads < 0 || !token_start ||
+      !first_pos || !k_pool || !v_pool || !page_table || !page_bounds ||
+      (num_tokens > 0 && (!k || !v || (num_qo_heads > 0 && (!q || !q_out)))))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
+  if (num_tokens == 0 || num_requests == 0) return D2SD_OK;
+  if (head_dim != 64 && head_dim != 128)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": head_dim must be 64 or 128");
+  if (dtype != D2SD_DTYPE_BF16 && dtype != D2SD_DTYPE_F16 && dtype != D2SD_DTYPE_F32)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": unknown dtype");
+  const bool scaled = k_scale != nullptr;
+  if (scaled != (v_scale != nullptr))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": k_scale and v_scale go together");
+  if ((q_weight != nullptr) != (k_weight != nullptr) && num_qo_heads > 0)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": q_weight and k_weight go together");
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16 != 0)
+    return fail(D2SD_ERR_UNSUPPORTED,
+                std::string(w) + ": rotary_dim must be a multiple of 16 up to head_dim");
+  if (rotary_dim > 0 && (!cos_table || !sin_table || table_rows <= 0 || table_stride < rotary_dim / 2))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": the rotary tables do not fit rotary_dim");
+  const int elem = dtype == D2SD_DTYPE_F32 ? 4 : 2;
+  if (!aligned16(k) || !aligned16(v) || !aligned16(k_pool) || !aligned16(v_pool) ||
+      !aligned16(q_weight) || !aligned16(k_weight) || !aligned_rows(k_stride_token, k_stride_head) ||
+      !aligned_rows(v_stride_token, v_stride_head) ||
+      (num_qo_heads > 0 && (!aligned16(q) || !aligned16(q_out) ||
+                            !aligned_rows(q_stride_token, q_stride_head) ||
+                            !aligned_rows(q_out_stride_token, q_out_stride_head))))
+    return fail(D2SD_ERR_INVALID_ARGUMENT,
+                std::string(w) + ": rows must be 16-byte aligned, strides multiples of 8");
+  AppendArgs a{};
+  int rc = make_page_geom(&a.g, w, head_dim, scaled ? 1 : elem, cache_stride_page, cache_stride_slot,
+                          cache_stride_head, page_size, num_pages, cache_format, scaled,
+                          scale_stride_page, scale_stride_head);
+  if (rc) return rc;
+  if (scaled && elem != 2)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": 8-bit rows are written from 16-bit values");
+  a.q = q, a.k = k, a.v = v, a.q_out = q_out;
+  a.q_st = q_stride_token, a.q_sh = q_stride_head, a.o_st = q_out_stride_token,
+  a.o_sh = q_out_stride_head, a.k_st = k_stride_token, a.k_sh = k_stride_head, a.v_st = v_stride_token,
+  a.v_sh = v_stride_head;
+  a.q_weight = q_weight ? q_weight : k_weight, a.k_weight = k_weight;
+  a.cos = cos_table, a.sin = sin_table, a.table_stride = table_stride, a.table_rows = table_rows;
+  a.token_start = token_start, a.first_pos = first_pos;
+  a.page_table = page_table, a.page_bounds = page_bounds;
+  a.k_pool = static_cast<uint8_t*>(k_pool), a.v_pool = static_cast<uint8_t*>(v_pool);
+  a.k_scale = static_cast<uint8_t*>(k_scale), a.v_scale = static_cast<uint8_t*>(v_scale);
+  a.status = status;
+  a.tokens = num_tokens;
+  a.eps = eps;
+  a.R = num_requests, a.Hq = num_qo_heads, a.Hk = num_kv_heads, a.half = rotary_dim / 2,
+  a.interleaved = interleaved;
+  const int64_t cap = static_cast<int64_t>(current_sm_count()) * 64;
+  const dim3 grid(static_cast<unsigned>(num_tokens < cap ? num_tokens : cap));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kThreads), 0, st, w, a); };
+  if (dtype == D2SD_DTYPE_F32) return head_dim == 128 ? go(append_kernel<float, 128, false>) : go(append_kernel<float, 64, false>);
+  if (dtype == D2SD_DTYPE_BF16) {
+    if (scaled) return head_dim == 128 ? go(append_kernel<__nv_bfloat16, 128, true>) : go(append_kernel<__nv_bfloat16, 64, true>);
+    return head_dim == 128 ? go(append_kernel<__nv_bfloat16, 128, false>) : go(append_kernel<__nv_bfloat16, 64, false>);
+  }
+  if (scaled) return head_dim == 128 ? go(append_kernel<__half, 128, true>) : go(append_kernel<__half, 64, true>);
+  return head_dim == 128 ? go(append_kernel<__half, 128, false>) : go(append_kernel<__half, 64, false>);
+}
+
+extern "C" int d2sd_read_kv(const void* k_pool, const void* v_pool, int64_t cache_stride_page,
+                            int64_t cache_stride_slot, int64_t cache_stride_head, int32_t page_size,
+                            int64_t num_pages, int32_t cache_format, const void* k_scale,
+                            const void* v_scale, int64_t scale_stride_page, int64_t scale_stride_head,
+                            const int32_t* page_table, const int32_t* page_bounds,
+                            const int32_t* token_start, const int32_t* first_pos, int32_t num_requests,
+                            int64_t num_tokens, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                            void* k_out, int64_t k_out_stride_token, int64_t k_out_stride_head,
+                            void* v_out, int64_t v_out_stride_token, int64_t v_out_stride_head,
+                            int32_t* status, void* stream) {
+  using namespace d2sd;
+  const char* const w = "d2sd_read_kv";
+  if (num_tokens < 0 || num_requests < 0 || num_kv_heads <= 0 || !token_start || !first_pos || !k_pool ||
+      !v_pool || !page_table || !page_bounds || (num_tokens > 0 && (!k_out || !v_out)))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
+  if (num_tokens == 0 || num_requests == 0) return D2SD_OK;
+  if (head_dim != 64 && head_dim != 128)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": head_dim must be 64 or 128");
+  if (dtype != D2SD_DTYPE_BF16 && dtype != D2SD_DTYPE_F16 && dtype != D2SD_DTYPE_F32)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": unknown dtype");
+  const bool scaled = k_scale != nullptr;
+  if (scaled != (v_scale != nullptr))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": k_scale and v_scale go together");
+  if (!aligned16(k_pool) || !aligned16(v_pool) || !aligned16(k_out) || !aligned16(v_out) ||
+      !aligned_rows(k_out_stride_token, k_out_stride_head) ||
+      !aligned_rows(v_out_stride_token, v_out_stride_head))
+    return fail(D2SD_ERR_INVALID_ARGUMENT,
+                std::string(w) + ": rows must be 16-byte aligned, strides multiples of 8");
+  const int elem = dtype == D2SD_DTYPE_F32 ? 4 : 2;
+  if (scaled && elem != 2)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": 8-bit rows are read into 16-bit values");
+  ReadArgs a{};
+  int rc = make_page_geom(&a.g, w, head_dim, scaled ? 1 : elem, cache_stride_page, cache_stride_slot,
+                          cache_stride_head, page_size, num_pages, cache_format, scaled,
+                          scale_stride_page, scale_stride_head);
+  if (rc) return rc;
+  a.k_pool = static_cast<const uint8_t*>(k_pool), a.v_pool = static_cast<const uint8_t*>(v_pool);
+  a.k_scale = static_cast<const uint8_t*>(k_scale), a.v_scale = static_cast<const uint8_t*>(v_scale);
+  a.k_out = k_out, a.v_out = v_out;
+  a.ko_st = k_out_stride_token, a.ko_sh = k_out_stride_head, a.vo_st = v_out_stride_token,
+  a.vo_sh = v_out_stride_head;
+  a.token_start = token_start, a.first_pos = first_pos, a.page_table = page_table,
+  a.page_bounds = page_bounds;
+  a.status = status;
+  a.tokens = num_tokens;
+  a.R = num_requests, a.Hk = num_kv_heads;
+  const int64_t cap = static_cast<int64_t>(current_sm_count()) * 64;
+  const dim3 grid(static_cast<unsigned>(num_tokens < cap ? num_tokens : cap));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kThreads), 0, st, w, a); };
+  if (dtype == D2SD_DTYPE_F32) return head_dim == 128 ? go(read_kernel<float, 128, false>) : go(read_kernel<float, 64, false>);
+  if (dtype == D2SD_DTYPE_BF16) {
+    if (scaled) return head_dim == 128 ? go(read_kernel<__nv_bfloat16, 128, true>) : go(read_kernel<__nv_bfloat16, 64, true>);
+    return head_dim == 128 ? go(read_kernel<__nv_bfloat16, 128, false>) : go(read_kernel<__nv_bfloat16, 64, false>);
+  }
+  if (scaled) return head_dim == 128 ? go(read_kernel<__half, 128, true>) : go(read_kernel<__half, 64, true>);
+  return head_dim == 128 ? go(read_kernel<__half, 128, false>) : go(read_kernel<__half, 64, false>);
+}
+
+extern "C" int d2sd_commit_kv_e4m3(const void* const* layer_ptrs, int32_t num_layers,
+                                   int32_t num_requests, int32_t num_kv_heads, int32_t head_dim,
+                                   int32_t dtype, int32_t block_len, int64_t new_stride_request,
+                                   int64_t new_stride_branch, int64_t new_stride_head,
+                                   int64_t new_stride_token, int64_t cache_stride_page,
+                                   int64_t cache_stride_head, int64_t num_pages,
+                                   int64_t scale_stride_page, int64_t scale_stride_head,
+                                   const int32_t* page_table, const int32_t* page_bounds,
+                                   const int32_t* accept_results, const int32_t* cache_lens,
+                                   int32_t* status, void* stream) {
+  using namespace d2sd;
+  const char* const w = "d2sd_commit_kv_e4m3";
+  if (!layer_ptrs || num_layers <= 0 || num_requests <= 0 || num_kv_heads <= 0 || block_len <= 0 ||
+      !page_table || !page_bounds || !accept_results || !cache_lens)
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": head_dim must be 64 or 128");
+  if (dtype != D2SD_DTYPE_BF16 && dtype != D2SD_DTYPE_F16)
+    return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": 8-bit rows are written from 16-bit values");
+  if (!aligned_rows(new_stride_request, new_stride_branch) ||
+      !aligned_rows(new_stride_head, new_stride_token))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": strides must be multiples of 8");
+  CommitArgs8 a{};
+  int rc = make_page_geom(&a.g, w, head_dim, 1, cache_stride_page, 0, cache_stride_head, 16, num_pages,
+                          D2SD_KV_UMMA_PAGES, true, scale_stride_page, scale_stride_head);
+  if (rc) return rc;
+  a.layer_ptrs = layer_ptrs;
+  a.n_sr = new_stride_request, a.n_sb = new_stride_branch, a.n_sh = new_stride_head,
+  a.n_st = new_stride_token;
+  a.page_table = page_table, a.page_bounds = page_bounds, a.accept_results = accept_results,
+  a.cache_lens = cache_lens, a.status = status;
+  a.R = num_requests, a.L = num_layers, a.Hk = num_kv_heads, a.TB = block_len;
+  const int64_t groups = static_cast<int64_t>(num_requests) * num_layers * 2 * num_kv_heads;
+  const int64_t per = kThreads / (head_dim / 8);
+  int64_t blocks = (groups + per - 1) / per;
+  const int64_t cap = static_cast<int64_t>(current_sm_count()) * 8;
+  if (blocks > cap) blocks = cap;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kThreads), 0, st, w, a); };
+  if (dtype == D2SD_DTYPE_BF16)
+    return head_dim == 128 ? go(commit_e4m3_kernel<__nv_bfloat16, 128>) : go(commit_e4m3_kernel<__nv_bfloat16, 64>);
+  return head_dim == 128 ? go(commit_e4m3_kernel<__half, 128>) : go(commit_e4m3_kernel<__half, 64>);
+}

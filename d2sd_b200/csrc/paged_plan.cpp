@@ -1,0 +1,177 @@
+// Host-side plan of the attention over the paged cache (paged_plan.h).
+#include <stdint.h>
+#include <string.h>
+
+#include <algorithm>
+#include <exception>
+#include <string>
+#include <vector>
+
+#include "../../include/d2sd.h"
+#include "paged_plan.h"
+
+namespace d2sd {
+void set_last_error(const std::string& msg);
+
+namespace {
+using namespace paged;
+
+int plan_fail(int code, const char* msg) {
+  set_last_error(std::string("d2sd_paged_plan: ") + msg);
+  return code;
+}
+
+struct Unit {
+  int32_t req, head, tok0, row0, nrows, key0, key1, pos0, page_off, kv_len;
+  int32_t tiles() const { return key1 > key0 ? (key1 - key0 + kTileKeys - 1) / kTileKeys : 0; }
+};
+
+// The units in order, cut where a CTA's share of the tiles ends. Every item
+// costs `fixed` tiles on top of its own (its start, its end and, for a split
+// unit, the joining), so a CTA of many small items gets fewer tiles.
+void cut(const std::vector<Unit>& units, int ctas, int fixed, int32_t window, std::vector<int32_t>& items,
+         std::vector<int32_t>& first, int32_t* slots, int32_t* tickets) {
+  int64_t total = 0;
+  for (const Unit& u : units) total += u.tiles() + fixed;
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>(ctas, total / (1 + fixed)));
+  *slots = *tickets = 0;
+  first.assign(1, 0);
+  int64_t done = 0;  // cost handed out so far
+  int32_t count = 0;
+  for (const Unit& u : units) {
+    const size_t at = items.size();
+    int32_t key = u.key0, parts = 0;
+    int left = u.tiles();
+    do {
+      // this CTA's share ends at cost total * k / n
+      const int64_t k = static_cast<int64_t>(first.size());
+      int64_t room = total * k / n - done - fixed;
+      if (k >= n) room = total;
+      int take = static_cast<int>(std::min<int64_t>(left, std::max<int64_t>(room, 1)));
+      if (left - take == 1 && take > 1 && room - take >= -1) take = left;  // no splinter of one tile
+      const int32_t end = (take == left) ? u.key1 : key + take * kTileKeys;
+      const int32_t it[kItemInts] = {u.req,  u.head, u.tok0,     u.row0,   u.nrows, key, end, u.pos0,
+                                     window, u.page_off, u.kv_len, parts,    0,       0,   0,   0};
+      items.insert(items.end(), it, it + kItemInts);
+      ++count;
+      ++parts;
+      left -= take;
+      done += take + fixed;
+      total += left > 0 ? fixed : 0;  // the next part's own fixed cost
+      key = end;
+      while (static_cast<int64_t>(first.size()) < n &&
+             done + fixed >= total * static_cast<int64_t>(first.size()) / n)
+        first.push_back(count);
+    } while (left > 0);
+    for (int p = 0; p < parts; ++p) {
+      int32_t* it = items.data() + at + static_cast<size_t>(p) * kItemInts;
+      it[P_SLOT] = parts > 1 ? *slots + p : -1;
+      it[P_FIRST_SLOT] = *slots;
+      it[P_PARTS] = parts;
+      it[P_TICKET] = *tickets;
+    }
+    if (parts > 1) {
+      *slots += parts;
+      ++*tickets;
+    }
+  }
+  first.push_back(count);
+}
+
+}  // namespace
+}  // namespace d2sd
+
+extern "C" int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_requests,
+                                            int32_t num_qo_heads, int32_t num_kv_heads,
+                                            int32_t num_ctas) {
+  using namespace d2sd::paged;
+  if (!q_lens || num_requests < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 ||
+      num_qo_heads % num_kv_heads || num_ctas <= 0)
+    return -1;
+  const int64_t G = num_qo_heads / num_kv_heads;
+  int64_t units = 0;
+  for (int r = 0; r < num_requests; ++r) {
+    if (q_lens[r] < 0) return -1;
+    units += (q_lens[r] * G + kRowsTile - 1) / kRowsTile * num_kv_heads;
+  }
+  // every CTA adds at most one cut
+  return kHeaderInts + (units + 2 * static_cast<int64_t>(num_ctas)) * kItemInts + 4 * (num_ctas + 2);
+}
+
+extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
+                               const int32_t* page_offsets, int32_t num_requests, int32_t num_qo_heads,
+                               int32_t num_kv_heads, int32_t causal, int32_t window, int32_t num_ctas,
+                               int32_t* plan, int64_t capacity, int64_t* used, int32_t* sections) {
+  using namespace d2sd;
+  using namespace d2sd::paged;
+  if (num_requests < 0 || (num_requests > 0 && (!q_lens || !kv_lens || !page_offsets)) || !plan ||
+      !used || !sections || num_ctas <= 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || window < 0)
+    return plan_fail(D2SD_ERR_INVALID_ARGUMENT, "invalid argument");
+  if (num_qo_heads % num_kv_heads)
+    return plan_fail(D2SD_ERR_INVALID_ARGUMENT, "query heads must be a multiple of kv heads");
+  if (window > 0 && !causal)
+    return plan_fail(D2SD_ERR_UNSUPPORTED, "a window needs a causal mask");
+  const int G = num_qo_heads / num_kv_heads;
+  try {
+    if (G > 128) return plan_fail(D2SD_ERR_UNSUPPORTED, "more than 128 query heads per kv head");
+    std::vector<Unit> units[kSections];
+    int64_t tok = 0;
+    for (int r = 0; r < num_requests; ++r) {
+      const int64_t n = q_lens[r], kv = kv_lens[r];
+      if (n < 0 || kv < 0 || page_offsets[r] < 0)
+        return plan_fail(D2SD_ERR_INVALID_ARGUMENT, "negative length or page offset");
+      if (kv >= kNoLimit || n * G >= kNoLimit || tok + n >= kNoLimit)
+        return plan_fail(D2SD_ERR_UNSUPPORTED, "lengths above 2^30");
+      const int64_t rows = n * G;
+      const int section = 0;
+      const int64_t tile = kRowsTile;
+      const int32_t pos0 = causal ? static_cast<int32_t>(kv - n) : kNoLimit;
+      for (int h = 0; h < num_kv_heads; ++h) {
+        for (int64_t row = 0; row < rows; row += tile) {
+          const int64_t nr = std::min(tile, rows - row);
+          const int64_t t0 = row / G, t1 = (row + nr - 1) / G;
+          int64_t lo = 0, hi = kv;
+          if (causal) {
+            hi = std::max<int64_t>(0, std::min<int64_t>(kv, pos0 + t1 + 1));
+            if (window) lo = std::max<int64_t>(0, pos0 + t0 + 1 - window);
+          }
+          lo = lo / kTileKeys * kTileKeys;
+          if (lo > hi) lo = hi;
+          units[section].push_back({r, h, static_cast<int32_t>(tok), static_cast<int32_t>(row),
+                                    static_cast<int32_t>(nr), static_cast<int32_t>(lo),
+                                    static_cast<int32_t>(hi), pos0, page_offsets[r],
+                                    static_cast<int32_t>(kv)});
+        }
+      }
+      tok += n;
+    }
+    std::vector<int32_t> out(kHeaderInts, 0);
+    out[H_MAGIC] = kMagic;
+    out[H_REQUESTS] = num_requests;
+    out[H_TOKENS] = static_cast<int32_t>(tok);
+    out[H_GROUP] = G;
+    out[H_KV_HEADS] = num_kv_heads;
+    for (int s = 0; s < kSections; ++s) {
+      int32_t sec[kSectionInts] = {0};
+      if (!units[s].empty()) {
+        std::vector<int32_t> items, first;
+        cut(units[s], num_ctas, 1, window, items, first, &sec[S_SLOTS], &sec[S_TICKETS]);
+        sec[S_CTAS] = static_cast<int32_t>(first.size()) - 1;
+        sec[S_ITEMS] = static_cast<int32_t>(items.size() / kItemInts);
+        sec[S_OFF_CTA] = static_cast<int32_t>(out.size());
+        out.insert(out.end(), first.begin(), first.end());
+        while (out.size() % 4) out.push_back(0);
+        sec[S_OFF_ITEMS] = static_cast<int32_t>(out.size());
+        out.insert(out.end(), items.begin(), items.end());
+      }
+      memcpy(out.data() + H_SECTION + s * kSectionInts, sec, sizeof(sec));
+      memcpy(sections + s * kSectionInts, sec, sizeof(sec));
+    }
+    *used = static_cast<int64_t>(out.size());
+    if (*used > capacity) return plan_fail(D2SD_ERR_WORKSPACE, "plan buffer too small");
+    memcpy(plan, out.data(), out.size() * sizeof(int32_t));
+  } catch (const std::exception& e) {  // out of host memory
+    return plan_fail(D2SD_ERR_INVALID_ARGUMENT, e.what());
+  }
+  return D2SD_OK;
+}

@@ -477,3 +477,163 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
         _stream(dev)), "d2sd_qk_norm_rope")
     return q_out, k_out
 
+
+
+# ---------------------------------------------------------------------------
+# The target's own tokens and the paged cache: write, read back
+# ---------------------------------------------------------------------------
+_E4M3 = torch.float8_e4m3fn
+
+
+def _int32(name: str, t: torch.Tensor, n: int | None = None) -> int:
+    if t.dtype != torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{name} must be a contiguous int32 tensor"
+                         + (f" with {n} entries" if n is not None else ""))
+    return t.data_ptr()
+
+
+def _pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale):
+    """The C arguments (strides, page size, pages, format, scales) of a K and V
+    pool, and its (heads, head_dim)."""
+    if not kv_layout.startswith("paged_"):
+        raise ValueError(f"a paged layout is needed, not {kv_layout!r}")
+    kv = kv_view(k_pool, kv_layout)
+    if v_pool.shape != k_pool.shape or v_pool.stride() != k_pool.stride() \
+            or v_pool.dtype != k_pool.dtype:
+        raise ValueError("k and v pools must share shape, strides and dtype")
+    sp = sh = 0
+    if k_pool.dtype == _E4M3:
+        if k_scale is None or v_scale is None:
+            raise ValueError("an e4m3 pool needs k_scale and v_scale")
+        if kv_layout != "paged_umma":
+            raise NotImplementedError("8-bit rows are kept in the paged_umma layout")
+        for s in (k_scale, v_scale):
+            if s.dtype != torch.uint8 or s.shape != k_pool.shape[:3] or s.stride(-1) != 1 \
+                    or s.stride() != k_scale.stride():
+                raise ValueError("scales must be uint8 [pages, Hk, 16], slots contiguous")
+        sp, sh = k_scale.stride(0), k_scale.stride(1)
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError("only e4m3 pools have scales")
+    args = (kv.stride_page, kv.stride_slot, kv.stride_head, kv.page_size, kv.num_pages,
+            _lib.KV_UMMA_PAGES if kv.native else _lib.KV_ROWS, _ptr(k_scale), _ptr(v_scale), sp, sh)
+    return args, kv.num_kv_heads, kv.head_dim
+
+
+def _row_strides(name: str, t: torch.Tensor, heads: int, dim: int):
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.stride(2) != 1:
+        raise ValueError(f"{name} must be [tokens, {heads}, {dim}] with a contiguous head_dim")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def _call(dev: torch.device, fn, args, what: str) -> None:
+    """Run a C entry point on dev's current stream, whatever the current device."""
+    if torch.cuda.current_device() == dev.index:
+        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
+        return
+    with torch.cuda.device(dev):
+        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
+
+
+def append_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+              kv_layout: str, page_table: torch.Tensor, page_bounds: torch.Tensor,
+              token_start: torch.Tensor, first_pos: torch.Tensor, *,
+              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+              q: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+              q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+              eps: float = 1e-6, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+              interleaved: bool = False, status: torch.Tensor | None = None):
+    """Write a ragged batch's new tokens into the paged cache (d2sd_append_kv).
+
+    k, v [tokens, Hk, D] (and q [tokens, Hq, D], optional) in the projections'
+    type; request r's tokens are rows token_start[r] .. token_start[r + 1] - 1 and
+    go to its positions first_pos[r] onward, in the pages page_table[page_bounds[r]
+    .. page_bounds[r + 1]). Pools per ``kv_layout`` hold the type of k, or
+    float8_e4m3fn with uint8 scales [pages, Hk, 16] ("paged_umma").
+
+    q_weight / k_weight [D]: per-head RMSNorm of q and k first. cos / sin fp32
+    [positions, rotary_dim / 2], indexed by position: the first rotary_dim elements
+    of each q and k head are rotated, in pairs (i, i + rotary_dim / 2) or, with
+    ``interleaved``, (2i, 2i + 1) (``rope_tables`` makes them). Both in fp32,
+    rounded once. Returns q_out (default: q, in place). A token with a bad position
+    or page is skipped and ``status`` (int32, optional) says why."""
+    dev = _require_cuda(k, v, k_pool, v_pool, page_table, page_bounds, token_start, first_pos,
+                        k_scale, v_scale, q, q_out, q_weight, k_weight, cos, sin, status)
+    pool, Hk, D = _pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale)
+    n = k.shape[0]
+    if v.shape[0] != n or v.dtype != k.dtype:
+        raise ValueError("k and v must have the same tokens and dtype")
+    if k_pool.dtype not in (k.dtype, _E4M3):
+        raise ValueError(f"a {k_pool.dtype} cache does not take {k.dtype} rows")
+    R = first_pos.numel()
+    q_args, o_args, Hq = (None, 0, 0), (None, 0, 0), 0
+    if q is not None:
+        q_out = q if q_out is None else q_out
+        Hq = q.shape[1]
+        if q.shape[0] != n or q.dtype != k.dtype or q_out.dtype != k.dtype or q_out.shape != q.shape:
+            raise ValueError("q and q_out must match k's tokens and dtype")
+        q_args, o_args = _row_strides("q", q, Hq, D), _row_strides("q_out", q_out, Hq, D)
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != k.dtype or w.shape != (D,) or not w.is_contiguous()):
+            raise ValueError("norm weights must be contiguous [head_dim] in the data dtype")
+    if q is not None and (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight go together")
+    rot = rows = stride = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    if cos is not None:
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape \
+                or cos.dim() != 2 or cos.stride() != sin.stride() or cos.stride(1) != 1:
+            raise ValueError("cos and sin must be fp32 [positions, rotary_dim / 2] with the same "
+                             "strides, columns contiguous")
+        rows, rot, stride = cos.shape[0], 2 * cos.shape[1], cos.stride(0)
+    args = (*q_args, *o_args, Hq, *_row_strides("k", k, Hk, D), *_row_strides("v", v, Hk, D), Hk, n,
+            D, dtype_code(k), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
+            stride, rows, rot, 1 if interleaved else 0, _int32("token_start", token_start, R + 1),
+            _int32("first_pos", first_pos), R, k_pool.data_ptr(), v_pool.data_ptr(), *pool,
+            _int32("page_table", page_table), _int32("page_bounds", page_bounds, R + 1),
+            _ptr(status))
+    _call(dev, load().d2sd_append_kv, args, "d2sd_append_kv")
+    return q_out
+
+
+def read_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, kv_layout: str, page_table: torch.Tensor,
+            page_bounds: torch.Tensor, token_start: torch.Tensor, first_pos: torch.Tensor,
+            k_out: torch.Tensor, v_out: torch.Tensor, *, k_scale: torch.Tensor | None = None,
+            v_scale: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """Rows of a ragged batch out of the paged cache (d2sd_read_kv): k_out, v_out
+    [tokens, Hk, D] rows token_start[r] .. from request r's positions first_pos[r]
+    on. An e4m3 cache is read into bf16 (exact) or fp16 rows, any other into rows
+    of its own type. Rows behind the last request stay as they are."""
+    dev = _require_cuda(k_pool, v_pool, page_table, page_bounds, token_start, first_pos, k_out,
+                        v_out, k_scale, v_scale, status)
+    pool, Hk, D = _pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale)
+    n, R = k_out.shape[0], first_pos.numel()
+    if v_out.shape[0] != n or v_out.dtype != k_out.dtype:
+        raise ValueError("k_out and v_out must have the same rows and dtype")
+    if k_pool.dtype not in (k_out.dtype, _E4M3):
+        raise ValueError(f"a {k_pool.dtype} cache is not read into {k_out.dtype} rows")
+    args = (k_pool.data_ptr(), v_pool.data_ptr(), *pool, _int32("page_table", page_table),
+            _int32("page_bounds", page_bounds, R + 1), _int32("token_start", token_start, R + 1),
+            _int32("first_pos", first_pos), R, n, Hk, D, dtype_code(k_out),
+            *_row_strides("k_out", k_out, Hk, D), *_row_strides("v_out", v_out, Hk, D),
+            _ptr(status))
+    _call(dev, load().d2sd_read_kv, args, "d2sd_read_kv")
+
+
+def commit_kv_e4m3(layer_ptrs: torch.Tensor, *, num_layers: int, num_requests: int,
+                   num_kv_heads: int, head_dim: int, dtype: torch.dtype, block_len: int,
+                   new_strides: tuple[int, int, int, int], cache_strides: tuple[int, int],
+                   num_pages: int, scale_strides: tuple[int, int], page_table: torch.Tensor,
+                   page_bounds: torch.Tensor, accept_results: torch.Tensor,
+                   cache_lens: torch.Tensor, status: torch.Tensor | None = None) -> None:
+    """``commit_kv_batch`` into an 8-bit cache (d2sd_commit_kv_e4m3). layer_ptrs:
+    int64 device tensor [L*6] of {new_k, new_v, cache_k, cache_v, k_scale, v_scale}
+    pointers; cache and scale strides are (page, head)."""
+    dev = _require_cuda(layer_ptrs, page_table, page_bounds, accept_results, cache_lens, status)
+    args = (layer_ptrs.data_ptr(), num_layers, num_requests, num_kv_heads, head_dim,
+            _DTYPES.get(dtype, -1), block_len, *new_strides, *cache_strides, num_pages,
+            *scale_strides, _int32("page_table", page_table),
+            _int32("page_bounds", page_bounds, num_requests + 1),
+            _int32("accept_results", accept_results), _int32("cache_lens", cache_lens),
+            _ptr(status))
+    _call(dev, load().d2sd_commit_kv_e4m3, args, "d2sd_commit_kv_e4m3")

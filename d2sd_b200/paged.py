@@ -1,0 +1,197 @@
+"""The target's own attention over its paged cache.
+
+``paged_attention`` runs a ragged batch of new tokens -- prompts in chunks, single
+tokens, drafted blocks taken as plain sequences -- against the cache that
+``ops.append_kv`` has just written them into: causal, with an optional sliding
+window and attention sinks, over 16-bit or e4m3 pages. ``PagedAttentionPlan`` is
+its plan/run split, as ``CascadePlan`` is kernel (a)'s: built on the host from the
+lengths once per step, used by every layer.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+from . import _lib, ops
+from ._lib import check, load
+
+_SINKS = {"reference": _lib.SINK_REFERENCE, "exact": _lib.SINK_EXACT}
+
+
+class PagedAttentionPlan:
+    """Work plan and workspace of ``paged_attention`` for one ragged batch.
+
+    q_lens / kv_lens: new tokens of each request and its cached positions, the new
+    ones included (the new tokens are the last of them). page_offsets: each
+    request's first entry in the page table (default: one request from entry 0, or
+    ``PagedKVPool.page_offsets_host``); a longer list (page bounds) is cut.
+    window: a row sees only the last ``window`` positions up to its own.
+
+    The plan owns the workspace of its calls: two calls that overlap on the GPU
+    need a plan each. ``update`` re-plans in place; with ``reserve=(requests,
+    tokens)`` the device buffers have room for that many, and the launch does not
+    depend on the lengths, so a captured ``paged_attention`` replays with the new
+    ones. Both must run where the next call sees them (the same stream, or ordered
+    before it).
+    """
+
+    def __init__(self, q_lens, kv_lens, num_qo_heads: int, num_kv_heads: int, head_dim: int,
+                 device: torch.device | str, *, causal: bool = True, window: int | None = None,
+                 page_offsets=None, reserve: tuple[int, int] | None = None):
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("PagedAttentionPlan needs a CUDA device")
+        if window is not None and window <= 0:
+            raise ValueError("window must be positive")
+        self.num_qo_heads, self.num_kv_heads, self.head_dim = num_qo_heads, num_kv_heads, head_dim
+        self.causal, self.window = causal, window
+        self.num_ctas = ops.num_sms(device)
+        self.fixed_grid = reserve is not None
+        host, sections, tokens = self._plan(q_lens, kv_lens, page_offsets)
+        need = len(host)
+        if reserve is not None:
+            # every request adds at most one short tile per kv head
+            rows, G = max(reserve[1], tokens), num_qo_heads // num_kv_heads
+            lens = np.ones(max(reserve[0], 1), dtype=np.int32)
+            lens[0] = rows
+            need = max(need, load().d2sd_paged_plan_capacity(
+                lens.ctypes.data, len(lens), num_qo_heads, num_kv_heads, self.num_ctas)
+                + 16 * num_kv_heads * len(lens) * -(-G // 16))
+        with torch.cuda.device(device):
+            self.plan = torch.zeros(need, dtype=torch.int32, device=device)
+            self.device = self.plan.device
+            nbytes = load().d2sd_paged_workspace_bytes(self.num_ctas, head_dim)
+            if nbytes < 0:
+                raise NotImplementedError("paged attention: head_dim must be 64 or 128")
+            self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            self.status = torch.zeros(1, dtype=torch.int32, device=device)
+            self._set(host, sections, tokens)
+            torch.cuda.current_stream(device).synchronize()  # usable on any stream from here
+
+    def _plan(self, q_lens, kv_lens, page_offsets):
+        q = np.ascontiguousarray(q_lens, dtype=np.int32)
+        kv = np.ascontiguousarray(kv_lens, dtype=np.int32)
+        R = len(q)
+        if q.ndim != 1 or kv.shape != q.shape:
+            raise ValueError("q_lens and kv_lens must be lists of the same length")
+        if page_offsets is None:
+            if R > 1:
+                raise ValueError("page_offsets are required for several requests")
+            page_offsets = [0] * R
+        off = np.ascontiguousarray(page_offsets, dtype=np.int32)[:R]
+        if len(off) != R:
+            raise ValueError("page_offsets must have an entry for each request")
+        lib = load()
+        cap = lib.d2sd_paged_plan_capacity(q.ctypes.data, R, self.num_qo_heads, self.num_kv_heads,
+                                           self.num_ctas)
+        if cap < 0:
+            raise ValueError("invalid plan sizes")
+        plan = np.empty(cap, dtype=np.int32)
+        used = np.zeros(1, dtype=np.int64)
+        sections = np.zeros(12, dtype=np.int32)
+        check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, R,
+                                  self.num_qo_heads, self.num_kv_heads, 1 if self.causal else 0,
+                                  self.window or 0, self.num_ctas, plan.ctypes.data, cap,
+                                  used.ctypes.data, sections.ctypes.data), "d2sd_paged_plan")
+        return plan[:int(used[0])], sections, int(q.sum())
+
+    def _set(self, host, sections, tokens):
+        if len(host) > self.plan.numel():
+            raise ValueError("the batch is larger than the plan's reserve")
+        self.plan[:len(host)].copy_(torch.from_numpy(host))
+        self.host_plan, self.sections, self.tokens = host, sections, tokens
+
+    def update(self, q_lens, kv_lens, page_offsets=None) -> None:
+        """Plan another batch into the same device buffers, on the current stream."""
+        new = self._plan(q_lens, kv_lens, page_offsets)
+        if len(new[0]) > self.plan.numel() and not self.fixed_grid:
+            self.plan = torch.empty(2 * len(new[0]), dtype=torch.int32, device=self.device)
+        self._set(*new)
+
+
+def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, kv_layout: str,
+                    page_table: torch.Tensor, plan: PagedAttentionPlan, *,
+                    sm_scale: float | None = None, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None, sinks: torch.Tensor | None = None,
+                    sink_mode: str = "exact", out: torch.Tensor | None = None,
+                    lse: torch.Tensor | None = None):
+    """q [tokens, Hq, D] (bf16 or fp16; bf16 with an e4m3 cache), the planned
+    requests' new tokens one after another; pools per ``kv_layout`` ("paged_umma",
+    "paged_hnd" or "paged_nhd") with their int32 ``page_table``; k_scale / v_scale
+    uint8 [pages, Hk, 16] for an e4m3 cache. sinks fp32 [Hq]: out times
+    sigmoid(lse - sink) (``sink_mode`` as in ``cascade_attention``).
+
+    Returns (out [tokens, Hq, D], lse [tokens, Hq] fp32, base 2), written into
+    ``out`` / ``lse`` when given; rows behind the plan's tokens are left alone. A
+    row that sees no key has out 0 and lse -inf. Cache slots past a request's last
+    position may hold anything. A NaN or an infinity in the value of a position that
+    some row of a tile sees may reach rows of that tile that do not see it."""
+    dev = ops._require_cuda(q, k_pool, v_pool, page_table, k_scale, v_scale, sinks, out, lse)
+    Hq, Hk, D = plan.num_qo_heads, plan.num_kv_heads, plan.head_dim
+    if dev != plan.device:
+        raise ValueError("the plan is for another device")
+    if q.dim() != 3 or q.shape[0] < plan.tokens:
+        raise ValueError(f"q must hold the plan's {plan.tokens} tokens")
+    pool, heads, dim = ops._pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale)
+    if heads != Hk or dim != D:
+        raise ValueError("the pools and the plan differ in kv heads or head_dim")
+    if k_pool.dtype != q.dtype and not (k_pool.dtype == torch.float8_e4m3fn):
+        raise ValueError(f"a {k_pool.dtype} cache does not take {q.dtype} queries")
+    if q.dtype == torch.float32:
+        raise NotImplementedError("paged attention takes bf16 or fp16 queries")
+    if sinks is not None and (sinks.dtype != torch.float32 or not sinks.is_contiguous()
+                              or sinks.numel() != Hq):
+        raise ValueError("sinks must be a contiguous fp32 tensor [num_qo_heads]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape[0] < plan.tokens:
+        raise ValueError("out must hold the plan's tokens in q's dtype")
+    if lse is None:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
+    elif lse.dtype != torch.float32 or lse.dim() != 2 or lse.stride(1) != 1 \
+            or lse.shape[0] < plan.tokens or lse.shape[1] != Hq:
+        raise ValueError("lse must be fp32 [tokens, num_qo_heads] with a contiguous head axis")
+    args = (*ops._row_strides("q", q, Hq, D), ops.dtype_code(q), k_pool.data_ptr(),
+            v_pool.data_ptr(), *pool, ops._int32("page_table", page_table), page_table.numel(), Hq,
+            Hk, D, D ** -0.5 if sm_scale is None else float(sm_scale), plan.plan.data_ptr(),
+            plan.sections.ctypes.data, plan.num_ctas, 1 if plan.fixed_grid else 0,
+            plan.workspace.data_ptr(), plan.workspace.numel(), ops._ptr(sinks),
+            _SINKS[sink_mode] if sinks is not None else 0, *ops._row_strides("out", out, Hq, D),
+            lse.data_ptr(), lse.stride(0), plan.status.data_ptr())
+    ops._call(dev, load().d2sd_paged_attention, args, "d2sd_paged_attention")
+    return out, lse
+
+
+def rope_tables(num_positions: int, rotary_dim: int, theta: float, device, *,
+                scaling: dict | None = None):
+    """cos and sin tables for ``ops.append_kv``: fp32 [num_positions, rotary_dim / 2],
+    angles in 64 bits. scaling: None; {"type": "linear", "factor": f} (positions
+    divided by f); {"type": "yarn", "factor": f, "original": L, "beta_fast": 32,
+    "beta_slow": 1} (wavelengths far below L keep their frequency, those far above
+    are divided by f, with a linear ramp between, and both tables are multiplied by
+    0.1 ln f + 1, as YaRN's paper defines them)."""
+    if rotary_dim <= 0 or rotary_dim % 2 or num_positions <= 0:
+        raise ValueError("rope_tables: positive sizes, an even rotary_dim")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    freq = theta ** (-i / rotary_dim)
+    gain = 1.0
+    if scaling is not None:
+        f = float(scaling["factor"])
+        if scaling["type"] == "linear":
+            freq = freq / f
+        elif scaling["type"] == "yarn":
+            L = float(scaling["original"])
+
+            def column(turns):  # the (real) column whose wave makes `turns` turns over L
+                return rotary_dim * math.log(L / (turns * 2 * math.pi)) / (2 * math.log(theta))
+            lo = max(math.floor(column(scaling.get("beta_fast", 32))), 0)
+            hi = min(math.ceil(column(scaling.get("beta_slow", 1))), rotary_dim - 1)
+            ramp = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+            freq = freq * (1 - ramp) + freq / f * ramp
+            gain = 0.1 * math.log(f) + 1.0 if f > 1 else 1.0
+        else:
+            raise NotImplementedError(f"rope_tables: scaling {scaling['type']!r}")
+    angle = torch.arange(num_positions, dtype=torch.float64)[:, None] * freq[None]
+    return ((angle.cos() * gain).float().to(device), (angle.sin() * gain).float().to(device))

@@ -505,6 +505,145 @@ int d2sd_commit_kv_hidden(const void* const* layer_ptrs, int32_t num_layers,
                           int64_t hidden_stride_token, void* hidden_dst,
                           int64_t hidden_dst_stride_token, void* stream);
 
+/* ---- the target's own forward over the paged cache ----------------------
+ *
+ * Three operators for the tokens a target model processes itself (prompts in
+ * chunks, single tokens, drafted blocks as plain sequences): write them into
+ * the cache, attend the cache, read rows back. They take a ragged batch of
+ * num_requests requests: request r's new tokens are rows token_start[r] ..
+ * token_start[r+1]-1 (device int32 [num_requests+1], ascending), its token i is
+ * at position first_pos[r] + i (device int32), and its positions live in pages
+ * page_table[page_bounds[r] + p / page_size] (device int32; page_bounds has
+ * num_requests+1 entries). Rows behind the last request are not touched.
+ *
+ * 8-bit caches (k_scale, v_scale != NULL): UMMA pages of e4m3 values, element
+ * (page, slot r, head h, d) at page*stride_page + h*stride_head + ((r/8)*
+ * (head_dim/16) + d/16)*128 + (r%8)*16 + d%16 bytes, and a scale byte for each
+ * row at page*scale_stride_page + h*scale_stride_head + r. The row's values are
+ * e4m3 * 2^(byte - 127); the byte is that of the smallest power of two from
+ * 2^-126 on with max|row| <= 448 * 2^e, the values are rounded to nearest even.
+ * A row with a NaN or an infinity reads back as NaN; a byte of 0 reads as 0.
+ *
+ * status (device int32, may be NULL) receives 4 when a position lies outside
+ * its request's pages, 5 for a page id outside the pool, 6 for a position
+ * outside the rotary tables; that token's rows are then not written. */
+
+/* Norm (optional), rotary position (optional) and cache write of a batch's new
+ * tokens in one launch; no reference counterpart (the reference's target forward
+ * is the HF model's, generation/d3_generator.py:77-88).
+ * q/q_out [num_tokens, num_qo_heads, head_dim] (num_qo_heads 0: no q), k, v
+ * [num_tokens, num_kv_heads, head_dim] in dtype (BF16, F16, F32); q_out may be q.
+ * q_weight/k_weight [head_dim] in dtype, or NULL: RMSNorm of q and k.
+ * cos_table/sin_table fp32 [table_rows, rotary_dim/2] (row stride table_stride),
+ * indexed by position: the first rotary_dim elements of every q and k head are
+ * rotated in pairs (i, i + rotary_dim/2), or (2i, 2i+1) when interleaved;
+ * rotary_dim is a multiple of 16, 0 for no rotation. All in fp32, rounded once.
+ * The cache holds dtype, or e4m3 rows (16-bit dtypes, UMMA pages).
+ * head_dim 64 or 128; rows 16-byte aligned. */
+int d2sd_append_kv(const void* q, int64_t q_stride_token, int64_t q_stride_head,
+                   void* q_out, int64_t q_out_stride_token,
+                   int64_t q_out_stride_head, int32_t num_qo_heads,
+                   const void* k, int64_t k_stride_token, int64_t k_stride_head,
+                   const void* v, int64_t v_stride_token, int64_t v_stride_head,
+                   int32_t num_kv_heads, int64_t num_tokens, int32_t head_dim,
+                   int32_t dtype, const void* q_weight, const void* k_weight,
+                   float eps, const float* cos_table, const float* sin_table,
+                   int64_t table_stride, int64_t table_rows, int32_t rotary_dim,
+                   int32_t interleaved, const int32_t* token_start,
+                   const int32_t* first_pos, int32_t num_requests, void* k_pool,
+                   void* v_pool, int64_t cache_stride_page,
+                   int64_t cache_stride_slot, int64_t cache_stride_head,
+                   int32_t page_size, int64_t num_pages, int32_t cache_format,
+                   void* k_scale, void* v_scale, int64_t scale_stride_page,
+                   int64_t scale_stride_head, const int32_t* page_table,
+                   const int32_t* page_bounds, int32_t* status, void* stream);
+
+/* Rows out of the cache: k_out/v_out [num_tokens, num_kv_heads, head_dim] in
+ * dtype (the cache's type; BF16 or F16 for an e4m3 cache, exact in BF16),
+ * request r's rows token_start[r] .. from its positions first_pos[r] on. */
+int d2sd_read_kv(const void* k_pool, const void* v_pool,
+                 int64_t cache_stride_page, int64_t cache_stride_slot,
+                 int64_t cache_stride_head, int32_t page_size,
+                 int64_t num_pages, int32_t cache_format, const void* k_scale,
+                 const void* v_scale, int64_t scale_stride_page,
+                 int64_t scale_stride_head, const int32_t* page_table,
+                 const int32_t* page_bounds, const int32_t* token_start,
+                 const int32_t* first_pos, int32_t num_requests,
+                 int64_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+                 int32_t dtype, void* k_out, int64_t k_out_stride_token,
+                 int64_t k_out_stride_head, void* v_out,
+                 int64_t v_out_stride_token, int64_t v_out_stride_head,
+                 int32_t* status, void* stream);
+
+/* d2sd_commit_kv_batch into an 8-bit cache. layer_ptrs: device array of
+ * num_layers*6 pointers {new_k, new_v, cache_k, cache_v, k_scale, v_scale};
+ * page_bounds [num_requests+1]; num_requests 1 is the single form. */
+int d2sd_commit_kv_e4m3(const void* const* layer_ptrs, int32_t num_layers,
+                        int32_t num_requests, int32_t num_kv_heads,
+                        int32_t head_dim, int32_t dtype, int32_t block_len,
+                        int64_t new_stride_request, int64_t new_stride_branch,
+                        int64_t new_stride_head, int64_t new_stride_token,
+                        int64_t cache_stride_page, int64_t cache_stride_head,
+                        int64_t num_pages, int64_t scale_stride_page,
+                        int64_t scale_stride_head, const int32_t* page_table,
+                        const int32_t* page_bounds,
+                        const int32_t* accept_results,
+                        const int32_t* cache_lens, int32_t* status,
+                        void* stream);
+
+/* Number of int32 entries a d2sd_paged_plan needs (upper bound), -1 if invalid. */
+int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_requests,
+                                 int32_t num_qo_heads, int32_t num_kv_heads,
+                                 int32_t num_ctas);
+
+/* Host-side work plan of d2sd_paged_attention (pure host code). Request r has
+ * q_lens[r] new tokens, the last of its kv_lens[r] cached positions (causal:
+ * token i sees positions up to kv_lens[r] - q_lens[r] + i, and with window > 0
+ * only the last `window` of them; not causal: every position), and its pages
+ * start at page_table[page_offsets[r]]. num_ctas is the grid (the SM count).
+ * plan[0 .. capacity) is written on the HOST (*used entries): copy it to the
+ * device. sections [12] is the host's copy of what the launch needs. */
+int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
+                    const int32_t* page_offsets, int32_t num_requests,
+                    int32_t num_qo_heads, int32_t num_kv_heads, int32_t causal,
+                    int32_t window, int32_t num_ctas, int32_t* plan,
+                    int64_t capacity, int64_t* used, int32_t* sections);
+
+/* Workspace bytes of d2sd_paged_attention for a grid of num_ctas: zeroed once
+ * before the first call (each call leaves its counters zero again). Calls that
+ * overlap on the GPU need a workspace each. */
+int64_t d2sd_paged_workspace_bytes(int32_t num_ctas, int32_t head_dim);
+
+/* Attention of the planned new tokens over the paged cache, which already holds
+ * them. q/out [tokens, num_qo_heads, head_dim] in dtype (BF16 or F16; BF16 with
+ * an 8-bit cache), requests in the plan's order; lse [tokens, num_qo_heads]
+ * base 2, or NULL. page_size is a multiple of 16 (UMMA pages: 16), head_dim 64
+ * or 128, at most 128 query heads per kv head. sinks fp32 [num_qo_heads] with a
+ * D2SD_SINK_* mode, or NULL. A row that sees no key gets out 0 and lse -inf.
+ * Slots past a request's last position may hold anything, NaN included; page
+ * ids outside the pool are read as its first or last page. fixed_grid: launch
+ * num_ctas CTAs whatever the plan says, so that a captured call stays valid
+ * when the plan's device buffer is rewritten. status receives 1 if a wait inside
+ * the kernel ran out of time (zero the workspace before using it again). */
+int d2sd_paged_attention(const void* q, int64_t q_stride_token,
+                         int64_t q_stride_head, int32_t dtype,
+                         const void* k_pool, const void* v_pool,
+                         int64_t cache_stride_page, int64_t cache_stride_slot,
+                         int64_t cache_stride_head, int32_t page_size,
+                         int64_t num_pages, int32_t cache_format,
+                         const void* k_scale, const void* v_scale,
+                         int64_t scale_stride_page, int64_t scale_stride_head,
+                         const int32_t* page_table, int64_t page_table_len,
+                         int32_t num_qo_heads, int32_t num_kv_heads,
+                         int32_t head_dim, float sm_scale, const int32_t* plan,
+                         const int32_t* sections, int32_t num_ctas,
+                         int32_t fixed_grid, void* workspace,
+                         int64_t workspace_bytes, const float* sinks,
+                         int32_t sink_mode, void* out, int64_t out_stride_token,
+                         int64_t out_stride_head, float* lse,
+                         int64_t lse_stride_token, int32_t* status,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

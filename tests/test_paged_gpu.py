@@ -1,0 +1,486 @@
+"""The operators of the target's own tokens on the GPU -- append, read, paged
+attention, commit into an 8-bit cache -- against float64 (oracle/paged.py).
+
+Error bounds, from the roundings the kernels make. Output o = sum p v / l: the
+weights are rounded to the value type (at most u = finfo.eps / 2 relative each,
+so u * sum p|v|), the output once more (u |o|); a score is an fp32 sum of D
+products and a scale, off by at most (D + 4) 2^-24 sum|q k| scale, and the weights
+by twice that relative to each other, with 2^-20 for the exponential and the fp32
+sums of a row. A log-sum-exp is off by the score's error and 2^-20, times
+log2 e."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as OP
+
+pytestmark = pytest.mark.gpu
+
+E4M3 = torch.float8_e4m3fn
+
+
+def make_cache(g, kv_lens, Hk, D, dtype, layout, device, page_size=16, garbage=False):
+    """Random cache of a ragged batch: pools (and scales) on the device, the page
+    table, bounds, and every request's rows in float64."""
+    pages = [-(-n // page_size) for n in kv_lens]
+    bounds = [0]
+    for p in pages:
+        bounds.append(bounds[-1] + p)
+    total = max(bounds[-1], 1) + 3
+    table = torch.randperm(total, generator=g)[:max(bounds[-1], 1)].to(torch.int32)
+    shape = (total, page_size, Hk, D) if layout == "paged_nhd" else (total, Hk, page_size, D)
+    pools, scales = [], []
+    for _ in range(2):
+        x = torch.randn(shape, generator=g)
+        if dtype == E4M3:
+            vals, byte = OP.e4m3_rows(x.double() * 2.0 ** torch.randint(-5, 3, (*shape[:3], 1),
+                                                                        generator=g))
+            unit = vals / (2.0 ** (byte.double() - 127))[..., None]
+            idx = OP.page_index(layout, D, 1).flatten()
+            flat = torch.empty(total, Hk, 16 * D, dtype=torch.uint8)
+            flat[..., idx] = unit.float().to(E4M3).view(torch.uint8).flatten(2)
+            pools.append(flat.view(shape).view(E4M3))
+            scales.append(byte)
+        else:
+            pools.append(x.to(dtype))
+    rows = [[OP.cached_rows(p, layout, table[bounds[r]:bounds[r + 1]].long(), n,
+                            scales[i] if scales else None) if page_size == 16 else
+             OP.block_rows(p[table[bounds[r]:bounds[r + 1]].long()], layout).transpose(1, 2)
+             .flatten(0, 1)[:n]
+             for r, n in enumerate(kv_lens)] for i, p in enumerate(pools)]
+    if garbage:  # NaN behind every request's last position, and in the pages nobody owns
+        used = torch.zeros(total, page_size, dtype=torch.bool)
+        for r, n in enumerate(kv_lens):
+            pos = torch.arange(n)
+            used[table[bounds[r]:bounds[r + 1]].long()[pos // page_size], pos % page_size] = True
+        pg, sl = (~used).nonzero(as_tuple=True)
+        for i, p in enumerate(pools):
+            if dtype == E4M3:
+                blk = p.view(torch.uint8).view(total, Hk, 2, D // 16, 8, 16)
+                blk[pg, :, sl // 8, :, sl % 8] = 0x7f
+                scales[i][pg, :, sl] = 255
+            elif layout == "paged_umma":
+                p.view(total, Hk, 2, D // 8, 8, 8)[pg, :, sl // 8, :, sl % 8] = float("nan")
+            elif layout == "paged_nhd":
+                p[pg, sl] = float("nan")
+            else:
+                p[pg, :, sl] = float("nan")
+    to = lambda t: t.to(device)  # noqa: E731
+    return dict(k=to(pools[0]), v=to(pools[1]), ks=to(scales[0]) if scales else None,
+                vs=to(scales[1]) if scales else None, table=to(table), bounds=bounds,
+                k_rows=rows[0], v_rows=rows[1], layout=layout)
+
+
+def check_attention(out, lse, q, c, q_lens, D, dtype, **kw):
+    u = torch.finfo(dtype).eps / 2
+    at = 0
+    for r, n in enumerate(q_lens):
+        qr = q[at:at + n].double().cpu()
+        o, l2, absv, big = OP.attention(qr, c["k_rows"][r], c["v_rows"][r], **kw)
+        serr = (D + 4) * 2.0 ** -24 * big
+        rel = (u + 2 * serr + 2.0 ** -20)[..., None]
+        tol = rel * absv * (1 + u) + u * o.abs() + 1e-30
+        got = out[at:at + n].double().cpu()
+        assert not got.isnan().any(), r
+        bad = (got - o).abs() - tol
+        assert (bad <= 0).all(), (r, n, float((got - o).abs().max()), float(bad.max()))
+        gl = lse[at:at + n].double().cpu()
+        empty = l2 == float("-inf")
+        assert torch.equal(gl == float("-inf"), empty), r
+        if n:
+            d = (gl - l2)[~empty].abs()
+            t = ((serr + 2.0 ** -20) * 1.4427 + l2.abs() * 2.0 ** -23)[~empty]
+            assert (d <= t).all(), (r, float(d.max()))
+        at += n
+
+
+# (q lengths, kv lengths): single tokens, lengths of zero, odd ones, pages that end
+# inside a tile, rows without a key (kv < q), more than one tile and many splits
+MIXED = ([1, 0, 5, 33, 2, 17, 3], [1, 40, 5, 130, 700, 17, 0])
+CASES = [
+    # Hq, Hk, D, type, store, layout, lens, window, sinks
+    (32, 8, 128, "bf16", "same", "paged_umma", ([1] * 6, [1, 15, 16, 17, 128, 3001]), None, False),
+    (32, 8, 128, "bf16", "same", "paged_umma", MIXED, None, False),
+    (64, 8, 64, "bf16", "same", "paged_umma", MIXED, 20, True),
+    (10, 2, 128, "f16", "same", "paged_umma", MIXED, None, True),
+    (6, 2, 64, "f16", "same", "paged_hnd", MIXED, 129, False),
+    (8, 8, 128, "bf16", "same", "paged_nhd", MIXED, None, False),
+    (32, 8, 128, "bf16", "e4m3", "paged_umma", MIXED, None, False),
+    (64, 8, 64, "bf16", "e4m3", "paged_umma", MIXED, 100, True),
+    (16, 1, 128, "bf16", "e4m3", "paged_umma", ([3, 1], [5000, 257]), None, False),
+    (32, 8, 128, "bf16", "same", "paged_umma", ([1], [20011]), None, False),
+    (4, 1, 64, "bf16", "same", "paged_umma", ([300], [450]), None, False),
+    (32, 8, 128, "bf16", "same", "paged_umma", ([257, 130], [257, 1000]), None, False),
+    (32, 8, 128, "bf16", "same", "paged_umma", ([257, 130], [300, 1000]), 70, True),
+    (40, 8, 128, "f16", "same", "paged_hnd", ([200], [333]), None, False),
+    (12, 4, 128, "bf16", "e4m3", "paged_umma", ([190, 1], [700, 90]), 300, False),
+    (128, 1, 64, "bf16", "same", "paged_umma", ([3, 40], [100, 41]), None, False),
+]
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.mark.parametrize("i", range(len(CASES)))
+@pytest.mark.parametrize("garbage", [False, True])
+def test_attention(cuda_device, i, garbage):
+    import d2sd_b200 as d
+    Hq, Hk, D, t, store, layout, (ql, kl), window, with_sinks = CASES[i]
+    dtype = TYPES[t]
+    g = torch.Generator().manual_seed(100 + i)
+    c = make_cache(g, kl, Hk, D, E4M3 if store == "e4m3" else dtype, layout, cuda_device,
+                   garbage=garbage)
+    n = sum(ql)
+    # a strided view (the projection's output) and rows behind the last request
+    q = torch.randn(n + 2, Hq + 3, D, generator=g).to(dtype).to(cuda_device)[:, 1:Hq + 1]
+    sinks = torch.randn(Hq, generator=g).to(cuda_device) if with_sinks else None
+    plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, window=window,
+                                page_offsets=c["bounds"])
+    out = torch.full((n + 2, Hq + 1, D), 7.0, dtype=dtype, device=cuda_device)[:, :Hq]
+    lse = torch.full((n + 2, Hq), 7.0, device=cuda_device)
+    for _ in range(2):  # the second call finds the workspace as the first left it
+        d.paged_attention(q, c["k"], c["v"], layout, c["table"], plan, k_scale=c["ks"],
+                          v_scale=c["vs"], sinks=sinks, out=out, lse=lse)
+        check_attention(out, lse, q, c, ql, D, dtype, window=window,
+                        sinks=None if sinks is None else sinks.cpu())
+    assert (out[n:] == 7).all() and (lse[n:] == 7).all()
+    assert int(plan.status) == 0
+    assert not plan.workspace[:4 * 2 * plan.num_ctas].any()  # the counters are zero again
+
+
+@pytest.mark.parametrize("store", ["same", "e4m3"])
+def test_attention_without_causal_mask(cuda_device, store):
+    import d2sd_b200 as d
+    Hq, Hk, D, ql, kl = 16, 4, 128, [4, 3, 50], [60, 0, 333]
+    g = torch.Generator().manual_seed(5)
+    c = make_cache(g, kl, Hk, D, E4M3 if store == "e4m3" else torch.bfloat16, "paged_umma",
+                   cuda_device, garbage=True)
+    q = torch.randn(sum(ql), Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, causal=False,
+                                page_offsets=c["bounds"])
+    out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, sm_scale=0.05,
+                                 k_scale=c["ks"], v_scale=c["vs"])
+    check_attention(out, lse, q, c, ql, D, torch.bfloat16, causal=False, scale=0.05)
+
+
+@pytest.mark.parametrize("layout,page_size", [("paged_hnd", 32), ("paged_nhd", 64)])
+def test_attention_larger_pages(cuda_device, layout, page_size):
+    import d2sd_b200 as d
+    Hq, Hk, D, ql, kl = 8, 2, 64, [2, 100], [77, 300]
+    g = torch.Generator().manual_seed(6)
+    c = make_cache(g, kl, Hk, D, torch.bfloat16, layout, cuda_device, page_size=page_size)
+    q = torch.randn(sum(ql), Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, page_offsets=c["bounds"])
+    out, lse = d.paged_attention(q, c["k"], c["v"], layout, c["table"], plan)
+    check_attention(out, lse, q, c, ql, D, torch.bfloat16)
+
+
+def test_attention_large_scores(cuda_device):
+    """Scores in the hundreds: the running maximum moves through the keys."""
+    import d2sd_b200 as d
+    Hq, Hk, D, ql, kl = 8, 2, 128, [1, 140], [2000, 900]
+    g = torch.Generator().manual_seed(7)
+    c = make_cache(g, kl, Hk, D, torch.bfloat16, "paged_umma", cuda_device)
+    q = (20 * torch.randn(sum(ql), Hq, D, generator=g)).to(torch.bfloat16).to(cuda_device)
+    plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, page_offsets=c["bounds"])
+    out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan)
+    check_attention(out, lse, q, c, ql, D, torch.bfloat16)
+
+
+def test_attention_bad_page_ids(cuda_device):
+    """Ids outside the pool are read as its first or last page: no fault, and the
+    other requests' rows are right."""
+    import d2sd_b200 as d
+    Hq, Hk, D, ql, kl = 8, 2, 128, [1, 1, 150], [50, 64, 400]
+    g = torch.Generator().manual_seed(8)
+    c = make_cache(g, kl, Hk, D, torch.bfloat16, "paged_umma", cuda_device)
+    c["table"][c["bounds"][1]] = 1 << 30
+    c["table"][c["bounds"][1] + 1] = -5
+    q = torch.randn(sum(ql), Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, page_offsets=c["bounds"])
+    out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan)
+    for r, (a, b) in ((0, (0, 1)), (2, (2, 152))):
+        one = dict(c, k_rows=[c["k_rows"][r]], v_rows=[c["v_rows"][r]])
+        check_attention(out[a:b], lse[a:b], q[a:b], one, [ql[r]], D, torch.bfloat16)
+
+
+def test_captured_call_replays_after_update(cuda_device):
+    """A reserved plan: one captured call, other lengths at every replay."""
+    import d2sd_b200 as d
+    Hq, Hk, D = 16, 4, 128
+    g = torch.Generator().manual_seed(9)
+    full = [900, 300, 2500]
+    c = make_cache(g, full, Hk, D, torch.bfloat16, "paged_umma", cuda_device)
+    q = torch.randn(400, Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    plan = d.PagedAttentionPlan([1, 1, 1], [9, 9, 9], Hq, Hk, D, cuda_device,
+                                page_offsets=c["bounds"], reserve=(3, 400))
+    out = torch.zeros_like(q)
+    lse = torch.zeros(400, Hq, device=cuda_device)
+    call = lambda: d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan,  # noqa
+                                     out=out, lse=lse)
+    call()
+    s = torch.cuda.Stream(cuda_device)
+    s.wait_stream(torch.cuda.current_stream(cuda_device))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s), torch.cuda.graph(graph, stream=s):
+        call()
+    torch.cuda.current_stream(cuda_device).wait_stream(s)
+    for ql, kl in (([1, 1, 1], [9, 9, 9]), ([1, 1, 1], [900, 16, 2500]), ([40, 0, 350], [41, 7, 2400]),
+                   ([0, 0, 0], [5, 5, 5]), ([1, 260, 1], [1, 290, 1])):
+        plan.update(ql, kl, c["bounds"])
+        graph.replay()
+        torch.cuda.synchronize(cuda_device)
+        cut = dict(c, k_rows=[x[:n] for x, n in zip(c["k_rows"], kl)],
+                   v_rows=[x[:n] for x, n in zip(c["v_rows"], kl)])
+        check_attention(out, lse, q, cut, ql, D, torch.bfloat16)
+    with pytest.raises(ValueError):
+        plan.update([4000] * 3, [4000] * 3, c["bounds"])
+    del graph
+
+
+def test_two_plans_on_two_streams(cuda_device):
+    import d2sd_b200 as d
+    Hq, Hk, D = 32, 8, 128
+    g = torch.Generator().manual_seed(10)
+    jobs = []
+    for kl in ([4000], [3000]):
+        c = make_cache(g, kl, Hk, D, torch.bfloat16, "paged_umma", cuda_device)
+        q = torch.randn(1, Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+        jobs.append((c, q, d.PagedAttentionPlan([1], kl, Hq, Hk, D, cuda_device),
+                     torch.cuda.Stream(cuda_device)))
+    torch.cuda.synchronize(cuda_device)
+    res = []
+    for _ in range(5):
+        for c, q, plan, s in jobs:
+            with torch.cuda.stream(s):
+                res.append(d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan))
+    torch.cuda.synchronize(cuda_device)
+    for x, (o, l) in enumerate(res):
+        c, q, _, _ = jobs[x % 2]
+        check_attention(o, l, q, c, [1], D, torch.bfloat16)
+
+
+# ---------------------------------------------------------------------------
+# append, read, commit
+# ---------------------------------------------------------------------------
+APPEND = [
+    # type, store, layout, Hq, Hk, D, norm, rotary, interleaved
+    ("bf16", "same", "paged_umma", 32, 8, 128, True, 128, False),
+    ("bf16", "same", "paged_umma", 64, 8, 64, False, 64, False),
+    ("f16", "same", "paged_hnd", 6, 2, 64, True, 32, True),
+    ("f32", "same", "paged_hnd", 4, 1, 128, True, 48, False),
+    ("f32", "same", "paged_nhd", 4, 2, 64, False, 16, True),
+    ("bf16", "same", "paged_nhd", 5, 5, 128, False, 0, False),
+    ("bf16", "e4m3", "paged_umma", 32, 8, 128, True, 128, False),
+    ("f16", "e4m3", "paged_umma", 8, 8, 64, False, 32, True),
+    ("bf16", "e4m3", "paged_umma", 0, 3, 128, False, 0, False),
+    ("bf16", "same", "paged_umma", 40, 8, 128, True, 96, False),
+]
+ALL_TYPES = dict(TYPES, f32=torch.float32)
+
+
+def new_pool(total, Hk, D, dtype, layout, device, g):
+    shape = (total, 16, Hk, D) if layout == "paged_nhd" else (total, Hk, 16, D)
+    x = torch.randint(1, 100, shape, generator=g)
+    if dtype == E4M3:
+        return (x.to(torch.uint8).view(E4M3).to(device),
+                torch.randint(100, 130, shape[:3], generator=g).to(torch.uint8).to(device))
+    return x.to(dtype).to(device), None
+
+
+@pytest.mark.parametrize("i", range(len(APPEND)))
+def test_append_and_read(cuda_device, i):
+    from d2sd_b200 import ops
+    t, store, layout, Hq, Hk, D, norm, rot, inter = APPEND[i]
+    dtype, dev = ALL_TYPES[t], cuda_device
+    g = torch.Generator().manual_seed(40 + i)
+    ql, first = [1, 0, 37, 16, 3], [0, 9, 5, 4000, 31]
+    R, n = len(ql), sum(ql)
+    starts, bounds = [0], [0]
+    for a, b in zip(ql, first):
+        starts.append(starts[-1] + a)
+        bounds.append(bounds[-1] + -(-(a + b) // 16))
+    total = bounds[-1] + 2
+    table = torch.randperm(total, generator=g)[:bounds[-1]].to(torch.int32)
+    kp, ks = new_pool(total, Hk, D, E4M3 if store == "e4m3" else dtype, layout, dev, g)
+    vp, vs = new_pool(total, Hk, D, E4M3 if store == "e4m3" else dtype, layout, dev, g)
+    k0, v0 = kp.clone(), vp.clone()
+    # q, k, v side by side, two rows behind the last request; rows of many sizes
+    size = 2.0 ** torch.randint(-12, 8, (n + 2, Hq + 2 * Hk, 1), generator=g)
+    qkv = (torch.randn(n + 2, Hq + 2 * Hk, D, generator=g) * size).to(dtype)
+    qkv[0, -1] = 0.0  # a row of zeros
+    q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + Hk], qkv[:, Hq + Hk:]
+    w = [(1 + 0.3 * torch.randn(D, generator=g)).to(dtype) if norm else None for _ in range(2)]
+    cos = sin = None
+    if rot:
+        from d2sd_b200 import rope_tables
+        cos, sin = rope_tables(4016, rot, 1e4, "cpu")
+    dq = qkv.to(dev)
+    up = lambda x: None if x is None else x.to(dev)  # noqa: E731
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    q_out = torch.full((n + 2, Hq, D), 3.0, dtype=dtype, device=dev) if Hq else None
+    ops.append_kv(dq[:, Hq:Hq + Hk], dq[:, Hq + Hk:], kp, vp, layout, up(table), ints(bounds),
+                  ints(starts), ints(first), k_scale=ks, v_scale=vs, q=dq[:, :Hq] if Hq else None,
+                  q_out=q_out, q_weight=up(w[0]) if Hq else None, k_weight=up(w[1]), eps=1e-5,
+                  cos=up(cos), sin=up(sin), interleaved=inter, status=status)
+    assert int(status) == 0
+    pos = torch.cat([torch.arange(b, b + a) for a, b in zip(ql, first)])
+    f64 = lambda x: x[:n].double()  # noqa: E731
+    want_k = OP.norm_rotate(f64(k), w[1], 1e-5, cos, sin, pos, inter)
+    want_v = f64(v)
+    # fp32 arithmetic: a norm of D squares and five products, (D / 2 + 16) 2^-24 of the pair's size
+    u = torch.finfo(dtype).eps / 2
+    fp32 = (D // 2 + 16) * 2.0 ** -24
+
+    def pair(x):  # size of the rotated pair each element comes from (sqrt 2 of its own at most)
+        return x.abs().amax(-1, keepdim=True) * 2 if rot else x.abs()
+    if Hq:
+        want_q = OP.norm_rotate(f64(q), w[0], 1e-5, cos, sin, pos, inter)
+        err = (q_out[:n].double().cpu() - want_q).abs()
+        tiny = torch.finfo(dtype).smallest_normal * u * 2
+        assert (err <= u * want_q.abs() + fp32 * pair(want_q) + tiny).all()
+        assert (q_out[n:] == 3).all()
+    # read back
+    out_t = torch.bfloat16 if store == "e4m3" and t == "bf16" else dtype
+    kr = torch.full((n + 1, Hk, D), 5.0, dtype=out_t, device=dev)
+    vr = torch.full((n + 1, Hk, D), 5.0, dtype=out_t, device=dev)
+    ops.read_kv(kp, vp, layout, up(table), ints(bounds), ints(starts), ints(first), kr, vr,
+                k_scale=ks, v_scale=vs, status=status)
+    assert int(status) == 0 and (kr[n:] == 5).all() and (vr[n:] == 5).all()
+    got_k, got_v = kr[:n].double().cpu(), vr[:n].double().cpu()
+    if store == "e4m3":
+        # e4m3: half a step is 2^-4 of the value, or of the smallest normal value
+        # 2^-6 * 2^e where the row's scale 2^e is at most 2 * max / 448
+        def bound(x):
+            floor = x.abs().amax(-1, keepdim=True) * 2 / 448 * 2.0 ** -6 * 2.0 ** -4
+            return torch.maximum(x.abs() * 2.0 ** -4, floor) + fp32 * pair(x)
+        if t == "bf16":  # exact values, without rotation or norm the very ones
+            assert torch.equal(got_v, OP.e4m3_rows(want_v)[0])
+            assert ((got_k - want_k).abs() <= bound(want_k)).all()
+            if not norm and not rot:
+                assert torch.equal(got_k, OP.e4m3_rows(want_k)[0])
+        else:  # read into fp16: small values are subnormal there
+            extra = 2.0 ** -25
+            assert ((got_v - want_v).abs() <= bound(want_v) * (1 + 2 ** -10) + extra).all()
+            assert ((got_k - want_k).abs() <= bound(want_k) * (1 + 2 ** -10) + extra).all()
+    else:
+        tiny = torch.finfo(dtype).smallest_normal * u * 2
+        assert torch.equal(got_v, want_v)
+        assert ((got_k - want_k).abs() <= u * want_k.abs() + fp32 * pair(want_k) + tiny).all()
+    # nothing else in the pools changed
+    for new, old in ((kp, k0), (vp, v0)):
+        a, b = (OP.block_rows(x.cpu(), layout) for x in (new, old))
+        touched = torch.zeros(total, 16, dtype=torch.bool)
+        req = torch.repeat_interleave(torch.arange(R), torch.tensor(ql))
+        touched[table[torch.tensor(bounds)[req] + pos // 16].long(), pos % 16] = True
+        keep = ~touched[:, None, :, None].expand_as(a)
+        assert torch.equal(a[keep], b[keep])
+
+
+def test_append_skips_bad_positions_and_pages(cuda_device):
+    from d2sd_b200 import ops, rope_tables
+    dev, Hk, D = cuda_device, 2, 64
+    g = torch.Generator().manual_seed(3)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    cos, sin = rope_tables(30, D, 1e4, dev)
+    cases = [(4, [0, 3], [0, 2], [30], None),         # runs past the request's two pages
+             (4, [0, 3], [0, 2], [-1], None),
+             (5, [0, 1], [0, 1], [3], [77]),          # a page id outside the pool
+             (5, [0, 1], [0, 1], [3], [-2]),
+             (6, [0, 3], [0, 3], [29], None)]         # past the rotary tables
+    for code, starts, bounds, first, table in cases:
+        table = ints(table or [0, 1, 2])
+        kp, _ = new_pool(4, Hk, D, torch.bfloat16, "paged_umma", dev, g)
+        vp = kp.clone()
+        before = kp.clone()
+        rows = torch.randn(starts[-1], Hk, D, generator=g).to(torch.bfloat16).to(dev)
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
+        q = rows.clone()
+        ops.append_kv(rows, rows, kp, vp, "paged_umma", table, ints(bounds), ints(starts),
+                      ints(first), q=q, cos=cos, sin=sin, status=status)
+        assert int(status) == code
+        changed = (kp != before).any(-1).any(1).sum().item()  # rows that were written
+        ok = {30: 2, -1: 2, 29: 1, 3: 0}[first[0]]
+        assert changed <= ok * D * 2
+        if ok == 0:
+            assert torch.equal(kp, before) and torch.equal(vp, before) and torch.equal(q, rows)
+        if code != 6:
+            out = torch.full_like(rows, 9.0)
+            status.zero_()
+            ops.read_kv(kp, vp, "paged_umma", table, ints(bounds), ints(starts), ints(first), out,
+                        out.clone(), status=status)
+            assert int(status) == code
+
+
+def test_quantised_row_with_nan_or_infinity_reads_as_nan(cuda_device):
+    from d2sd_b200 import ops
+    dev, Hk, D = cuda_device, 1, 64
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    rows = torch.ones(4, Hk, D, dtype=torch.bfloat16, device=dev)
+    rows[1, 0, 5], rows[2, 0, 63] = float("nan"), float("-inf")
+    rows[3] *= 3e38
+    kp = torch.zeros(1, Hk, 16, D, dtype=torch.uint8, device=dev).view(E4M3)
+    vp = kp.clone()
+    ks = torch.zeros(1, Hk, 16, dtype=torch.uint8, device=dev)
+    vs = ks.clone()
+    args = ("paged_umma", ints([0]), ints([0, 1]), ints([0, 4]), ints([0]))
+    ops.append_kv(rows, rows, kp, vp, *args, k_scale=ks, v_scale=vs)
+    ko, vo = torch.zeros_like(rows), torch.zeros_like(rows)
+    ops.read_kv(kp, vp, *args, ko, vo, k_scale=ks, v_scale=vs)
+    assert ko[1].isnan().all() and ko[2].isnan().all() and (ko[0] == 1).all()
+    assert torch.equal(ko[3].double().cpu(), OP.e4m3_rows(rows[3].double().cpu())[0])
+
+
+def test_refusals(cuda_device):
+    import d2sd_b200 as d
+    from d2sd_b200 import ops
+    dev = cuda_device
+    z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t, device=dev)  # noqa: E731
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    kp, k = z(4, 2, 16, 64), z(3, 2, 64)
+    one = (ints([0, 1, 2, 3]), ints([0, 4]), ints([0, 3]), ints([0]))
+
+    def refused(err, *a, **kw):
+        with pytest.raises(err):
+            ops.append_kv(*a, **kw)
+    refused(ValueError, k.float(), k.float(), kp, kp, "paged_umma", *one)      # cache type
+    refused(ValueError, k, k, kp, kp, "nhd", *one)                             # not paged
+    refused(ValueError, k[:, :1], k, kp, kp, "paged_umma", *one)               # heads
+    refused(ValueError, k, k, kp, kp, "paged_umma", one[0].long(), *one[1:])   # int64 table
+    refused(ValueError, k, k, kp, kp, "paged_umma", one[0], ints([0]), *one[2:])
+    refused(ValueError, k, k, kp.view(E4M3) if False else z(4, 2, 16, 64, t=torch.uint8).view(E4M3),
+            z(4, 2, 16, 64, t=torch.uint8).view(E4M3), "paged_umma", *one)     # no scales
+    refused(ValueError, k, k, kp, kp, "paged_umma", *one, cos=z(9, 32, t=torch.float32))
+    refused(NotImplementedError, k, k, kp, kp, "paged_umma", *one, cos=z(9, 20, t=torch.float32),
+            sin=z(9, 20, t=torch.float32))                                     # rotary_dim 40
+    refused(NotImplementedError, k[..., :32], k[..., :32], z(4, 2, 16, 32), z(4, 2, 16, 32),
+            "paged_umma", *one)                                                # head_dim 32
+    refused(ValueError, z(3, 2, 65)[..., 1:], k, kp, kp, "paged_umma", *one)   # alignment
+    refused(ValueError, k.cpu(), k, kp, kp, "paged_umma", *one)
+    with pytest.raises(ValueError):
+        ops.read_kv(kp, kp, "paged_umma", *one, k.half(), k.half())
+    # attention
+    P = d.PagedAttentionPlan
+    for bad in (dict(q_lens=[1], kv_lens=[1, 2]), dict(q_lens=[-1], kv_lens=[1]),
+                dict(q_lens=[1, 1], kv_lens=[1, 1])):
+        with pytest.raises(ValueError):
+            P(bad["q_lens"], bad["kv_lens"], 4, 2, 64, dev)
+    with pytest.raises(ValueError):
+        P([1], [1], 5, 2, 64, dev)
+    with pytest.raises(NotImplementedError):
+        P([1], [1], 4, 2, 96, dev)
+    with pytest.raises(NotImplementedError):
+        P([1], [1], 4, 2, 64, dev, causal=False, window=3)
+    with pytest.raises(NotImplementedError):
+        P([1], [1], 129, 1, 64, dev)
+    plan = P([3], [3], 4, 2, 64, dev)
+    q = z(3, 4, 64)
+    for err, a, kw in [
+            (ValueError, (q[:2], kp, kp, "paged_umma", one[0], plan), {}),
+            (ValueError, (q.half(), kp, kp, "paged_umma", one[0], plan), {}),
+            (NotImplementedError, (q.float(), kp.float(), kp.float(), "paged_hnd", one[0], plan), {}),
+            (ValueError, (q, kp, kp, "paged_umma", one[0], plan), {"sinks": z(3, t=torch.float32)}),
+            (ValueError, (q, kp[:, :1], kp[:, :1], "paged_hnd", one[0], plan), {}),
+            (ValueError, (q, kp, kp, "paged_umma", one[0], plan), {"out": z(2, 4, 64)}),
+            (NotImplementedError, (q, z(4, 2, 8, 64), z(4, 2, 8, 64), "paged_hnd", one[0], plan), {})]:
+        with pytest.raises(err):
+            d.paged_attention(*a, **kw)

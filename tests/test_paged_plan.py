@@ -1,0 +1,134 @@
+"""The host-side plan of the paged attention (CPU only): every (row, visible key
+tile) of every request in exactly one item, spans in order, slots and tickets, and
+the balance over the CTAs."""
+import numpy as np
+import pytest
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from d2sd_b200 import build
+    build.build()
+    from d2sd_b200 import _lib
+    return _lib.load()
+
+
+def make(lib, q, kv, off, Hq, Hk, causal, window, ctas):
+    from d2sd_b200._lib import check
+    q, kv, off = (np.ascontiguousarray(x, dtype=np.int32) for x in (q, kv, off))
+    cap = lib.d2sd_paged_plan_capacity(q.ctypes.data, len(q), Hq, Hk, ctas)
+    plan, used, sec = np.zeros(cap, np.int32), np.zeros(1, np.int64), np.zeros(12, np.int32)
+    check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, len(q), Hq, Hk, causal,
+                              window, ctas, plan.ctypes.data, cap, used.ctypes.data,
+                              sec.ctypes.data), "plan")
+    return plan[:int(used[0])], sec
+
+
+@pytest.mark.parametrize("q,kv,Hq,Hk,causal,window,ctas", [
+    ([1] * 64, list(range(512, 8193, 120))[:64], 32, 8, 1, 0, 148),
+    ([1], [1000], 32, 8, 1, 0, 148),
+    ([1], [1], 8, 8, 1, 0, 148),
+    ([5, 0, 16, 1], [5, 40, 300, 0], 10, 2, 1, 0, 7),
+    ([900, 3], [900, 5000], 32, 8, 1, 0, 148),
+    ([900, 3], [1900, 5000], 64, 8, 1, 128, 148),
+    ([4, 9], [70, 0], 16, 4, 0, 0, 148),
+    ([2048], [32768], 32, 8, 1, 0, 148),
+    ([100], [40], 4, 2, 1, 0, 5),
+    ([3] * 300, [77] * 300, 8, 1, 1, 0, 3),
+])
+def test_plan_covers_every_tile_once(lib, q, kv, Hq, Hk, causal, window, ctas):
+    off = np.cumsum([0] + [-(-n // 16) for n in kv])[:-1]
+    plan, sec = make(lib, q, kv, off, Hq, Hk, causal, window, ctas)
+    G = Hq // Hk
+    starts = np.cumsum([0] + list(q))
+    seen = {}
+    for s in range(2):
+        nct, nit, nslots, ntick, oc, oi = sec[6 * s:6 * s + 6]
+        assert list(plan[5 + 6 * s:11 + 6 * s]) == [nct, nit, nslots, ntick, oc, oi]
+        if nit == 0:
+            continue
+        cta = plan[oc:oc + nct + 1]
+        assert nct <= ctas and cta[0] == 0 and cta[-1] == nit and (np.diff(cta) >= 0).all()
+        assert nslots <= 2 * ctas and ntick <= 2 * ctas and oi % 4 == 0
+        items = plan[oi:oi + 16 * nit].reshape(-1, 16)
+        slots, ticket_of = set(), {}
+        for it in items:
+            r, h, tok0, row0, nrows, k0, k1, pos0, win, po, kvl, slot, first, parts, tick, _ = it
+            assert tok0 == starts[r] and po == off[r] and kvl == kv[r] and win == window
+            assert nrows > 0 and row0 + nrows <= q[r] * G and k0 % 128 == 0 and k1 <= kv[r]
+            unit = seen.setdefault((r, h, row0), [nrows, []])
+            unit[1].append((k0, k1))
+            if parts == 1:
+                assert slot == -1
+            else:
+                assert slot not in slots and first <= slot < first + parts
+                assert slot == first + len(unit[1]) - 1  # spans in slot order
+                slots.add(slot)
+                assert ticket_of.setdefault(tick, (r, h, row0)) == (r, h, row0)
+        assert slots == set(range(nslots)) and sorted(ticket_of) == list(range(ntick))
+        # balance: the largest CTA within the mean, one item's cost and the rounding
+        cost = [sum(-(-(i[6] - i[5]) // 128) + 1 for i in items[a:b]) for a, b in zip(cta, cta[1:])]
+        assert max(cost) <= sum(cost) / nct + 5
+    for r in range(len(q)):
+        rows = q[r] * G
+        for h in range(Hk):
+            units = sorted((k[2], v) for k, v in seen.items() if k[:2] == (r, h))
+            at = 0
+            for row0, (n, spans) in units:
+                assert row0 == at
+                at += n
+                pos0 = kv[r] - q[r]
+                hi, lo = kv[r], 0
+                if causal:
+                    hi = max(0, min(kv[r], pos0 + (row0 + n - 1) // G + 1))
+                    lo = max(0, pos0 + row0 // G + 1 - window) if window else 0
+                lo = min(lo // 128 * 128, hi)
+                assert spans[0][0] == lo and spans[-1][1] == hi
+                for a, b in zip(spans, spans[1:]):
+                    assert a[1] == b[0] and b[1] > b[0]
+            assert at == rows
+
+
+def test_plan_refusals(lib):
+    with pytest.raises(ValueError):
+        make(lib, [1], [-1], [0], 4, 2, 1, 0, 8)
+    with pytest.raises(ValueError):
+        make(lib, [1], [1], [-1], 4, 2, 1, 0, 8)
+    with pytest.raises(ValueError):
+        make(lib, [1], [1], [0], 4, 2, 1, -3, 8)
+    with pytest.raises(NotImplementedError):
+        make(lib, [1], [1], [0], 4, 2, 0, 16, 8)
+    with pytest.raises(NotImplementedError):
+        make(lib, [1], [1 << 30], [0], 4, 2, 1, 0, 8)
+    with pytest.raises(NotImplementedError):
+        make(lib, [1], [1], [0], 129, 1, 1, 0, 8)
+    import ctypes
+    n = np.ones(1, np.int32)
+    buf, used, sec = np.zeros(4, np.int32), np.zeros(1, np.int64), np.zeros(12, np.int32)
+    rc = lib.d2sd_paged_plan(n.ctypes.data, n.ctypes.data, ctypes.c_void_p(np.zeros(1, np.int32).ctypes.data),
+                             1, 4, 2, 1, 0, 8, buf.ctypes.data, 4, used.ctypes.data, sec.ctypes.data)
+    assert rc == 3 and "small" in lib.d2sd_last_error().decode()
+    assert lib.d2sd_paged_plan_capacity(n.ctypes.data, 1, 5, 2, 8) == -1
+    assert lib.d2sd_paged_workspace_bytes(148, 96) == -1
+
+
+def test_empty_batches(lib):
+    plan, sec = make(lib, [], [], [], 4, 2, 1, 0, 8)
+    assert sec[1] == 0 and sec[7] == 0
+    plan, sec = make(lib, [0, 0], [7, 0], [0, 1], 4, 2, 1, 0, 8)
+    assert sec[1] == 0 and sec[7] == 0
+
+
+def test_e4m3_oracle_against_the_type():
+    """The oracle's 8-bit rows against torch's own rounding to float8_e4m3fn."""
+    import torch
+    from oracle import paged as OP
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(500, 64, generator=g) * 2.0 ** torch.randint(-130, 20, (500, 1), generator=g).float()
+    x[0] = 0
+    vals, byte = OP.e4m3_rows(x.double())
+    e = byte.double() - 127
+    top = x.double().abs().amax(-1)
+    assert (top <= 448 * 2.0 ** e).all() and ((top > 448 * 2.0 ** (e - 1)) | (e == -126)).all()
+    y = x.double() / (2.0 ** e)[:, None]
+    assert torch.equal(y.float().to(torch.float8_e4m3fn).double() * (2.0 ** e)[:, None], vals)
