@@ -21,6 +21,11 @@ constexpr int kStatusPosition = 4;  // a position outside the request's pages
 constexpr int kStatusPage = 5;      // a page id outside the pool
 constexpr int kStatusTable = 6;     // a position outside the rotary tables
 
+// The smallest code of a launch stays, whichever token reports first.
+__device__ __forceinline__ void report(int32_t* status, int code) {
+  if (status && atomicCAS(status, 0, code) > code) atomicMin(status, code);
+}
+
 // One pool (K and V alike): byte strides, so 8- and 16-bit values share it.
 struct PageGeom {
   int64_t stride_page, stride_slot, stride_head;  // bytes

@@ -31,8 +31,7 @@
 #include <atomic>
 #include <string>
 
-#include "paged.cuh"
-#include "paged_plan.h"
+#include "paged_attn.cuh"
 
 namespace d2sd {
 namespace {
@@ -41,24 +40,6 @@ using namespace paged;
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-
-struct AttnArgs {
-  const void* q;
-  void* out;
-  float* lse;
-  int64_t q_st, q_sh, o_st, o_sh, lse_st;  // element strides
-  const uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
-  const int32_t* page_table;
-  int64_t page_table_len;
-  const int32_t* plan;
-  float* slots;      // partial states: [slot][rows * (D + 2)]
-  uint32_t* tickets;
-  const float* sinks;
-  int32_t* status;
-  PageGeom g;
-  float scale_log2;
-  int32_t sink_mode;
-};
 
 template <int D, int ELEM>
 struct RowsCfg {
@@ -104,48 +85,8 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) { return pack_bf16x2(lo, hi); }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
-// Bytes 0 and 2 (even) or 1 and 3 (odd) of x, e4m3, to two bf16. Moving sign and
-// magnitude into a bf16's places gives value * 2^-120 (the exponent biases differ
-// by 120; subnormals likewise), so a product with 2^120 ends it. NaN (0x7f) is
-// not one after this; the writer marks such rows in their scale byte.
-__device__ __forceinline__ uint32_t mul_2p120(uint32_t x) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7b807b80u));
-  return r;
-}
-__device__ __forceinline__ uint32_t e4m3_even(uint32_t x) {
-  return mul_2p120(((x & 0x00800080u) << 8) | ((x & 0x007f007fu) << 4));
-}
-__device__ __forceinline__ uint32_t e4m3_odd(uint32_t x) {
-  return mul_2p120((x & 0x80008000u) | ((x & 0x7f007f00u) >> 4));
-}
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-
-// Factor of the attention sink: o *= sigmoid(lse - sink) (include/d2sd.h).
-__device__ __forceinline__ float sink_factor(float lse2, float sink, int mode) {
-  const float x = (mode == D2SD_SINK_EXACT ? lse2 * kLn2 : lse2) - sink;
-  return 1.f / (1.f + expf(-x));
-}
-
-// One 16-byte chunk of zeros is written over rows [r0, r1) of a page in smem.
-template <int D, int ELEM>
-__device__ __forceinline__ void zero_rows(uint8_t* page, int r0, int r1) {
-  constexpr int C = D * ELEM / 16;
-  const int lane = threadIdx.x & 31;
-  for (int i = lane; i < 16 * C; i += 32) {
-    const int r = i & 15, c = i >> 4;
-    if (r >= r0 && r < r1)
-      *reinterpret_cast<uint4*>(page + ((r >> 3) * C + c) * 128 + (r & 7) * 16) = make_uint4(0, 0, 0, 0);
-  }
 }
 
 // ELEM: bytes of a cached value (2: T, 1: e4m3); UMMA: pages in core-matrix order,
@@ -541,19 +482,28 @@ int launch_rows(const AttnArgs& a, int ctas, cudaStream_t stream) {
                     "rows_kernel", a);
 }
 
+int run_rows(const AttnArgs& a, int32_t dtype, int32_t head_dim, bool scaled, int ctas, cudaStream_t st) {
+  const bool d128 = head_dim == 128, umma = a.g.umma != 0;
+  if (scaled) return d128 ? launch_rows<__nv_bfloat16, 128, 1, true>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 1, true>(a, ctas, st);
+  if (dtype == D2SD_DTYPE_BF16) {
+    if (umma) return d128 ? launch_rows<__nv_bfloat16, 128, 2, true>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 2, true>(a, ctas, st);
+    return d128 ? launch_rows<__nv_bfloat16, 128, 2, false>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 2, false>(a, ctas, st);
+  }
+  if (umma) return d128 ? launch_rows<__half, 128, 2, true>(a, ctas, st) : launch_rows<__half, 64, 2, true>(a, ctas, st);
+  return d128 ? launch_rows<__half, 128, 2, false>(a, ctas, st) : launch_rows<__half, 64, 2, false>(a, ctas, st);
+}
+
 }  // namespace
 }  // namespace d2sd
 
-// Tickets first, then the slots: a CTA's first and last item can be spans of split
-// units, so 2 per CTA bounds both.
 extern "C" int64_t d2sd_paged_workspace_bytes(int32_t num_ctas, int32_t head_dim) {
-  using namespace d2sd::paged;
   if (num_ctas <= 0 || (head_dim != 64 && head_dim != 128)) return -1;
-  return ticket_bytes(num_ctas) + 2 * static_cast<int64_t>(num_ctas) * kRowsTile * (head_dim + 2) * 4;
+  return d2sd::paged::workspace_bytes(num_ctas, head_dim);
 }
 
 extern "C" int d2sd_paged_attention(
-    const void* q, int64_t q_stride_token, int64_t q_stride_head, int32_t dtype, const void* k_pool,
+    const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t num_tokens, int32_t dtype,
+    const void* k_pool,
     const void* v_pool, int64_t cache_stride_page, int64_t cache_stride_slot, int64_t cache_stride_head,
     int32_t page_size, int64_t num_pages, int32_t cache_format, const void* k_scale, const void* v_scale,
     int64_t scale_stride_page, int64_t scale_stride_head, const int32_t* page_table,
@@ -566,8 +516,11 @@ extern "C" int d2sd_paged_attention(
   const char* const w = "d2sd_paged_attention";
   if (!plan || !sections || num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads % num_kv_heads)
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
-  if (sections[S_ITEMS] == 0 && !fixed_grid) return D2SD_OK;  // no query rows
-  if (!q || !out || !k_pool || !v_pool || !page_table || page_table_len < 0)
+  const int32_t* tiles = sections + kSectionInts;
+  if (sections[S_ITEMS] == 0 && tiles[S_ITEMS] == 0 && !fixed_grid) return D2SD_OK;  // no query rows
+  if (!(sm_scale > 0.f))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": sm_scale must be positive");
+  if (!q || !out || !k_pool || !v_pool || !page_table || page_table_len < 0 || num_tokens <= 0)
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
   if (head_dim != 64 && head_dim != 128)
     return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": head_dim must be 64 or 128");
@@ -585,8 +538,12 @@ extern "C" int d2sd_paged_attention(
       out_stride_token % 8 || out_stride_head % 8 || scale_stride_page % 16 || scale_stride_head % 16)
     return fail(D2SD_ERR_INVALID_ARGUMENT,
                 std::string(w) + ": rows must be 16-byte aligned, strides multiples of 8");
-  if (num_ctas <= 0 || sections[S_CTAS] > num_ctas || sections[S_TICKETS] > 2 * num_ctas ||
-      sections[S_SLOTS] > 2 * num_ctas)
+  bool fits = num_ctas > 0;
+  for (int s = 0; s < kSections; ++s) {
+    const int32_t* sec = sections + s * kSectionInts;
+    fits = fits && sec[S_CTAS] <= num_ctas && sec[S_TICKETS] <= 2 * num_ctas && sec[S_SLOTS] <= 2 * num_ctas;
+  }
+  if (!fits)
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": the plan is for another grid");
   if (workspace_bytes < d2sd_paged_workspace_bytes(num_ctas, head_dim) || !workspace ||
       !aligned16(workspace))
@@ -610,14 +567,16 @@ extern "C" int d2sd_paged_attention(
   a.sinks = sinks, a.sink_mode = sink_mode;
   a.status = status;
   a.scale_log2 = sm_scale * kLog2e;
-  const int ctas = fixed_grid ? num_ctas : sections[S_CTAS];
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool d128 = head_dim == 128, umma = a.g.umma != 0;
-  if (scaled) return d128 ? launch_rows<__nv_bfloat16, 128, 1, true>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 1, true>(a, ctas, st);
-  if (dtype == D2SD_DTYPE_BF16) {
-    if (umma) return d128 ? launch_rows<__nv_bfloat16, 128, 2, true>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 2, true>(a, ctas, st);
-    return d128 ? launch_rows<__nv_bfloat16, 128, 2, false>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 2, false>(a, ctas, st);
+  if (sections[S_ITEMS] > 0 || fixed_grid) {
+    rc = run_rows(a, dtype, head_dim, scaled, fixed_grid ? num_ctas : sections[S_CTAS], st);
+    if (rc) return rc;
   }
-  if (umma) return d128 ? launch_rows<__half, 128, 2, true>(a, ctas, st) : launch_rows<__half, 64, 2, true>(a, ctas, st);
-  return d128 ? launch_rows<__half, 128, 2, false>(a, ctas, st) : launch_rows<__half, 64, 2, false>(a, ctas, st);
+  if (tiles[S_ITEMS] > 0 || fixed_grid) {
+    a.tickets += tile_tickets_at(num_ctas);
+    a.slots += tile_slots_at(num_ctas, head_dim);
+    rc = launch_tiles(a, dtype, head_dim, scaled, num_tokens, num_qo_heads, num_kv_heads,
+                      fixed_grid ? num_ctas : tiles[S_CTAS], stream);
+  }
+  return rc;
 }

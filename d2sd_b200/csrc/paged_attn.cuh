@@ -1,0 +1,73 @@
+// Shared by the two kernels of the attention over the paged cache.
+#pragma once
+
+#include "paged.cuh"
+#include "paged_plan.h"
+
+namespace d2sd {
+namespace paged {
+
+struct AttnArgs {
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_st, q_sh, o_st, o_sh, lse_st;  // element strides
+  const uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
+  const int32_t* page_table;
+  int64_t page_table_len;
+  const int32_t* plan;
+  float* slots;      // partial states: [slot][rows * (D + 2)]
+  uint32_t* tickets;
+  const float* sinks;
+  int32_t* status;
+  PageGeom g;
+  float scale_log2;
+  int32_t sink_mode;
+};
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) { return pack_bf16x2(lo, hi); }
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// Bytes 0 and 2 (even) or 1 and 3 (odd) of x, e4m3, to two bf16. Moving sign and
+// magnitude into a bf16's places gives value * 2^-120 (the exponent biases differ
+// by 120; subnormals likewise), so a product with 2^120 ends it. NaN (0x7f) is
+// not one after this; the writer marks such rows in their scale byte.
+__device__ __forceinline__ uint32_t mul_2p120(uint32_t x) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7b807b80u));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_even(uint32_t x) {
+  return mul_2p120(((x & 0x00800080u) << 8) | ((x & 0x007f007fu) << 4));
+}
+__device__ __forceinline__ uint32_t e4m3_odd(uint32_t x) {
+  return mul_2p120((x & 0x80008000u) | ((x & 0x7f007f00u) >> 4));
+}
+
+// Factor of the attention sink: o *= sigmoid(lse - sink) (include/d2sd.h).
+__device__ __forceinline__ float sink_factor(float lse2, float sink, int mode) {
+  const float x = (mode == D2SD_SINK_EXACT ? lse2 * kLn2 : lse2) - sink;
+  return 1.f / (1.f + expf(-x));
+}
+
+// One 16-byte chunk of zeros is written over rows [r0, r1) of a page in smem.
+template <int D, int ELEM>
+__device__ __forceinline__ void zero_rows(uint8_t* page, int r0, int r1) {
+  constexpr int C = D * ELEM / 16;
+  const int lane = threadIdx.x & 31;
+  for (int i = lane; i < 16 * C; i += 32) {
+    const int r = i & 15, c = i >> 4;
+    if (r >= r0 && r < r1)
+      *reinterpret_cast<uint4*>(page + ((r >> 3) * C + c) * 128 + (r & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Units of more than 16 query rows (paged_tiles.cu); dims of q for its copies.
+int launch_tiles(const AttnArgs& a, int32_t dtype, int32_t head_dim, bool scaled, int64_t num_tokens,
+                 int32_t num_qo_heads, int32_t num_kv_heads, int ctas, void* stream);
+
+}  // namespace paged
+}  // namespace d2sd

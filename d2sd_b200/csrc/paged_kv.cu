@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
       else if (a.half && pos >= a.table_rows) err = kStatusTable;
     }
     if (err) {  // the token's rows are not written at all
-      if (threadIdx.x == 0 && a.status) atomicExch(a.status, err);
+      if (threadIdx.x == 0) report(a.status, err);
       continue;
     }
     // this lane's cos and sin: columns of its 8 elements' pairs
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
       if (page < 0 || page >= a.g.num_pages) err = kStatusPage;
     }
     if (err) {
-      if (threadIdx.x == 0 && a.status) atomicExch(a.status, err);
+      if (threadIdx.x == 0) report(a.status, err);
       continue;
     }
     const int slot = static_cast<int>(pos % a.g.page_size);
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads) commit_e4m3_kernel(const CommitArgs8
         }
         if (err) {
           ok = false;
-          if (part == 0 && a.status) atomicExch(a.status, err);
+          if (part == 0) report(a.status, err);
         } else {
           Vec8<T> v;
           v.load(src + t * a.n_st);

@@ -23,17 +23,21 @@ int plan_fail(int code, const char* msg) {
 
 struct Unit {
   int32_t req, head, tok0, row0, nrows, key0, key1, pos0, page_off, kv_len;
+  int32_t weight;  // cost of a tile
   int32_t tiles() const { return key1 > key0 ? (key1 - key0 + kTileKeys - 1) / kTileKeys : 0; }
 };
 
-// The units in order, cut where a CTA's share of the tiles ends. Every item
-// costs `fixed` tiles on top of its own (its start, its end and, for a split
-// unit, the joining), so a CTA of many small items gets fewer tiles.
-void cut(const std::vector<Unit>& units, int ctas, int fixed, int32_t window, std::vector<int32_t>& items,
-         std::vector<int32_t>& first, int32_t* slots, int32_t* tickets) {
-  int64_t total = 0;
-  for (const Unit& u : units) total += u.tiles() + fixed;
-  const int64_t n = std::max<int64_t>(1, std::min<int64_t>(ctas, total / (1 + fixed)));
+// The units in order, cut where a CTA's share of the cost ends. An item costs its
+// tiles, each of the unit's weight, and `fixed` on top (its start, its end and, for
+// a split unit, the joining), so a CTA of many small items gets fewer tiles.
+void cut(const std::vector<Unit>& units, int ctas, int64_t fixed, int32_t window,
+         std::vector<int32_t>& items, std::vector<int32_t>& first, int32_t* slots, int32_t* tickets) {
+  int64_t total = 0, tiles = 0;
+  for (const Unit& u : units) {
+    total += static_cast<int64_t>(u.tiles()) * u.weight + fixed;
+    tiles += std::max(1, u.tiles());
+  }
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>(ctas, tiles));
   *slots = *tickets = 0;
   first.assign(1, 0);
   int64_t done = 0;  // cost handed out so far
@@ -41,26 +45,29 @@ void cut(const std::vector<Unit>& units, int ctas, int fixed, int32_t window, st
   for (const Unit& u : units) {
     const size_t at = items.size();
     int32_t key = u.key0, parts = 0;
-    int left = u.tiles();
+    int64_t left = u.tiles();
     do {
       // this CTA's share ends at cost total * k / n
       const int64_t k = static_cast<int64_t>(first.size());
-      int64_t room = total * k / n - done - fixed;
-      if (k >= n) room = total;
-      int take = static_cast<int>(std::min<int64_t>(left, std::max<int64_t>(room, 1)));
-      if (left - take == 1 && take > 1 && room - take >= -1) take = left;  // no splinter of one tile
-      const int32_t end = (take == left) ? u.key1 : key + take * kTileKeys;
-      const int32_t it[kItemInts] = {u.req,  u.head, u.tok0,     u.row0,   u.nrows, key, end, u.pos0,
-                                     window, u.page_off, u.kv_len, parts,    0,       0,   0,   0};
+      int64_t take = left;
+      if (k < n) {
+        const int64_t room = (total * k / n - done - fixed) / u.weight;
+        take = std::min(left, std::max<int64_t>(room, 1));
+        if (left - take == 1 && take > 1) take = left;  // no splinter of one tile
+      }
+      const int32_t end = take == left ? u.key1 : key + static_cast<int32_t>(take) * kTileKeys;
+      const int32_t it[kItemInts] = {u.req,  u.head,     u.tok0,   u.row0, u.nrows, key, end, u.pos0,
+                                     window, u.page_off, u.kv_len, parts,  0,       0,   0,   0};
       items.insert(items.end(), it, it + kItemInts);
       ++count;
       ++parts;
       left -= take;
-      done += take + fixed;
-      total += left > 0 ? fixed : 0;  // the next part's own fixed cost
+      done += take * u.weight + fixed;
+      if (left > 0) total += fixed;  // the next part's own
       key = end;
+      // the next item starts in the CTA whose share still has room for a tile
       while (static_cast<int64_t>(first.size()) < n &&
-             done + fixed >= total * static_cast<int64_t>(first.size()) / n)
+             done + fixed + u.weight > total * static_cast<int64_t>(first.size()) / n)
         first.push_back(count);
     } while (left > 0);
     for (int p = 0; p < parts; ++p) {
@@ -123,8 +130,11 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
       if (kv >= kNoLimit || n * G >= kNoLimit || tok + n >= kNoLimit)
         return plan_fail(D2SD_ERR_UNSUPPORTED, "lengths above 2^30");
       const int64_t rows = n * G;
-      const int section = 0;
-      const int64_t tile = kRowsTile;
+      // few rows: tiles of 16 rows; else pairs of q tiles of whole tokens, where a
+      // unit of one q tile works on two key tiles at a time
+      const int section = rows <= kRowsLimit ? 0 : 1;
+      const int64_t q_tile = static_cast<int64_t>(128 / G) * G;
+      const int64_t tile = section == 0 ? kRowsTile : 2 * q_tile;
       const int32_t pos0 = causal ? static_cast<int32_t>(kv - n) : kNoLimit;
       for (int h = 0; h < num_kv_heads; ++h) {
         for (int64_t row = 0; row < rows; row += tile) {
@@ -140,7 +150,8 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
           units[section].push_back({r, h, static_cast<int32_t>(tok), static_cast<int32_t>(row),
                                     static_cast<int32_t>(nr), static_cast<int32_t>(lo),
                                     static_cast<int32_t>(hi), pos0, page_offsets[r],
-                                    static_cast<int32_t>(kv)});
+                                    static_cast<int32_t>(kv),
+                                    section == 1 && nr > q_tile ? 2 : 1});
         }
       }
       tok += n;
@@ -155,7 +166,7 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
       int32_t sec[kSectionInts] = {0};
       if (!units[s].empty()) {
         std::vector<int32_t> items, first;
-        cut(units[s], num_ctas, 1, window, items, first, &sec[S_SLOTS], &sec[S_TICKETS]);
+        cut(units[s], num_ctas, s == 0 ? 1 : 4, window, items, first, &sec[S_SLOTS], &sec[S_TICKETS]);
         sec[S_CTAS] = static_cast<int32_t>(first.size()) - 1;
         sec[S_ITEMS] = static_cast<int32_t>(items.size() / kItemInts);
         sec[S_OFF_CTA] = static_cast<int32_t>(out.size());

@@ -16,6 +16,7 @@ namespace paged {
 
 constexpr int kTileKeys = 128;
 constexpr int kRowsTile = 16;    // query rows of a unit of the rows kernel
+constexpr int kRowsLimit = 16;   // requests of more rows per kv head go to the tiles kernel
 constexpr int kMagic = 0x50474131;
 
 // header: magic, then one section per kernel (S_*), kSectionInts ints each
@@ -45,7 +46,20 @@ enum {
 };
 constexpr int kNoLimit = 1 << 30;
 
-constexpr int64_t ticket_bytes(int num_ctas) { return (2 * 4 * static_cast<int64_t>(num_ctas) + 127) / 128 * 128; }
+// Workspace: tickets of the rows units (2 per CTA: a CTA's first and last item can
+// be spans of split units) and of the tiles units (one for each of two q tiles),
+// then the slots in the same order.
+constexpr int64_t tile_tickets_at(int num_ctas) { return 2 * static_cast<int64_t>(num_ctas); }
+constexpr int64_t ticket_bytes(int num_ctas) { return (6 * 4 * static_cast<int64_t>(num_ctas) + 127) / 128 * 128; }
+constexpr int64_t rows_slot_floats(int head_dim) { return kRowsTile * (head_dim + 2); }
+constexpr int64_t tile_slot_floats(int head_dim) { return 128 * (head_dim + 2); }
+constexpr int64_t tile_slots_at(int num_ctas, int head_dim) {  // floats behind the first slot
+  return 2 * static_cast<int64_t>(num_ctas) * rows_slot_floats(head_dim);
+}
+constexpr int64_t workspace_bytes(int num_ctas, int head_dim) {
+  return ticket_bytes(num_ctas) +
+         4 * (tile_slots_at(num_ctas, head_dim) + 4 * static_cast<int64_t>(num_ctas) * tile_slot_floats(head_dim));
+}
 
 }  // namespace paged
 }  // namespace d2sd

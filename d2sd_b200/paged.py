@@ -132,7 +132,7 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     Hq, Hk, D = plan.num_qo_heads, plan.num_kv_heads, plan.head_dim
     if dev != plan.device:
         raise ValueError("the plan is for another device")
-    if q.dim() != 3 or q.shape[0] < plan.tokens:
+    if q.dim() != 3 or q.shape[0] < max(plan.tokens, 1):
         raise ValueError(f"q must hold the plan's {plan.tokens} tokens")
     pool, heads, dim = ops._pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale)
     if heads != Hk or dim != D:
@@ -153,7 +153,7 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     elif lse.dtype != torch.float32 or lse.dim() != 2 or lse.stride(1) != 1 \
             or lse.shape[0] < plan.tokens or lse.shape[1] != Hq:
         raise ValueError("lse must be fp32 [tokens, num_qo_heads] with a contiguous head axis")
-    args = (*ops._row_strides("q", q, Hq, D), ops.dtype_code(q), k_pool.data_ptr(),
+    args = (*ops._row_strides("q", q, Hq, D), q.shape[0], ops.dtype_code(q), k_pool.data_ptr(),
             v_pool.data_ptr(), *pool, ops._int32("page_table", page_table), page_table.numel(), Hq,
             Hk, D, D ** -0.5 if sm_scale is None else float(sm_scale), plan.plan.data_ptr(),
             plan.sections.ctypes.data, plan.num_ctas, 1 if plan.fixed_grid else 0,

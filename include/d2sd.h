@@ -526,7 +526,8 @@ int d2sd_commit_kv_hidden(const void* const* layer_ptrs, int32_t num_layers,
  *
  * status (device int32, may be NULL) receives 4 when a position lies outside
  * its request's pages, 5 for a page id outside the pool, 6 for a position
- * outside the rotary tables; that token's rows are then not written. */
+ * outside the rotary tables (the smallest of them, if several); that token's
+ * rows are then not written. */
 
 /* Norm (optional), rotary position (optional) and cache write of a batch's new
  * tokens in one launch; no reference counterpart (the reference's target forward
@@ -615,10 +616,10 @@ int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
 int64_t d2sd_paged_workspace_bytes(int32_t num_ctas, int32_t head_dim);
 
 /* Attention of the planned new tokens over the paged cache, which already holds
- * them. q/out [tokens, num_qo_heads, head_dim] in dtype (BF16 or F16; BF16 with
+ * them. q/out [num_tokens, num_qo_heads, head_dim] in dtype (BF16 or F16; BF16 with
  * an 8-bit cache), requests in the plan's order; lse [tokens, num_qo_heads]
  * base 2, or NULL. page_size is a multiple of 16 (UMMA pages: 16), head_dim 64
- * or 128, at most 128 query heads per kv head. sinks fp32 [num_qo_heads] with a
+ * or 128, at most 128 query heads per kv head, sm_scale > 0. sinks fp32 [num_qo_heads] with a
  * D2SD_SINK_* mode, or NULL. A row that sees no key gets out 0 and lse -inf.
  * Slots past a request's last position may hold anything, NaN included; page
  * ids outside the pool are read as its first or last page. fixed_grid: launch
@@ -626,8 +627,8 @@ int64_t d2sd_paged_workspace_bytes(int32_t num_ctas, int32_t head_dim);
  * when the plan's device buffer is rewritten. status receives 1 if a wait inside
  * the kernel ran out of time (zero the workspace before using it again). */
 int d2sd_paged_attention(const void* q, int64_t q_stride_token,
-                         int64_t q_stride_head, int32_t dtype,
-                         const void* k_pool, const void* v_pool,
+                         int64_t q_stride_head, int64_t num_tokens,
+                         int32_t dtype, const void* k_pool, const void* v_pool,
                          int64_t cache_stride_page, int64_t cache_stride_slot,
                          int64_t cache_stride_head, int32_t page_size,
                          int64_t num_pages, int32_t cache_format,

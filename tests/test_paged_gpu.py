@@ -115,6 +115,10 @@ CASES = [
     (40, 8, 128, "f16", "same", "paged_hnd", ([200], [333]), None, False),
     (12, 4, 128, "bf16", "e4m3", "paged_umma", ([190, 1], [700, 90]), 300, False),
     (128, 1, 64, "bf16", "same", "paged_umma", ([3, 40], [100, 41]), None, False),
+    # many short units for each CTA, whose first and last key tiles are both cut
+    (64, 8, 64, "bf16", "same", "paged_umma", ([1300, 900, 33], [1300, 2000, 300]), 128, True),
+    (64, 8, 64, "bf16", "e4m3", "paged_umma", ([1300, 900, 33], [1300, 2000, 300]), 128, False),
+    (32, 8, 128, "f16", "same", "paged_hnd", ([1000, 70], [1000, 500]), 50, False),
 ]
 TYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
 
