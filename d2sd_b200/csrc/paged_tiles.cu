@@ -25,8 +25,8 @@
 //
 // Online softmax in the log2 domain with a lazy maximum: O is rescaled in TMEM
 // only when the running maximum grows by more than 8 (weights stay below 2^8,
-// inside f16). Weights are rounded to nearest (ties up for bf16) for the second
-// product; their fp32 values go into the sum. Tiles that every row sees whole skip
+// inside f16). Weights are rounded to nearest for the second product; their fp32
+// values go into the sum. Tiles that every row sees whole skip
 // the mask; the others compare each key with the row's [lo, hi).
 #include <atomic>
 #include <string>
@@ -77,6 +77,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   const bool ok = mbar_wait(bar, parity, abort);
   return __all_sync(0xffffffffu, ok);
 }
+// One lane of the warp. The compiler knows that a branch on it runs a single
+// thread, so what tcgen05 takes from uniform registers is computed there; behind
+// `lane == 0` every operand of every product is moved over one by one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -90,13 +98,6 @@ __device__ __forceinline__ uint64_t desc_at(uint64_t d, uint32_t bytes) {
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
   return r;
 }
-
-// Two weights to 16 bits. bf16: half a last place is added and the low half cut
-// (weights are not negative; ties go up), one add and half a permute each.
-__device__ __forceinline__ uint32_t pack_weights(float lo, float hi, __nv_bfloat16) {
-  return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632);
-}
-__device__ __forceinline__ uint32_t pack_weights(float lo, float hi, __half) { return pack2(lo, hi, __half()); }
 
 // What every role derives from an item.
 struct Item {
@@ -188,14 +189,13 @@ __device__ void producer(const CUtensorMap* tm_q, const CUtensorMap* tm_k, const
         if (MODE == kRows) {
           if (lane == 0) mbar_arrive_expect_tx(full, C::kTileBytes);
           uint8_t* dst = smem + (kv ? C::kSmemV : C::kSmemK) + st * C::kTileBytes;
-          for (int b = 0; b < boxes; ++b) {
-            const int pg = __shfl_sync(0xffffffffu, page, b);
-            if (lane == 0) {
+          __syncwarp();
+          if (lane < boxes) {
+            const int slot = box_slot(t, lane);
 #pragma unroll
-              for (int pn = 0; pn < C::kPanels; ++pn)
-                tma_load_4d(dst + pn * kPanelBytes + b * rpb * 128, kv ? tm_v : tm_k, full, pn * 64,
-                            box_slot(t, b), I.head, pg);
-            }
+            for (int pn = 0; pn < C::kPanels; ++pn)
+              tma_load_4d(dst + pn * kPanelBytes + lane * rpb * 128, kv ? tm_v : tm_k, full, pn * 64, slot,
+                          I.head, page);
           }
         } else {
           constexpr int kBlock = 16 * D * (MODE == kE4m3 ? 1 : 2);  // a page of one head
@@ -445,7 +445,6 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       // TMEM where there are no registers for all 128
       uint32_t s[kTwoPass ? 32 : 128];
       auto mask = [&](int c, uint32_t* v) {
-        if (!edge) return;
 #pragma unroll
         for (int e = 0; e < 32; ++e)
           if (c * 32 + e >= h || c * 32 + e < l) v[e] = 0xff800000u;  // -inf
@@ -453,12 +452,20 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       float mx[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) mx[e] = -INFINITY;
-      if constexpr (!kTwoPass) tmem_ld128_wait(lane_base + s_col(i), s);
+      if constexpr (!kTwoPass) {
+        tmem_ld128_wait(lane_base + s_col(i), s);
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mask(c, s + c * 32);
+        }
+      }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t* v = kTwoPass ? s : s + c * 32;
-        if constexpr (kTwoPass) tmem_ld32_wait(lane_base + s_col(i) + c * 32, s);
-        mask(c, v);
+        if constexpr (kTwoPass) {
+          tmem_ld32_wait(lane_base + s_col(i) + c * 32, s);
+          if (edge) mask(c, s);
+        }
 #pragma unroll
         for (int e = 0; e < 32; e += 16) {
 #pragma unroll
@@ -488,7 +495,7 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
         const uint32_t* v = kTwoPass ? s : s + c * 32;
         if constexpr (kTwoPass) {
           tmem_ld32_wait(lane_base + s_col(i) + c * 32, s);
-          mask(c, s);
+          if (edge) mask(c, s);
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -497,7 +504,7 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
           f2_unpack(x2, x0, x1);
           const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
           acc2[e & 3] = f2_add(acc2[e & 3], f2_pack(p0, p1));
-          pk[e] = pack_weights(p0, p1, T());
+          pk[e] = pack2(p0, p1, T());
         }
         tmem_st16(lane_base + s_col(i) + c * 16, pk);
         if (c == 1 && early) {
@@ -751,7 +758,7 @@ __global__ void __launch_bounds__(Cfg<D, MODE>::kThreads, 1)
       producer<D, MODE>(&tm_q, &tm_k, &tm_v, a, smem, bars, abort, items, item0, item1, G, TT, rpb);
       __syncwarp();
     } else if (warp == kMmaWarp) {
-      if (lane == 0) mma_issuer<T, D, MODE>(smem, bars, tmem, abort, items, item0, item1, G, TT);
+      if (elect_one()) mma_issuer<T, D, MODE>(smem, bars, tmem, abort, items, item0, item1, G, TT);
       __syncwarp();
     } else if (warp == kFixWarp && MODE != kE4m3) {
       fixer<D, MODE>(smem, bars, abort, items, item0, item1, G, TT);
