@@ -70,6 +70,14 @@ struct Cfg {
   static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 };
 
+__device__ __forceinline__ float fmin3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
+}
 __device__ __forceinline__ uint32_t s_col(int i) { return static_cast<uint32_t>(i * 128); }
 __device__ __forceinline__ uint32_t o_col(int i) { return static_cast<uint32_t>(256 + i * 128); }
 
@@ -139,20 +147,8 @@ __device__ void producer(const CUtensorMap* tm_q, const CUtensorMap* tm_k, const
   bool alive = true;
   for (int it = item0; it < item1 && alive; ++it) {
     const Item I(items + it * kItemInts, G, TT);
+    if (it + 2 < item1) prefetch_l1(items + (it + 2) * kItemInts);  // for every role
     if (I.tiles == 0) continue;
-    if (lane == 0) {
-      if (kitem > 0 && !mbar_wait(&bars[C::B_QFREE], (kitem - 1) & 1, abort)) alive = false;
-      if (alive) {
-        const int nq = I.split ? 1 : 2;
-        mbar_arrive_expect_tx(&bars[C::B_QFULL], nq * C::kPanels * TT * G * 128);
-        for (int i = 0; i < nq; ++i)
-          for (int pn = 0; pn < C::kPanels; ++pn)
-            tma_load_3d(smem + C::kSmemQ + i * C::kTileBytes + pn * kPanelBytes, tm_q,
-                        &bars[C::B_QFULL], pn * 64, I.head * G, I.tok0 + I.tokb + i * TT);
-      }
-    }
-    ++kitem;
-    alive = __shfl_sync(0xffffffffu, alive ? 1 : 0, 0) != 0;
     // lane b: the page of box b of tile t (slots behind the last position are
     // filled from the last page and masked), clamped to the pool
     const int last = (I.kv_len - 1) / rpb;
@@ -214,6 +210,22 @@ __device__ void producer(const CUtensorMap* tm_q, const CUtensorMap* tm_k, const
         }
       }
       page = next;
+      if (t > 0) continue;
+      // q behind the first tile's keys and values: its buffer is free only when the
+      // previous item's last S is done, and their copies need not wait for that
+      if (lane == 0) {
+        if (kitem > 0 && !mbar_wait(&bars[C::B_QFREE], (kitem - 1) & 1, abort)) alive = false;
+        if (alive) {
+          const int nq = I.split ? 1 : 2;
+          mbar_arrive_expect_tx(&bars[C::B_QFULL], nq * C::kPanels * TT * G * 128);
+          for (int i = 0; i < nq; ++i)
+            for (int pn = 0; pn < C::kPanels; ++pn)
+              tma_load_3d(smem + C::kSmemQ + i * C::kTileBytes + pn * kPanelBytes, tm_q,
+                          &bars[C::B_QFULL], pn * 64, I.head * G, I.tok0 + I.tokb + i * TT);
+        }
+      }
+      ++kitem;
+      alive = __shfl_sync(0xffffffffu, alive ? 1 : 0, 0) != 0;
     }
   }
 }
@@ -417,14 +429,17 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
   const float sl2 = a.scale_log2;
   float2* join = reinterpret_cast<float2*>(smem + C::kSmemJoin);
   uint32_t scount = 0, kitem = 0;
+  const int row_tok = row / G, row_g = row % G;
   // a wait ran out of time: the warp does no more work, but goes through the
   // named barriers, which the other warps may be waiting at
   bool dead = false;
   for (int it = item0; it < item1; ++it) {
     const Item I(items + it * kItemInts, G, TT);
-    const int tok = I.tokb + (I.split ? 0 : i * TT) + row / G;  // inside the request
+    const int tok = I.tokb + (I.split ? 0 : i * TT) + row_tok;  // inside the request
     const int tok_end = I.tokb + (I.split ? I.ntok : min(I.ntok, (i + 1) * TT));
     const bool valid = row < TT * G && tok < tok_end;
+    const int hq = I.head * G + row_g;
+    const float sink = a.sinks && valid ? a.sinks[hq] : 0.f;
     const int hi = valid ? I.row_hi(tok) : 0, lo = valid ? I.row_lo(tok) : 0;
     // keys every valid row of this tile sees
     const int first_tok = I.tokb + (I.split ? 0 : i * TT);
@@ -440,14 +455,25 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       tc_fence_after();
       const int key = I.key0 + I.tile(i, j) * kTileKeys;
       const bool edge = key + kTileKeys > hi_all || key < lo_all;
-      const int h = hi - key, l = lo - key;
-      // the scores of 32 keys, those the row does not see at -inf; two passes over
-      // TMEM where there are no registers for all 128
+      // The scores of 32 keys, those the row does not see at -inf: key e is kept by
+      // a minimum with (h - e) * inf, which is +inf below h and -inf above (h half
+      // an integer), and likewise for the window's end -- two multiplications on
+      // the idle FMA pipe and one three-way minimum, where comparing and selecting
+      // costs three operations of the pipe that also takes the row maximum. Two
+      // passes over TMEM where there are no registers for all 128 keys.
+      const float h = static_cast<float>(hi - key) - 0.5f, l = static_cast<float>(lo - key) - 0.5f;
       uint32_t s[kTwoPass ? 32 : 128];
       auto mask = [&](int c, uint32_t* v) {
+        const float hc = h - c * 32, lc = c * 32 - l;
+        if (I.window) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (c * 32 + e >= h || c * 32 + e < l) v[e] = 0xff800000u;  // -inf
+          for (int e = 0; e < 32; ++e)
+            v[e] = __float_as_uint(fmin3(__uint_as_float(v[e]), (hc - e) * INFINITY, (lc + e) * INFINITY));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            v[e] = __float_as_uint(fminf(__uint_as_float(v[e]), (hc - e) * INFINITY));
+        }
       };
       float mx[8];
 #pragma unroll
@@ -595,12 +621,11 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       }
       ++kitem;
     };
-    const int hq = I.head * G + row % G;
     const int64_t gtok = static_cast<int64_t>(I.tok0) + tok;
     auto factor = [&](float m, float l, float& lse2) {
       lse2 = l > 0.f ? m + log2f(l) : (l == 0.f ? -INFINITY : l);
       float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      if (a.sinks) f *= sink_factor(lse2, a.sinks[hq], a.sink_mode);
+      if (a.sinks) f *= sink_factor(lse2, sink, a.sink_mode);
       return f;
     };
     auto store_o = [&](int c, const float (&o)[32], float f) {
