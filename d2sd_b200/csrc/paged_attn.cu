@@ -17,7 +17,7 @@
 // 8-row x 16-byte core matrices, exactly what ldmatrix fetches, without bank
 // conflicts and without a swizzle; pages of plain rows are put into that order by
 // the copy. At the end the warps' states are joined in shared memory, and for a
-// unit of several spans the last CTA joins the spans.
+// unit of several spans join_kernel joins the spans.
 //
 // e4m3 pages: the fragments are widened to bf16 in registers (sign and the seven
 // magnitude bits moved into place, then a product with 2^120, all exact). A
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
   float* sm_m = reinterpret_cast<float*>(smem + C::kSmemMl);
   float* sm_l = sm_m + kWarps * 16;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kSmemBars);
-  volatile int* flags = reinterpret_cast<volatile int*>(smem + C::kSmemFlags);  // abort, last
+  volatile int* flags = reinterpret_cast<volatile int*>(smem + C::kSmemFlags);  // abort
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   uint8_t* ring = smem + warp * C::kRing;
   uint64_t* full = bars + warp * 8;
@@ -413,45 +413,23 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) acc[e] = fmaf(ow[e], f, acc[e]);
     }
-    const int parts = I[P_PARTS];
-    bool write = true;
-    if (parts > 1) {
-      constexpr int kSlot = 16 * (D + 2);
-      float* mine_s = a.slots + static_cast<int64_t>(I[P_SLOT]) * kSlot;
+    if (I[P_PARTS] > 1) {  // a span of a unit: leave the state in its slot (join_kernel)
+      float* own = a.slots + static_cast<int64_t>(I[P_SLOT]) * rows_slot_floats(D);
+      if (row < nrows) {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) mine_s[row * D + dcol + e] = acc[e];
-      if (dcol == 0) {
-        mine_s[16 * D + row] = M;
-        mine_s[16 * D + 16 + row] = L;
-      }
-      __syncthreads();
-      if (threadIdx.x == 0)
-        flags[1] = atom_add_acq_rel_gpu(&a.tickets[I[P_TICKET]], 1u) == static_cast<uint32_t>(parts - 1);
-      __syncthreads();
-      write = flags[1] != 0;
-      if (write) {  // the last span: join all of them, in slot order
-        if (threadIdx.x == 0) a.tickets[I[P_TICKET]] = 0;
-        const float* s0 = a.slots + static_cast<int64_t>(I[P_FIRST_SLOT]) * kSlot;
-        M = -INFINITY;
-        for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(s0 + p * kSlot + 16 * D + row));
-        const float mr = M == -INFINITY ? 0.f : M;
-        L = 0.f;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-        for (int p = 0; p < parts; ++p) {
-          const float* sp = s0 + p * kSlot;
-          const float f = fast_exp2(__ldcg(sp + 16 * D + row) - mr);
-          L += __ldcg(sp + 16 * D + 16 + row) * f;
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) acc[e] = fmaf(__ldcg(sp + row * D + dcol + e), f, acc[e]);
+        for (int e = 0; e < kPer; e += 4)
+          reinterpret_cast<float4*>(own)[(dcol + e) / 4 * 16 + row] =
+              make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+        if (dcol == 0) {
+          own[16 * D + row] = M;
+          own[16 * D + 16 + row] = L;
         }
       }
-    }
-    if (write && row < nrows) {
+    } else if (row < nrows) {
       const int64_t tok = tok0 + static_cast<int64_t>((row0 + row) / G);
       const int hq = head * G + (row0 + row) % G;
-      const float lse2 = L > 0.f ? M + log2f(L) : (L == 0.f ? -INFINITY : L);
-      float f = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+      float lse2;
+      float f = row_factor(M, L, lse2);
       if (a.sinks) f *= sink_factor(lse2, a.sinks[hq], a.sink_mode);
       T* op = static_cast<T*>(a.out) + tok * a.o_st + hq * a.o_sh + dcol;
 #pragma unroll
@@ -463,6 +441,75 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
     if (flags[0]) break;
   }
   if (threadIdx.x == 0 && flags[0] && a.status) atomicExch(a.status, 1);
+}
+
+// Joins the spans of split units: an entry of the join list is RB rows (or fewer)
+// whose partial states lie `step` slots apart,
+//   M = max m_p, L = sum l_p 2^(m_p - M), o = sum o_p 2^(m_p - M) / L,
+// in slot order. A thread takes a row and every (256 / RB)-th group of 4 columns.
+template <typename T, int D, int SECTION>
+__global__ void __launch_bounds__(256) join_kernel(const AttnArgs a) {
+  constexpr int RB = kJoinRows[SECTION];
+  constexpr int kSlotRows = SECTION == 0 ? kRowsTile : 128;
+  constexpr int kGroups = 256 / RB, kCols = D / 4 / kGroups;
+  constexpr int64_t kSlot = SECTION == 0 ? rows_slot_floats(D) : tile_slot_floats(D);
+  const int r = threadIdx.x % RB, group = threadIdx.x / RB;
+  grid_dep_wait();
+  const int32_t* sec = a.plan + H_SECTION + SECTION * kSectionInts;
+  const int G = a.plan[H_GROUP], n = sec[S_JOINS];
+  const int32_t* list = a.plan + sec[S_OFF_JOINS];
+  for (int b = blockIdx.x; b < n; b += gridDim.x) {
+    const int32_t* J = list + b * kJoinInts;
+    if (r >= J[J_ROWS]) continue;
+    const int parts = J[J_PARTS], rq = J[J_ROW0] + r;
+    const float* s0 = a.slots + J[J_SLOT] * kSlot;
+    const int64_t step = J[J_STEP] * kSlot;
+    const int at = J[J_SLOT_ROW] + r;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) M = fmaxf(M, s0[p * step + kSlotRows * D + at]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float4 acc[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+      const float* sp = s0 + p * step;
+      const float w = fast_exp2(sp[kSlotRows * D + at] - ref);
+      L = fmaf(sp[kSlotRows * D + kSlotRows + at], w, L);
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        const float4 v = reinterpret_cast<const float4*>(sp)[(c * kGroups + group) * kSlotRows + at];
+        acc[c].x = fmaf(v.x, w, acc[c].x);
+        acc[c].y = fmaf(v.y, w, acc[c].y);
+        acc[c].z = fmaf(v.z, w, acc[c].z);
+        acc[c].w = fmaf(v.w, w, acc[c].w);
+      }
+    }
+    const int64_t tok = J[J_TOK0] + static_cast<int64_t>(rq / G);
+    const int hq = J[J_HEAD] * G + rq % G;
+    float lse2;
+    float f = row_factor(M, L, lse2);
+    if (a.sinks) f *= sink_factor(lse2, a.sinks[hq], a.sink_mode);
+    T* op = static_cast<T*>(a.out) + tok * a.o_st + hq * a.o_sh;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      uint2 v;
+      v.x = pack2(acc[c].x * f, acc[c].y * f, T());
+      v.y = pack2(acc[c].z * f, acc[c].w * f, T());
+      *reinterpret_cast<uint2*>(op + (c * kGroups + group) * 4) = v;
+    }
+    if (a.lse && group == 0) a.lse[tok * a.lse_st + hq] = lse2;
+  }
+}
+
+template <int SECTION>
+int run_join(const AttnArgs& a, int32_t dtype, int32_t head_dim, int entries, int num_ctas, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(entries < 8 * num_ctas ? entries : 8 * num_ctas));
+  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(256), 0, st, "join_kernel", a); };
+  if (dtype == D2SD_DTYPE_BF16)
+    return head_dim == 128 ? go(join_kernel<__nv_bfloat16, 128, SECTION>) : go(join_kernel<__nv_bfloat16, 64, SECTION>);
+  return head_dim == 128 ? go(join_kernel<__half, 128, SECTION>) : go(join_kernel<__half, 64, SECTION>);
 }
 
 template <typename T, int D, int ELEM, bool UMMA>
@@ -541,7 +588,7 @@ extern "C" int d2sd_paged_attention(
   bool fits = num_ctas > 0;
   for (int s = 0; s < kSections; ++s) {
     const int32_t* sec = sections + s * kSectionInts;
-    fits = fits && sec[S_CTAS] <= num_ctas && sec[S_TICKETS] <= 2 * num_ctas && sec[S_SLOTS] <= 2 * num_ctas;
+    fits = fits && sec[S_CTAS] <= num_ctas && sec[S_SLOTS] <= 2 * num_ctas;
   }
   if (!fits)
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": the plan is for another grid");
@@ -562,21 +609,27 @@ extern "C" int d2sd_paged_attention(
   a.k_scale = static_cast<const uint8_t*>(k_scale), a.v_scale = static_cast<const uint8_t*>(v_scale);
   a.page_table = page_table, a.page_table_len = page_table_len;
   a.plan = plan;
-  a.tickets = static_cast<uint32_t*>(workspace);
-  a.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ticket_bytes(num_ctas));
+  a.slots = static_cast<float*>(workspace);
   a.sinks = sinks, a.sink_mode = sink_mode;
   a.status = status;
   a.scale_log2 = sm_scale * kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  AttnArgs t = a;  // the tiles kernel's half of the workspace
+  t.slots += tile_slots_at(num_ctas, head_dim);
   if (sections[S_ITEMS] > 0 || fixed_grid) {
     rc = run_rows(a, dtype, head_dim, scaled, fixed_grid ? num_ctas : sections[S_CTAS], st);
     if (rc) return rc;
   }
   if (tiles[S_ITEMS] > 0 || fixed_grid) {
-    a.tickets += tile_tickets_at(num_ctas);
-    a.slots += tile_slots_at(num_ctas, head_dim);
-    rc = launch_tiles(a, dtype, head_dim, scaled, num_tokens, num_qo_heads, num_kv_heads,
+    rc = launch_tiles(t, dtype, head_dim, scaled, num_tokens, num_qo_heads, num_kv_heads,
                       fixed_grid ? num_ctas : tiles[S_CTAS], stream);
+    if (rc) return rc;
   }
+  if (sections[S_JOINS] > 0 || fixed_grid) {
+    rc = run_join<0>(a, dtype, head_dim, fixed_grid ? num_ctas : sections[S_JOINS], num_ctas, st);
+    if (rc) return rc;
+  }
+  if (tiles[S_JOINS] > 0 || fixed_grid)
+    rc = run_join<1>(t, dtype, head_dim, fixed_grid ? 2 * num_ctas : tiles[S_JOINS], num_ctas, st);
   return rc;
 }

@@ -16,8 +16,7 @@ struct AttnArgs {
   const int32_t* page_table;
   int64_t page_table_len;
   const int32_t* plan;
-  float* slots;      // partial states: [slot][rows * (D + 2)]
-  uint32_t* tickets;
+  float* slots;  // partial states (paged_plan.h)
   const float* sinks;
   int32_t* status;
   PageGeom g;
@@ -47,6 +46,12 @@ __device__ __forceinline__ uint32_t e4m3_odd(uint32_t x) {
   return mul_2p120((x & 0x80008000u) | ((x & 0x7f007f00u) >> 4));
 }
 
+// 1 / sum and log-sum-exp (base 2) of a row with maximum m and sum l: 0 and -inf for
+// a row that saw no key, NaN for one with a NaN.
+__device__ __forceinline__ float row_factor(float m, float l, float& lse2) {
+  lse2 = l > 0.f ? m + log2f(l) : (l == 0.f ? -INFINITY : l);
+  return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+}
 // Factor of the attention sink: o *= sigmoid(lse - sink) (include/d2sd.h).
 __device__ __forceinline__ float sink_factor(float lse2, float sink, int mode) {
   const float x = (mode == D2SD_SINK_EXACT ? lse2 * kLn2 : lse2) - sink;

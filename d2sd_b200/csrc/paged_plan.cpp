@@ -28,22 +28,25 @@ struct Unit {
 };
 
 // The units in order, cut where a CTA's share of the cost ends. An item costs its
-// tiles, each of the unit's weight, and `fixed` on top (its start, its end and, for
-// a split unit, the joining), so a CTA of many small items gets fewer tiles.
-void cut(const std::vector<Unit>& units, int ctas, int64_t fixed, int32_t window,
-         std::vector<int32_t>& items, std::vector<int32_t>& first, int32_t* slots, int32_t* tickets) {
+// tiles and `extra` more (its start, its end and, for a split unit, the joining),
+// each of the unit's weight, so a CTA of many small items gets fewer tiles.
+void cut(const std::vector<Unit>& units, int ctas, int section, int32_t group, int32_t window,
+         std::vector<int32_t>& items, std::vector<int32_t>& first, std::vector<int32_t>& joins, int32_t* slots) {
+  const int extra = section == 0 ? 1 : 4;
+  const int q_tile = section == 0 ? kRowsTile : 128 / group * group, per = section == 0 ? 1 : 2;
   int64_t total = 0, tiles = 0;
   for (const Unit& u : units) {
-    total += static_cast<int64_t>(u.tiles()) * u.weight + fixed;
+    total += static_cast<int64_t>(u.tiles() + extra) * u.weight;
     tiles += std::max(1, u.tiles());
   }
   const int64_t n = std::max<int64_t>(1, std::min<int64_t>(ctas, tiles));
-  *slots = *tickets = 0;
+  *slots = 0;
   first.assign(1, 0);
   int64_t done = 0;  // cost handed out so far
   int32_t count = 0;
   for (const Unit& u : units) {
     const size_t at = items.size();
+    const int64_t fixed = static_cast<int64_t>(extra) * u.weight;
     int32_t key = u.key0, parts = 0;
     int64_t left = u.tiles();
     do {
@@ -57,7 +60,7 @@ void cut(const std::vector<Unit>& units, int ctas, int64_t fixed, int32_t window
       }
       const int32_t end = take == left ? u.key1 : key + static_cast<int32_t>(take) * kTileKeys;
       const int32_t it[kItemInts] = {u.req,  u.head,     u.tok0,   u.row0, u.nrows, key, end, u.pos0,
-                                     window, u.page_off, u.kv_len, parts,  0,       0,   0,   0};
+                                     window, u.page_off, u.kv_len, parts,  0,       u.row0 / group, 0, 0};
       items.insert(items.end(), it, it + kItemInts);
       ++count;
       ++parts;
@@ -73,14 +76,17 @@ void cut(const std::vector<Unit>& units, int ctas, int64_t fixed, int32_t window
     for (int p = 0; p < parts; ++p) {
       int32_t* it = items.data() + at + static_cast<size_t>(p) * kItemInts;
       it[P_SLOT] = parts > 1 ? *slots + p : -1;
-      it[P_FIRST_SLOT] = *slots;
       it[P_PARTS] = parts;
-      it[P_TICKET] = *tickets;
     }
-    if (parts > 1) {
-      *slots += parts;
-      ++*tickets;
+    if (parts == 1) continue;
+    for (int r = 0; r < u.nrows;) {  // rows of one q tile at a time
+      const int tile = r / q_tile, in_tile = r % q_tile;
+      const int n = std::min({kJoinRows[section], u.nrows - r, q_tile - in_tile});
+      const int32_t j[kJoinInts] = {*slots * per + tile, per, parts, in_tile, n, u.row0 + r, u.tok0, u.head};
+      joins.insert(joins.end(), j, j + kJoinInts);
+      r += n;
     }
+    *slots += parts;
   }
   first.push_back(count);
 }
@@ -101,8 +107,9 @@ extern "C" int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_r
     if (q_lens[r] < 0) return -1;
     units += (q_lens[r] * G + kRowsTile - 1) / kRowsTile * num_kv_heads;
   }
-  // every CTA adds at most one cut
-  return kHeaderInts + (units + 2 * static_cast<int64_t>(num_ctas)) * kItemInts + 4 * (num_ctas + 2);
+  // every CTA adds at most one cut; a cut unit has at most 256 rows to join
+  return kHeaderInts + (units + 2 * static_cast<int64_t>(num_ctas)) * kItemInts + 4 * (num_ctas + 2) +
+         static_cast<int64_t>(num_ctas) * 8 * kJoinInts;
 }
 
 extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
@@ -165,8 +172,8 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
     for (int s = 0; s < kSections; ++s) {
       int32_t sec[kSectionInts] = {0};
       if (!units[s].empty()) {
-        std::vector<int32_t> items, first;
-        cut(units[s], num_ctas, s == 0 ? 1 : 4, window, items, first, &sec[S_SLOTS], &sec[S_TICKETS]);
+        std::vector<int32_t> items, first, joins;
+        cut(units[s], num_ctas, s, G, window, items, first, joins, &sec[S_SLOTS]);
         sec[S_CTAS] = static_cast<int32_t>(first.size()) - 1;
         sec[S_ITEMS] = static_cast<int32_t>(items.size() / kItemInts);
         sec[S_OFF_CTA] = static_cast<int32_t>(out.size());
@@ -174,6 +181,9 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
         while (out.size() % 4) out.push_back(0);
         sec[S_OFF_ITEMS] = static_cast<int32_t>(out.size());
         out.insert(out.end(), items.begin(), items.end());
+        sec[S_JOINS] = static_cast<int32_t>(joins.size() / kJoinInts);
+        sec[S_OFF_JOINS] = static_cast<int32_t>(out.size());
+        out.insert(out.end(), joins.begin(), joins.end());
       }
       memcpy(out.data() + H_SECTION + s * kSectionInts, sec, sizeof(sec));
       memcpy(sections + s * kSectionInts, sec, sizeof(sec));

@@ -4,9 +4,9 @@
 // A unit is (request, kv head, row tile): consecutive query rows of one kv head,
 // row = token * G + g. A unit's visible keys are cut into spans of whole 128-key
 // tiles; an item is one span. A unit of one item is written out directly; the
-// items of a split unit leave partial states in consecutive slots, and the CTA
-// that finishes last (one ticket per split unit) joins them in slot order, so the
-// result does not depend on which one that is.
+// items of a split unit leave partial states in consecutive slots, which a second
+// kernel joins in slot order (kept apart so that all SMs join, and no state stays
+// behind in the workspace), 16 or 64 rows to an entry of the join list.
 #pragma once
 
 #include <stdint.h>
@@ -21,7 +21,7 @@ constexpr int kMagic = 0x50474131;
 
 // header: magic, then one section per kernel (S_*), kSectionInts ints each
 enum { H_MAGIC = 0, H_REQUESTS, H_TOKENS, H_GROUP, H_KV_HEADS, H_SECTION, };
-enum { S_CTAS = 0, S_ITEMS, S_SLOTS, S_TICKETS, S_OFF_CTA, S_OFF_ITEMS, kSectionInts };
+enum { S_CTAS = 0, S_ITEMS, S_SLOTS, S_JOINS, S_OFF_CTA, S_OFF_ITEMS, S_OFF_JOINS, kSectionInts };
 constexpr int kSections = 2;  // 0: rows kernel, 1: tiles kernel
 constexpr int kHeaderInts = 32;
 
@@ -37,28 +37,39 @@ enum {
   P_WINDOW,    // 0: none
   P_PAGE_OFF,  // the request's first entry in the page table
   P_KV_LEN,
-  P_SLOT,        // this item's slot, -1: the unit's only item
-  P_FIRST_SLOT,  // of the unit
-  P_PARTS,
-  P_TICKET,
-  P_PAD,
+  P_SLOT,         // this item's slot, -1: the unit's only item
+  P_PARTS,        // items of the unit
+  P_FIRST_TOKEN,  // of the unit, inside the request (P_ROW0 / G)
+  P_PAD0,
+  P_PAD1,
   kItemInts
 };
 constexpr int kNoLimit = 1 << 30;
 
-// Workspace: tickets of the rows units (2 per CTA: a CTA's first and last item can
-// be spans of split units) and of the tiles units (one for each of two q tiles),
-// then the slots in the same order.
-constexpr int64_t tile_tickets_at(int num_ctas) { return 2 * static_cast<int64_t>(num_ctas); }
-constexpr int64_t ticket_bytes(int num_ctas) { return (6 * 4 * static_cast<int64_t>(num_ctas) + 127) / 128 * 128; }
+// Entry of a join list: rows J_ROW0 .. of one q tile (tiles: slots 2 * slot + tile).
+enum {
+  J_SLOT = 0,  // the unit's first slot (tiles: of this q tile)
+  J_STEP,      // slots from one part to the next
+  J_PARTS,
+  J_SLOT_ROW,  // first row inside the slot
+  J_ROWS,      // rows of the entry
+  J_ROW0,      // first row inside the request
+  J_TOK0,      // q row of the request's first token
+  J_HEAD,
+  kJoinInts
+};
+constexpr int kJoinRows[kSections] = {16, 64};
+
+// A slot holds [head_dim / 4][rows] of four columns each, then the rows' m and l.
+// A CTA's first and last item can be spans of split units, so 2 slots per CTA do
+// (tiles: 4, one for each q tile). Workspace: the rows slots, then the tiles slots.
 constexpr int64_t rows_slot_floats(int head_dim) { return kRowsTile * (head_dim + 2); }
 constexpr int64_t tile_slot_floats(int head_dim) { return 128 * (head_dim + 2); }
-constexpr int64_t tile_slots_at(int num_ctas, int head_dim) {  // floats behind the first slot
+constexpr int64_t tile_slots_at(int num_ctas, int head_dim) {  // floats
   return 2 * static_cast<int64_t>(num_ctas) * rows_slot_floats(head_dim);
 }
 constexpr int64_t workspace_bytes(int num_ctas, int head_dim) {
-  return ticket_bytes(num_ctas) +
-         4 * (tile_slots_at(num_ctas, head_dim) + 4 * static_cast<int64_t>(num_ctas) * tile_slot_floats(head_dim));
+  return 4 * (tile_slots_at(num_ctas, head_dim) + 4 * static_cast<int64_t>(num_ctas) * tile_slot_floats(head_dim));
 }
 
 }  // namespace paged

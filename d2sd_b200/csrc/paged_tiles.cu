@@ -107,18 +107,23 @@ __device__ __forceinline__ uint64_t desc_at(uint64_t d, uint32_t bytes) {
   return r;
 }
 
-// What every role derives from an item.
+// What every role derives from an item. rG = 1 / G: the unit's rows are at most 256
+// and a multiple of G, so the rounded product is their number of tokens.
 struct Item {
-  int head, tok0, tokb, ntok, key0, key1, pos0, window, kv_len, parts, slot, first_slot, ticket;
-  int64_t page_off;
+  int head, tok0, tokb, ntok, key0, key1, pos0, window, kv_len, parts, slot, page_off;
   int tiles;
   bool split;  // both streams on the same q tile, every other key tile
-  __device__ __forceinline__ Item(const int32_t* I, int G, int TT) {
-    head = I[P_HEAD], tok0 = I[P_TOK0], key0 = I[P_KEY0], key1 = I[P_KEY1], pos0 = I[P_POS0];
-    window = I[P_WINDOW], kv_len = I[P_KV_LEN], parts = I[P_PARTS], slot = I[P_SLOT];
-    first_slot = I[P_FIRST_SLOT], ticket = I[P_TICKET], page_off = I[P_PAGE_OFF];
-    tokb = I[P_ROW0] / G;        // first token of the unit, inside the request
-    ntok = I[P_NROWS] / G;       // tokens of the unit
+  Item() = default;
+  __device__ __forceinline__ Item(const int32_t* items, int it, float rG, int TT) {
+    const int4* p = reinterpret_cast<const int4*>(items + it * kItemInts);
+    const int4 a = __ldg(p), b = __ldg(p + 1), c = __ldg(p + 2), d = __ldg(p + 3);
+    static_assert(P_HEAD == 1 && P_TOK0 == 2 && P_NROWS == 4 && P_KEY0 == 5 && P_KEY1 == 6 && P_POS0 == 7 &&
+                      P_WINDOW == 8 && P_PAGE_OFF == 9 && P_KV_LEN == 10 && P_SLOT == 11 && P_PARTS == 12 &&
+                      P_FIRST_TOKEN == 13 && kItemInts == 16,
+                  "the layout read here");
+    head = a.y, tok0 = a.z, key0 = b.y, key1 = b.z, pos0 = b.w, window = c.x, page_off = c.y, kv_len = c.z;
+    slot = c.w, parts = d.x, tokb = d.y;
+    ntok = __float2int_rn(b.x * rG);
     tiles = (key1 - key0 + kTileKeys - 1) / kTileKeys;
     split = ntok <= TT;
   }
@@ -139,14 +144,14 @@ struct Item {
 template <int D, int MODE>
 __device__ void producer(const CUtensorMap* tm_q, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
                          const AttnArgs& a, uint8_t* smem, uint64_t* bars, volatile int* abort,
-                         const int32_t* items, int item0, int item1, int G, int TT, int rpb) {
+                         const int32_t* items, int item0, int item1, int G, float rG, int TT, int rpb) {
   using C = Cfg<D, MODE>;
   const int lane = threadIdx.x & 31;
   const int boxes = kTileKeys / rpb;  // copies of a K or V tile (<= 8 ... 16)
   uint32_t kt = 0, kitem = 0;
   bool alive = true;
   for (int it = item0; it < item1 && alive; ++it) {
-    const Item I(items + it * kItemInts, G, TT);
+    const Item I(items, it, rG, TT);
     if (it + 2 < item1) prefetch_l1(items + (it + 2) * kItemInts);  // for every role
     if (I.tiles == 0) continue;
     // lane b: the page of box b of tile t (slots behind the last position are
@@ -253,7 +258,7 @@ __device__ __forceinline__ void issue_pv(uint32_t tmem_o, uint32_t tmem_p, uint6
 
 template <typename T, int D, int MODE>
 __device__ void mma_issuer(uint8_t* smem, uint64_t* bars, uint32_t tmem, volatile int* abort,
-                           const int32_t* items, int item0, int item1, int G, int TT) {
+                           const int32_t* items, int item0, int item1, float rG, int TT) {
   using C = Cfg<D, MODE>;
   constexpr bool SWZ = MODE == kRows;
   constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
@@ -267,7 +272,7 @@ __device__ void mma_issuer(uint8_t* smem, uint64_t* bars, uint32_t tmem, volatil
   uint32_t kt = 0, kitem = 0;
   uint32_t pcount[2] = {0, 0};
   for (int it = item0; it < item1; ++it) {
-    const Item I(items + it * kItemInts, G, TT);
+    const Item I(items, it, rG, TT);
     if (I.tiles == 0) continue;
     const int n = I.tiles;
     // S of stream i's step j
@@ -324,12 +329,12 @@ __device__ void mma_issuer(uint8_t* smem, uint64_t* bars, uint32_t tmem, volatil
 // on to the MMA issuer (a barrier for each stage, so that no phase is skipped).
 template <int D, int MODE>
 __device__ void fixer(uint8_t* smem, uint64_t* bars, volatile int* abort, const int32_t* items, int item0,
-                      int item1, int G, int TT) {
+                      int item1, float rG, int TT) {
   using C = Cfg<D, MODE>;
   const int lane = threadIdx.x & 31;
   uint32_t kt = 0;
   for (int it = item0; it < item1; ++it) {
-    const Item I(items + it * kItemInts, G, TT);
+    const Item I(items, it, rG, TT);
     for (int t = 0; t < I.tiles; ++t, ++kt) {
       const uint32_t st = kt % C::kStages;
       if (!warp_wait(&bars[C::B_VFULL + st], (kt / C::kStages) & 1, abort)) return;
@@ -356,12 +361,17 @@ __device__ void fixer(uint8_t* smem, uint64_t* bars, volatile int* abort, const 
 // thread takes 16-byte chunks: 16 elements of one row.
 template <int D>
 __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, const int32_t* items, int item0,
-                        int item1, int G, int TT) {
+                        int item1, float rG, int TT) {
   using C = Cfg<D, kE4m3>;
   const int tid = threadIdx.x - 384, lane = threadIdx.x & 31;
+  // a page is D chunks; this thread's chunk of a page: row group, chunk, row
+  constexpr int kPagesPer = 128 / D;  // pages that the 128 threads take at once
+  const int y = tid % D, g = y / (D / 2), c = (y / 8) % (D / 16), r = y % 8;
+  const int row0 = tid / D * 16 + g * 8 + r;
+  const int dst0 = tid / D * (32 * D) + (g * (D / 8) + 2 * c) * 128 + r * 16;
   uint32_t kt = 0;
   for (int it = item0; it < item1; ++it) {
-    const Item I(items + it * kItemInts, G, TT);
+    const Item I(items, it, rG, TT);
     const int hi = I.hi_max(), lo = I.lo_min();
     for (int t = 0; t < I.tiles; ++t, ++kt) {
       const uint32_t st = kt % C::kStages, use = kt / C::kStages;
@@ -370,24 +380,24 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
       for (int kv = 0; kv < 2; ++kv) {
         if (!warp_wait(&bars[C::B_LFULL + kv], kt & 1, abort)) return;
         if (use > 0 && !warp_wait(&bars[(kv ? C::B_VEMPTY : C::B_KEMPTY) + st], (use - 1) & 1, abort)) return;
-        const uint8_t* src = smem + C::kSmemLand + kv * C::kLandBytes;
-        const uint8_t* scales = smem + C::kSmemLand + 2 * C::kLandBytes + kv * 128;
-        uint8_t* dst = smem + (kv ? C::kSmemV : C::kSmemK) + st * C::kTileBytes;
-#pragma unroll 4
-        for (int x = tid; x < 128 * (D / 16); x += 128) {
-          const int page = x / D, y = x % D;  // D chunks of a 16-row page
-          const int g = y / (D / 2), c = (y / 8) % (D / 16), r = y % 8;
-          const int row = page * 16 + g * 8 + r;
-          const uint4 w = *reinterpret_cast<const uint4*>(src + x * 16);
-          // 2^(120 + e) as bf16, in two factors where it is above 2^127
-          const int byte = scales[row];
-          int e0 = byte == 0 ? 0 : byte + 120, e1 = 127;  // exponent fields
-          if (e0 > 254) e1 = e0 - 254 + 127, e0 = 254;
-          uint32_t f0 = static_cast<uint32_t>(e0) << 7, f1 = static_cast<uint32_t>(e1) << 7;
-          if (byte == 255) f0 = 0x7fc0u;                                     // NaN
-          if (kv == 1 && (key + row >= hi || key + row < lo)) f0 = 0u;       // seen by no row
+        const uint8_t* src = smem + C::kSmemLand + kv * C::kLandBytes + tid * 16;
+        const uint8_t* scales = smem + C::kSmemLand + 2 * C::kLandBytes + kv * 128 + row0;
+        uint8_t* dst = smem + (kv ? C::kSmemV : C::kSmemK) + st * C::kTileBytes + dst0;
+        const bool fix = kv == 1 && (key + kTileKeys > hi || key < lo);
+#pragma unroll 2
+        for (int x = 0; x < D / 16; ++x) {  // chunk tid + 128 x: kPagesPer pages further on
+          const uint4 w = *reinterpret_cast<const uint4*>(src + x * 2048);
+          const uint32_t byte = scales[x * kPagesPer * 16];
+          // 2^(120 + e) as a bf16; the exponent field ends at 254, the rest of a
+          // scale above 2^7 is a second factor
+          uint32_t f0 = min(byte + 120u, 254u) << 7;
+          if (byte == 0u) f0 = 0u;
+          if (byte == 255u) f0 = 0x7fc0u;  // NaN
+          if (fix) {
+            const int k = key + row0 + x * kPagesPer * 16;
+            if (k >= hi || k < lo) f0 = 0u;  // a value no row sees
+          }
           f0 |= f0 << 16;
-          f1 |= f1 << 16;
           uint32_t o[8];
           const uint32_t in[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -397,11 +407,16 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
               const uint32_t b = __byte_perm(in[i], 0u, h ? 0x3424 : 0x1404);  // bytes into the high halves
               uint32_t v = (b & 0x80008000u) | ((b & 0x7f007f00u) >> 4);
               asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(f0));
-              if (e1 != 127) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(f1));
               o[2 * i + h] = v;
             }
           }
-          uint8_t* at = dst + page * (32 * D) + (g * (D / 8) + 2 * c) * 128 + r * 16;
+          if (byte > 134u && byte < 255u) {
+            uint32_t f1 = (byte + 120u - 254u + 127u) << 7;
+            f1 |= f1 << 16;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[i]) : "r"(f1));
+          }
+          uint8_t* at = dst + x * kPagesPer * (32 * D);
           *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
           *reinterpret_cast<uint4*>(at + 128) = make_uint4(o[4], o[5], o[6], o[7]);
         }
@@ -419,8 +434,8 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
 // ---------------------------------------------------------------------------
 template <typename T, int D, int MODE>
 __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, uint32_t tmem,
-                             volatile int* abort, volatile int* last_flag, const int32_t* items, int item0,
-                             int item1, int G, int TT) {
+                             volatile int* abort, const int32_t* items, int item0,
+                             int item1, int G, float rG, int TT) {
   using C = Cfg<D, MODE>;
   constexpr bool kTwoPass = MODE == kE4m3;
   const int i = threadIdx.x / 128, wq = (threadIdx.x / 32) & 3, lane = threadIdx.x & 31;
@@ -430,20 +445,25 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
   float2* join = reinterpret_cast<float2*>(smem + C::kSmemJoin);
   uint32_t scount = 0, kitem = 0;
   const int row_tok = row / G, row_g = row % G;
+  // tokens of the warp's first and last row
+  const int warp_tok0 = wq * 32 / G, warp_tok1 = min(wq * 32 + 31, TT * G - 1) / G;
   // a wait ran out of time: the warp does no more work, but goes through the
   // named barriers, which the other warps may be waiting at
   bool dead = false;
   for (int it = item0; it < item1; ++it) {
-    const Item I(items + it * kItemInts, G, TT);
-    const int tok = I.tokb + (I.split ? 0 : i * TT) + row_tok;  // inside the request
+    const Item I(items, it, rG, TT);
+    const int base = I.tokb + (I.split ? 0 : i * TT);  // first token of the tile, inside the request
+    const int tok = base + row_tok;
     const int tok_end = I.tokb + (I.split ? I.ntok : min(I.ntok, (i + 1) * TT));
     const bool valid = row < TT * G && tok < tok_end;
     const int hq = I.head * G + row_g;
     const float sink = a.sinks && valid ? a.sinks[hq] : 0.f;
     const int hi = valid ? I.row_hi(tok) : 0, lo = valid ? I.row_lo(tok) : 0;
-    // keys every valid row of this tile sees
-    const int first_tok = I.tokb + (I.split ? 0 : i * TT);
-    const int hi_all = I.row_hi(first_tok), lo_all = I.row_lo(tok_end - 1);
+    // keys that every row, and that some row, of this warp sees
+    const bool warp_any = wq * 32 < TT * G && base + warp_tok0 < tok_end;
+    const int w0 = base + warp_tok0, w1 = min(base + warp_tok1, tok_end - 1);
+    const int all_hi = warp_any ? I.row_hi(w0) : 0, any_hi = warp_any ? I.row_hi(w1) : 0;
+    const int any_lo = I.row_lo(w0), all_lo = I.row_lo(w1);
     float m_run = -INFINITY, l_run = 0.f;
     const int steps = I.count(i);
     for (int j = 0; j < steps && !dead; ++j) {
@@ -453,76 +473,57 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       }
       ++scount;
       tc_fence_after();
+      if (!warp_any) {  // rows that are not there: whatever S holds may be their P
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars[C::B_PHALF + i]);
+          mbar_arrive(&bars[C::B_PFULL + i]);
+        }
+        continue;
+      }
       const int key = I.key0 + I.tile(i, j) * kTileKeys;
-      const bool edge = key + kTileKeys > hi_all || key < lo_all;
-      // The scores of 32 keys, those the row does not see at -inf: key e is kept by
-      // a minimum with (h - e) * inf, which is +inf below h and -inf above (h half
-      // an integer), and likewise for the window's end -- two multiplications on
-      // the idle FMA pipe and one three-way minimum, where comparing and selecting
-      // costs three operations of the pipe that also takes the row maximum. Two
-      // passes over TMEM where there are no registers for all 128 keys.
+      const bool edge = key + kTileKeys > all_hi || key < all_lo;
+      // In a tile that not every row of the warp sees whole, chunks of 32 keys that
+      // no row sees are skipped and those between are masked: key e is kept by a
+      // minimum with (h - e) * inf, which is +inf below h and -inf above (h half an
+      // integer), and likewise at the window's end -- multiplications on the idle
+      // FMA pipe and one three-way minimum, where comparing and selecting costs
+      // three operations of the pipe that also takes the row maximum.
       const float h = static_cast<float>(hi - key) - 0.5f, l = static_cast<float>(lo - key) - 0.5f;
-      uint32_t s[kTwoPass ? 32 : 128];
+      auto skip = [&](int c) { return key + c * 32 >= any_hi || key + c * 32 + 32 <= any_lo; };
       auto mask = [&](int c, uint32_t* v) {
         const float hc = h - c * 32, lc = c * 32 - l;
-        if (I.window) {
+        if (key + c * 32 < all_lo) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             v[e] = __float_as_uint(fmin3(__uint_as_float(v[e]), (hc - e) * INFINITY, (lc + e) * INFINITY));
-        } else {
+        } else if (key + c * 32 + 32 > all_hi) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             v[e] = __float_as_uint(fminf(__uint_as_float(v[e]), (hc - e) * INFINITY));
         }
       };
-      float mx[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) mx[e] = -INFINITY;
-      if constexpr (!kTwoPass) {
-        tmem_ld128_wait(lane_base + s_col(i), s);
-        if (edge) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) mask(c, s + c * 32);
+      float f = 1.f, neg_m = 0.f;
+      bool early = true;
+      // the row's maximum of this tile (raw) -> reference and rescaling factor
+      auto new_max = [&](float (&mx)[8]) {
+        mx[0] = fmax3(mx[0], mx[1], mx[2]);
+        mx[3] = fmax3(mx[3], mx[4], mx[5]);
+        mx[6] = fmaxf(mx[6], mx[7]);
+        const float m_tile = fmax3(mx[0], mx[3], mx[6]) * sl2;
+        if (j == 0) {
+          m_run = m_tile;
+        } else if (m_tile > m_run + 8.f) {
+          f = fast_exp2(m_run - m_tile);  // 0 while the row has seen no key
+          m_run = m_tile;
         }
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t* v = kTwoPass ? s : s + c * 32;
-        if constexpr (kTwoPass) {
-          tmem_ld32_wait(lane_base + s_col(i) + c * 32, s);
-          if (edge) mask(c, s);
-        }
-#pragma unroll
-        for (int e = 0; e < 32; e += 16) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mx[k] = fmax3(mx[k], __uint_as_float(v[e + k]), __uint_as_float(v[e + 8 + k]));
-        }
-      }
-      mx[0] = fmax3(mx[0], mx[1], mx[2]);
-      mx[3] = fmax3(mx[3], mx[4], mx[5]);
-      mx[6] = fmaxf(mx[6], mx[7]);
-      const float m_tile = fmax3(mx[0], mx[3], mx[6]) * sl2;
-      float f = 1.f;
-      if (j == 0) {
-        m_run = m_tile;
-      } else if (m_tile > m_run + 8.f) {
-        f = fast_exp2(m_run - m_tile);  // 0 while the row has seen no key
-        m_run = m_tile;
-      }
-      const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-      // the first half of P is released early, unless a lane must rescale O first
-      const bool early = __all_sync(0xffffffffu, f == 1.f);
-      const uint64_t sc2 = f2_pack(sl2, sl2), nm2 = f2_pack(neg_m, neg_m);
+        neg_m = m_run == -INFINITY ? 0.f : -m_run;
+        // the first half of P is released early, unless a lane must rescale O first
+        early = __all_sync(0xffffffffu, f == 1.f);
+      };
       uint64_t acc2[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
-        const uint32_t* v = kTwoPass ? s : s + c * 32;
-        if constexpr (kTwoPass) {
-          tmem_ld32_wait(lane_base + s_col(i) + c * 32, s);
-          if (edge) mask(c, s);
-        }
+      auto weights = [&](const uint32_t* v, uint32_t (&pk)[16], uint64_t sc2, uint64_t nm2) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, nm2);
@@ -532,12 +533,70 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
           acc2[e & 3] = f2_add(acc2[e & 3], f2_pack(p0, p1));
           pk[e] = pack2(p0, p1, T());
         }
+      };
+      auto store_p = [&](int c, const uint32_t (&pk)[16]) {
         tmem_st16(lane_base + s_col(i) + c * 16, pk);
         if (c == 1 && early) {
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars[C::B_PHALF + i]);
+        }
+      };
+      auto max32 = [&](const uint32_t* v, float (&mx)[8]) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 16) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mx[k] = fmax3(mx[k], __uint_as_float(v[e + k]), __uint_as_float(v[e + 8 + k]));
+        }
+      };
+      float mx[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx[e] = -INFINITY;
+      if (kTwoPass || (edge && I.window)) {
+        // 32 scores at a time, twice, so that chunks no row sees are skipped (a
+        // window leaves many; 117 us against 137 with the masks below at six chunks
+        // of about 850 tokens, window 128) and no more than 32 are in registers
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          if (edge && skip(c)) continue;
+          uint32_t v[32];
+          tmem_ld32_wait(lane_base + s_col(i) + c * 32, v);
+          if (edge) mask(c, v);
+          max32(v, mx);
+        }
+        new_max(mx);
+        const uint64_t sc2 = f2_pack(sl2, sl2), nm2 = f2_pack(neg_m, neg_m);
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+          if (edge && skip(c)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[e] = 0u;
+          } else {
+            uint32_t v[32];
+            tmem_ld32_wait(lane_base + s_col(i) + c * 32, v);
+            if (edge) mask(c, v);
+            weights(v, pk, sc2, nm2);
+          }
+          store_p(c, pk);
+        }
+      } else if constexpr (!kTwoPass) {
+        uint32_t s[128];
+        tmem_ld128_wait(lane_base + s_col(i), s);
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mask(c, s + c * 32);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) max32(s + c * 32, mx);
+        new_max(mx);
+        const uint64_t sc2 = f2_pack(sl2, sl2), nm2 = f2_pack(neg_m, neg_m);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+          weights(s + c * 32, pk, sc2, nm2);
+          store_p(c, pk);
         }
       }
       if (!early) {
@@ -568,7 +627,16 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
         mbar_arrive(&bars[C::B_PFULL + i]);
       }
     }
-    if (I.tiles > 0) {
+    // while the last products run: the row's factor, and the next item
+    auto factor = [&](float m, float l, float& lse2) {
+      float f = row_factor(m, l, lse2);
+      if (a.sinks) f *= sink_factor(lse2, sink, a.sink_mode);
+      return f;
+    };
+    float lse_own = 0.f, f_row = 0.f;
+    if (valid) f_row = factor(m_run, l_run, lse_own);
+    const Item& cur = I;
+    if (cur.tiles > 0) {
       if (!dead && !warp_wait(&bars[C::B_OFINAL + i], kitem & 1, abort)) dead = true;
       tc_fence_after();
     }
@@ -576,12 +644,12 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
     // ---- a split unit: stream 0 takes over stream 1's state ----
     float f_own = 1.f, f_other = 0.f;  // factors of this stream's O and of stream 1's
     float m = m_run, l = l_run;
-    if (I.split) {
+    if (cur.split) {
       if (i == 1) {
         join[row] = make_float2(m_run, l_run);
         named_sync(3, 256);
         named_sync(3, 256);  // it is read
-        if (I.tiles > 0) ++kitem;
+        if (cur.tiles > 0) ++kitem;
         continue;  // stream 0 reads O1 and frees it
       }
       named_sync(3, 256);
@@ -590,14 +658,14 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       m = fmaxf(m_run, o1.x);
       const float mr = m == -INFINITY ? 0.f : m;
       f_own = fast_exp2(m_run - mr);
-      f_other = I.count(1) > 0 ? fast_exp2(o1.x - mr) : 0.f;
+      f_other = cur.count(1) > 0 ? fast_exp2(o1.x - mr) : 0.f;
       l = l_run * f_own + o1.y * f_other;
     }
-    const bool has_other = I.split && I.count(1) > 0;
+    const bool has_other = cur.split && cur.count(1) > 0;
     // 32 columns of this row's (joined, unnormalised) O
     auto load_o = [&](int c, float (&o)[32]) {
       uint32_t r[32];
-      if (I.tiles == 0) {
+      if (cur.tiles == 0) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = 0.f;
         return;
@@ -612,22 +680,16 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       }
     };
     auto free_o = [&] {
-      if (I.tiles == 0) return;
+      if (cur.tiles == 0) return;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&bars[C::B_OFREE + i]);
-        if (I.split) mbar_arrive(&bars[C::B_OFREE + 1]);
+        if (cur.split) mbar_arrive(&bars[C::B_OFREE + 1]);
       }
       ++kitem;
     };
-    const int64_t gtok = static_cast<int64_t>(I.tok0) + tok;
-    auto factor = [&](float m, float l, float& lse2) {
-      lse2 = l > 0.f ? m + log2f(l) : (l == 0.f ? -INFINITY : l);
-      float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      if (a.sinks) f *= sink_factor(lse2, sink, a.sink_mode);
-      return f;
-    };
+    const int64_t gtok = static_cast<int64_t>(cur.tok0) + tok;
     auto store_o = [&](int c, const float (&o)[32], float f) {
       T* op = static_cast<T*>(a.out) + gtok * a.o_st + hq * a.o_sh + c * 32;
 #pragma unroll
@@ -640,24 +702,20 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
         *reinterpret_cast<uint4*>(op + e * 8) = v;
       }
     };
-    if (I.parts == 1) {
-      float lse2 = 0.f, f = 0.f;
-      if (valid) f = factor(m, l, lse2);
+    if (cur.parts == 1) {
+      if (cur.split && valid) f_row = factor(m, l, lse_own);
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float o[32];
         load_o(c, o);
-        if (valid) store_o(c, o, f);
+        if (valid) store_o(c, o, f_row);
       }
-      if (valid && a.lse) a.lse[gtok * a.lse_st + hq] = lse2;
+      if (valid && a.lse) a.lse[gtok * a.lse_st + hq] = lse_own;
       free_o();
       continue;
     }
-    // ---- a span of a unit: leave the state in its slot; the last span joins ----
-    // slot: [D / 4][128 rows] of four columns, then m and l of the rows
-    constexpr int kSlot = 128 * (D + 2);
-    const int per = 2;  // slots of an item: one for each q tile
-    float* own = a.slots + static_cast<int64_t>(I.slot * per + i) * kSlot;
+    // ---- a span of a unit: leave the state in its slot (join_kernel) ----
+    float* own = a.slots + static_cast<int64_t>(cur.slot * 2 + i) * tile_slot_floats(D);
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       float o[32];
@@ -674,44 +732,6 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       own[128 * D + 128 + row] = l;
     }
     free_o();
-    named_sync(1 + i, 128);
-    if (row == 0)
-      last_flag[i] = atom_add_acq_rel_gpu(&a.tickets[I.ticket * 2 + i], 1u) == static_cast<uint32_t>(I.parts - 1);
-    named_sync(1 + i, 128);
-    const bool last = last_flag[i] != 0;
-    named_sync(1 + i, 128);  // the flag is read before the next item writes it
-    if (!last) continue;
-    if (row == 0) a.tickets[I.ticket * 2 + i] = 0;
-    if (!valid) continue;
-    const float* s0 = a.slots + static_cast<int64_t>(I.first_slot * per + i) * kSlot;
-    const int64_t step = static_cast<int64_t>(per) * kSlot;
-    float M = -INFINITY, L = 0.f;
-    for (int p = 0; p < I.parts; ++p) M = fmaxf(M, __ldcg(s0 + p * step + 128 * D + row));
-    const float Mr = M == -INFINITY ? 0.f : M;
-    for (int p = 0; p < I.parts; ++p)
-      L += __ldcg(s0 + p * step + 128 * D + 128 + row) * fast_exp2(__ldcg(s0 + p * step + 128 * D + row) - Mr);
-    float lse2;
-    const float f = factor(M, L, lse2);
-#pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      float o[32];
-#pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = 0.f;
-#pragma unroll 1
-      for (int p = 0; p < I.parts; ++p) {
-        const float w = fast_exp2(__ldcg(s0 + p * step + 128 * D + row) - Mr);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(s0 + p * step) + (c * 8 + e) * 128 + row);
-          o[4 * e] = fmaf(v.x, w, o[4 * e]);
-          o[4 * e + 1] = fmaf(v.y, w, o[4 * e + 1]);
-          o[4 * e + 2] = fmaf(v.z, w, o[4 * e + 2]);
-          o[4 * e + 3] = fmaf(v.w, w, o[4 * e + 3]);
-        }
-      }
-      store_o(c, o, f);
-    }
-    if (a.lse) a.lse[gtok * a.lse_st + hq] = lse2;
   }
 }
 
@@ -726,7 +746,6 @@ __global__ void __launch_bounds__(Cfg<D, MODE>::kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kSmemBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* last_flag = abort + 1;  // one for each stream
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&bars[C::B_QFULL], 1);
@@ -772,6 +791,7 @@ __global__ void __launch_bounds__(Cfg<D, MODE>::kThreads, 1)
   const int32_t* sec = a.plan + H_SECTION + kSectionInts;
   const int G = a.plan[H_GROUP];
   const int TT = 128 / G;
+  const float rG = 1.f / G;
   const bool spare = static_cast<int>(blockIdx.x) >= sec[S_CTAS];  // of a fixed grid
   const int item0 = spare ? 0 : a.plan[sec[S_OFF_CTA] + blockIdx.x];
   const int item1 = spare ? 0 : a.plan[sec[S_OFF_CTA] + blockIdx.x + 1];
@@ -780,21 +800,21 @@ __global__ void __launch_bounds__(Cfg<D, MODE>::kThreads, 1)
   if (warp >= 8) {
     if constexpr (MODE != kE4m3) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kSideRegs));
     if (warp == kTmaWarp) {
-      producer<D, MODE>(&tm_q, &tm_k, &tm_v, a, smem, bars, abort, items, item0, item1, G, TT, rpb);
+      producer<D, MODE>(&tm_q, &tm_k, &tm_v, a, smem, bars, abort, items, item0, item1, G, rG, TT, rpb);
       __syncwarp();
     } else if (warp == kMmaWarp) {
-      if (elect_one()) mma_issuer<T, D, MODE>(smem, bars, tmem, abort, items, item0, item1, G, TT);
+      if (elect_one()) mma_issuer<T, D, MODE>(smem, bars, tmem, abort, items, item0, item1, rG, TT);
       __syncwarp();
     } else if (warp == kFixWarp && MODE != kE4m3) {
-      fixer<D, MODE>(smem, bars, abort, items, item0, item1, G, TT);
+      fixer<D, MODE>(smem, bars, abort, items, item0, item1, rG, TT);
       __syncwarp();
     } else if (warp >= 12) {
-      if constexpr (MODE == kE4m3) widener<D>(smem, bars, abort, items, item0, item1, G, TT);
+      if constexpr (MODE == kE4m3) widener<D>(smem, bars, abort, items, item0, item1, rG, TT);
       __syncwarp();
     }
   } else {
     if constexpr (MODE != kE4m3) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
-    softmax_role<T, D, MODE>(a, smem, bars, tmem, abort, last_flag, items, item0, item1, G, TT);
+    softmax_role<T, D, MODE>(a, smem, bars, tmem, abort, items, item0, item1, G, rG, TT);
   }
 
   tc_fence_before();

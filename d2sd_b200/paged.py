@@ -30,11 +30,11 @@ class PagedAttentionPlan:
     window: a row sees only the last ``window`` positions up to its own.
 
     The plan owns the workspace of its calls: two calls that overlap on the GPU
-    need a plan each. ``update`` re-plans in place; with ``reserve=(requests,
-    tokens)`` the device buffers have room for that many, and the launch does not
-    depend on the lengths, so a captured ``paged_attention`` replays with the new
-    ones. Both must run where the next call sees them (the same stream, or ordered
-    before it).
+    need a plan each. ``update`` re-plans in place, on the current stream. With
+    ``reserve=(requests, tokens)`` the device buffers have room for that many, the
+    tensors of a call must hold that many tokens, and the launch does not depend on
+    the lengths: a captured ``paged_attention`` replays with the updated ones (of a
+    plan without a reserve it must not be replayed after an update).
     """
 
     def __init__(self, q_lens, kv_lens, num_qo_heads: int, num_kv_heads: int, head_dim: int,
@@ -49,23 +49,22 @@ class PagedAttentionPlan:
         self.causal, self.window = causal, window
         self.num_ctas = ops.num_sms(device)
         self.fixed_grid = reserve is not None
+        self.reserve = reserve
         host, sections, tokens = self._plan(q_lens, kv_lens, page_offsets)
         need = len(host)
         if reserve is not None:
-            # every request adds at most one short tile per kv head
-            rows, G = max(reserve[1], tokens), num_qo_heads // num_kv_heads
-            lens = np.ones(max(reserve[0], 1), dtype=np.int32)
-            lens[0] = rows
-            need = max(need, load().d2sd_paged_plan_capacity(
-                lens.ctypes.data, len(lens), num_qo_heads, num_kv_heads, self.num_ctas)
-                + 16 * num_kv_heads * len(lens) * -(-G // 16))
+            # most units: one long request and the others of one token each
+            lens = np.ones(reserve[0], dtype=np.int32)
+            lens[0] = reserve[1]
+            need = load().d2sd_paged_plan_capacity(lens.ctypes.data, len(lens), num_qo_heads,
+                                                   num_kv_heads, self.num_ctas)
         with torch.cuda.device(device):
             self.plan = torch.zeros(need, dtype=torch.int32, device=device)
             self.device = self.plan.device
             nbytes = load().d2sd_paged_workspace_bytes(self.num_ctas, head_dim)
             if nbytes < 0:
                 raise NotImplementedError("paged attention: head_dim must be 64 or 128")
-            self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
             self.status = torch.zeros(1, dtype=torch.int32, device=device)
             self._set(host, sections, tokens)
             torch.cuda.current_stream(device).synchronize()  # usable on any stream from here
@@ -80,6 +79,8 @@ class PagedAttentionPlan:
             if R > 1:
                 raise ValueError("page_offsets are required for several requests")
             page_offsets = [0] * R
+        if self.reserve is not None and (R > self.reserve[0] or int(q.sum()) > self.reserve[1]):
+            raise ValueError(f"the batch is larger than the plan's reserve {self.reserve}")
         off = np.ascontiguousarray(page_offsets, dtype=np.int32)[:R]
         if len(off) != R:
             raise ValueError("page_offsets must have an entry for each request")
@@ -90,7 +91,7 @@ class PagedAttentionPlan:
             raise ValueError("invalid plan sizes")
         plan = np.empty(cap, dtype=np.int32)
         used = np.zeros(1, dtype=np.int64)
-        sections = np.zeros(12, dtype=np.int32)
+        sections = np.zeros(14, dtype=np.int32)
         check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, R,
                                   self.num_qo_heads, self.num_kv_heads, 1 if self.causal else 0,
                                   self.window or 0, self.num_ctas, plan.ctypes.data, cap,
@@ -98,8 +99,6 @@ class PagedAttentionPlan:
         return plan[:int(used[0])], sections, int(q.sum())
 
     def _set(self, host, sections, tokens):
-        if len(host) > self.plan.numel():
-            raise ValueError("the batch is larger than the plan's reserve")
         self.plan[:len(host)].copy_(torch.from_numpy(host))
         self.host_plan, self.sections, self.tokens = host, sections, tokens
 
@@ -132,8 +131,9 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     Hq, Hk, D = plan.num_qo_heads, plan.num_kv_heads, plan.head_dim
     if dev != plan.device:
         raise ValueError("the plan is for another device")
-    if q.dim() != 3 or q.shape[0] < max(plan.tokens, 1):
-        raise ValueError(f"q must hold the plan's {plan.tokens} tokens")
+    tokens = plan.reserve[1] if plan.reserve else plan.tokens
+    if q.dim() != 3 or q.shape[0] < max(tokens, 1):
+        raise ValueError(f"q must hold the plan's {tokens} tokens")
     pool, heads, dim = ops._pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale)
     if heads != Hk or dim != D:
         raise ValueError("the pools and the plan differ in kv heads or head_dim")
@@ -146,12 +146,12 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("sinks must be a contiguous fp32 tensor [num_qo_heads]")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.shape[0] < plan.tokens:
+    elif out.dtype != q.dtype or out.shape[0] < tokens:
         raise ValueError("out must hold the plan's tokens in q's dtype")
     if lse is None:
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
     elif lse.dtype != torch.float32 or lse.dim() != 2 or lse.stride(1) != 1 \
-            or lse.shape[0] < plan.tokens or lse.shape[1] != Hq:
+            or lse.shape[0] < tokens or lse.shape[1] != Hq:
         raise ValueError("lse must be fp32 [tokens, num_qo_heads] with a contiguous head axis")
     args = (*ops._row_strides("q", q, Hq, D), q.shape[0], ops.dtype_code(q), k_pool.data_ptr(),
             v_pool.data_ptr(), *pool, ops._int32("page_table", page_table), page_table.numel(), Hq,

@@ -603,16 +603,16 @@ int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_requests,
  * only the last `window` of them; not causal: every position), and its pages
  * start at page_table[page_offsets[r]]. num_ctas is the grid (the SM count).
  * plan[0 .. capacity) is written on the HOST (*used entries): copy it to the
- * device. sections [12] is the host's copy of what the launch needs. */
+ * device. sections [14] is the host's copy of what the launch needs. */
 int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
                     const int32_t* page_offsets, int32_t num_requests,
                     int32_t num_qo_heads, int32_t num_kv_heads, int32_t causal,
                     int32_t window, int32_t num_ctas, int32_t* plan,
                     int64_t capacity, int64_t* used, int32_t* sections);
 
-/* Workspace bytes of d2sd_paged_attention for a grid of num_ctas: zeroed once
- * before the first call (each call leaves its counters zero again). Calls that
- * overlap on the GPU need a workspace each. */
+/* Workspace bytes of d2sd_paged_attention for a grid of num_ctas; it holds
+ * nothing from one call to the next. Calls that overlap on the GPU need a
+ * workspace each. */
 int64_t d2sd_paged_workspace_bytes(int32_t num_ctas, int32_t head_dim);
 
 /* Attention of the planned new tokens over the paged cache, which already holds
@@ -625,7 +625,7 @@ int64_t d2sd_paged_workspace_bytes(int32_t num_ctas, int32_t head_dim);
  * ids outside the pool are read as its first or last page. fixed_grid: launch
  * num_ctas CTAs whatever the plan says, so that a captured call stays valid
  * when the plan's device buffer is rewritten. status receives 1 if a wait inside
- * the kernel ran out of time (zero the workspace before using it again). */
+ * the kernel ran out of time. */
 int d2sd_paged_attention(const void* q, int64_t q_stride_token,
                          int64_t q_stride_head, int64_t num_tokens,
                          int32_t dtype, const void* k_pool, const void* v_pool,

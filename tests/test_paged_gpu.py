@@ -147,7 +147,6 @@ def test_attention(cuda_device, i, garbage):
                         sinks=None if sinks is None else sinks.cpu())
     assert (out[n:] == 7).all() and (lse[n:] == 7).all()
     assert int(plan.status) == 0
-    assert not plan.workspace[:4 * 2 * plan.num_ctas].any()  # the counters are zero again
 
 
 @pytest.mark.parametrize("store", ["same", "e4m3"])

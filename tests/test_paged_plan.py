@@ -1,6 +1,6 @@
 """The host-side plan of the paged attention (CPU only): every (row, visible key
-tile) of every request in exactly one item, spans in order, slots and tickets, and
-the balance over the CTAs."""
+tile) of every request in exactly one item, spans in order, the slots and the list
+of rows to join, and the balance over the CTAs."""
 import numpy as np
 import pytest
 
@@ -17,7 +17,7 @@ def make(lib, q, kv, off, Hq, Hk, causal, window, ctas):
     from d2sd_b200._lib import check
     q, kv, off = (np.ascontiguousarray(x, dtype=np.int32) for x in (q, kv, off))
     cap = lib.d2sd_paged_plan_capacity(q.ctypes.data, len(q), Hq, Hk, ctas)
-    plan, used, sec = np.zeros(cap, np.int32), np.zeros(1, np.int64), np.zeros(12, np.int32)
+    plan, used, sec = np.zeros(cap, np.int32), np.zeros(1, np.int64), np.zeros(14, np.int32)
     check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, len(q), Hq, Hk, causal,
                               window, ctas, plan.ctypes.data, cap, used.ctypes.data,
                               sec.ctypes.data), "plan")
@@ -43,32 +43,51 @@ def test_plan_covers_every_tile_once(lib, q, kv, Hq, Hk, causal, window, ctas):
     starts = np.cumsum([0] + list(q))
     seen = {}
     for s in range(2):
-        nct, nit, nslots, ntick, oc, oi = sec[6 * s:6 * s + 6]
-        assert list(plan[5 + 6 * s:11 + 6 * s]) == [nct, nit, nslots, ntick, oc, oi]
+        nct, nit, nslots, njoin, oc, oi, oj = sec[7 * s:7 * s + 7]
+        assert list(plan[5 + 7 * s:12 + 7 * s]) == list(sec[7 * s:7 * s + 7])
         if nit == 0:
             continue
+        q_tile = 16 if s == 0 else 128 // G * G
         cta = plan[oc:oc + nct + 1]
         assert nct <= ctas and cta[0] == 0 and cta[-1] == nit and (np.diff(cta) >= 0).all()
-        assert nslots <= 2 * ctas and ntick <= 2 * ctas and oi % 4 == 0
+        assert nslots <= 2 * ctas and oi % 4 == 0
         items = plan[oi:oi + 16 * nit].reshape(-1, 16)
-        slots, ticket_of = set(), {}
+        slots, split = set(), {}
         for it in items:
-            r, h, tok0, row0, nrows, k0, k1, pos0, win, po, kvl, slot, first, parts, tick, _ = it
+            r, h, tok0, row0, nrows, k0, k1, pos0, win, po, kvl, slot, parts, tokb, *_ = it
             assert tok0 == starts[r] and po == off[r] and kvl == kv[r] and win == window
-            assert nrows > 0 and row0 + nrows <= q[r] * G and k0 % 128 == 0 and k1 <= kv[r]
+            assert 0 < nrows <= (q_tile if s == 0 else 2 * q_tile)
+            assert row0 + nrows <= q[r] * G and k0 % 128 == 0 and k1 <= kv[r]
+            assert tokb == row0 // G and (s == 0 or (row0 % G == 0 and nrows % G == 0))
             unit = seen.setdefault((r, h, row0), [nrows, []])
             unit[1].append((k0, k1))
             if parts == 1:
                 assert slot == -1
             else:
-                assert slot not in slots and first <= slot < first + parts
-                assert slot == first + len(unit[1]) - 1  # spans in slot order
+                first = split.setdefault((r, h, row0), (slot, parts, nrows, tok0))[0]
+                assert slot == first + len(unit[1]) - 1 and slot not in slots  # spans in slot order
                 slots.add(slot)
-                assert ticket_of.setdefault(tick, (r, h, row0)) == (r, h, row0)
-        assert slots == set(range(nslots)) and sorted(ticket_of) == list(range(ntick))
-        # balance: the largest CTA within the mean, one item's cost and the rounding
-        cost = [sum(-(-(i[6] - i[5]) // 128) + 1 for i in items[a:b]) for a, b in zip(cta, cta[1:])]
-        assert max(cost) <= sum(cost) / nct + 5
+        assert slots == set(range(nslots))
+        # join list: every row of every split unit once, with its slot
+        joined = {}
+        for j in plan[oj:oj + 8 * njoin].reshape(-1, 8):
+            slot, step, parts, srow, n, row0, tok0, head = j
+            assert 0 < n <= (16, 64)[s] and step == (1, 2)[s] and srow + n <= q_tile
+            for x in range(n):
+                key = (tok0, head, row0 + x)
+                assert key not in joined
+                joined[key] = (slot, parts, srow + x)
+        want = {}
+        for (r, h, row0), (first, parts, nrows, tok0) in split.items():
+            for x in range(nrows):
+                tile, rest = divmod(x, q_tile)
+                want[tok0, h, row0 + x] = (first * (1, 2)[s] + tile, parts, rest)
+        assert joined == want
+        # balance: the largest CTA within the mean and two items' fixed costs
+        extra = 1 if s == 0 else 4
+        cost = [sum((-(-(i[6] - i[5]) // 128) + extra) * (2 if s == 1 and i[4] > q_tile else 1)
+                    for i in items[a:b]) for a, b in zip(cta, cta[1:])]
+        assert max(cost) <= sum(cost) / nct + 2 * (extra + 2) * 2
     for r in range(len(q)):
         rows = q[r] * G
         for h in range(Hk):
@@ -104,7 +123,7 @@ def test_plan_refusals(lib):
         make(lib, [1], [1], [0], 129, 1, 1, 0, 8)
     import ctypes
     n = np.ones(1, np.int32)
-    buf, used, sec = np.zeros(4, np.int32), np.zeros(1, np.int64), np.zeros(12, np.int32)
+    buf, used, sec = np.zeros(4, np.int32), np.zeros(1, np.int64), np.zeros(14, np.int32)
     rc = lib.d2sd_paged_plan(n.ctypes.data, n.ctypes.data, ctypes.c_void_p(np.zeros(1, np.int32).ctypes.data),
                              1, 4, 2, 1, 0, 8, buf.ctypes.data, 4, used.ctypes.data, sec.ctypes.data)
     assert rc == 3 and "small" in lib.d2sd_last_error().decode()
@@ -114,9 +133,9 @@ def test_plan_refusals(lib):
 
 def test_empty_batches(lib):
     plan, sec = make(lib, [], [], [], 4, 2, 1, 0, 8)
-    assert sec[1] == 0 and sec[7] == 0
+    assert sec[1] == 0 and sec[8] == 0
     plan, sec = make(lib, [0, 0], [7, 0], [0, 1], 4, 2, 1, 0, 8)
-    assert sec[1] == 0 and sec[7] == 0
+    assert sec[1] == 0 and sec[8] == 0
 
 
 def test_e4m3_oracle_against_the_type():
