@@ -110,6 +110,8 @@ class D2SDError(RuntimeError):
 def load() -> ctypes.CDLL:
     """Load ``libd2sd.so`` (once). Raises if it has not been built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not LIB_PATH.exists():

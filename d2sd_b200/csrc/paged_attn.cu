@@ -446,14 +446,14 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
 // Joins the spans of split units: an entry of the join list is RB rows (or fewer)
 // whose partial states lie `step` slots apart,
 //   M = max m_p, L = sum l_p 2^(m_p - M), o = sum o_p 2^(m_p - M) / L,
-// in slot order. A thread takes a row and every (256 / RB)-th group of 4 columns.
+// in slot order. A thread takes four columns of a row, and few rows go to a block,
+// so that a unit of many spans is spread over the SMs and many loads are in flight.
 template <typename T, int D, int SECTION>
-__global__ void __launch_bounds__(256) join_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kJoinRows[SECTION] * D / 4) join_kernel(const AttnArgs a) {
   constexpr int RB = kJoinRows[SECTION];
   constexpr int kSlotRows = SECTION == 0 ? kRowsTile : 128;
-  constexpr int kGroups = 256 / RB, kCols = D / 4 / kGroups;
   constexpr int64_t kSlot = SECTION == 0 ? rows_slot_floats(D) : tile_slot_floats(D);
-  const int r = threadIdx.x % RB, group = threadIdx.x / RB;
+  const int r = threadIdx.x % RB, col = threadIdx.x / RB;
   grid_dep_wait();
   const int32_t* sec = a.plan + H_SECTION + SECTION * kSectionInts;
   const int G = a.plan[H_GROUP], n = sec[S_JOINS];
@@ -469,44 +469,36 @@ __global__ void __launch_bounds__(256) join_kernel(const AttnArgs a) {
 #pragma unroll 8
     for (int p = 0; p < parts; ++p) M = fmaxf(M, s0[p * step + kSlotRows * D + at]);
     const float ref = M == -INFINITY ? 0.f : M;
-    float4 acc[kCols];
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
     for (int p = 0; p < parts; ++p) {
       const float* sp = s0 + p * step;
+      const float4 v = reinterpret_cast<const float4*>(sp)[col * kSlotRows + at];
       const float w = fast_exp2(sp[kSlotRows * D + at] - ref);
       L = fmaf(sp[kSlotRows * D + kSlotRows + at], w, L);
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        const float4 v = reinterpret_cast<const float4*>(sp)[(c * kGroups + group) * kSlotRows + at];
-        acc[c].x = fmaf(v.x, w, acc[c].x);
-        acc[c].y = fmaf(v.y, w, acc[c].y);
-        acc[c].z = fmaf(v.z, w, acc[c].z);
-        acc[c].w = fmaf(v.w, w, acc[c].w);
-      }
+      acc.x = fmaf(v.x, w, acc.x);
+      acc.y = fmaf(v.y, w, acc.y);
+      acc.z = fmaf(v.z, w, acc.z);
+      acc.w = fmaf(v.w, w, acc.w);
     }
     const int64_t tok = J[J_TOK0] + static_cast<int64_t>(rq / G);
     const int hq = J[J_HEAD] * G + rq % G;
     float lse2;
     float f = row_factor(M, L, lse2);
     if (a.sinks) f *= sink_factor(lse2, a.sinks[hq], a.sink_mode);
-    T* op = static_cast<T*>(a.out) + tok * a.o_st + hq * a.o_sh;
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      uint2 v;
-      v.x = pack2(acc[c].x * f, acc[c].y * f, T());
-      v.y = pack2(acc[c].z * f, acc[c].w * f, T());
-      *reinterpret_cast<uint2*>(op + (c * kGroups + group) * 4) = v;
-    }
-    if (a.lse && group == 0) a.lse[tok * a.lse_st + hq] = lse2;
+    uint2 v;
+    v.x = pack2(acc.x * f, acc.y * f, T());
+    v.y = pack2(acc.z * f, acc.w * f, T());
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + tok * a.o_st + hq * a.o_sh + col * 4) = v;
+    if (a.lse && col == 0) a.lse[tok * a.lse_st + hq] = lse2;
   }
 }
 
 template <int SECTION>
 int run_join(const AttnArgs& a, int32_t dtype, int32_t head_dim, int entries, int num_ctas, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(entries < 8 * num_ctas ? entries : 8 * num_ctas));
-  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(256), 0, st, "join_kernel", a); };
+  const dim3 grid(static_cast<unsigned>(entries < 16 * num_ctas ? entries : 16 * num_ctas));
+  const dim3 block(static_cast<unsigned>(kJoinRows[SECTION] * head_dim / 4));
+  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, st, "join_kernel", a); };
   if (dtype == D2SD_DTYPE_BF16)
     return head_dim == 128 ? go(join_kernel<__nv_bfloat16, 128, SECTION>) : go(join_kernel<__nv_bfloat16, 64, SECTION>);
   return head_dim == 128 ? go(join_kernel<__half, 128, SECTION>) : go(join_kernel<__half, 64, SECTION>);
@@ -626,10 +618,10 @@ extern "C" int d2sd_paged_attention(
     if (rc) return rc;
   }
   if (sections[S_JOINS] > 0 || fixed_grid) {
-    rc = run_join<0>(a, dtype, head_dim, fixed_grid ? num_ctas : sections[S_JOINS], num_ctas, st);
+    rc = run_join<0>(a, dtype, head_dim, fixed_grid ? 4 * num_ctas : sections[S_JOINS], num_ctas, st);
     if (rc) return rc;
   }
   if (tiles[S_JOINS] > 0 || fixed_grid)
-    rc = run_join<1>(t, dtype, head_dim, fixed_grid ? 2 * num_ctas : tiles[S_JOINS], num_ctas, st);
+    rc = run_join<1>(t, dtype, head_dim, fixed_grid ? 8 * num_ctas : tiles[S_JOINS], num_ctas, st);
   return rc;
 }

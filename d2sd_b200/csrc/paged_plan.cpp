@@ -109,7 +109,7 @@ extern "C" int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_r
   }
   // every CTA adds at most one cut; a cut unit has at most 256 rows to join
   return kHeaderInts + (units + 2 * static_cast<int64_t>(num_ctas)) * kItemInts + 4 * (num_ctas + 2) +
-         static_cast<int64_t>(num_ctas) * 8 * kJoinInts;
+         static_cast<int64_t>(num_ctas) * (256 / 8) * kJoinInts;
 }
 
 extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,

@@ -6,7 +6,7 @@
 // tiles; an item is one span. A unit of one item is written out directly; the
 // items of a split unit leave partial states in consecutive slots, which a second
 // kernel joins in slot order (kept apart so that all SMs join, and no state stays
-// behind in the workspace), 16 or 64 rows to an entry of the join list.
+// behind in the workspace), 4 or 8 rows to an entry of the join list.
 #pragma once
 
 #include <stdint.h>
@@ -58,7 +58,7 @@ enum {
   J_HEAD,
   kJoinInts
 };
-constexpr int kJoinRows[kSections] = {16, 64};
+constexpr int kJoinRows[kSections] = {4, 8};
 
 // A slot holds [head_dim / 4][rows] of four columns each, then the rows' m and l.
 // A CTA's first and last item can be spans of split units, so 2 slots per CTA do

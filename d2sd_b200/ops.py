@@ -482,7 +482,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
 # ---------------------------------------------------------------------------
 # The target's own tokens and the paged cache: write, read back
 # ---------------------------------------------------------------------------
+# These calls are made for every layer of every step, single tokens included, so
+# the checks below read each tensor's shape and strides once and build nothing.
 _E4M3 = torch.float8_e4m3fn
+
+
+def _same_device(dev: int, *ts) -> None:
+    """Every tensor (or None) on CUDA device dev."""
+    if dev < 0:
+        raise ValueError("d2sd kernels take CUDA tensors (there is no CPU path)")
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("all tensors must be on the same CUDA device")
 
 
 def _int32(name: str, t: torch.Tensor, n: int | None = None) -> int:
@@ -495,43 +506,58 @@ def _int32(name: str, t: torch.Tensor, n: int | None = None) -> int:
 def _pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale):
     """The C arguments (strides, page size, pages, format, scales) of a K and V
     pool, and its (heads, head_dim)."""
-    if not kv_layout.startswith("paged_"):
-        raise ValueError(f"a paged layout is needed, not {kv_layout!r}")
-    kv = kv_view(k_pool, kv_layout)
-    if v_pool.shape != k_pool.shape or v_pool.stride() != k_pool.stride() \
-            or v_pool.dtype != k_pool.dtype:
+    shape, st = k_pool.shape, k_pool.stride()
+    if len(shape) != 4 or st[3] != 1:
+        raise ValueError("pools are 4-D with a contiguous head dimension")
+    if v_pool.shape != shape or v_pool.stride() != st or v_pool.dtype != k_pool.dtype:
         raise ValueError("k and v pools must share shape, strides and dtype")
-    sp = sh = 0
+    if kv_layout == "paged_umma":
+        pages, heads, page, dim = shape
+        slot, head, fmt = dim, st[1], _lib.KV_UMMA_PAGES
+        if page != 16 or st[2] != dim or head != 16 * dim:
+            raise ValueError("paged_umma pools are contiguous [pages, Hk, 16, D] blocks")
+    elif kv_layout == "paged_hnd":
+        pages, heads, page, dim = shape
+        slot, head, fmt = st[2], st[1], _lib.KV_ROWS
+    elif kv_layout == "paged_nhd":
+        pages, page, heads, dim = shape
+        slot, head, fmt = st[1], st[2], _lib.KV_ROWS
+    else:
+        raise ValueError(f"a paged layout is needed, not {kv_layout!r}")
     if k_pool.dtype == _E4M3:
         if k_scale is None or v_scale is None:
             raise ValueError("an e4m3 pool needs k_scale and v_scale")
-        if kv_layout != "paged_umma":
+        if fmt != _lib.KV_UMMA_PAGES:
             raise NotImplementedError("8-bit rows are kept in the paged_umma layout")
+        ss = k_scale.stride()
         for s in (k_scale, v_scale):
-            if s.dtype != torch.uint8 or s.shape != k_pool.shape[:3] or s.stride(-1) != 1 \
-                    or s.stride() != k_scale.stride():
+            if s.dtype != torch.uint8 or s.shape != shape[:3] or s.stride() != ss or ss[2] != 1:
                 raise ValueError("scales must be uint8 [pages, Hk, 16], slots contiguous")
-        sp, sh = k_scale.stride(0), k_scale.stride(1)
-    elif k_scale is not None or v_scale is not None:
+        return (st[0], slot, head, page, pages, fmt, k_scale.data_ptr(), v_scale.data_ptr(), ss[0],
+                ss[1]), heads, dim
+    if k_scale is not None or v_scale is not None:
         raise ValueError("only e4m3 pools have scales")
-    args = (kv.stride_page, kv.stride_slot, kv.stride_head, kv.page_size, kv.num_pages,
-            _lib.KV_UMMA_PAGES if kv.native else _lib.KV_ROWS, _ptr(k_scale), _ptr(v_scale), sp, sh)
-    return args, kv.num_kv_heads, kv.head_dim
+    return (st[0], slot, head, page, pages, fmt, None, None, 0, 0), heads, dim
 
 
-def _row_strides(name: str, t: torch.Tensor, heads: int, dim: int):
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.stride(2) != 1:
-        raise ValueError(f"{name} must be [tokens, {heads}, {dim}] with a contiguous head_dim")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+def _rows(name: str, t: torch.Tensor, tokens: int, heads: int, dim: int, dtype):
+    """(pointer, token stride, head stride) of a [tokens, heads, dim] view."""
+    st = t.stride()
+    if t.shape != (tokens, heads, dim) or st[2] != 1 or t.dtype != dtype:
+        raise ValueError(f"{name} must be [{tokens}, {heads}, {dim}] of {dtype} with a contiguous "
+                         "head_dim")
+    return t.data_ptr(), st[0], st[1]
 
 
-def _call(dev: torch.device, fn, args, what: str) -> None:
-    """Run a C entry point on dev's current stream, whatever the current device."""
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
-        return
-    with torch.cuda.device(dev):
-        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
+def _call(dev: int, fn, args, what: str) -> None:
+    """Run a C entry point on the device's current stream, whatever the current device."""
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, what)
 
 
 def append_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -556,38 +582,40 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     ``interleaved``, (2i, 2i + 1) (``rope_tables`` makes them). Both in fp32,
     rounded once. Returns q_out (default: q, in place). A token with a bad position
     or page is skipped and ``status`` (int32, optional) says why."""
-    dev = _require_cuda(k, v, k_pool, v_pool, page_table, page_bounds, token_start, first_pos,
-                        k_scale, v_scale, q, q_out, q_weight, k_weight, cos, sin, status)
+    dev = k.get_device()
+    _same_device(dev, v, k_pool, v_pool, page_table, page_bounds, token_start, first_pos, k_scale,
+                 v_scale, q, q_out, q_weight, k_weight, cos, sin, status)
     pool, Hk, D = _pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale)
-    n = k.shape[0]
-    if v.shape[0] != n or v.dtype != k.dtype:
-        raise ValueError("k and v must have the same tokens and dtype")
-    if k_pool.dtype not in (k.dtype, _E4M3):
-        raise ValueError(f"a {k_pool.dtype} cache does not take {k.dtype} rows")
+    n, dtype = k.shape[0], k.dtype
+    if k_pool.dtype != dtype and k_pool.dtype != _E4M3:
+        raise ValueError(f"a {k_pool.dtype} cache does not take {dtype} rows")
     R = first_pos.numel()
-    q_args, o_args, Hq = (None, 0, 0), (None, 0, 0), 0
+    q_args = o_args = (None, 0, 0)
+    Hq = 0
     if q is not None:
-        q_out = q if q_out is None else q_out
         Hq = q.shape[1]
-        if q.shape[0] != n or q.dtype != k.dtype or q_out.dtype != k.dtype or q_out.shape != q.shape:
-            raise ValueError("q and q_out must match k's tokens and dtype")
-        q_args, o_args = _row_strides("q", q, Hq, D), _row_strides("q_out", q_out, Hq, D)
+        q_args = o_args = _rows("q", q, n, Hq, D, dtype)
+        if q_out is None:
+            q_out = q
+        else:
+            o_args = _rows("q_out", q_out, n, Hq, D, dtype)
+        if (q_weight is None) != (k_weight is None):
+            raise ValueError("q_weight and k_weight go together")
     for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != k.dtype or w.shape != (D,) or not w.is_contiguous()):
+        if w is not None and (w.dtype != dtype or w.shape != (D,) or not w.is_contiguous()):
             raise ValueError("norm weights must be contiguous [head_dim] in the data dtype")
-    if q is not None and (q_weight is None) != (k_weight is None):
-        raise ValueError("q_weight and k_weight go together")
     rot = rows = stride = 0
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if cos is not None:
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape \
-                or cos.dim() != 2 or cos.stride() != sin.stride() or cos.stride(1) != 1:
+        shape, st = cos.shape, cos.stride()
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or sin.shape != shape \
+                or len(shape) != 2 or sin.stride() != st or st[1] != 1:
             raise ValueError("cos and sin must be fp32 [positions, rotary_dim / 2] with the same "
                              "strides, columns contiguous")
-        rows, rot, stride = cos.shape[0], 2 * cos.shape[1], cos.stride(0)
-    args = (*q_args, *o_args, Hq, *_row_strides("k", k, Hk, D), *_row_strides("v", v, Hk, D), Hk, n,
-            D, dtype_code(k), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
+        rows, rot, stride = shape[0], 2 * shape[1], st[0]
+    args = (*q_args, *o_args, Hq, *_rows("k", k, n, Hk, D, dtype), *_rows("v", v, n, Hk, D, dtype),
+            Hk, n, D, dtype_code(k), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
             stride, rows, rot, 1 if interleaved else 0, _int32("token_start", token_start, R + 1),
             _int32("first_pos", first_pos), R, k_pool.data_ptr(), v_pool.data_ptr(), *pool,
             _int32("page_table", page_table), _int32("page_bounds", page_bounds, R + 1),
@@ -604,18 +632,17 @@ def read_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, kv_layout: str, page_tab
     [tokens, Hk, D] rows token_start[r] .. from request r's positions first_pos[r]
     on. An e4m3 cache is read into bf16 (exact) or fp16 rows, any other into rows
     of its own type. Rows behind the last request stay as they are."""
-    dev = _require_cuda(k_pool, v_pool, page_table, page_bounds, token_start, first_pos, k_out,
-                        v_out, k_scale, v_scale, status)
+    dev = k_pool.get_device()
+    _same_device(dev, v_pool, page_table, page_bounds, token_start, first_pos, k_out, v_out, k_scale,
+                 v_scale, status)
     pool, Hk, D = _pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale)
-    n, R = k_out.shape[0], first_pos.numel()
-    if v_out.shape[0] != n or v_out.dtype != k_out.dtype:
-        raise ValueError("k_out and v_out must have the same rows and dtype")
-    if k_pool.dtype not in (k_out.dtype, _E4M3):
-        raise ValueError(f"a {k_pool.dtype} cache is not read into {k_out.dtype} rows")
+    n, R, dtype = k_out.shape[0], first_pos.numel(), k_out.dtype
+    if k_pool.dtype != dtype and k_pool.dtype != _E4M3:
+        raise ValueError(f"a {k_pool.dtype} cache is not read into {dtype} rows")
     args = (k_pool.data_ptr(), v_pool.data_ptr(), *pool, _int32("page_table", page_table),
             _int32("page_bounds", page_bounds, R + 1), _int32("token_start", token_start, R + 1),
             _int32("first_pos", first_pos), R, n, Hk, D, dtype_code(k_out),
-            *_row_strides("k_out", k_out, Hk, D), *_row_strides("v_out", v_out, Hk, D),
+            *_rows("k_out", k_out, n, Hk, D, dtype), *_rows("v_out", v_out, n, Hk, D, dtype),
             _ptr(status))
     _call(dev, load().d2sd_read_kv, args, "d2sd_read_kv")
 
@@ -629,7 +656,8 @@ def commit_kv_e4m3(layer_ptrs: torch.Tensor, *, num_layers: int, num_requests: i
     """``commit_kv_batch`` into an 8-bit cache (d2sd_commit_kv_e4m3). layer_ptrs:
     int64 device tensor [L*6] of {new_k, new_v, cache_k, cache_v, k_scale, v_scale}
     pointers; cache and scale strides are (page, head)."""
-    dev = _require_cuda(layer_ptrs, page_table, page_bounds, accept_results, cache_lens, status)
+    dev = layer_ptrs.get_device()
+    _same_device(dev, page_table, page_bounds, accept_results, cache_lens, status)
     args = (layer_ptrs.data_ptr(), num_layers, num_requests, num_kv_heads, head_dim,
             _DTYPES.get(dtype, -1), block_len, *new_strides, *cache_strides, num_pages,
             *scale_strides, _int32("page_table", page_table),

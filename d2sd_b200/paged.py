@@ -101,6 +101,10 @@ class PagedAttentionPlan:
     def _set(self, host, sections, tokens):
         self.plan[:len(host)].copy_(torch.from_numpy(host))
         self.host_plan, self.sections, self.tokens = host, sections, tokens
+        # what every call passes on
+        self._args = (self.plan.data_ptr(), sections.ctypes.data, self.num_ctas,
+                      1 if self.fixed_grid else 0, self.workspace.data_ptr(),
+                      self.workspace.numel())
 
     def update(self, q_lens, kv_lens, page_offsets=None) -> None:
         """Plan another batch into the same device buffers, on the current stream."""
@@ -127,39 +131,44 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     row that sees no key has out 0 and lse -inf. Cache slots past a request's last
     position may hold anything. A NaN or an infinity in the value of a position that
     some row of a tile sees may reach rows of that tile that do not see it."""
-    dev = ops._require_cuda(q, k_pool, v_pool, page_table, k_scale, v_scale, sinks, out, lse)
+    dev = q.get_device()
+    ops._same_device(dev, plan.status, k_pool, v_pool, page_table, k_scale, v_scale, sinks, out, lse)
     Hq, Hk, D = plan.num_qo_heads, plan.num_kv_heads, plan.head_dim
-    if dev != plan.device:
-        raise ValueError("the plan is for another device")
+    dtype, n = q.dtype, q.shape[0]
     tokens = plan.reserve[1] if plan.reserve else plan.tokens
-    if q.dim() != 3 or q.shape[0] < max(tokens, 1):
+    if n < tokens or n < 1:
         raise ValueError(f"q must hold the plan's {tokens} tokens")
     pool, heads, dim = ops._pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale)
     if heads != Hk or dim != D:
         raise ValueError("the pools and the plan differ in kv heads or head_dim")
-    if k_pool.dtype != q.dtype and not (k_pool.dtype == torch.float8_e4m3fn):
-        raise ValueError(f"a {k_pool.dtype} cache does not take {q.dtype} queries")
-    if q.dtype == torch.float32:
+    if k_pool.dtype != dtype and k_pool.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"a {k_pool.dtype} cache does not take {dtype} queries")
+    if dtype == torch.float32:
         raise NotImplementedError("paged attention takes bf16 or fp16 queries")
     if sinks is not None and (sinks.dtype != torch.float32 or not sinks.is_contiguous()
                               or sinks.numel() != Hq):
         raise ValueError("sinks must be a contiguous fp32 tensor [num_qo_heads]")
+    q_args = ops._rows("q", q, n, Hq, D, dtype)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.shape[0] < tokens:
-        raise ValueError("out must hold the plan's tokens in q's dtype")
+        out = torch.empty((n, Hq, D), dtype=dtype, device=plan.device)
+        o_args = (out.data_ptr(), Hq * D, D)
+    else:
+        if out.shape[0] < tokens:
+            raise ValueError(f"out must hold the plan's {tokens} tokens")
+        o_args = ops._rows("out", out, out.shape[0], Hq, D, dtype)
     if lse is None:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
-    elif lse.dtype != torch.float32 or lse.dim() != 2 or lse.stride(1) != 1 \
-            or lse.shape[0] < tokens or lse.shape[1] != Hq:
-        raise ValueError("lse must be fp32 [tokens, num_qo_heads] with a contiguous head axis")
-    args = (*ops._row_strides("q", q, Hq, D), q.shape[0], ops.dtype_code(q), k_pool.data_ptr(),
-            v_pool.data_ptr(), *pool, ops._int32("page_table", page_table), page_table.numel(), Hq,
-            Hk, D, D ** -0.5 if sm_scale is None else float(sm_scale), plan.plan.data_ptr(),
-            plan.sections.ctypes.data, plan.num_ctas, 1 if plan.fixed_grid else 0,
-            plan.workspace.data_ptr(), plan.workspace.numel(), ops._ptr(sinks),
-            _SINKS[sink_mode] if sinks is not None else 0, *ops._row_strides("out", out, Hq, D),
-            lse.data_ptr(), lse.stride(0), plan.status.data_ptr())
+        lse = torch.empty((n, Hq), dtype=torch.float32, device=plan.device)
+        l_stride = Hq
+    else:
+        l_stride = lse.stride(0)
+        if lse.dtype != torch.float32 or lse.dim() != 2 or lse.stride(1) != 1 \
+                or lse.shape[0] < tokens or lse.shape[1] != Hq:
+            raise ValueError("lse must be fp32 [tokens, num_qo_heads] with a contiguous head axis")
+    args = (*q_args, n, ops.dtype_code(q), k_pool.data_ptr(), v_pool.data_ptr(), *pool,
+            ops._int32("page_table", page_table), page_table.numel(), Hq, Hk, D,
+            D ** -0.5 if sm_scale is None else float(sm_scale), *plan._args, ops._ptr(sinks),
+            _SINKS[sink_mode] if sinks is not None else 0, *o_args, lse.data_ptr(), l_stride,
+            plan.status.data_ptr())
     ops._call(dev, load().d2sd_paged_attention, args, "d2sd_paged_attention")
     return out, lse
 

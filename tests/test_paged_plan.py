@@ -72,7 +72,7 @@ def test_plan_covers_every_tile_once(lib, q, kv, Hq, Hk, causal, window, ctas):
         joined = {}
         for j in plan[oj:oj + 8 * njoin].reshape(-1, 8):
             slot, step, parts, srow, n, row0, tok0, head = j
-            assert 0 < n <= (16, 64)[s] and step == (1, 2)[s] and srow + n <= q_tile
+            assert 0 < n <= (4, 8)[s] and step == (1, 2)[s] and srow + n <= q_tile
             for x in range(n):
                 key = (tok0, head, row0 + x)
                 assert key not in joined
