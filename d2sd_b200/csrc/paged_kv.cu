@@ -15,7 +15,12 @@
 //
 // head_dim / 8 lanes hold one (token, head) row, 8 elements each: the norm's sum
 // and the row's largest magnitude are shuffles inside that group, and the rotary
-// partner is either in the lane (interleaved) or rotary/16 lanes away.
+// partner is either in the lane (interleaved) or rotary/16 lanes away. A group
+// stays with one token and takes its heads in turn, four rows' loads in flight:
+// the chain of dependent loads that finds a token's page (request, position, page
+// table) and its cos and sin are paid once for all its heads, and a warp's
+// neighbouring tokens fill whole 32-byte sectors of the pages, whose rows of eight
+// values lie 16 bytes apart. Few tokens spread their heads over several blocks.
 #include <string>
 
 #include "paged.cuh"
@@ -111,124 +116,171 @@ struct AppendArgs {
   int32_t R, Hq, Hk, half, interleaved;  // half: rotary_dim / 2, 0 without rotation
 };
 
-// A CTA takes one token at a time; its groups take the token's q, k and v heads
-// in turn, so the position, the page and the lane's cos and sin are found once.
+// What a group knows of its token.
+struct Place {
+  int64_t pos, page;
+  int slot, err;  // err < 0: the token belongs to no request
+};
+
+// The places of a warp's tokens: lane group t % (32 / W) has token t. Every lane of
+// the warp calls it.
+template <int W>
+__device__ __forceinline__ Place find_place(int64_t t, int64_t tokens, const int32_t* token_start,
+                                            const int32_t* first_pos, int R, const int32_t* page_table,
+                                            const int32_t* page_bounds, const PageGeom& g) {
+  int r = R;
+#pragma unroll
+  for (int k = 0; k < 32 / W; ++k) {
+    const int64_t tk = __shfl_sync(0xffffffffu, t, k * W);
+    const int rk = find_request(token_start, R, tk);
+    if ((threadIdx.x & 31) / W == k) r = rk;
+  }
+  Place p{0, 0, 0, -1};
+  if (t >= tokens || r >= R) return p;
+  const int64_t start = token_start[r];
+  if (t < start) return p;
+  const int64_t lo = page_bounds[r], n = page_bounds[r + 1] - lo;
+  p.pos = static_cast<int64_t>(first_pos[r]) + (t - start);
+  p.err = kStatusPosition;
+  if (p.pos < 0 || p.pos / g.page_size >= n) return p;
+  p.page = page_table[lo + p.pos / g.page_size];
+  p.slot = static_cast<int>(p.pos % g.page_size);
+  p.err = p.page < 0 || p.page >= g.num_pages ? kStatusPage : 0;
+  return p;
+}
+
 template <typename T, int D, bool Q8>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a, const int rows_per_block) {
   constexpr int W = D / 8;               // lanes of a row
-  constexpr int kGroups = kThreads / W;  // rows a CTA holds at once
-  const int group = threadIdx.x / W, part = threadIdx.x % W;
+  constexpr int kGroups = kThreads / W;  // tokens of a block
+  const int part = threadIdx.x % W;
+  const int64_t t = blockIdx.x * static_cast<int64_t>(kGroups) + threadIdx.x / W;
+  const int rows = a.Hq + 2 * a.Hk;
+  const int row0 = blockIdx.y * rows_per_block, row1 = min(rows, row0 + rows_per_block);
   grid_dep_wait();
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    const int r = find_request(a.token_start, a.R, t);
-    if (r >= a.R || t < a.token_start[r]) continue;  // behind the last sequence
-    const int64_t pos = static_cast<int64_t>(a.first_pos[r]) + (t - a.token_start[r]);
-    const int64_t lo = a.page_bounds[r], n = a.page_bounds[r + 1] - lo;
-    int err = 0;
-    int64_t page = 0;
-    int slot = 0;
-    if (pos < 0 || pos / a.g.page_size >= n) {
-      err = kStatusPosition;
+  Place p = find_place<W>(t, a.tokens, a.token_start, a.first_pos, a.R, a.page_table, a.page_bounds, a.g);
+  if (p.err == 0 && a.half && p.pos >= a.table_rows) p.err = kStatusTable;
+  if (p.err > 0 && part == 0 && row0 == 0) report(a.status, p.err);
+  const bool ok = p.err == 0;  // else the token's rows are not written at all
+  if (!__any_sync(0xffffffffu, ok)) return;
+  // where row `row` of this token is read
+  auto source = [&](int row) {
+    const bool is_q = row < a.Hq, is_k = !is_q && row < a.Hq + a.Hk;
+    const int head = is_q ? row : (is_k ? row - a.Hq : row - a.Hq - a.Hk);
+    return static_cast<const T*>(is_q ? a.q : (is_k ? a.k : a.v)) + t * (is_q ? a.q_st : (is_k ? a.k_st : a.v_st)) +
+           head * (is_q ? a.q_sh : (is_k ? a.k_sh : a.v_sh)) + part * 8;
+  };
+  constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // rows in flight
+  Vec8<T> in[kAhead];
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (ok && r0 + u < row1) in[u].load(source(r0 + u));
+  };
+  fetch(row0);
+  // this lane's cos and sin: columns of its 8 elements' pairs
+  float c[8], s[8];
+  const int rot_lanes = a.half / 4;  // lanes that hold rotated elements
+  const bool rotated = part < rot_lanes, first = part < rot_lanes / 2;
+  const int lane = threadIdx.x & 31;
+  const int from = rotated ? (first ? lane + rot_lanes / 2 : lane - rot_lanes / 2) : lane;
+  if (rotated && ok && row0 < a.Hq + a.Hk) {
+    const float* cr = a.cos + p.pos * a.table_stride;
+    const float* sr = a.sin + p.pos * a.table_stride;
+    if (a.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[2 * i] = c[2 * i + 1] = __ldg(cr + part * 4 + i);
+        s[2 * i + 1] = __ldg(sr + part * 4 + i);
+        s[2 * i] = -s[2 * i + 1];
+      }
     } else {
-      page = a.page_table[lo + pos / a.g.page_size];
-      slot = static_cast<int>(pos % a.g.page_size);
-      if (page < 0 || page >= a.g.num_pages) err = kStatusPage;
-      else if (a.half && pos >= a.table_rows) err = kStatusTable;
-    }
-    if (err) {  // the token's rows are not written at all
-      if (threadIdx.x == 0) report(a.status, err);
-      continue;
-    }
-    // this lane's cos and sin: columns of its 8 elements' pairs
-    float c[8], s[8];
-    const int rot_lanes = a.half / 4;  // lanes that hold rotated elements
-    const bool rotated = part < rot_lanes;
-    if (rotated) {
-      const float* cr = a.cos + pos * a.table_stride;
-      const float* sr = a.sin + pos * a.table_stride;
-      if (a.interleaved) {
+      const int col = part * 8 - (first ? 0 : a.half);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          c[2 * i] = c[2 * i + 1] = __ldg(cr + part * 4 + i);
-          s[2 * i] = s[2 * i + 1] = __ldg(sr + part * 4 + i);
-        }
-      } else {
-        const int col = part * 8 - (part >= rot_lanes / 2 ? a.half : 0);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          c[i] = __ldg(cr + col + i);
-          s[i] = __ldg(sr + col + i);
-        }
+      for (int i = 0; i < 8; ++i) {
+        c[i] = __ldg(cr + col + i);
+        s[i] = __ldg(sr + col + i);
+        if (first) s[i] = -s[i];
       }
     }
-    const int rows = a.Hq + 2 * a.Hk;
-    for (int r0 = 0; r0 < rows; r0 += kGroups) {
-      const int row = r0 + group;
-      const bool live = row < rows;
-      const bool is_q = row < a.Hq, is_k = !is_q && row < a.Hq + a.Hk;
-      const int head = is_q ? row : (is_k ? row - a.Hq : row - a.Hq - a.Hk);
-      const T* src = static_cast<const T*>(is_q ? a.q : (is_k ? a.k : a.v));
-      const int64_t off = t * (is_q ? a.q_st : (is_k ? a.k_st : a.v_st)) +
-                          head * (is_q ? a.q_sh : (is_k ? a.k_sh : a.v_sh)) + part * 8;
-      Vec8<T> x;
-      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (live) {
-        x.load(src + off);
-        x.get(f);
-      }
-      if (a.q_weight) {
+  }
+  float w[8];
+  const void* w_of = nullptr;  // the weight that w holds
+  auto one_row = [&](int row, const Vec8<T>& raw) {
+    const bool is_q = row < a.Hq, is_k = !is_q && row < a.Hq + a.Hk;
+    const int head = is_q ? row : (is_k ? row - a.Hq : row - a.Hq - a.Hk);
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (ok) raw.get(f);
+    if (is_q || is_k) {
+      const void* wp = is_q ? a.q_weight : a.k_weight;
+      if (wp) {
+        if (wp != w_of) {
+          Vec8<T> wv;
+          wv.load(static_cast<const T*>(wp) + part * 8);
+          wv.get(w);
+          w_of = wp;
+        }
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
         const float inv = rsqrtf(group_sum<W>(ss) * (1.f / D) + a.eps);
-        if (is_q || is_k) {
-          Vec8<T> wv;
-          float w[8];
-          wv.load(static_cast<const T*>(is_q ? a.q_weight : a.k_weight) + part * 8);
-          wv.get(w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
-        }
+        for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
       }
       if (a.half) {
-        float p[8];  // the partners
+        float x[8];  // the partners
         if (a.interleaved) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) p[i] = (i & 1) ? f[i - 1] : -f[i + 1];
+          for (int i = 0; i < 8; ++i) x[i] = f[i ^ 1];
         } else {
-          const bool first = part < rot_lanes / 2;
-          const int lane = threadIdx.x & 31;
-          const int from = rotated ? (first ? lane + rot_lanes / 2 : lane - rot_lanes / 2) : lane;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            p[i] = __shfl_sync(0xffffffffu, f[i], from);
-            if (first) p[i] = -p[i];
-          }
+          for (int i = 0; i < 8; ++i) x[i] = __shfl_sync(0xffffffffu, f[i], from);
         }
-        if (rotated && (is_q || is_k)) {
+        if (rotated) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + p[i] * s[i];
-        }
-      }
-      if (Q8) {
-        const bool kv = live && !is_q;
-        store_e4m3<D>(f, part, is_k ? a.k_pool : a.v_pool, is_k ? a.k_scale : a.v_scale, a.g, page,
-                      kv ? head : 0, slot, kv);
-      }
-      if (live && (is_q || !Q8)) {
-        x.set(f);
-        if (is_q) {
-          x.store(static_cast<T*>(a.q_out) + t * a.o_st + head * a.o_sh + part * 8);
-        } else {
-          uint8_t* pool = is_k ? a.k_pool : a.v_pool;
-          if (sizeof(T) == 2)
-            x.store(pool + page_chunk(a.g, page, head, slot, part, D / 8));
-          else
-            x.store(pool + page_chunk(a.g, page, head, slot, part * 2, D / 4));
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + x[i] * s[i];
         }
       }
     }
+    if (is_q) {
+      if (ok) {
+        Vec8<T> v;
+        v.set(f);
+        v.store(static_cast<T*>(a.q_out) + t * a.o_st + head * a.o_sh + part * 8);
+      }
+      return;
+    }
+    uint8_t* pool = is_k ? a.k_pool : a.v_pool;
+    if (Q8) {
+      store_e4m3<D>(f, part, pool, is_k ? a.k_scale : a.v_scale, a.g, p.page, head, p.slot, ok);
+    } else if (ok) {
+      Vec8<T> v;
+      v.set(f);
+      v.store(pool + (sizeof(T) == 2 ? page_chunk(a.g, p.page, head, p.slot, part, D / 8)
+                                     : page_chunk(a.g, p.page, head, p.slot, part * 2, D / 4)));
+    }
+  };
+  for (int r0 = row0; r0 < row1; r0 += kAhead) {
+    Vec8<T> now[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) now[u] = in[u];
+    fetch(r0 + kAhead);
+#pragma unroll 1
+    for (int u = 0; u < kAhead; ++u) {
+      if (r0 + u < row1) one_row(r0 + u, now[0]);
+#pragma unroll
+      for (int x = 0; x + 1 < kAhead; ++x) now[x] = now[x + 1];
+    }
   }
+}
+
+// Heads of a token that one block takes: all of them when there are tokens enough
+// for four blocks on each SM, else as few as fill them.
+int rows_per_block(int64_t token_blocks, int rows) {
+  const int64_t want = static_cast<int64_t>(current_sm_count()) * 4;
+  int64_t splits = (want + token_blocks - 1) / token_blocks;
+  if (splits > rows) splits = rows;
+  return static_cast<int>((rows + splits - 1) / splits);
 }
 
 struct ReadArgs {
@@ -243,54 +295,57 @@ struct ReadArgs {
 };
 
 template <typename T, int D, bool Q8>
-__global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a, const int rows_per_block) {
   constexpr int W = D / 8;
   constexpr int kGroups = kThreads / W;
-  const int group = threadIdx.x / W, part = threadIdx.x % W;
+  constexpr int kAhead = 4;  // rows in flight
+  const int part = threadIdx.x % W;
+  const int64_t t = blockIdx.x * static_cast<int64_t>(kGroups) + threadIdx.x / W;
+  const int row0 = blockIdx.y * rows_per_block, row1 = min(2 * a.Hk, row0 + rows_per_block);
   grid_dep_wait();
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    const int r = find_request(a.token_start, a.R, t);
-    if (r >= a.R || t < a.token_start[r]) continue;
-    const int64_t pos = static_cast<int64_t>(a.first_pos[r]) + (t - a.token_start[r]);
-    const int64_t lo = a.page_bounds[r], n = a.page_bounds[r + 1] - lo;
-    int64_t page = -1;
-    int err = 0;
-    if (pos < 0 || pos / a.g.page_size >= n) {
-      err = kStatusPosition;
-    } else {
-      page = a.page_table[lo + pos / a.g.page_size];
-      if (page < 0 || page >= a.g.num_pages) err = kStatusPage;
-    }
-    if (err) {
-      if (threadIdx.x == 0) report(a.status, err);
-      continue;
-    }
-    const int slot = static_cast<int>(pos % a.g.page_size);
-    for (int row = group; row < 2 * a.Hk; row += kGroups) {
+  const Place p =
+      find_place<W>(t, a.tokens, a.token_start, a.first_pos, a.R, a.page_table, a.page_bounds, a.g);
+  if (p.err > 0 && part == 0 && row0 == 0) report(a.status, p.err);
+  if (p.err != 0) return;
+  for (int r0 = row0; r0 < row1; r0 += kAhead) {
+    Vec8<T> x[kAhead];
+    uint2 q[kAhead];
+    uint32_t byte[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int row = r0 + u;
+      if (row >= row1) break;
       const bool is_k = row < a.Hk;
       const int head = is_k ? row : row - a.Hk;
       const uint8_t* pool = is_k ? a.k_pool : a.v_pool;
-      Vec8<T> x;
       if (Q8) {
-        const uint2 q = *reinterpret_cast<const uint2*>(
-            pool + page_chunk(a.g, page, head, slot, part >> 1, D / 16) + (part & 1) * 8);
-        const float sc = e4m3_scale(
-            (is_k ? a.k_scale : a.v_scale)[page * a.g.scale_page + head * a.g.scale_head + slot]);
+        q[u] = *reinterpret_cast<const uint2*>(pool + page_chunk(a.g, p.page, head, p.slot, part >> 1, D / 16) +
+                                               (part & 1) * 8);
+        byte[u] = (is_k ? a.k_scale : a.v_scale)[p.page * a.g.scale_page + head * a.g.scale_head + p.slot];
+      } else {
+        x[u].load(pool + (sizeof(T) == 2 ? page_chunk(a.g, p.page, head, p.slot, part, D / 8)
+                                         : page_chunk(a.g, p.page, head, p.slot, part * 2, D / 4)));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int row = r0 + u;
+      if (row >= row1) break;
+      const bool is_k = row < a.Hk;
+      const int head = is_k ? row : row - a.Hk;
+      if (Q8) {
+        const float sc = e4m3_scale(byte[u]);
         float f[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 p = e4m3x2_to_f((i < 2 ? q.x : q.y) >> ((i & 1) * 16));
-          f[2 * i] = p.x * sc;
-          f[2 * i + 1] = p.y * sc;
+          const float2 v = e4m3x2_to_f((i < 2 ? q[u].x : q[u].y) >> ((i & 1) * 16));
+          f[2 * i] = v.x * sc;
+          f[2 * i + 1] = v.y * sc;
         }
-        x.set(f);
-      } else {
-        x.load(pool + (sizeof(T) == 2 ? page_chunk(a.g, page, head, slot, part, D / 8)
-                                      : page_chunk(a.g, page, head, slot, part * 2, D / 4)));
+        x[u].set(f);
       }
-      T* out = static_cast<T*>(is_k ? a.k_out : a.v_out) + t * (is_k ? a.ko_st : a.vo_st) +
-               head * (is_k ? a.ko_sh : a.vo_sh) + part * 8;
-      x.store(out);
+      x[u].store(static_cast<T*>(is_k ? a.k_out : a.v_out) + t * (is_k ? a.ko_st : a.vo_st) +
+                 head * (is_k ? a.ko_sh : a.vo_sh) + part * 8);
     }
   }
 }
@@ -429,10 +484,13 @@ extern "C" int d2sd_append_kv(
   a.eps = eps;
   a.R = num_requests, a.Hq = num_qo_heads, a.Hk = num_kv_heads, a.half = rotary_dim / 2,
   a.interleaved = interleaved;
-  const int64_t cap = static_cast<int64_t>(current_sm_count()) * 64;
-  const dim3 grid(static_cast<unsigned>(num_tokens < cap ? num_tokens : cap));
+  const int rows = num_qo_heads + 2 * num_kv_heads;
+  const int64_t per = kThreads / (head_dim / 8), blocks = (num_tokens + per - 1) / per;
+  if (blocks > 0x7fffffff) return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": too many tokens");
+  const int rpb = rows_per_block(blocks, rows);
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((rows + rpb - 1) / rpb));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kThreads), 0, st, w, a); };
+  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kThreads), 0, st, w, a, rpb); };
   if (dtype == D2SD_DTYPE_F32) return head_dim == 128 ? go(append_kernel<float, 128, false>) : go(append_kernel<float, 64, false>);
   if (dtype == D2SD_DTYPE_BF16) {
     if (scaled) return head_dim == 128 ? go(append_kernel<__nv_bfloat16, 128, true>) : go(append_kernel<__nv_bfloat16, 64, true>);
@@ -488,10 +546,13 @@ extern "C" int d2sd_read_kv(const void* k_pool, const void* v_pool, int64_t cach
   a.status = status;
   a.tokens = num_tokens;
   a.R = num_requests, a.Hk = num_kv_heads;
-  const int64_t cap = static_cast<int64_t>(current_sm_count()) * 64;
-  const dim3 grid(static_cast<unsigned>(num_tokens < cap ? num_tokens : cap));
+  const int rows = 2 * num_kv_heads;
+  const int64_t per = kThreads / (head_dim / 8), blocks = (num_tokens + per - 1) / per;
+  if (blocks > 0x7fffffff) return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": too many tokens");
+  const int rpb = rows_per_block(blocks, rows);
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((rows + rpb - 1) / rpb));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kThreads), 0, st, w, a); };
+  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(kThreads), 0, st, w, a, rpb); };
   if (dtype == D2SD_DTYPE_F32) return head_dim == 128 ? go(read_kernel<float, 128, false>) : go(read_kernel<float, 64, false>);
   if (dtype == D2SD_DTYPE_BF16) {
     if (scaled) return head_dim == 128 ? go(read_kernel<__nv_bfloat16, 128, true>) : go(read_kernel<__nv_bfloat16, 64, true>);
