@@ -9,7 +9,7 @@
 // o = 0 and lse2 = -inf.
 //
 // rows_kernel: a CTA takes 16 query rows of one kv head against a span of keys
-// (paged_plan.h); its eight warps take the span's 16-key pages in turn, each with
+// (paged_plan.h); its warps take the span's 16-key pages in turn, each with
 // a ring of pages of its own in shared memory, so the loop has no CTA barrier and
 // about 190 KB of loads are in flight per SM -- the bound is HBM. The products
 // are m16n8k16 matrix instructions: one 16-row tile is all the rows there are,
@@ -38,18 +38,21 @@ namespace {
 
 using namespace paged;
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-
 template <int D, int ELEM>
 struct RowsCfg {
+  // 8-bit pages take half of the bytes and more instructions (they are widened): 16
+  // warps, with q's fragments in shared memory so that 128 registers suffice. 16-bit
+  // pages need their bytes in flight: 8 warps with three stages each.
+  static constexpr int kWarps = ELEM == 1 ? 16 : 8;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kPageBytes = 16 * D * ELEM;        // one of K, V
   static constexpr int kStageBytes = 2 * kPageBytes + (ELEM == 1 ? 32 : 0);  // + 16 + 16 scale bytes
-  static constexpr int kRing = 24576;                     // bytes of a warp's ring
+  static constexpr int kRing = ELEM == 1 ? 12416 : 24576;  // bytes of a warp's ring
   static constexpr int kStages = (kRing / kStageBytes) < 8 ? (kRing / kStageBytes) : 8;
   static constexpr int kState = 16 * D * 4;               // a warp's O, over its ring at the end
   static constexpr int kSmemMl = kWarps * kRing;          // [warps][16] m, then l
-  static constexpr int kSmemBars = kSmemMl + 2 * kWarps * 16 * 4;
+  static constexpr int kSmemQ = kSmemMl + 2 * kWarps * 16 * 4;  // [D / 16][32 lanes][16 bytes] (8-bit)
+  static constexpr int kSmemBars = kSmemQ + (ELEM == 1 ? 16 * D * 2 : 0);
   static constexpr int kSmemFlags = kSmemBars + kWarps * 8 * 8;
   static constexpr int kSmemBytes = kSmemFlags + 16 + 128;
   static_assert(kState <= kRing, "the state fits the ring");
@@ -92,14 +95,16 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 // ELEM: bytes of a cached value (2: T, 1: e4m3); UMMA: pages in core-matrix order,
 // fetched with one bulk copy each (else rows, 16-byte cp.async).
 template <typename T, int D, int ELEM, bool UMMA>
-__global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(const AttnArgs a) {
   using C = RowsCfg<D, ELEM>;
+  constexpr int kWarps = C::kWarps, kThreads = C::kThreads;
   constexpr int kChunks = D * ELEM / 16;  // 16-byte chunks of a row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) &
                                              ~static_cast<uintptr_t>(127));
   float* sm_m = reinterpret_cast<float*>(smem + C::kSmemMl);
   float* sm_l = sm_m + kWarps * 16;
+  uint4* sm_q = reinterpret_cast<uint4*>(smem + C::kSmemQ);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kSmemBars);
   volatile int* flags = reinterpret_cast<volatile int*>(smem + C::kSmemFlags);  // abort
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
@@ -135,34 +140,33 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
     const int lo_min = row_lo(0), lo_max = row_lo(nrows - 1);
 
     // ---- q fragments (A operand, 16 rows x 16 of d per step) ----
-    uint32_t qf[D / 16][4];
+    const T* q0 = nullptr;
+    const T* q1 = nullptr;
     {
       const T* qb = static_cast<const T*>(a.q);
-      const T* q0 = nullptr;
-      const T* q1 = nullptr;
       if (qr < nrows)
         q0 = qb + (tok0 + static_cast<int64_t>((row0 + qr) / G)) * a.q_st + (head * G + (row0 + qr) % G) * a.q_sh;
       if (qr + 8 < nrows)
         q1 = qb + (tok0 + static_cast<int64_t>((row0 + qr + 8) / G)) * a.q_st +
              (head * G + (row0 + qr + 8) % G) * a.q_sh;
+    }
+    uint32_t qf[ELEM == 2 ? D / 16 : 1][4];
+    if constexpr (ELEM == 2) {
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        if (ELEM == 2) {
-          const int d = ks * 16 + qc * 2;
-          qf[ks][0] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + d) : 0u;
-          qf[ks][1] = q1 ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
-          qf[ks][2] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + d + 8) : 0u;
-          qf[ks][3] = q1 ? *reinterpret_cast<const uint32_t*>(q1 + d + 8) : 0u;
-        } else {  // the four elements this lane's K bytes belong to: even ones, then odd ones
-          const int d = ks * 16 + qc * 4;
-          const uint2 x = q0 ? *reinterpret_cast<const uint2*>(q0 + d) : make_uint2(0u, 0u);
-          const uint2 y = q1 ? *reinterpret_cast<const uint2*>(q1 + d) : make_uint2(0u, 0u);
-          qf[ks][0] = __byte_perm(x.x, x.y, 0x5410);
-          qf[ks][2] = __byte_perm(x.x, x.y, 0x7632);
-          qf[ks][1] = __byte_perm(y.x, y.y, 0x5410);
-          qf[ks][3] = __byte_perm(y.x, y.y, 0x7632);
-        }
+        const int d = ks * 16 + qc * 2;
+        qf[ks][0] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + d) : 0u;
+        qf[ks][1] = q1 ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
+        qf[ks][2] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + d + 8) : 0u;
+        qf[ks][3] = q1 ? *reinterpret_cast<const uint32_t*>(q1 + d + 8) : 0u;
       }
+    } else if (warp < D / 16) {
+      // step `warp` of the four elements a lane's K bytes belong to: even ones, then odd ones
+      const int d = warp * 16 + qc * 4;
+      const uint2 x = q0 ? *reinterpret_cast<const uint2*>(q0 + d) : make_uint2(0u, 0u);
+      const uint2 y = q1 ? *reinterpret_cast<const uint2*>(q1 + d) : make_uint2(0u, 0u);
+      sm_q[warp * 32 + lane] = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(y.x, y.y, 0x5410),
+                                          __byte_perm(x.x, x.y, 0x7632), __byte_perm(y.x, y.y, 0x7632));
     }
     float o[D / 8][4];
 #pragma unroll
@@ -221,6 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
       if (j < mine) issue(j);
       commit();
     }
+    if (ELEM == 1) __syncthreads();  // q is in shared memory
     bool alive = true;
     int j = 0;
     for (; j < mine; ++j) {
@@ -267,10 +272,13 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
         for (int ks = 0; ks < D / 16; ks += 2) {
           uint32_t b[4];  // (keys 0-7, chunk ks), (8-15, ks), (0-7, ks + 1), (8-15, ks + 1)
           ldsm4(ka + ((mt & 1) * kChunks + ks + (mt >> 1)) * 128, b);
-          mma16816<T>(c[0], qf[ks], e4m3_even(b[0]), e4m3_odd(b[0]));
-          mma16816<T>(c[1], qf[ks], e4m3_even(b[1]), e4m3_odd(b[1]));
-          mma16816<T>(c[0], qf[ks + 1], e4m3_even(b[2]), e4m3_odd(b[2]));
-          mma16816<T>(c[1], qf[ks + 1], e4m3_even(b[3]), e4m3_odd(b[3]));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 q = sm_q[(ks + h) * 32 + lane];
+            const uint32_t qa[4] = {q.x, q.y, q.z, q.w};
+            mma16816<T>(c[0], qa, e4m3_even(b[2 * h]), e4m3_odd(b[2 * h]));
+            mma16816<T>(c[1], qa, e4m3_even(b[2 * h + 1]), e4m3_odd(b[2 * h + 1]));
+          }
         }
       }
       float vs[2][2] = {{1.f, 1.f}, {1.f, 1.f}};  // value scales of this lane's four keys
@@ -417,9 +425,9 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const AttnArgs a) {
       float* own = a.slots + static_cast<int64_t>(I[P_SLOT]) * rows_slot_floats(D);
       if (row < nrows) {
 #pragma unroll
-        for (int e = 0; e < kPer; e += 4)
-          reinterpret_cast<float4*>(own)[(dcol + e) / 4 * 16 + row] =
-              make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+        for (int e = 0; e < kPer; e += 2)
+          reinterpret_cast<float2*>(own)[((dcol + e) / 4 * 16 + row) * 2 + (dcol + e) / 2 % 2] =
+              make_float2(acc[e], acc[e + 1]);
         if (dcol == 0) {
           own[16 * D + row] = M;
           own[16 * D + 16 + row] = L;
@@ -517,7 +525,7 @@ int launch_rows(const AttnArgs& a, int ctas, cudaStream_t stream) {
       return fail(D2SD_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
     if (dev < 64) configured.fetch_or(1ull << dev);
   }
-  return launch_pdl(rows_kernel<T, D, ELEM, UMMA>, dim3(ctas), dim3(kThreads), C::kSmemBytes, stream,
+  return launch_pdl(rows_kernel<T, D, ELEM, UMMA>, dim3(ctas), dim3(C::kThreads), C::kSmemBytes, stream,
                     "rows_kernel", a);
 }
 

@@ -22,6 +22,7 @@
 // neighbouring tokens fill whole 32-byte sectors of the pages, whose rows of eight
 // values lie 16 bytes apart. Few tokens spread their heads over several blocks.
 #include <string>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -72,12 +73,11 @@ __device__ __forceinline__ float group_max(float x) {
   return x;
 }
 
-// Lane `part` of the row's group holds elements 8 part .. 8 part + 7. Writes the
-// row's 8-bit form to slot s of (page, head) of a pool and its scale pool. The
-// whole group calls it; rows with store == false only take part in the shuffles.
+// Lane `part` of a row's group holds elements 8 part .. 8 part + 7. Writes them to
+// `at` (this lane's 8 bytes of the page) and the row's scale byte. The whole group
+// calls it; rows with store == false only take part in the shuffles.
 template <int D>
-__device__ __forceinline__ void store_e4m3(const float (&f)[8], int part, uint8_t* pool, uint8_t* scale,
-                                           const PageGeom& g, int64_t page, int head, int s,
+__device__ __forceinline__ void store_e4m3(const float (&f)[8], int part, uint8_t* at, uint8_t* scale,
                                            bool store) {
   float m = 0.f;
   bool bad = false;
@@ -95,8 +95,8 @@ __device__ __forceinline__ void store_e4m3(const float (&f)[8], int part, uint8_
   q.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
   if (!finite) q.x = q.y = 0x7f7f7f7fu;
   if (!store) return;
-  *reinterpret_cast<uint2*>(pool + page_chunk(g, page, head, s, part >> 1, D / 16) + (part & 1) * 8) = q;
-  if (part == 0) scale[page * g.scale_page + head * g.scale_head + s] = static_cast<uint8_t>(byte);
+  *reinterpret_cast<uint2*>(at) = q;
+  if (part == 0) *scale = static_cast<uint8_t>(byte);
 }
 
 struct AppendArgs {
@@ -150,7 +150,7 @@ __device__ __forceinline__ Place find_place(int64_t t, int64_t tokens, const int
 }
 
 template <typename T, int D, bool Q8>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a, const int rows_per_block) {
+__global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a, const int rows_per_block) {
   constexpr int W = D / 8;               // lanes of a row
   constexpr int kGroups = kThreads / W;  // tokens of a block
   const int part = threadIdx.x % W;
@@ -163,21 +163,6 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a, co
   if (p.err > 0 && part == 0 && row0 == 0) report(a.status, p.err);
   const bool ok = p.err == 0;  // else the token's rows are not written at all
   if (!__any_sync(0xffffffffu, ok)) return;
-  // where row `row` of this token is read
-  auto source = [&](int row) {
-    const bool is_q = row < a.Hq, is_k = !is_q && row < a.Hq + a.Hk;
-    const int head = is_q ? row : (is_k ? row - a.Hq : row - a.Hq - a.Hk);
-    return static_cast<const T*>(is_q ? a.q : (is_k ? a.k : a.v)) + t * (is_q ? a.q_st : (is_k ? a.k_st : a.v_st)) +
-           head * (is_q ? a.q_sh : (is_k ? a.k_sh : a.v_sh)) + part * 8;
-  };
-  constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // rows in flight
-  Vec8<T> in[kAhead];
-  auto fetch = [&](int r0) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (ok && r0 + u < row1) in[u].load(source(r0 + u));
-  };
-  fetch(row0);
   // this lane's cos and sin: columns of its 8 elements' pairs
   float c[8], s[8];
   const int rot_lanes = a.half / 4;  // lanes that hold rotated elements
@@ -204,74 +189,77 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a, co
       }
     }
   }
-  float w[8];
-  const void* w_of = nullptr;  // the weight that w holds
-  auto one_row = [&](int row, const Vec8<T>& raw) {
-    const bool is_q = row < a.Hq, is_k = !is_q && row < a.Hq + a.Hk;
-    const int head = is_q ? row : (is_k ? row - a.Hq : row - a.Hq - a.Hk);
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (ok) raw.get(f);
-    if (is_q || is_k) {
-      const void* wp = is_q ? a.q_weight : a.k_weight;
-      if (wp) {
-        if (wp != w_of) {
-          Vec8<T> wv;
-          wv.load(static_cast<const T*>(wp) + part * 8);
-          wv.get(w);
-          w_of = wp;
-        }
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
-        const float inv = rsqrtf(group_sum<W>(ss) * (1.f / D) + a.eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
-      }
-      if (a.half) {
-        float x[8];  // the partners
-        if (a.interleaved) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = f[i ^ 1];
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = __shfl_sync(0xffffffffu, f[i], from);
-        }
-        if (rotated) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + x[i] * s[i];
-        }
-      }
+  // heads h0 .. h1 - 1 of q (0), k (1) or v (2): four rows' loads, then their work
+  constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+  auto heads = [&](auto kind, int h0, int h1, const void* src_p, int64_t st, int64_t sh, const void* weight,
+                   uint8_t* dst, int64_t dst_sh, uint8_t* scale) {
+    constexpr int kKind = decltype(kind)::value;
+    if (h0 >= h1) return;
+    const T* src = static_cast<const T*>(src_p) + t * st + h0 * sh + part * 8;
+    dst += h0 * dst_sh;
+    if (Q8 && kKind != 0) scale += h0 * a.g.scale_head;
+    float w[8];
+    if (kKind != 2 && weight) {
+      Vec8<T> wv;
+      wv.load(static_cast<const T*>(weight) + part * 8);
+      wv.get(w);
     }
-    if (is_q) {
-      if (ok) {
-        Vec8<T> v;
-        v.set(f);
-        v.store(static_cast<T*>(a.q_out) + t * a.o_st + head * a.o_sh + part * 8);
+    for (int h = h0; h < h1; h += kAhead) {
+      Vec8<T> in[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (ok && h + u < h1) in[u].load(src + u * sh);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (h + u >= h1) break;
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (ok) in[u].get(f);
+        if (kKind != 2 && weight) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
+          const float inv = rsqrtf(group_sum<W>(ss) * (1.f / D) + a.eps);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
+        }
+        if (kKind != 2 && a.half) {
+          float x[8];  // the partners
+          if (a.interleaved) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = f[i ^ 1];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __shfl_sync(0xffffffffu, f[i], from);
+          }
+          if (rotated) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + x[i] * s[i];
+          }
+        }
+        if (Q8 && kKind != 0) {
+          store_e4m3<D>(f, part, dst + u * dst_sh, scale + u * a.g.scale_head, ok);
+        } else if (ok) {
+          Vec8<T> v;
+          v.set(f);
+          v.store(dst + u * dst_sh);
+        }
       }
-      return;
-    }
-    uint8_t* pool = is_k ? a.k_pool : a.v_pool;
-    if (Q8) {
-      store_e4m3<D>(f, part, pool, is_k ? a.k_scale : a.v_scale, a.g, p.page, head, p.slot, ok);
-    } else if (ok) {
-      Vec8<T> v;
-      v.set(f);
-      v.store(pool + (sizeof(T) == 2 ? page_chunk(a.g, p.page, head, p.slot, part, D / 8)
-                                     : page_chunk(a.g, p.page, head, p.slot, part * 2, D / 4)));
+      src += kAhead * sh;
+      dst += kAhead * dst_sh;
+      if (Q8 && kKind != 0) scale += kAhead * a.g.scale_head;
     }
   };
-  for (int r0 = row0; r0 < row1; r0 += kAhead) {
-    Vec8<T> now[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) now[u] = in[u];
-    fetch(r0 + kAhead);
-#pragma unroll 1
-    for (int u = 0; u < kAhead; ++u) {
-      if (r0 + u < row1) one_row(r0 + u, now[0]);
-#pragma unroll
-      for (int x = 0; x + 1 < kAhead; ++x) now[x] = now[x + 1];
-    }
-  }
+  // this lane's part of the token's row of head 0 in a page
+  const int64_t at = page_chunk(a.g, p.page, 0, p.slot, Q8 ? part >> 1 : part * static_cast<int>(sizeof(T)) / 2,
+                                (Q8 ? 1 : static_cast<int>(sizeof(T))) * D / 16) + (Q8 ? (part & 1) * 8 : 0);
+  const int64_t sat = Q8 ? p.page * a.g.scale_page + p.slot : 0;
+  heads(std::integral_constant<int, 0>(), row0, min(row1, a.Hq), a.q, a.q_st, a.q_sh, a.q_weight,
+        static_cast<uint8_t*>(a.q_out) + (t * a.o_st + part * 8) * static_cast<int64_t>(sizeof(T)),
+        a.o_sh * static_cast<int64_t>(sizeof(T)), nullptr);
+  heads(std::integral_constant<int, 1>(), max(row0, a.Hq) - a.Hq, min(row1, a.Hq + a.Hk) - a.Hq, a.k, a.k_st,
+        a.k_sh, a.k_weight, a.k_pool + at, a.g.stride_head, a.k_scale + sat);
+  heads(std::integral_constant<int, 2>(), max(row0, a.Hq + a.Hk) - a.Hq - a.Hk, row1 - a.Hq - a.Hk, a.v, a.v_st,
+        a.v_sh, nullptr, a.v_pool + at, a.g.stride_head, a.v_scale + sat);
 }
 
 // Heads of a token that one block takes: all of them when there are tokens enough
@@ -410,7 +398,9 @@ __global__ void __launch_bounds__(kThreads) commit_e4m3_kernel(const CommitArgs8
           v.get(f);
         }
       }
-      store_e4m3<D>(f, part, pool, scale, a.g, ok ? page : 0, h, static_cast<int>(pos & 15), ok);
+      const int slot = static_cast<int>(pos & 15);
+      store_e4m3<D>(f, part, pool + page_chunk(a.g, page, h, slot, part >> 1, D / 16) + (part & 1) * 8,
+                    scale + page * a.g.scale_page + h * a.g.scale_head + slot, ok);
     }
   }
 }
@@ -473,7 +463,7 @@ extern "C" int d2sd_append_kv(
   a.q_st = q_stride_token, a.q_sh = q_stride_head, a.o_st = q_out_stride_token,
   a.o_sh = q_out_stride_head, a.k_st = k_stride_token, a.k_sh = k_stride_head, a.v_st = v_stride_token,
   a.v_sh = v_stride_head;
-  a.q_weight = q_weight ? q_weight : k_weight, a.k_weight = k_weight;
+  a.q_weight = q_weight, a.k_weight = k_weight;
   a.cos = cos_table, a.sin = sin_table, a.table_stride = table_stride, a.table_rows = table_rows;
   a.token_start = token_start, a.first_pos = first_pos;
   a.page_table = page_table, a.page_bounds = page_bounds;
