@@ -19,15 +19,18 @@
 // the copy. At the end the warps' states are joined in shared memory, and for a
 // unit of several spans join_kernel joins the spans.
 //
-// e4m3 pages: the fragments are widened to bf16 in registers (sign and the seven
-// magnitude bits moved into place, then a product with 2^120, all exact). A
-// 16-byte row of a core matrix holds 16 elements of d; ldmatrix hands a lane four
-// neighbouring ones, and since the order of the summed index is free, q's
-// fragment takes the same four (K), or two neighbouring output columns (V). The
-// key's scale multiplies the score, the value's scale the weight, in fp32.
-//
-// Weights are rounded to the value type (bf16: 2^-8 relative, f16: 2^-11) for the
-// second product; maximum, sum and output stay in fp32.
+// e4m3 pages: their values are widened to f16 in registers (one conversion for two,
+// exact) and both products are f16. A 16-byte row of a core matrix holds 16 elements
+// of d; ldmatrix hands a lane four neighbouring ones, and since the order of the
+// summed index is free, q's fragment takes the same four (K); for V the lane's four
+// bytes are two keys by two neighbouring columns. f16's range is met by powers of
+// two, which cost no precision: q's rows are scaled to 2^14 .. 2^15, and with e_j
+// the exponent of value row j the weights are
+//   w_j = 2^(s_j + e_j - M), M the running maximum of s_j + e_j,
+// at most 1 whatever the rows' sizes are; the sum of plain weights keeps its own
+// maximum m. The key's scale multiplies the score in fp32.
+// Weights are rounded to 16 bits (bf16: 2^-8 relative, f16: 2^-11) for the second
+// product; maximum, sum and output stay in fp32.
 #include <atomic>
 #include <string>
 
@@ -40,10 +43,12 @@ using namespace paged;
 
 template <int D, int ELEM>
 struct RowsCfg {
-  // 8-bit pages take half of the bytes and more instructions (they are widened): 16
-  // warps, with q's fragments in shared memory so that 128 registers suffice. 16-bit
-  // pages need their bytes in flight: 8 warps with three stages each.
-  static constexpr int kWarps = ELEM == 1 ? 16 : 8;
+  // Four small CTAs share an SM, so that one's start and end (an item's entry, its q
+  // and its first pages come one after another, about 5 us, and then the join) pass
+  // under the others' loads. 8-bit pages take half of the bytes and more
+  // instructions: twice the warps, with q's fragments in shared memory so that 128
+  // registers suffice.
+  static constexpr int kWarps = ELEM == 1 ? 4 : 2;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kPageBytes = 16 * D * ELEM;        // one of K, V
   static constexpr int kStageBytes = 2 * kPageBytes + (ELEM == 1 ? 32 : 0);  // + 16 + 16 scale bytes
@@ -56,6 +61,7 @@ struct RowsCfg {
   static constexpr int kSmemFlags = kSmemBars + kWarps * 8 * 8;
   static constexpr int kSmemBytes = kSmemFlags + 16 + 128;
   static_assert(kState <= kRing, "the state fits the ring");
+  static_assert(kRowsCtas * (kSmemBytes + 1024) <= 227 * 1024 + 1024, "the CTAs of an SM");
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -88,6 +94,13 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The four e4m3 values of x as two pairs of f16 (bytes 0 and 1, bytes 2 and 3).
+__device__ __forceinline__ void e4m3x4_f16(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(x));
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -95,7 +108,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 // ELEM: bytes of a cached value (2: T, 1: e4m3); UMMA: pages in core-matrix order,
 // fetched with one bulk copy each (else rows, 16-byte cp.async).
 template <typename T, int D, int ELEM, bool UMMA>
-__global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_kernel(const AttnArgs a) {
   using C = RowsCfg<D, ELEM>;
   constexpr int kWarps = C::kWarps, kThreads = C::kThreads;
   constexpr int kChunks = D * ELEM / 16;  // 16-byte chunks of a row
@@ -111,7 +124,7 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
   uint8_t* ring = smem + warp * C::kRing;
   uint64_t* full = bars + warp * 8;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kWarps * 8; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < kWarps * 8; ++i) mbar_init(&bars[i], ELEM == 1 ? 3 : 1);
     flags[0] = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -121,6 +134,7 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
 
   const int32_t* sec = a.plan + H_SECTION;
   const int G = a.plan[H_GROUP];
+  grid_dep_launch();  // the join's blocks wait beside this kernel
   if (static_cast<int>(blockIdx.x) >= sec[S_CTAS]) return;  // a fixed grid's spare CTA
   const int item0 = a.plan[sec[S_OFF_CTA] + blockIdx.x], item1 = a.plan[sec[S_OFF_CTA] + blockIdx.x + 1];
   const int qr = lane >> 2, qc = lane & 3;
@@ -160,18 +174,49 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
         qf[ks][2] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + d + 8) : 0u;
         qf[ks][3] = q1 ? *reinterpret_cast<const uint32_t*>(q1 + d + 8) : 0u;
       }
-    } else if (warp < D / 16) {
-      // step `warp` of the four elements a lane's K bytes belong to: even ones, then odd ones
-      const int d = warp * 16 + qc * 4;
-      const uint2 x = q0 ? *reinterpret_cast<const uint2*>(q0 + d) : make_uint2(0u, 0u);
-      const uint2 y = q1 ? *reinterpret_cast<const uint2*>(q1 + d) : make_uint2(0u, 0u);
-      sm_q[warp * 32 + lane] = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(y.x, y.y, 0x5410),
-                                          __byte_perm(x.x, x.y, 0x7632), __byte_perm(y.x, y.y, 0x7632));
+    }
+    float row_scale[2] = {a.scale_log2, a.scale_log2};
+    if constexpr (ELEM == 1) {
+      // rows scaled by 2^k to 2^14 <= max|q| < 2^15 and their scores by 2^-k
+      float q_scale[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const T* qp = h ? q1 : q0;
+        float m = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint2 x = qp ? *reinterpret_cast<const uint2*>(qp + ks * 16 + qc * 4) : make_uint2(0u, 0u);
+          const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(Num<T>::to_f(e[i])));
+        }
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int e = static_cast<int>(__float_as_uint(m) >> 23);  // 2^(e - 127) <= m
+        const int k = min(141 - e, 126);
+        q_scale[h] = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+        row_scale[h] *= __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+      }
+      for (int ks = warp; ks < D / 16; ks += kWarps) {  // the four elements a lane's K bytes belong to
+        const int d = ks * 16 + qc * 4;
+        uint4 f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const T* qp = h ? q1 : q0;
+          const uint2 x = qp ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0u, 0u);
+          const T* e = reinterpret_cast<const T*>(&x);
+          const float sc = q_scale[h];
+          (h ? f.y : f.x) = pack2(Num<T>::to_f(e[0]) * sc, Num<T>::to_f(e[1]) * sc, __half());
+          (h ? f.w : f.z) = pack2(Num<T>::to_f(e[2]) * sc, Num<T>::to_f(e[3]) * sc, __half());
+        }
+        sm_q[ks * 32 + lane] = f;
+      }
     }
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float M0 = -INFINITY, M1 = -INFINITY, g0 = 0.f, g1 = 0.f;  // e4m3: of s_j + e_j, 2^(m - M)
 
     // ---- this warp's pages of 16 keys: b0 + warp, b0 + warp + 8, ... ----
     const int b0 = key0 / 16, nb = (key1 - key0 + 15) / 16;
@@ -194,14 +239,14 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
       const int64_t off = page * a.g.stride_page + head * a.g.stride_head;
       if (UMMA) {
         if (lane == 0) {
-          mbar_arrive_expect_tx(&full[st], C::kStageBytes);
+          mbar_arrive_expect_tx(&full[st], 2 * C::kPageBytes);
           bulk_load(dst, a.k_pool + off, C::kPageBytes, &full[st]);
           bulk_load(dst + C::kPageBytes, a.v_pool + off, C::kPageBytes, &full[st]);
-          if (ELEM == 1) {
-            const int64_t so = page * a.g.scale_page + head * a.g.scale_head;
-            bulk_load(dst + 2 * C::kPageBytes, a.k_scale + so, 16, &full[st]);
-            bulk_load(dst + 2 * C::kPageBytes + 16, a.v_scale + so, 16, &full[st]);
-          }
+        }
+        if (ELEM == 1 && lane < 2) {  // the scales: two more bulk copies would cost as much as the pages
+          cp_async16(smem_u32(dst + 2 * C::kPageBytes + lane * 16),
+                     (lane ? a.v_scale : a.k_scale) + page * a.g.scale_page + head * a.g.scale_head);
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
         }
       } else {
         const int slot0 = (b0 + warp + j * kWarps) * 16 % a.g.page_size;
@@ -276,28 +321,30 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
           for (int h = 0; h < 2; ++h) {
             const uint4 q = sm_q[(ks + h) * 32 + lane];
             const uint32_t qa[4] = {q.x, q.y, q.z, q.w};
-            mma16816<T>(c[0], qa, e4m3_even(b[2 * h]), e4m3_odd(b[2 * h]));
-            mma16816<T>(c[1], qa, e4m3_even(b[2 * h + 1]), e4m3_odd(b[2 * h + 1]));
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              uint32_t lo, hi;
+              e4m3x4_f16(b[2 * h + n], lo, hi);
+              mma16816<__half>(c[n], qa, lo, hi);
+            }
           }
         }
       }
-      float vs[2][2] = {{1.f, 1.f}, {1.f, 1.f}};  // value scales of this lane's four keys
+      uint32_t vb[2] = {0u, 0u};  // value scale bytes of this lane's four keys
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        float s0 = a.scale_log2, s1 = a.scale_log2;
+        float k0 = 1.f, k1 = 1.f;
         if (ELEM == 1) {
           const uint8_t* sp = kp + 2 * C::kPageBytes + n * 8 + qc * 2;
           const uint32_t kb = *reinterpret_cast<const uint16_t*>(sp);
-          const uint32_t vb = *reinterpret_cast<const uint16_t*>(sp + 16);
-          s0 *= e4m3_scale(kb & 255u);
-          s1 *= e4m3_scale(kb >> 8);
-          vs[n][0] = e4m3_scale(vb & 255u);
-          vs[n][1] = e4m3_scale(vb >> 8);
+          vb[n] = *reinterpret_cast<const uint16_t*>(sp + 16);
+          k0 = e4m3_scale(kb & 255u);
+          k1 = e4m3_scale(kb >> 8);
         }
-        c[n][0] *= s0;
-        c[n][1] *= s1;
-        c[n][2] *= s0;
-        c[n][3] *= s1;
+        c[n][0] *= row_scale[0] * k0;
+        c[n][1] *= row_scale[0] * k1;
+        c[n][2] *= row_scale[1] * k0;
+        c[n][3] *= row_scale[1] * k1;
       }
       if (edge) {
 #pragma unroll
@@ -307,23 +354,51 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
             const int x = key + n * 8 + qc * 2 + e;
             if (x >= hi0 || x < lo0) c[n][e] = -INFINITY;
             if (x >= hi1 || x < lo1) c[n][2 + e] = -INFINITY;
-            if (x >= hi_max || x < lo_min) vs[n][e] = 0.f;  // a scale byte no row sees
+            // a scale byte no row sees
+            if (ELEM == 1 && (x >= hi_max || x < lo_min)) vb[n] &= e ? 0x00ffu : 0xff00u;
           }
       }
-      // ---- running maximum and sum; o is rescaled only when a maximum grew ----
-      float x0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
-      float x1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+      // ---- running maxima and sum; o is rescaled only when its maximum grew ----
+      auto row_max = [](float x) {  // over the four lanes of a row
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      };
+      const float x0 = row_max(fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1])));
+      const float x1 = row_max(fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3])));
+      float vs[2][2];           // 2^e_j
+      float y0 = x0, y1 = x1;   // maxima of s_j + e_j
+      if (ELEM == 1) {
+        float ve[2][2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t byte = (vb[n] >> (8 * e)) & 255u;
+            vs[n][e] = e4m3_scale(byte);
+            ve[n][e] = byte == 0u ? -INFINITY : static_cast<float>(static_cast<int>(byte) - 127);
+          }
+        y0 = row_max(fmaxf(fmaxf(c[0][0] + ve[0][0], c[0][1] + ve[0][1]),
+                           fmaxf(c[1][0] + ve[1][0], c[1][1] + ve[1][1])));
+        y1 = row_max(fmaxf(fmaxf(c[0][2] + ve[0][0], c[0][3] + ve[0][1]),
+                           fmaxf(c[1][2] + ve[1][0], c[1][3] + ve[1][1])));
+      }
+      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1 || (ELEM == 1 && (y0 > M0 || y1 > M1)))) {
         const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-        const float f0 = m0 == n0 ? 1.f : fast_exp2(m0 - n0), f1 = m1 == n1 ? 1.f : fast_exp2(m1 - n1);
+        float f0 = m0 == n0 ? 1.f : fast_exp2(m0 - n0), f1 = m1 == n1 ? 1.f : fast_exp2(m1 - n1);
         m0 = n0;
         m1 = n1;
         l0 *= f0;
         l1 *= f1;
+        if (ELEM == 1) {
+          const float N0 = fmaxf(M0, y0), N1 = fmaxf(M1, y1);
+          f0 = M0 == N0 ? 1.f : fast_exp2(M0 - N0);
+          f1 = M1 == N1 ? 1.f : fast_exp2(M1 - N1);
+          M0 = N0;
+          M1 = N1;
+          // 2^(m - M), 0 while the row has seen no value
+          g0 = M0 == -INFINITY ? 0.f : fast_exp2(m0 - M0);
+          g1 = M1 == -INFINITY ? 0.f : fast_exp2(m1 - M1);
+        }
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           o[i][0] *= f0;
@@ -340,8 +415,13 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
         const float p2 = fast_exp2(c[n][2] - r1), p3 = fast_exp2(c[n][3] - r1);
         l0 += p0 + p1;
         l1 += p2 + p3;
-        p[2 * n] = pack2(p0 * vs[n][0], p1 * vs[n][1], T());
-        p[2 * n + 1] = pack2(p2 * vs[n][0], p3 * vs[n][1], T());
+        if (ELEM == 1) {
+          p[2 * n] = pack2(p0 * g0 * vs[n][0], p1 * g0 * vs[n][1], __half());
+          p[2 * n + 1] = pack2(p2 * g1 * vs[n][0], p3 * g1 * vs[n][1], __half());
+        } else {
+          p[2 * n] = pack2(p0, p1, T());
+          p[2 * n + 1] = pack2(p2, p3, T());
+        }
       }
       // ---- o += p v ----
       const uint32_t va = smem_u32(vp) + (lane & 7) * 16;
@@ -358,10 +438,15 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
         for (int i = 0; i < D / 16; i += 2) {
           uint32_t b[4];  // pairs of neighbouring d, transposed
           ldsm4_t(va + ((mt & 1) * kChunks + i + (mt >> 1)) * 128, b);
-          mma16816<T>(o[2 * i], p, e4m3_even(b[0]), e4m3_even(b[1]));
-          mma16816<T>(o[2 * i + 1], p, e4m3_odd(b[0]), e4m3_odd(b[1]));
-          mma16816<T>(o[2 * i + 2], p, e4m3_even(b[2]), e4m3_even(b[3]));
-          mma16816<T>(o[2 * i + 3], p, e4m3_odd(b[2]), e4m3_odd(b[3]));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // (key, d): bytes (0, 0) (0, 1) (1, 0) (1, 1) -> even d's pair of keys, odd d's
+            uint32_t e0, d0, e1, d1;
+            e4m3x4_f16(__byte_perm(b[2 * h], 0u, 0x3120), e0, d0);
+            e4m3x4_f16(__byte_perm(b[2 * h + 1], 0u, 0x3120), e1, d1);
+            mma16816<__half>(o[2 * (i + h)], p, e0, e1);
+            mma16816<__half>(o[2 * (i + h) + 1], p, d0, d1);
+          }
         }
       }
       __syncwarp();  // the stage is free for block j + kStages
@@ -386,6 +471,16 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
     // ---- join the warps: O over the warp's own ring, m and l beside it ----
     __syncwarp();
     float* os = reinterpret_cast<float*>(ring);
+    if (ELEM == 1) {  // back from the reference M to m
+      const float f0 = M0 == -INFINITY ? 0.f : fast_exp2(M0 - m0), f1 = M1 == -INFINITY ? 0.f : fast_exp2(M1 - m1);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i][0] *= f0;
+        o[i][1] *= f0;
+        o[i][2] *= f1;
+        o[i][3] *= f1;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) {
       // 16-bit: columns of tile i are d = 8 i + n. 8-bit: tiles 2 j, 2 j + 1 hold
@@ -454,32 +549,37 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, 1) rows_kernel(con
 // Joins the spans of split units: an entry of the join list is RB rows (or fewer)
 // whose partial states lie `step` slots apart,
 //   M = max m_p, L = sum l_p 2^(m_p - M), o = sum o_p 2^(m_p - M) / L,
-// in slot order. A thread takes four columns of a row, and few rows go to a block,
-// so that a unit of many spans is spread over the SMs and many loads are in flight.
-template <typename T, int D, int SECTION>
-__global__ void __launch_bounds__(kJoinRows[SECTION] * D / 4) join_kernel(const AttnArgs a) {
-  constexpr int RB = kJoinRows[SECTION];
+// in slot order. A thread takes four columns of a row; few rows go to a block, and
+// GROUPS groups of threads share the spans (joined in shared memory, in order), so
+// that a unit of many spans has many loads in flight.
+template <typename T, int D, int SECTION, int GROUPS>
+__global__ void __launch_bounds__(kJoinRows[SECTION] * D / 4 * GROUPS) join_kernel(const AttnArgs a) {
+  constexpr int RB = kJoinRows[SECTION], kThreads = RB * D / 4;  // of a group
   constexpr int kSlotRows = SECTION == 0 ? kRowsTile : 128;
   constexpr int64_t kSlot = SECTION == 0 ? rows_slot_floats(D) : tile_slot_floats(D);
-  const int r = threadIdx.x % RB, col = threadIdx.x / RB;
+  __shared__ float4 sm_o[GROUPS > 1 ? GROUPS * kThreads : 1];
+  __shared__ float2 sm_ml[GROUPS > 1 ? GROUPS * RB : 1];
+  const int group = threadIdx.x / kThreads, t = threadIdx.x % kThreads;
+  const int r = t % RB, col = t / RB;
   grid_dep_wait();
   const int32_t* sec = a.plan + H_SECTION + SECTION * kSectionInts;
   const int G = a.plan[H_GROUP], n = sec[S_JOINS];
   const int32_t* list = a.plan + sec[S_OFF_JOINS];
   for (int b = blockIdx.x; b < n; b += gridDim.x) {
     const int32_t* J = list + b * kJoinInts;
-    if (r >= J[J_ROWS]) continue;
+    const bool live = r < J[J_ROWS];
     const int parts = J[J_PARTS], rq = J[J_ROW0] + r;
+    const int p0 = parts * group / GROUPS, p1 = live ? parts * (group + 1) / GROUPS : p0;
     const float* s0 = a.slots + J[J_SLOT] * kSlot;
     const int64_t step = J[J_STEP] * kSlot;
     const int at = J[J_SLOT_ROW] + r;
     float M = -INFINITY, L = 0.f;
 #pragma unroll 8
-    for (int p = 0; p < parts; ++p) M = fmaxf(M, s0[p * step + kSlotRows * D + at]);
-    const float ref = M == -INFINITY ? 0.f : M;
+    for (int p = p0; p < p1; ++p) M = fmaxf(M, s0[p * step + kSlotRows * D + at]);
+    float ref = M == -INFINITY ? 0.f : M;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-    for (int p = 0; p < parts; ++p) {
+    for (int p = p0; p < p1; ++p) {
       const float* sp = s0 + p * step;
       const float4 v = reinterpret_cast<const float4*>(sp)[col * kSlotRows + at];
       const float w = fast_exp2(sp[kSlotRows * D + at] - ref);
@@ -489,6 +589,32 @@ __global__ void __launch_bounds__(kJoinRows[SECTION] * D / 4) join_kernel(const 
       acc.z = fmaf(v.z, w, acc.z);
       acc.w = fmaf(v.w, w, acc.w);
     }
+    if (GROUPS > 1) {
+      sm_o[threadIdx.x] = acc;
+      if (col == 0) sm_ml[group * RB + r] = make_float2(M, L);
+      __syncthreads();
+      if (group == 0) {
+        M = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) M = fmaxf(M, sm_ml[g * RB + r].x);
+        ref = M == -INFINITY ? 0.f : M;
+        L = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const float2 ml = sm_ml[g * RB + r];
+          const float4 v = sm_o[g * kThreads + t];
+          const float w = fast_exp2(ml.x - ref);
+          L = fmaf(ml.y, w, L);
+          acc.x = fmaf(v.x, w, acc.x);
+          acc.y = fmaf(v.y, w, acc.y);
+          acc.z = fmaf(v.z, w, acc.z);
+          acc.w = fmaf(v.w, w, acc.w);
+        }
+      }
+      __syncthreads();
+    }
+    if (group > 0 || !live) continue;
     const int64_t tok = J[J_TOK0] + static_cast<int64_t>(rq / G);
     const int hq = J[J_HEAD] * G + rq % G;
     float lse2;
@@ -502,14 +628,27 @@ __global__ void __launch_bounds__(kJoinRows[SECTION] * D / 4) join_kernel(const 
   }
 }
 
-template <int SECTION>
-int run_join(const AttnArgs& a, int32_t dtype, int32_t head_dim, int entries, int num_ctas, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(entries < 16 * num_ctas ? entries : 16 * num_ctas));
-  const dim3 block(static_cast<unsigned>(kJoinRows[SECTION] * head_dim / 4));
+template <int SECTION, int GROUPS>
+int launch_join(const AttnArgs& a, int32_t dtype, int32_t head_dim, int blocks, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(blocks));
+  const dim3 block(static_cast<unsigned>(kJoinRows[SECTION] * head_dim / 4 * GROUPS));
   auto go = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, st, "join_kernel", a); };
   if (dtype == D2SD_DTYPE_BF16)
-    return head_dim == 128 ? go(join_kernel<__nv_bfloat16, 128, SECTION>) : go(join_kernel<__nv_bfloat16, 64, SECTION>);
-  return head_dim == 128 ? go(join_kernel<__half, 128, SECTION>) : go(join_kernel<__half, 64, SECTION>);
+    return head_dim == 128 ? go(join_kernel<__nv_bfloat16, 128, SECTION, GROUPS>)
+                           : go(join_kernel<__nv_bfloat16, 64, SECTION, GROUPS>);
+  return head_dim == 128 ? go(join_kernel<__half, 128, SECTION, GROUPS>)
+                         : go(join_kernel<__half, 64, SECTION, GROUPS>);
+}
+
+// Groups share the spans where a unit has more of them than one thread keeps in
+// flight (one token against 32k keys: 74 spans a unit).
+template <int SECTION>
+int run_join(const AttnArgs& a, int32_t dtype, int32_t head_dim, const int32_t* sec, int num_ctas,
+             bool fixed_grid, cudaStream_t st) {
+  const int most = 16 * num_ctas;
+  const int blocks = fixed_grid ? 8 * num_ctas : (sec[S_JOINS] < most ? sec[S_JOINS] : most);
+  if (fixed_grid || sec[S_PARTS] > 8) return launch_join<SECTION, SECTION == 0 ? 8 : 4>(a, dtype, head_dim, blocks, st);
+  return launch_join<SECTION, 1>(a, dtype, head_dim, blocks, st);
 }
 
 template <typename T, int D, int ELEM, bool UMMA>
@@ -588,7 +727,7 @@ extern "C" int d2sd_paged_attention(
   bool fits = num_ctas > 0;
   for (int s = 0; s < kSections; ++s) {
     const int32_t* sec = sections + s * kSectionInts;
-    fits = fits && sec[S_CTAS] <= num_ctas && sec[S_SLOTS] <= 2 * num_ctas;
+    fits = fits && sec[S_CTAS] <= section_ctas(s, num_ctas) && sec[S_SLOTS] <= 2 * section_ctas(s, num_ctas);
   }
   if (!fits)
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": the plan is for another grid");
@@ -617,7 +756,7 @@ extern "C" int d2sd_paged_attention(
   AttnArgs t = a;  // the tiles kernel's half of the workspace
   t.slots += tile_slots_at(num_ctas, head_dim);
   if (sections[S_ITEMS] > 0 || fixed_grid) {
-    rc = run_rows(a, dtype, head_dim, scaled, fixed_grid ? num_ctas : sections[S_CTAS], st);
+    rc = run_rows(a, dtype, head_dim, scaled, fixed_grid ? section_ctas(0, num_ctas) : sections[S_CTAS], st);
     if (rc) return rc;
   }
   if (tiles[S_ITEMS] > 0 || fixed_grid) {
@@ -626,10 +765,9 @@ extern "C" int d2sd_paged_attention(
     if (rc) return rc;
   }
   if (sections[S_JOINS] > 0 || fixed_grid) {
-    rc = run_join<0>(a, dtype, head_dim, fixed_grid ? 4 * num_ctas : sections[S_JOINS], num_ctas, st);
+    rc = run_join<0>(a, dtype, head_dim, sections, num_ctas, fixed_grid != 0, st);
     if (rc) return rc;
   }
-  if (tiles[S_JOINS] > 0 || fixed_grid)
-    rc = run_join<1>(t, dtype, head_dim, fixed_grid ? 8 * num_ctas : tiles[S_JOINS], num_ctas, st);
+  if (tiles[S_JOINS] > 0 || fixed_grid) rc = run_join<1>(t, dtype, head_dim, tiles, num_ctas, fixed_grid != 0, st);
   return rc;
 }

@@ -30,22 +30,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// Bytes 0 and 2 (even) or 1 and 3 (odd) of x, e4m3, to two bf16. Moving sign and
-// magnitude into a bf16's places gives value * 2^-120 (the exponent biases differ
-// by 120; subnormals likewise), so a product with 2^120 ends it. NaN (0x7f) is
-// not one after this; the writer marks such rows in their scale byte.
-__device__ __forceinline__ uint32_t mul_2p120(uint32_t x) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7b807b80u));
-  return r;
-}
-__device__ __forceinline__ uint32_t e4m3_even(uint32_t x) {
-  return mul_2p120(((x & 0x00800080u) << 8) | ((x & 0x007f007fu) << 4));
-}
-__device__ __forceinline__ uint32_t e4m3_odd(uint32_t x) {
-  return mul_2p120((x & 0x80008000u) | ((x & 0x7f007f00u) >> 4));
-}
-
 // 1 / sum and log-sum-exp (base 2) of a row with maximum m and sum l: 0 and -inf for
 // a row that saw no key, NaN for one with a NaN.
 __device__ __forceinline__ float row_factor(float m, float l, float& lse2) {

@@ -31,7 +31,7 @@ struct Unit {
 // tiles and `extra` more (its start, its end and, for a split unit, the joining),
 // each of the unit's weight, so a CTA of many small items gets fewer tiles.
 void cut(const std::vector<Unit>& units, int ctas, int section, int32_t group, int32_t window,
-         std::vector<int32_t>& items, std::vector<int32_t>& first, std::vector<int32_t>& joins, int32_t* slots) {
+         std::vector<int32_t>& items, std::vector<int32_t>& first, std::vector<int32_t>& joins, int32_t* slots, int32_t* most) {
   const int extra = section == 0 ? 1 : 4;
   const int q_tile = section == 0 ? kRowsTile : 128 / group * group, per = section == 0 ? 1 : 2;
   int64_t total = 0, tiles = 0;
@@ -41,6 +41,7 @@ void cut(const std::vector<Unit>& units, int ctas, int section, int32_t group, i
   }
   const int64_t n = std::max<int64_t>(1, std::min<int64_t>(ctas, tiles));
   *slots = 0;
+  *most = 1;
   first.assign(1, 0);
   int64_t done = 0;  // cost handed out so far
   int32_t count = 0;
@@ -87,6 +88,7 @@ void cut(const std::vector<Unit>& units, int ctas, int section, int32_t group, i
       r += n;
     }
     *slots += parts;
+    *most = std::max(*most, parts);
   }
   first.push_back(count);
 }
@@ -108,8 +110,10 @@ extern "C" int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_r
     units += (q_lens[r] * G + kRowsTile - 1) / kRowsTile * num_kv_heads;
   }
   // every CTA adds at most one cut; a cut unit has at most 256 rows to join
-  return kHeaderInts + (units + 2 * static_cast<int64_t>(num_ctas)) * kItemInts + 4 * (num_ctas + 2) +
-         static_cast<int64_t>(num_ctas) * (256 / 8) * kJoinInts;
+  const int64_t ctas = section_ctas(0, num_ctas) + section_ctas(1, num_ctas);
+  return kHeaderInts + (units + 2 * ctas) * kItemInts + 2 * (ctas + 8) +
+         (static_cast<int64_t>(section_ctas(0, num_ctas)) * (kRowsTile / kJoinRows[0]) +
+          static_cast<int64_t>(num_ctas) * (256 / kJoinRows[1])) * kJoinInts;
 }
 
 extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
@@ -173,7 +177,7 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
       int32_t sec[kSectionInts] = {0};
       if (!units[s].empty()) {
         std::vector<int32_t> items, first, joins;
-        cut(units[s], num_ctas, s, G, window, items, first, joins, &sec[S_SLOTS]);
+        cut(units[s], section_ctas(s, num_ctas), s, G, window, items, first, joins, &sec[S_SLOTS], &sec[S_PARTS]);
         sec[S_CTAS] = static_cast<int32_t>(first.size()) - 1;
         sec[S_ITEMS] = static_cast<int32_t>(items.size() / kItemInts);
         sec[S_OFF_CTA] = static_cast<int32_t>(out.size());

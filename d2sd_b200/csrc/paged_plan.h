@@ -16,12 +16,13 @@ namespace paged {
 
 constexpr int kTileKeys = 128;
 constexpr int kRowsTile = 16;    // query rows of a unit of the rows kernel
+constexpr int kRowsCtas = 4;     // CTAs of the rows kernel on an SM
 constexpr int kRowsLimit = 16;   // requests of more rows per kv head go to the tiles kernel
 constexpr int kMagic = 0x50474131;
 
 // header: magic, then one section per kernel (S_*), kSectionInts ints each
 enum { H_MAGIC = 0, H_REQUESTS, H_TOKENS, H_GROUP, H_KV_HEADS, H_SECTION, };
-enum { S_CTAS = 0, S_ITEMS, S_SLOTS, S_JOINS, S_OFF_CTA, S_OFF_ITEMS, S_OFF_JOINS, kSectionInts };
+enum { S_CTAS = 0, S_ITEMS, S_SLOTS, S_JOINS, S_OFF_CTA, S_OFF_ITEMS, S_OFF_JOINS, S_PARTS, kSectionInts };  // S_PARTS: most spans of a unit
 constexpr int kSections = 2;  // 0: rows kernel, 1: tiles kernel
 constexpr int kHeaderInts = 32;
 
@@ -63,10 +64,11 @@ constexpr int kJoinRows[kSections] = {4, 8};
 // A slot holds [head_dim / 4][rows] of four columns each, then the rows' m and l.
 // A CTA's first and last item can be spans of split units, so 2 slots per CTA do
 // (tiles: 4, one for each q tile). Workspace: the rows slots, then the tiles slots.
+constexpr int section_ctas(int section, int num_ctas) { return section == 0 ? kRowsCtas * num_ctas : num_ctas; }
 constexpr int64_t rows_slot_floats(int head_dim) { return kRowsTile * (head_dim + 2); }
 constexpr int64_t tile_slot_floats(int head_dim) { return 128 * (head_dim + 2); }
 constexpr int64_t tile_slots_at(int num_ctas, int head_dim) {  // floats
-  return 2 * static_cast<int64_t>(num_ctas) * rows_slot_floats(head_dim);
+  return 2 * static_cast<int64_t>(section_ctas(0, num_ctas)) * rows_slot_floats(head_dim);
 }
 constexpr int64_t workspace_bytes(int num_ctas, int head_dim) {
   return 4 * (tile_slots_at(num_ctas, head_dim) + 4 * static_cast<int64_t>(num_ctas) * tile_slot_floats(head_dim));

@@ -17,7 +17,7 @@ def make(lib, q, kv, off, Hq, Hk, causal, window, ctas):
     from d2sd_b200._lib import check
     q, kv, off = (np.ascontiguousarray(x, dtype=np.int32) for x in (q, kv, off))
     cap = lib.d2sd_paged_plan_capacity(q.ctypes.data, len(q), Hq, Hk, ctas)
-    plan, used, sec = np.zeros(cap, np.int32), np.zeros(1, np.int64), np.zeros(14, np.int32)
+    plan, used, sec = np.zeros(cap, np.int32), np.zeros(1, np.int64), np.zeros(16, np.int32)
     check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, len(q), Hq, Hk, causal,
                               window, ctas, plan.ctypes.data, cap, used.ctypes.data,
                               sec.ctypes.data), "plan")
@@ -43,14 +43,15 @@ def test_plan_covers_every_tile_once(lib, q, kv, Hq, Hk, causal, window, ctas):
     starts = np.cumsum([0] + list(q))
     seen = {}
     for s in range(2):
-        nct, nit, nslots, njoin, oc, oi, oj = sec[7 * s:7 * s + 7]
-        assert list(plan[5 + 7 * s:12 + 7 * s]) == list(sec[7 * s:7 * s + 7])
+        nct, nit, nslots, njoin, oc, oi, oj, most_parts = sec[8 * s:8 * s + 8]
+        assert list(plan[5 + 8 * s:13 + 8 * s]) == list(sec[8 * s:8 * s + 8])
         if nit == 0:
             continue
         q_tile = 16 if s == 0 else 128 // G * G
         cta = plan[oc:oc + nct + 1]
-        assert nct <= ctas and cta[0] == 0 and cta[-1] == nit and (np.diff(cta) >= 0).all()
-        assert nslots <= 2 * ctas and oi % 4 == 0
+        most = 4 * ctas if s == 0 else ctas
+        assert nct <= most and cta[0] == 0 and cta[-1] == nit and (np.diff(cta) >= 0).all()
+        assert nslots <= 2 * most and oi % 4 == 0
         items = plan[oi:oi + 16 * nit].reshape(-1, 16)
         slots, split = set(), {}
         for it in items:
@@ -68,6 +69,7 @@ def test_plan_covers_every_tile_once(lib, q, kv, Hq, Hk, causal, window, ctas):
                 assert slot == first + len(unit[1]) - 1 and slot not in slots  # spans in slot order
                 slots.add(slot)
         assert slots == set(range(nslots))
+        assert most_parts == max([x[1] for x in split.values()], default=1)
         # join list: every row of every split unit once, with its slot
         joined = {}
         for j in plan[oj:oj + 8 * njoin].reshape(-1, 8):
@@ -123,7 +125,7 @@ def test_plan_refusals(lib):
         make(lib, [1], [1], [0], 129, 1, 1, 0, 8)
     import ctypes
     n = np.ones(1, np.int32)
-    buf, used, sec = np.zeros(4, np.int32), np.zeros(1, np.int64), np.zeros(14, np.int32)
+    buf, used, sec = np.zeros(4, np.int32), np.zeros(1, np.int64), np.zeros(16, np.int32)
     rc = lib.d2sd_paged_plan(n.ctypes.data, n.ctypes.data, ctypes.c_void_p(np.zeros(1, np.int32).ctypes.data),
                              1, 4, 2, 1, 0, 8, buf.ctypes.data, 4, used.ctypes.data, sec.ctypes.data)
     assert rc == 3 and "small" in lib.d2sd_last_error().decode()
@@ -133,9 +135,9 @@ def test_plan_refusals(lib):
 
 def test_empty_batches(lib):
     plan, sec = make(lib, [], [], [], 4, 2, 1, 0, 8)
-    assert sec[1] == 0 and sec[8] == 0
+    assert sec[1] == 0 and sec[9] == 0
     plan, sec = make(lib, [0, 0], [7, 0], [0, 1], 4, 2, 1, 0, 8)
-    assert sec[1] == 0 and sec[8] == 0
+    assert sec[1] == 0 and sec[9] == 0
 
 
 def test_e4m3_oracle_against_the_type():
