@@ -94,6 +94,13 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// 2^e of a scale byte. A row marked NaN (255, here 2^128) has NaN values too, so the
+// product is NaN; e of byte 0 (factor 0) is only a reference for the weights.
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+__device__ __forceinline__ float exponent_of(uint32_t byte) {  // byte - 127
+  return __uint_as_float(0x4b000000u | byte) - (8388608.f + 127.f);
+}
+
 // The four e4m3 values of x as two pairs of f16 (bytes 0 and 1, bytes 2 and 3).
 __device__ __forceinline__ void e4m3x4_f16(uint32_t x, uint32_t& lo, uint32_t& hi) {
   asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
@@ -138,7 +145,9 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
   if (static_cast<int>(blockIdx.x) >= sec[S_CTAS]) return;  // a fixed grid's spare CTA
   const int item0 = a.plan[sec[S_OFF_CTA] + blockIdx.x], item1 = a.plan[sec[S_OFF_CTA] + blockIdx.x + 1];
   const int qr = lane >> 2, qc = lane & 3;
-  uint32_t uses = 0;  // stages this warp has consumed so far (ring position and parity)
+  // ring positions of this warp: the stage to fill next; the stage to read next and
+  // the parity of its phase
+  uint32_t fill = 0, read = 0, parity = 0;
 
   for (int it = item0; it < item1; ++it) {
     const int32_t* I = a.plan + sec[S_OFF_ITEMS] + it * kItemInts;
@@ -234,7 +243,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
     auto issue = [&](int j) {  // fetch block j of mine into its stage
       if ((j & 31) == 0) fetch_ids(j);
       const int64_t page = __shfl_sync(0xffffffffu, ids, j & 31);
-      const uint32_t st = (uses + j) % C::kStages;
+      const uint32_t st = fill;
+      fill = fill + 1 == C::kStages ? 0 : fill + 1;
       uint8_t* dst = ring + st * C::kStageBytes;
       const int64_t off = page * a.g.stride_page + head * a.g.stride_head;
       if (UMMA) {
@@ -277,9 +287,9 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       // the stage freed by block j - 1 takes block j + kStages - 1
       if (j + C::kStages - 1 < mine) issue(j + C::kStages - 1);
       commit();
-      const uint32_t st = (uses + j) % C::kStages;
+      const uint32_t st = read;
       if (UMMA) {
-        const bool ok = mbar_wait(&full[st], ((uses + j) / C::kStages) & 1, flags);
+        const bool ok = mbar_wait(&full[st], parity, flags);
         if (!__all_sync(0xffffffffu, ok)) {
           alive = false;
           break;
@@ -338,8 +348,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
           const uint8_t* sp = kp + 2 * C::kPageBytes + n * 8 + qc * 2;
           const uint32_t kb = *reinterpret_cast<const uint16_t*>(sp);
           vb[n] = *reinterpret_cast<const uint16_t*>(sp + 16);
-          k0 = e4m3_scale(kb & 255u);
-          k1 = e4m3_scale(kb >> 8);
+          k0 = scale_of(kb & 255u);
+          k1 = scale_of(kb >> 8);
         }
         c[n][0] *= row_scale[0] * k0;
         c[n][1] *= row_scale[0] * k1;
@@ -374,8 +384,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t byte = (vb[n] >> (8 * e)) & 255u;
-            vs[n][e] = e4m3_scale(byte);
-            ve[n][e] = byte == 0u ? -INFINITY : static_cast<float>(static_cast<int>(byte) - 127);
+            vs[n][e] = scale_of(byte);
+            ve[n][e] = exponent_of(byte);
           }
         y0 = row_max(fmaxf(fmaxf(c[0][0] + ve[0][0], c[0][1] + ve[0][1]),
                            fmaxf(c[1][0] + ve[1][0], c[1][1] + ve[1][1])));
@@ -450,6 +460,7 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
         }
       }
       __syncwarp();  // the stage is free for block j + kStages
+      if (++read == C::kStages) read = 0, parity ^= 1;
     }
     if (!alive) {
       // give up: wait (bounded) for the copies in flight, so that none lands in
@@ -457,12 +468,11 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       flags[0] = 1;
       for (int x = j; x < min(j + C::kStages, mine); ++x) {
         const uint64_t t0 = global_timer_ns();
-        while (!mbar_try_wait(&full[(uses + x) % C::kStages], ((uses + x) / C::kStages) & 1) &&
-               global_timer_ns() - t0 < kWaitTimeoutNs) {
+        while (!mbar_try_wait(&full[read], parity) && global_timer_ns() - t0 < kWaitTimeoutNs) {
         }
+        if (++read == C::kStages) read = 0, parity ^= 1;
       }
     }
-    uses += mine;
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
