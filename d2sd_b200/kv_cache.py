@@ -15,6 +15,11 @@ tensor core's no-swizzle core-matrix order -- [2 groups of 8 rows][D/8 chunks of
 and feeds it to tcgen05.mma as it lands, whatever the page table's order. With
 layout="hnd" a block holds plain rows (fetched through TMA tensor boxes). Pools
 are zero-initialised so every slot past a sequence's length holds finite values.
+
+``dtype=torch.float8_e4m3fn`` keeps rows in 8 bits: e4m3 values and one scale byte
+for each (layer, page, head, slot) in ``k_scale`` / ``v_scale`` (a power of two; see
+include/d2sd.h), half of a bf16 cache's bytes. ``append`` and ``commit`` quantise as
+they write, ``ops.read_kv`` (``read``, ``gather``) and ``paged_attention`` read it.
 """
 from __future__ import annotations
 
@@ -29,7 +34,11 @@ class PagedKVCache:
                  page_order: torch.Tensor | None = None, layout: str = "umma"):
         if layout not in ("umma", "hnd"):
             raise ValueError("layout must be 'umma' or 'hnd'")
-        if layout == "umma" and (page_size != 16 or head_dim % 8 or dtype.itemsize != 2):
+        self.quantised = dtype == torch.float8_e4m3fn
+        if self.quantised and (layout != "umma" or page_size != 16 or head_dim not in (64, 128)):
+            raise ValueError("8-bit rows are kept in umma pages of 16 rows, head_dim 64 or 128")
+        if layout == "umma" and (page_size != 16 or head_dim % 8
+                                 or (dtype.itemsize != 2 and not self.quantised)):
             raise ValueError("umma pages hold 16 rows of 16-bit values")
         self.layout = layout
         self.num_layers, self.num_kv_heads, self.head_dim = num_layers, num_kv_heads, head_dim
@@ -40,12 +49,18 @@ class PagedKVCache:
         shape = (num_layers, self.num_pages, num_kv_heads, page_size, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=self.device)
         self.v = torch.zeros(shape, dtype=dtype, device=self.device)
+        self.k_scale = self.v_scale = None
+        if self.quantised:
+            self.k_scale = torch.zeros(shape[:4], dtype=torch.uint8, device=self.device)
+            self.v_scale = torch.zeros_like(self.k_scale)
         # logical page i of the sequence -> physical page page_table[i]
         if page_order is None:
             page_order = torch.arange(self.num_pages)
         if page_order.numel() != self.num_pages:
             raise ValueError("page_order must list every page once")
         self.page_table = page_order.to(torch.int32).to(self.device)
+        # first page-table entry of each sequence, and the end (one sequence here)
+        self.page_bounds = torch.tensor([0, self.num_pages], dtype=torch.int32, device=self.device)
         self.length = 0
         self._ptr_cache: dict = {}
 
@@ -53,6 +68,10 @@ class PagedKVCache:
     def layer(self, l: int):
         """(k_pool, v_pool) of layer l, [num_pages, Hk, page_size, D]."""
         return self.k[l], self.v[l]
+
+    def scales(self, l: int):
+        """(k_scale, v_scale) of layer l, uint8 [num_pages, Hk, 16]; Nones unless 8-bit."""
+        return (self.k_scale[l], self.v_scale[l]) if self.quantised else (None, None)
 
     @property
     def kv_layout(self) -> str:
@@ -69,10 +88,56 @@ class PagedKVCache:
         pt = self.page_table.to(pos.device).long()
         return pt[pos // self.page_size], pos % self.page_size
 
+    # -- the target's own tokens ---------------------------------------------
+    def append(self, l: int, k: torch.Tensor, v: torch.Tensor, token_start: torch.Tensor,
+               first_pos: torch.Tensor, **kw):
+        """``ops.append_kv`` into layer l: sequence r's new rows are token_start[r] ..
+        token_start[r + 1] - 1 of k, v (int32 [sequences + 1], device) and go to its
+        positions first_pos[r] onward (int32, device). Takes its keyword arguments
+        (q, q_out, q_weight, k_weight, eps, cos, sin, interleaved, status) and returns
+        the rotated q. The caller advances the lengths, once all layers are written."""
+        ks, vs = self.scales(l)
+        return ops.append_kv(k, v, self.k[l], self.v[l], self.kv_layout, self.page_table,
+                             self.page_bounds, token_start, first_pos, k_scale=ks, v_scale=vs, **kw)
+
+    def read(self, l: int, token_start: torch.Tensor, first_pos: torch.Tensor, k_out: torch.Tensor,
+             v_out: torch.Tensor, status: torch.Tensor | None = None) -> None:
+        """``ops.read_kv`` out of layer l: rows token_start[r] .. of k_out, v_out
+        [tokens, Hk, D] from sequence r's positions first_pos[r] on."""
+        ks, vs = self.scales(l)
+        ops.read_kv(self.k[l], self.v[l], self.kv_layout, self.page_table, self.page_bounds,
+                    token_start, first_pos, k_out, v_out, k_scale=ks, v_scale=vs, status=status)
+
+    def _span(self, n: int) -> torch.Tensor:
+        """int32 [0, n] on the device, without a copy from the host (n > 0)."""
+        return torch.arange(0, n + 1, n, dtype=torch.int32, device=self.device)
+
+    def _rows_of(self, l: int, s: int, n: int, dtype=torch.bfloat16):
+        """The first n rows of sequence s of an 8-bit layer, [n, Hk, D]."""
+        out = torch.empty(2, n, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
+        if n > 0:
+            ks, vs = self.scales(l)
+            ops.read_kv(self.k[l], self.v[l], self.kv_layout, self.page_table,
+                        self.page_bounds[s:s + 2], self._span(n),
+                        torch.zeros(1, dtype=torch.int32, device=self.device), out[0], out[1],
+                        k_scale=ks, v_scale=vs)
+        return out[0], out[1]
+
     # -- host-side set-up (not on the hot path) ------------------------------
     def write(self, l: int, k: torch.Tensor, v: torch.Tensor, start: int = 0) -> None:
         """Write k, v [n, Hk, D] at positions start .. start+n-1 of layer l."""
         n = k.shape[0]
+        if self.quantised:
+            pages = self.page_table.numel()
+            if start + n > pages * self.page_size:
+                raise ValueError("cache capacity exceeded")
+            if n > 0:
+                ks, vs = self.scales(l)
+                ops.append_kv(k, v, self.k[l], self.v[l], self.kv_layout, self.page_table,
+                              self._span(pages), self._span(n),
+                              torch.full((1,), start, dtype=torch.int32, device=self.device),
+                              k_scale=ks, v_scale=vs)
+            return
         pos = torch.arange(start, start + n, device=self.device)
         page, slot = self.positions_to_slots(pos)
         if self.layout == "hnd":
@@ -87,6 +152,8 @@ class PagedKVCache:
     def gather(self, l: int, length: int | None = None):
         """Layer l as contiguous [length, Hk, D] tensors (for checks)."""
         n = self.length if length is None else length
+        if self.quantised:
+            return self._rows_of(l, 0, n)
         pos = torch.arange(n, device=self.device)
         page, slot = self.positions_to_slots(pos)
         if self.layout == "hnd":
@@ -107,11 +174,30 @@ class PagedKVCache:
             for l in range(self.num_layers):
                 vals += [new_k[l].data_ptr(), new_v[l].data_ptr(), self.k[l].data_ptr(),
                          self.v[l].data_ptr()]
+                if self.quantised:
+                    vals += [self.k_scale[l].data_ptr(), self.v_scale[l].data_ptr()]
             ptrs = torch.tensor(vals, dtype=torch.int64).to(self.device)
             if len(self._ptr_cache) > 16:
                 self._ptr_cache.clear()
             self._ptr_cache[key] = ptrs
         return ptrs
+
+    def _row_dtype(self, new: torch.Tensor) -> torch.dtype:
+        """The dtype of rows a commit takes: the cache's, 16-bit ones for an 8-bit cache."""
+        if not self.quantised:
+            return self.dtype
+        return new.dtype if new.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+
+    def _commit_e4m3(self, new_k, new_v, new_strides, sequences, accept_results, cache_lens):
+        kl, sl = self.k[0], self.k_scale[0]
+        ops.commit_kv_e4m3(self._layer_ptrs(new_k, new_v), num_layers=self.num_layers,
+                           num_requests=sequences, num_kv_heads=new_k[0].shape[1],
+                           head_dim=new_k[0].shape[3], dtype=new_k[0].dtype,
+                           block_len=new_k[0].shape[2], new_strides=new_strides,
+                           cache_strides=(kl.stride(0), kl.stride(1)), num_pages=kl.shape[0],
+                           scale_strides=(sl.stride(0), sl.stride(1)), page_table=self.page_table,
+                           page_bounds=self.page_bounds, accept_results=accept_results,
+                           cache_lens=cache_lens)
 
     def commit(self, new_k, new_v, accept_result: torch.Tensor, advance_by: int | None = None,
                cache_len: int | None = None, target_hidden=None) -> None:
@@ -137,12 +223,20 @@ class PagedKVCache:
             raise ValueError("one new K/V tensor per layer is required")
         s = new_k[0].stride()
         for t in list(new_k) + list(new_v):
-            if t.stride() != s or t.dtype != self.dtype or t.stride(-1) != 1:
+            if t.stride() != s or t.dtype != self._row_dtype(new_k[0]) or t.stride(-1) != 1:
                 raise ValueError("new K/V tensors must share strides and the cache dtype")
         B, Hk, T, D = new_k[0].shape
         start = self.length if cache_len is None else cache_len
         if start + T > self.num_pages * self.page_size:
             raise ValueError("cache capacity exceeded")
+        if self.quantised:
+            if target_hidden is not None:
+                raise NotImplementedError("target_hidden with an 8-bit cache: gather it separately")
+            self._commit_e4m3(new_k, new_v, (0, s[0], s[1], s[2]), 1, accept_result,
+                              torch.full((1,), start, dtype=torch.int32, device=self.device))
+            if advance_by is not None:
+                self.length = start + int(advance_by)
+            return
         kl = self.k[0]
         hkw = {}
         if target_hidden is not None:
@@ -202,6 +296,7 @@ class PagedKVPool(PagedKVCache):
         self.capacities = caps
         self.page_offsets_host = offsets
         self.page_offsets = torch.tensor(offsets, dtype=torch.int32, device=self.device)
+        self.page_bounds = torch.tensor(offsets + [cur], dtype=torch.int32, device=self.device)
         self.lengths = [0] * len(caps)
         self.lengths_dev = torch.zeros(len(caps), dtype=torch.int32, device=self.device)
 
@@ -213,6 +308,16 @@ class PagedKVPool(PagedKVCache):
         self.lengths = [int(x) for x in lengths]
         self.lengths_dev.copy_(torch.tensor(self.lengths, dtype=torch.int32))
 
+    def plan(self, q_lens, num_qo_heads: int, **kw):
+        """A ``PagedAttentionPlan`` of every sequence's q_lens[s] newest tokens, which
+        ``append`` has written and ``lengths`` counts (its keyword arguments: causal,
+        window, reserve)."""
+        from .paged import PagedAttentionPlan
+        if len(q_lens) != self.num_seqs:
+            raise ValueError("q_lens must have an entry for each sequence")
+        return PagedAttentionPlan(q_lens, self.lengths, num_qo_heads, self.num_kv_heads, self.head_dim,
+                                  self.device, page_offsets=self.page_offsets_host, **kw)
+
     def write_seq(self, l: int, s: int, k: torch.Tensor, v: torch.Tensor, start: int = 0) -> None:
         """Write k, v [n, Hk, D] at positions start.. of sequence s, layer l."""
         if start + k.shape[0] > self.capacities[s]:
@@ -221,6 +326,8 @@ class PagedKVPool(PagedKVCache):
 
     def gather_seq(self, l: int, s: int, length: int):
         """Sequence s of layer l as contiguous [length, Hk, D] tensors (for checks)."""
+        if self.quantised:
+            return self._rows_of(l, s, length)
         base = self.page_offsets_host[s] * self.page_size
         pos = torch.arange(base, base + length, device=self.device)
         page, slot = self.positions_to_slots(pos)
@@ -248,11 +355,15 @@ class PagedKVPool(PagedKVCache):
             raise ValueError("one new K/V tensor per layer is required")
         s = new_k[0].stride()
         for t in list(new_k) + list(new_v):
-            if t.stride() != s or t.dtype != self.dtype or t.stride(-1) != 1:
+            if t.stride() != s or t.dtype != self._row_dtype(new_k[0]) or t.stride(-1) != 1:
                 raise ValueError("new K/V tensors must share strides and the cache dtype")
         RB, Hk, T, D = new_k[0].shape
         if RB != self.num_seqs * num_branches:
             raise ValueError("new K/V rows must be sequences x branches")
+        if self.quantised:
+            self._commit_e4m3(new_k, new_v, (num_branches * s[0], s[0], s[1], s[2]), self.num_seqs,
+                              accept_results, self.lengths_dev)
+            return
         kl = self.k[0]
         ops.commit_kv_batch(self._layer_ptrs(new_k, new_v), num_layers=self.num_layers,
                             num_requests=self.num_seqs, num_kv_heads=Hk, head_dim=D,

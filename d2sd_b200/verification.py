@@ -16,7 +16,8 @@ the sink rescale (:152-176). The GPT-OSS sliding layers see the last
 holding the same prefix (its ``length`` positions of every layer); with the
 paged cache the whole D3 step -- this forward, ``verify`` and
 ``PagedKVCache.commit`` -- runs without the reference's per-step
-reallocation of the cache.
+reallocation of the cache. An 8-bit cache's rows are read back into bf16 layer by
+layer.
 
 ``cascade_graph_runner`` is accepted for call compatibility; the fused kernel
 (b) already does what the runner's graph did.
@@ -40,6 +41,9 @@ def _prefix(past_key_values, idx):
     [1, Hk, P, D] is read in place as an HND tensor."""
     if isinstance(past_key_values, PagedKVCache):
         c = past_key_values
+        if c.quantised:  # kernel (a) takes 16-bit rows: the layer's rows, read back
+            k, v = c.gather(idx)
+            return k, v, "nhd", c.length, None
         return c.k[idx], c.v[idx], c.kv_layout, c.length, c.page_table
     layer = past_key_values.layers[idx]
     return layer.keys[0], layer.values[0], "hnd", layer.keys.shape[2], None

@@ -487,3 +487,145 @@ def test_refusals(cuda_device):
             (NotImplementedError, (q, z(4, 2, 8, 64), z(4, 2, 8, 64), "paged_hnd", one[0], plan), {})]:
         with pytest.raises(err):
             d.paged_attention(*a, **kw)
+
+
+# ---------------------------------------------------------------------------
+# the operators together, through the caches
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,layout", [(torch.bfloat16, "umma"), (torch.bfloat16, "hnd"),
+                                          (E4M3, "umma")])
+def test_serving_steps_through_the_pool(cuda_device, dtype, layout):
+    """Prompts in two chunks, then single tokens, of three sequences through one
+    pool: each step appends (norm, rotary) and attends, against the same steps in
+    float64 from the rows that the cache holds."""
+    import d2sd_b200 as d
+    dev = cuda_device
+    L, Hq, Hk, D = 2, 8, 2, 128
+    g = torch.Generator().manual_seed(77)
+    pool = d.PagedKVPool(L, Hk, D, [400, 90, 300], dtype=dtype, device=dev, shuffle_seed=1,
+                         layout=layout)
+    cos, sin = d.rope_tables(512, D, 1e6, dev)
+    w = [(1 + 0.2 * torch.randn(D, generator=g)).to(torch.bfloat16) for _ in range(2)]
+    lens = [0, 0, 0]
+    kept = [[[], []] for _ in range(3)]  # float64 k and v of each sequence, layer 1
+    for new in ([150, 60, 9], [201, 0, 88], [1, 1, 1], [1, 1, 1]):
+        n = sum(new)
+        starts = torch.tensor([0] + list(np.cumsum(new)), dtype=torch.int32, device=dev)
+        pool.set_lengths(lens)
+        qkv = [torch.randn(n, Hq + 2 * Hk, D, generator=g).to(torch.bfloat16) for _ in range(L)]
+        qs = []
+        for l in range(L):
+            x = qkv[l].to(dev)
+            qs.append(pool.append(l, x[:, Hq:Hq + Hk], x[:, Hq + Hk:], starts, pool.lengths_dev,
+                                  q=x[:, :Hq], q_weight=w[0].to(dev), k_weight=w[1].to(dev),
+                                  cos=cos, sin=sin))
+        pos = torch.cat([torch.arange(a, a + b) for a, b in zip(lens, new)])
+        lens = [a + b for a, b in zip(lens, new)]
+        pool.set_lengths(lens)
+        plan = pool.plan(new, Hq)
+        for l in range(L):
+            ks, vs = pool.scales(l)
+            out, lse = d.paged_attention(qs[l], pool.k[l], pool.v[l], pool.kv_layout,
+                                         pool.page_table, plan, k_scale=ks, v_scale=vs)
+        # layer 1: what append computes, then the attention of the rows the cache holds
+        x = qkv[1].double()
+        rot = lambda y, i: OP.norm_rotate(y, w[i], 1e-6, cos.cpu(), sin.cpu(), pos, False)  # noqa
+        q64, k64 = rot(x[:, :Hq], 0), rot(x[:, Hq:Hq + Hk], 1)
+        u = 2.0 ** -8
+        got = qs[1].double().cpu()
+        assert ((got - q64).abs() <= u * q64.abs() + 2.0 ** -17 * q64.abs().amax(-1, True) + 1e-30).all()
+        at = 0
+        for s, m in enumerate(new):
+            kept[s][0].append(k64[at:at + m])
+            kept[s][1].append(x[at:at + m, Hq + Hk:])
+            at += m
+        rows = [pool.gather_seq(1, s, lens[s]) for s in range(3)]
+        for s in range(3):
+            for i in range(2):
+                want = torch.cat(kept[s][i])
+                err = (rows[s][i].double().cpu() - want).abs()
+                top = want.abs().amax(-1, keepdim=True)
+                tol = ((2.0 ** -8 * want.abs() + 2.0 ** -17 * top) if dtype != E4M3 else
+                       torch.maximum(want.abs() * 2.0 ** -4, top * 2 / 448 * 2.0 ** -10)
+                       + 2.0 ** -17 * top)
+                assert (err <= tol + 1e-30).all(), (s, i)
+        c = dict(k_rows=[r[0].double().cpu() for r in rows], v_rows=[r[1].double().cpu() for r in rows])
+        check_attention(out, lse, qs[1], c, new, D, torch.bfloat16)
+    with pytest.raises(ValueError):
+        pool.plan([1, 1], Hq)
+
+
+@pytest.mark.parametrize("pooled", [False, True])
+def test_commit_into_an_8bit_cache(cuda_device, pooled):
+    import d2sd_b200 as d
+    dev = cuda_device
+    L, B, T, Hk, D = 3, 4, 16, 2, 64
+    g = torch.Generator().manual_seed(12)
+    S = 3 if pooled else 1
+    lens = [37, 0, 16][:S]
+    if pooled:
+        cache = d.PagedKVPool(L, Hk, D, [80, 40, 33], dtype=E4M3, device=dev, shuffle_seed=3)
+        cache.set_lengths(lens)
+    else:
+        cache = d.PagedKVCache(L, Hk, D, 80, dtype=E4M3, device=dev,
+                               page_order=torch.randperm(5, generator=g))
+        cache.length = 37
+    old = []
+    for s in range(S):
+        x = torch.randn(lens[s], Hk, D, generator=g).to(torch.bfloat16)
+        for l in range(L):
+            if lens[s]:
+                (cache.write_seq(l, s, x.to(dev), -x.to(dev)) if pooled else
+                 cache.write(l, x.to(dev), -x.to(dev)))
+        old.append(OP.e4m3_rows(x.double())[0])
+    # the projections' token-major rows seen as [B, Hk, T, D]
+    new = [torch.randn(2, S * B, T, Hk, D, generator=g).to(torch.bfloat16).to(dev) for _ in range(L)]
+    nk, nv = [x[0].transpose(1, 2) for x in new], [x[1].transpose(1, 2) for x in new]
+    res = torch.tensor([[5, 2], [16, 0], [1, 3]][:S], dtype=torch.int32, device=dev)
+    if pooled:
+        cache.commit_batch(nk, nv, res, B)
+    else:
+        cache.commit(nk, nv, res[0], advance_by=5)
+        assert cache.length == 42
+    for s in range(S):
+        acc, b = res[s].tolist()
+        for l in range(L):
+            gk, gv = (cache.gather_seq(l, s, lens[s] + acc) if pooled else cache.gather(l))
+            for i, (got, sign) in enumerate(((gk, 1), (gv, -1))):
+                rows = new[l][i, s * B + b, :acc].double().cpu()
+                want = torch.cat([sign * old[s], OP.e4m3_rows(rows)[0]])
+                assert torch.equal(got.double().cpu(), want), (s, l, i)
+    if not pooled:
+        with pytest.raises(NotImplementedError):
+            cache.commit(nk, nv, res[0], target_hidden=([torch.zeros(B, T, 64, device=dev)],
+                                                        torch.zeros(T, 64, device=dev)))
+        with pytest.raises(ValueError):
+            d.PagedKVCache(1, Hk, D, 16, dtype=E4M3, device=dev, layout="hnd")
+        with pytest.raises(ValueError):
+            cache.write(0, torch.zeros(90, Hk, D, dtype=torch.bfloat16, device=dev),
+                        torch.zeros(90, Hk, D, dtype=torch.bfloat16, device=dev))
+
+
+def test_verify_forward_over_an_8bit_cache(cuda_device):
+    """``cascade_verify_forward`` with an 8-bit PagedKVCache equals the same forward
+    over a 16-bit cache of the rows that the 8-bit one stands for."""
+    import d2sd_b200 as d
+    from test_verification_gpu import tiny
+    dev = cuda_device
+    model = tiny("qwen3", dev)
+    nl = len(model.model.layers)
+    Hk, D = model.config.num_key_value_heads, model.model.layers[0].self_attn.head_dim
+    g = torch.Generator().manual_seed(2)
+    P, B, T = 137, 3, 8
+    c8 = d.PagedKVCache(nl, Hk, D, 160, dtype=E4M3, device=dev)
+    c16 = d.PagedKVCache(nl, Hk, D, 160, device=dev)
+    for l in range(nl):
+        k, v = (torch.randn(P, Hk, D, generator=g).to(torch.bfloat16).to(dev) for _ in range(2))
+        c8.write(l, k, v)
+        c16.write(l, *c8.gather(l, P))
+    c8.length = c16.length = P
+    ids = torch.randint(0, 512, (B, T), generator=g).to(dev)
+    pos = torch.arange(P, P + T, device=dev).unsqueeze(0)
+    a = d.cascade_verify_forward(model, ids, pos, c8)[0]
+    b = d.cascade_verify_forward(model, ids, pos, c16)[0]
+    assert torch.equal(a, b)
