@@ -120,6 +120,11 @@ struct Vec8<float> {
   }
 };
 
+// Widen 8-bit pages into bf16 ones, one for each page-table entry (paged_kv.cu).
+int launch_widen(const uint8_t* k_pool, const uint8_t* v_pool, const uint8_t* k_scale, const uint8_t* v_scale,
+                 const PageGeom& g, const int32_t* page_table, int64_t entries, int num_kv_heads, int head_dim,
+                 void* k_out, void* v_out, void* stream);
+
 // Fill a PageGeom from the C arguments (strides in elements), or report what is
 // wrong with them. elem is the bytes of a cached value.
 int make_page_geom(PageGeom* g, const char* what, int32_t head_dim, int32_t elem, int64_t stride_page,

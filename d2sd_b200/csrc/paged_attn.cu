@@ -705,7 +705,7 @@ extern "C" int d2sd_paged_attention(
     int64_t scale_stride_page, int64_t scale_stride_head, const int32_t* page_table,
     int64_t page_table_len, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, float sm_scale,
     const int32_t* plan, const int32_t* sections, int32_t num_ctas, int32_t fixed_grid, void* workspace, int64_t workspace_bytes,
-    const float* sinks, int32_t sink_mode, void* out, int64_t out_stride_token, int64_t out_stride_head,
+    void* wide_k, void* wide_v, const float* sinks, int32_t sink_mode, void* out, int64_t out_stride_token, int64_t out_stride_head,
     float* lse, int64_t lse_stride_token, int32_t* status, void* stream) {
   using namespace d2sd;
   using namespace d2sd::paged;
@@ -727,6 +727,8 @@ extern "C" int d2sd_paged_attention(
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": k_scale and v_scale go together");
   if (scaled && dtype != D2SD_DTYPE_BF16)
     return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": 8-bit pages take bf16 queries");
+  if ((wide_k != nullptr) != (wide_v != nullptr) || (wide_k && !scaled) || !aligned16(wide_k) || !aligned16(wide_v))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": wide_k and wide_v go together, with an 8-bit cache");
   if (sinks && sink_mode != D2SD_SINK_REFERENCE && sink_mode != D2SD_SINK_EXACT)
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": unknown sink_mode");
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_pool) || !aligned16(v_pool) ||
@@ -770,7 +772,22 @@ extern "C" int d2sd_paged_attention(
     if (rc) return rc;
   }
   if (tiles[S_ITEMS] > 0 || fixed_grid) {
-    rc = launch_tiles(t, dtype, head_dim, scaled, num_tokens, num_qo_heads, num_kv_heads,
+    if (wide_k) {  // 8-bit pages that many row tiles go over: widened once
+      const int32_t lo = sections[kSections * kSectionInts + 1], hi = sections[kSections * kSectionInts + 2];
+      if (lo < 0 || hi <= lo || hi > page_table_len)
+        return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": the page table is shorter than the plan's");
+      rc = launch_widen(a.k_pool, a.v_pool, a.k_scale, a.v_scale, a.g, page_table + lo, hi - lo, num_kv_heads,
+                        head_dim, wide_k, wide_v, stream);
+      if (rc) return rc;
+      t.k_pool = static_cast<const uint8_t*>(wide_k), t.v_pool = static_cast<const uint8_t*>(wide_v);
+      t.k_scale = t.v_scale = nullptr;
+      t.page_table = nullptr;
+      t.first_entry = lo;
+      t.g.stride_head = 32 * static_cast<int64_t>(head_dim);
+      t.g.stride_page = num_kv_heads * t.g.stride_head;
+      t.g.num_pages = hi - lo;
+    }
+    rc = launch_tiles(t, dtype, head_dim, scaled && !wide_k, num_tokens, num_qo_heads, num_kv_heads,
                       fixed_grid ? num_ctas : tiles[S_CTAS], stream);
     if (rc) return rc;
   }

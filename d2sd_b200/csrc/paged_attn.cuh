@@ -15,6 +15,7 @@ struct AttnArgs {
   const uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
   const int32_t* page_table;
   int64_t page_table_len;
+  int64_t first_entry;  // page_table null: entry first_entry is page 0, and so on
   const int32_t* plan;
   float* slots;  // partial states (paged_plan.h)
   const float* sinks;

@@ -338,6 +338,48 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a, const 
   }
 }
 
+// The 8-bit pages of page-table entries [0, entries) as bf16 UMMA pages, entry e at
+// page e: a 16-byte core-matrix row becomes two (exact, see paged.cuh). For attention
+// that goes over the same keys many times.
+__global__ void __launch_bounds__(kThreads)
+    widen_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const uint8_t* k_scale, const uint8_t* v_scale,
+                 const PageGeom g, const int32_t* __restrict__ page_table, int64_t entries, int Hk, int D,
+                 uint8_t* k_out, uint8_t* v_out) {
+  grid_dep_wait();
+  const int chunks = D;  // 16-byte chunks of a (page, head) block of 16 * D bytes
+  const int64_t total = entries * Hk * chunks;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int x = static_cast<int>(i % chunks);
+    const int64_t eh = i / chunks;
+    const int h = static_cast<int>(eh % Hk);
+    const int64_t e = eh / Hk;
+    int64_t page = page_table[e];
+    page = page < 0 ? 0 : (page >= g.num_pages ? g.num_pages - 1 : page);
+    const int row_chunks = D / 16;
+    const int row = x / (8 * row_chunks) * 8 + x % 8, c = x / 8 % row_chunks;
+    const int64_t src = page * g.stride_page + h * g.stride_head + x * 16;
+    const int64_t sc = page * g.scale_page + h * g.scale_head + row;
+    const int64_t dst = eh * (32 * D) + ((row >> 3) * (D / 8) + 2 * c) * 128 + (row & 7) * 16;
+    const uint4 in[2] = {*reinterpret_cast<const uint4*>(k_pool + src), *reinterpret_cast<const uint4*>(v_pool + src)};
+    const float f[2] = {e4m3_scale(k_scale[sc]), e4m3_scale(v_scale[sc])};
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint32_t w[4] = {in[kv].x, in[kv].y, in[kv].z, in[kv].w};
+      uint32_t o[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 lo = e4m3x2_to_f(w[j]), hi = e4m3x2_to_f(w[j] >> 16);
+        o[2 * j] = pack_bf16x2(lo.x * f[kv], lo.y * f[kv]);
+        o[2 * j + 1] = pack_bf16x2(hi.x * f[kv], hi.y * f[kv]);
+      }
+      uint8_t* at = (kv ? v_out : k_out) + dst;
+      *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(at + 128) = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+  }
+}
+
 struct CommitArgs8 {
   const void* const* layer_ptrs;  // [L][6] {new_k, new_v, cache_k, cache_v, k_scale, v_scale}
   int64_t n_sr, n_sb, n_sh, n_st;
@@ -408,6 +450,17 @@ __global__ void __launch_bounds__(kThreads) commit_e4m3_kernel(const CommitArgs8
 bool aligned_rows(int64_t a, int64_t b) { return a % 8 == 0 && b % 8 == 0; }
 
 }  // namespace
+
+int launch_widen(const uint8_t* k_pool, const uint8_t* v_pool, const uint8_t* k_scale, const uint8_t* v_scale,
+                 const PageGeom& g, const int32_t* page_table, int64_t entries, int num_kv_heads, int head_dim,
+                 void* k_out, void* v_out, void* stream) {
+  const int64_t total = entries * num_kv_heads * head_dim;
+  const int64_t blocks = (total + kThreads - 1) / kThreads, most = static_cast<int64_t>(current_sm_count()) * 32;
+  return launch_pdl(widen_kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(kThreads), 0,
+                    static_cast<cudaStream_t>(stream), "widen_kernel", k_pool, v_pool, k_scale, v_scale, g,
+                    page_table, entries, num_kv_heads, head_dim, static_cast<uint8_t*>(k_out),
+                    static_cast<uint8_t*>(v_out));
+}
 }  // namespace d2sd
 
 extern "C" int d2sd_append_kv(

@@ -192,6 +192,21 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
       memcpy(out.data() + H_SECTION + s * kSectionInts, sec, sizeof(sec));
       memcpy(sections + s * kSectionInts, sec, sizeof(sec));
     }
+    // the page-table entries that the tiles kernel's requests span, and how often its
+    // units go over them
+    int64_t visits = 0, lo = kNoLimit, hi = 0;
+    for (const Unit& u : units[1]) {
+      visits += static_cast<int64_t>(u.tiles()) * (kTileKeys / 16);
+      lo = std::min<int64_t>(lo, u.page_off);
+      hi = std::max<int64_t>(hi, u.page_off + static_cast<int64_t>(u.kv_len + 15) / 16);
+    }
+    int32_t* host = sections + kSections * kSectionInts;
+    host[0] = host[1] = host[2] = 0;
+    if (hi > lo && hi < kNoLimit) {
+      host[0] = static_cast<int32_t>(std::min<int64_t>(visits / ((hi - lo) * num_kv_heads), kNoLimit));
+      host[1] = static_cast<int32_t>(lo);
+      host[2] = static_cast<int32_t>(hi);
+    }
     *used = static_cast<int64_t>(out.size());
     if (*used > capacity) return plan_fail(D2SD_ERR_WORKSPACE, "plan buffer too small");
     memcpy(plan, out.data(), out.size() * sizeof(int32_t));

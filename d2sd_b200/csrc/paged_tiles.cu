@@ -162,6 +162,7 @@ __device__ void producer(const CUtensorMap* tm_q, const CUtensorMap* tm_k, const
       if (b > last) b = last;
       const int64_t e = I.page_off + static_cast<int64_t>(b) * rpb / a.g.page_size;
       if (lane >= boxes || e >= a.page_table_len) return 0;
+      if (!a.page_table) return static_cast<int>(e - a.first_entry);  // widened pages
       const int64_t id = a.page_table[e];
       return static_cast<int>(id < 0 ? 0 : (id >= a.g.num_pages ? a.g.num_pages - 1 : id));
     };

@@ -91,7 +91,7 @@ class PagedAttentionPlan:
             raise ValueError("invalid plan sizes")
         plan = np.empty(cap, dtype=np.int32)
         used = np.zeros(1, dtype=np.int64)
-        sections = np.zeros(16, dtype=np.int32)
+        sections = np.zeros(19, dtype=np.int32)
         check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, R,
                                   self.num_qo_heads, self.num_kv_heads, 1 if self.causal else 0,
                                   self.window or 0, self.num_ctas, plan.ctypes.data, cap,
@@ -101,6 +101,11 @@ class PagedAttentionPlan:
     def _set(self, host, sections, tokens):
         self.plan[:len(host)].copy_(torch.from_numpy(host))
         self.host_plan, self.sections, self.tokens = host, sections, tokens
+        # an 8-bit cache is widened first where its keys are gone over four times or
+        # more (2048 tokens over 32k: 32 times; 1000 us against 1330), not where the
+        # launch has to fit any batch
+        self.widen = int(sections[16]) >= 4 and not self.fixed_grid
+        self.wide_pages = int(sections[18] - sections[17])
         # what every call passes on
         self._args = (self.plan.data_ptr(), sections.ctypes.data, self.num_ctas,
                       1 if self.fixed_grid else 0, self.workspace.data_ptr(),
@@ -128,7 +133,8 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
 
     Returns (out [tokens, Hq, D], lse [tokens, Hq] fp32, base 2), written into
     ``out`` / ``lse`` when given; rows behind the plan's tokens are left alone. A
-    row that sees no key has out 0 and lse -inf. Cache slots past a request's last
+    row that sees no key has out 0 and lse -inf. Prompt chunks over an e4m3 cache
+    take scratch of 4 * Hk * D bytes for each of their positions. Cache slots past a request's last
     position may hold anything. A NaN or an infinity in the value of a position that
     some row of a tile sees may reach rows of that tile that do not see it."""
     dev = q.get_device()
@@ -164,9 +170,13 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         if lse.dtype != torch.float32 or lse.dim() != 2 or lse.stride(1) != 1 \
                 or lse.shape[0] < tokens or lse.shape[1] != Hq:
             raise ValueError("lse must be fp32 [tokens, num_qo_heads] with a contiguous head axis")
+    wide = (None, None)
+    if k_scale is not None and plan.widen:
+        scratch = torch.empty((2, plan.wide_pages, Hk, 16, D), dtype=dtype, device=plan.device)
+        wide = (scratch.data_ptr(), scratch.data_ptr() + scratch.numel())
     args = (*q_args, n, ops.dtype_code(q), k_pool.data_ptr(), v_pool.data_ptr(), *pool,
             ops._int32("page_table", page_table), page_table.numel(), Hq, Hk, D,
-            D ** -0.5 if sm_scale is None else float(sm_scale), *plan._args, ops._ptr(sinks),
+            D ** -0.5 if sm_scale is None else float(sm_scale), *plan._args, *wide, ops._ptr(sinks),
             _SINKS[sink_mode] if sinks is not None else 0, *o_args, lse.data_ptr(), l_stride,
             plan.status.data_ptr())
     ops._call(dev, load().d2sd_paged_attention, args, "d2sd_paged_attention")

@@ -603,7 +603,7 @@ int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_requests,
  * only the last `window` of them; not causal: every position), and its pages
  * start at page_table[page_offsets[r]]. num_ctas is the grid (the SM count).
  * plan[0 .. capacity) is written on the HOST (*used entries): copy it to the
- * device. sections [16] is the host's copy of what the launch needs. */
+ * device. sections [19] is the host's copy of what the launch needs. */
 int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
                     const int32_t* page_offsets, int32_t num_requests,
                     int32_t num_qo_heads, int32_t num_kv_heads, int32_t causal,
@@ -624,7 +624,11 @@ int64_t d2sd_paged_workspace_bytes(int32_t num_ctas, int32_t head_dim);
  * Slots past a request's last position may hold anything, NaN included; page
  * ids outside the pool are read as its first or last page. fixed_grid: launch
  * num_ctas CTAs whatever the plan says, so that a captured call stays valid
- * when the plan's device buffer is rewritten. status receives 1 if a wait inside
+ * when the plan's device buffer is rewritten. wide_k, wide_v (8-bit caches, or
+ * NULL): scratch of (sections[18] - sections[17]) * num_kv_heads * 16 * head_dim
+ * bf16 values each, into which the pages of those page-table entries, the span of
+ * the requests of many rows, are widened first; sections[16] says how often their
+ * row tiles go over them on average. status receives 1 if a wait inside
  * the kernel ran out of time. */
 int d2sd_paged_attention(const void* q, int64_t q_stride_token,
                          int64_t q_stride_head, int64_t num_tokens,
@@ -639,8 +643,8 @@ int d2sd_paged_attention(const void* q, int64_t q_stride_token,
                          int32_t head_dim, float sm_scale, const int32_t* plan,
                          const int32_t* sections, int32_t num_ctas,
                          int32_t fixed_grid, void* workspace,
-                         int64_t workspace_bytes, const float* sinks,
-                         int32_t sink_mode, void* out, int64_t out_stride_token,
+                         int64_t workspace_bytes, void* wide_k, void* wide_v,
+                         const float* sinks, int32_t sink_mode, void* out, int64_t out_stride_token,
                          int64_t out_stride_head, float* lse,
                          int64_t lse_stride_token, int32_t* status,
                          void* stream);

@@ -149,6 +149,25 @@ def test_attention(cuda_device, i, garbage):
     assert int(plan.status) == 0
 
 
+def test_attention_widens_the_span_of_long_chunks(cuda_device):
+    """A chunk that goes over its 8-bit keys often enough to widen them first, between
+    requests of single tokens whose pages lie around it."""
+    import d2sd_b200 as d
+    Hq, Hk, D, ql, kl = 16, 2, 128, [1, 300, 200, 1], [200, 310, 1000, 77]
+    g = torch.Generator().manual_seed(21)
+    c = make_cache(g, kl, Hk, D, E4M3, "paged_umma", cuda_device, garbage=True)
+    q = torch.randn(sum(ql), Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, page_offsets=c["bounds"])
+    assert plan.widen and plan.wide_pages == c["bounds"][3] - c["bounds"][1]
+    for _ in range(2):
+        out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan,
+                                     k_scale=c["ks"], v_scale=c["vs"])
+        check_attention(out, lse, q, c, ql, D, torch.bfloat16)
+    with pytest.raises(ValueError):  # a page table that ends inside the span
+        d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"][:30], plan, k_scale=c["ks"],
+                          v_scale=c["vs"])
+
+
 @pytest.mark.parametrize("store", ["same", "e4m3"])
 def test_attention_without_causal_mask(cuda_device, store):
     import d2sd_b200 as d
