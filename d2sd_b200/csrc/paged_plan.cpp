@@ -156,7 +156,7 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
             hi = std::max<int64_t>(0, std::min<int64_t>(kv, pos0 + t1 + 1));
             if (window) lo = std::max<int64_t>(0, pos0 + t0 + 1 - window);
           }
-          lo = lo / kTileKeys * kTileKeys;
+          lo = lo / 16 * 16;  // whole pages
           if (lo > hi) lo = hi;
           units[section].push_back({r, h, static_cast<int32_t>(tok), static_cast<int32_t>(row),
                                     static_cast<int32_t>(nr), static_cast<int32_t>(lo),

@@ -2,8 +2,8 @@
 // (paged_plan.cpp), read by the kernels.
 //
 // A unit is (request, kv head, row tile): consecutive query rows of one kv head,
-// row = token * G + g. A unit's visible keys are cut into spans of whole 128-key
-// tiles; an item is one span. A unit of one item is written out directly; the
+// row = token * G + g. A unit's visible keys, from the first one's page of 16 on, are
+// cut into spans of whole 128-key tiles; an item is one span. A unit of one item is written out directly; the
 // items of a split unit leave partial states in consecutive slots, which a second
 // kernel joins in slot order (kept apart so that all SMs join, and no state stays
 // behind in the workspace), 4 or 8 rows to an entry of the join list.
@@ -32,7 +32,7 @@ enum {
   P_TOK0,      // q row of the request's first token
   P_ROW0,      // first row of the unit, inside the request
   P_NROWS,     // rows of the unit
-  P_KEY0,      // span [key0, key1): multiples of 128, key1 cut at the last visible key
+  P_KEY0,      // span [key0, key1): from a page's first key, whole tiles up to the last one
   P_KEY1,
   P_POS0,      // position of the request's token 0 (non-causal: kNoLimit)
   P_WINDOW,    // 0: none

@@ -96,6 +96,16 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+// Lanes `step` apart exchange: the lower keeps a and takes the other's a as b, the
+// upper (up = 1) keeps b and takes the other's b as a.
+__device__ __forceinline__ void quad_swap(uint4& a, uint4& b, int up, int step) {
+  uint4 s = up ? a : b;
+  s.x = __shfl_xor_sync(0xffffffffu, s.x, step);
+  s.y = __shfl_xor_sync(0xffffffffu, s.y, step);
+  s.z = __shfl_xor_sync(0xffffffffu, s.z, step);
+  s.w = __shfl_xor_sync(0xffffffffu, s.w, step);
+  if (up) a = s; else b = s;
+}
 // a shared-memory descriptor moved by `bytes` (its start address is the low 14
 // bits, address >> 4; shared addresses are below 256 KB, so nothing is carried)
 __device__ __forceinline__ uint64_t desc_at(uint64_t d, uint32_t bytes) {
@@ -691,25 +701,38 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       ++kitem;
     };
     const int64_t gtok = static_cast<int64_t>(cur.tok0) + tok;
-    auto store_o = [&](int c, const float (&o)[32], float f) {
-      T* op = static_cast<T*>(a.out) + gtok * a.o_st + hq * a.o_sh + c * 32;
+    // 32 columns of the warp's rows. A thread has its own row; four neighbours
+    // exchange 16-byte pieces, so that a store covers 64 bytes of a row each four
+    // lanes and touches 8 lines instead of 32.
+    auto store_o = [&](int c, const float (&o)[32], float f, const int64_t (&at)[4]) {
+      uint4 v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        uint4 v;
-        v.x = pack2(o[8 * e + 0] * f, o[8 * e + 1] * f, T());
-        v.y = pack2(o[8 * e + 2] * f, o[8 * e + 3] * f, T());
-        v.z = pack2(o[8 * e + 4] * f, o[8 * e + 5] * f, T());
-        v.w = pack2(o[8 * e + 6] * f, o[8 * e + 7] * f, T());
-        *reinterpret_cast<uint4*>(op + e * 8) = v;
+        v[e].x = pack2(o[8 * e + 0] * f, o[8 * e + 1] * f, T());
+        v[e].y = pack2(o[8 * e + 2] * f, o[8 * e + 3] * f, T());
+        v[e].z = pack2(o[8 * e + 4] * f, o[8 * e + 5] * f, T());
+        v[e].w = pack2(o[8 * e + 6] * f, o[8 * e + 7] * f, T());
       }
+      quad_swap(v[0], v[1], lane & 1, 1);
+      quad_swap(v[2], v[3], lane & 1, 1);
+      quad_swap(v[0], v[2], (lane >> 1) & 1, 2);
+      quad_swap(v[1], v[3], (lane >> 1) & 1, 2);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (at[k] >= 0)
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at[k] + c * 32 + (lane & 3) * 8) = v[k];
     };
     if (cur.parts == 1) {
       if (cur.split && valid) f_row = factor(m, l, lse_own);
+      int64_t at[4];  // where the quad's rows go, -1: not a row
+      const int64_t own = valid ? gtok * a.o_st + hq * a.o_sh : -1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) at[k] = __shfl_sync(0xffffffffu, own, (lane & ~3) + k);
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float o[32];
         load_o(c, o);
-        if (valid) store_o(c, o, f_row);
+        store_o(c, o, f_row, at);
       }
       if (valid && a.lse) a.lse[gtok * a.lse_st + hq] = lse_own;
       free_o();
@@ -867,12 +890,9 @@ int launch_tiles(const AttnArgs& a, int32_t dtype, int32_t head_dim, bool scaled
     int rc = encode_tensor_map(&tq, type, a.q, 3, dims, strides, box, "q");
     if (rc) return rc;
   }
-  int rpb = 16;
+  constexpr int rpb = 16;  // rows of a box: a span starts at any multiple of 16 keys
   tk = tv = tq;  // unused with UMMA pages
   if (!a.g.umma) {
-    // the largest power of two up to 128 that divides the page: boxes of a tile
-    // are whole and lie in one page
-    while (rpb < 128 && a.g.page_size % (2 * rpb) == 0) rpb *= 2;
     const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(a.g.page_size),
                               static_cast<uint64_t>(num_kv_heads), static_cast<uint64_t>(a.g.num_pages)};
     const uint64_t strides[3] = {static_cast<uint64_t>(a.g.stride_slot), static_cast<uint64_t>(a.g.stride_head),

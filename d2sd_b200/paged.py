@@ -101,10 +101,11 @@ class PagedAttentionPlan:
     def _set(self, host, sections, tokens):
         self.plan[:len(host)].copy_(torch.from_numpy(host))
         self.host_plan, self.sections, self.tokens = host, sections, tokens
-        # an 8-bit cache is widened first where its keys are gone over four times or
-        # more (2048 tokens over 32k: 32 times; 1000 us against 1330), not where the
-        # launch has to fit any batch
-        self.widen = int(sections[16]) >= 4 and not self.fixed_grid
+        # an 8-bit cache is widened first where its keys are gone over three times or
+        # more (32 query heads over 16k tokens: 128 new tokens 76 us either way, 256
+        # 106 against 117, 2048 over 32k 1060 against 1330), not where the launch has
+        # to fit any batch
+        self.widen = int(sections[16]) >= 3 and not self.fixed_grid
         self.wide_pages = int(sections[18] - sections[17])
         # what every call passes on
         self._args = (self.plan.data_ptr(), sections.ctypes.data, self.num_ctas,

@@ -58,7 +58,7 @@ def test_plan_covers_every_tile_once(lib, q, kv, Hq, Hk, causal, window, ctas):
             r, h, tok0, row0, nrows, k0, k1, pos0, win, po, kvl, slot, parts, tokb, *_ = it
             assert tok0 == starts[r] and po == off[r] and kvl == kv[r] and win == window
             assert 0 < nrows <= (q_tile if s == 0 else 2 * q_tile)
-            assert row0 + nrows <= q[r] * G and k0 % 128 == 0 and k1 <= kv[r]
+            assert row0 + nrows <= q[r] * G and k0 % 16 == 0 and k1 <= kv[r]
             assert tokb == row0 // G and (s == 0 or (row0 % G == 0 and nrows % G == 0))
             unit = seen.setdefault((r, h, row0), [nrows, []])
             unit[1].append((k0, k1))
@@ -103,10 +103,10 @@ def test_plan_covers_every_tile_once(lib, q, kv, Hq, Hk, causal, window, ctas):
                 if causal:
                     hi = max(0, min(kv[r], pos0 + (row0 + n - 1) // G + 1))
                     lo = max(0, pos0 + row0 // G + 1 - window) if window else 0
-                lo = min(lo // 128 * 128, hi)
+                lo = min(lo // 16 * 16, hi)
                 assert spans[0][0] == lo and spans[-1][1] == hi
                 for a, b in zip(spans, spans[1:]):
-                    assert a[1] == b[0] and b[1] > b[0]
+                    assert a[1] == b[0] and b[1] > b[0] and (a[1] - a[0]) % 128 == 0
             assert at == rows
 
 
