@@ -70,11 +70,6 @@ struct Cfg {
   static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 };
 
-__device__ __forceinline__ float fmin3(float a, float b, float c) {
-  float r;
-  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 __device__ __forceinline__ void prefetch_l1(const void* p) {
   asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
 }
@@ -498,22 +493,28 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
       // In a tile that not every row of the warp sees whole, chunks of 32 keys that
       // no row sees are skipped and those between are masked: key e is kept by a
       // minimum with (h - e) * inf, which is +inf below h and -inf above (h half an
-      // integer), and likewise at the window's end -- multiplications on the idle
-      // FMA pipe and one three-way minimum, where comparing and selecting costs
-      // three operations of the pipe that also takes the row maximum.
+      // integer), and likewise at the window's end -- two operations of the idle FMA
+      // pipe for two keys, where comparing and selecting costs more operations of the
+      // pipe that also takes the row maximum.
       const float h = static_cast<float>(hi - key) - 0.5f, l = static_cast<float>(lo - key) - 0.5f;
       auto skip = [&](int c) { return key + c * 32 >= any_hi || key + c * 32 + 32 <= any_lo; };
-      auto mask = [&](int c, uint32_t* v) {
-        const float hc = h - c * 32, lc = c * 32 - l;
-        if (key + c * 32 < all_lo) {
+      auto bound = [](uint32_t* v, float first, float step) {  // element e against first + e step
+        const uint64_t inf2 = f2_pack(INFINITY, INFINITY), two = f2_pack(2.f * step, 2.f * step);
+        uint64_t x = f2_pack(first, first + step);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            v[e] = __float_as_uint(fmin3(__uint_as_float(v[e]), (hc - e) * INFINITY, (lc + e) * INFINITY));
-        } else if (key + c * 32 + 32 > all_hi) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            v[e] = __float_as_uint(fminf(__uint_as_float(v[e]), (hc - e) * INFINITY));
+        for (int e = 0; e < 32; e += 2) {
+          float t0, t1;
+          f2_unpack(f2_mul(x, inf2), t0, t1);
+          v[e] = __float_as_uint(fminf(__uint_as_float(v[e]), t0));
+          v[e + 1] = __float_as_uint(fminf(__uint_as_float(v[e + 1]), t1));
+          x = f2_add(x, two);
         }
+      };
+      auto cut_hi = [&](int c) { return key + c * 32 + 32 > all_hi; };
+      auto cut_lo = [&](int c) { return key + c * 32 < all_lo; };
+      auto mask = [&](int c, uint32_t* v) {
+        if (cut_hi(c)) bound(v, h - c * 32, -1.f);
+        if (cut_lo(c)) bound(v, c * 32 - l, 1.f);
       };
       float f = 1.f, neg_m = 0.f;
       bool early = true;
@@ -573,9 +574,13 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
           if (edge && skip(c)) continue;
           uint32_t v[32];
           tmem_ld32_wait(lane_base + s_col(i) + c * 32, v);
-          if (edge) mask(c, v);
+          if (edge && (cut_hi(c) || cut_lo(c))) {  // masked once, for the second pass too
+            mask(c, v);
+            tmem_st32(lane_base + s_col(i) + c * 32, v);
+          }
           max32(v, mx);
         }
+        tmem_st_wait();
         new_max(mx);
         const uint64_t sc2 = f2_pack(sl2, sl2), nm2 = f2_pack(neg_m, neg_m);
 #pragma unroll 1
@@ -587,7 +592,6 @@ __device__ void softmax_role(const AttnArgs& a, uint8_t* smem, uint64_t* bars, u
           } else {
             uint32_t v[32];
             tmem_ld32_wait(lane_base + s_col(i) + c * 32, v);
-            if (edge) mask(c, v);
             weights(v, pk, sc2, nm2);
           }
           store_p(c, pk);
