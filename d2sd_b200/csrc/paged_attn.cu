@@ -788,6 +788,7 @@ extern "C" int d2sd_paged_attention(
       t.g.num_pages = hi - lo;
     }
     rc = launch_tiles(t, dtype, head_dim, scaled && !wide_k, num_tokens, num_qo_heads, num_kv_heads,
+                      !fixed_grid && sections[kSections * kSectionInts + 3] == 0,
                       fixed_grid ? num_ctas : tiles[S_CTAS], stream);
     if (rc) return rc;
   }

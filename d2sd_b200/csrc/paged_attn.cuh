@@ -55,9 +55,10 @@ __device__ __forceinline__ void zero_rows(uint8_t* page, int r0, int r1) {
   }
 }
 
-// Units of more than 16 query rows (paged_tiles.cu); dims of q for its copies.
+// Units of more than 16 query rows (paged_tiles.cu); num_tokens of q for its copies;
+// split: no unit of the plan has more rows than one q tile.
 int launch_tiles(const AttnArgs& a, int32_t dtype, int32_t head_dim, bool scaled, int64_t num_tokens,
-                 int32_t num_qo_heads, int32_t num_kv_heads, int ctas, void* stream);
+                 int32_t num_qo_heads, int32_t num_kv_heads, bool split, int ctas, void* stream);
 
 }  // namespace paged
 }  // namespace d2sd

@@ -201,7 +201,8 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
       hi = std::max<int64_t>(hi, u.page_off + static_cast<int64_t>(u.kv_len + 15) / 16);
     }
     int32_t* host = sections + kSections * kSectionInts;
-    host[0] = host[1] = host[2] = 0;
+    host[0] = host[1] = host[2] = host[3] = 0;
+    for (const Unit& u : units[1]) host[3] |= u.weight > 1;  // a unit of two q tiles
     if (hi > lo && hi < kNoLimit) {
       host[0] = static_cast<int32_t>(std::min<int64_t>(visits / ((hi - lo) * num_kv_heads), kNoLimit));
       host[1] = static_cast<int32_t>(lo);

@@ -91,7 +91,7 @@ class PagedAttentionPlan:
             raise ValueError("invalid plan sizes")
         plan = np.empty(cap, dtype=np.int32)
         used = np.zeros(1, dtype=np.int64)
-        sections = np.zeros(19, dtype=np.int32)
+        sections = np.zeros(20, dtype=np.int32)
         check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, R,
                                   self.num_qo_heads, self.num_kv_heads, 1 if self.causal else 0,
                                   self.window or 0, self.num_ctas, plan.ctypes.data, cap,

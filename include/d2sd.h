@@ -603,7 +603,7 @@ int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_requests,
  * only the last `window` of them; not causal: every position), and its pages
  * start at page_table[page_offsets[r]]. num_ctas is the grid (the SM count).
  * plan[0 .. capacity) is written on the HOST (*used entries): copy it to the
- * device. sections [19] is the host's copy of what the launch needs. */
+ * device. sections [20] is the host's copy of what the launch needs. */
 int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
                     const int32_t* page_offsets, int32_t num_requests,
                     int32_t num_qo_heads, int32_t num_kv_heads, int32_t causal,

@@ -17,7 +17,7 @@ def make(lib, q, kv, off, Hq, Hk, causal, window, ctas):
     from d2sd_b200._lib import check
     q, kv, off = (np.ascontiguousarray(x, dtype=np.int32) for x in (q, kv, off))
     cap = lib.d2sd_paged_plan_capacity(q.ctypes.data, len(q), Hq, Hk, ctas)
-    plan, used, sec = np.zeros(cap, np.int32), np.zeros(1, np.int64), np.zeros(19, np.int32)
+    plan, used, sec = np.zeros(cap, np.int32), np.zeros(1, np.int64), np.zeros(20, np.int32)
     check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, len(q), Hq, Hk, causal,
                               window, ctas, plan.ctypes.data, cap, used.ctypes.data,
                               sec.ctypes.data), "plan")
@@ -125,7 +125,7 @@ def test_plan_refusals(lib):
         make(lib, [1], [1], [0], 129, 1, 1, 0, 8)
     import ctypes
     n = np.ones(1, np.int32)
-    buf, used, sec = np.zeros(4, np.int32), np.zeros(1, np.int64), np.zeros(19, np.int32)
+    buf, used, sec = np.zeros(4, np.int32), np.zeros(1, np.int64), np.zeros(20, np.int32)
     rc = lib.d2sd_paged_plan(n.ctypes.data, n.ctypes.data, ctypes.c_void_p(np.zeros(1, np.int32).ctypes.data),
                              1, 4, 2, 1, 0, 8, buf.ctypes.data, 4, used.ctypes.data, sec.ctypes.data)
     assert rc == 3 and "small" in lib.d2sd_last_error().decode()
