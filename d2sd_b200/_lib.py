@@ -89,7 +89,7 @@ SIGNATURES = {
     "d2sd_commit_kv_e4m3": (i32, [vp, i32, i32, i32, i32, i32, i32, i64, i64, i64, i64, i64, i64,
                                   i64, i64, i64, vp, vp, vp, vp, vp, vp]),
     "d2sd_paged_plan_capacity": (i64, [vp, i32, i32, i32, i32]),
-    "d2sd_paged_plan": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, i64, vp, vp]),
+    "d2sd_paged_plan": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, i64, vp, vp]),
     "d2sd_paged_workspace_bytes": (i64, [i32, i32]),
     "d2sd_paged_attention": (i32, [vp, i64, i64, i64, i32, vp, vp, i64, i64, i64, i32, i64, i32, vp, vp,
                                    i64, i64, vp, i64, i32, i32, i32, f32, vp, vp, i32, i32, vp, i64,

@@ -118,8 +118,8 @@ extern "C" int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_r
 
 extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
                                const int32_t* page_offsets, int32_t num_requests, int32_t num_qo_heads,
-                               int32_t num_kv_heads, int32_t causal, int32_t window, int32_t num_ctas,
-                               int32_t* plan, int64_t capacity, int64_t* used, int32_t* sections) {
+                               int32_t num_kv_heads, int32_t causal, int32_t window, int32_t eight_bit,
+                               int32_t num_ctas, int32_t* plan, int64_t capacity, int64_t* used, int32_t* sections) {
   using namespace d2sd;
   using namespace d2sd::paged;
   if (num_requests < 0 || (num_requests > 0 && (!q_lens || !kv_lens || !page_offsets)) || !plan ||
@@ -143,7 +143,7 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
       const int64_t rows = n * G;
       // few rows: tiles of 16 rows; else pairs of q tiles of whole tokens, where a
       // unit of one q tile works on two key tiles at a time
-      const int section = rows <= kRowsLimit ? 0 : 1;
+      const int section = rows <= (eight_bit ? kRowsLimit8 : kRowsLimit) ? 0 : 1;
       const int64_t q_tile = static_cast<int64_t>(128 / G) * G;
       const int64_t tile = section == 0 ? kRowsTile : 2 * q_tile;
       const int32_t pos0 = causal ? static_cast<int32_t>(kv - n) : kNoLimit;

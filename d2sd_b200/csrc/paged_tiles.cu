@@ -63,13 +63,17 @@ struct Cfg {
   static constexpr int kSmemV = kSmemK + kStages * kTileBytes;
   static constexpr int kSmemLand = kSmemV + kStages * kTileBytes;  // 8-bit K, V tiles, their scales
   static constexpr int kLandBytes = 128 * D;
-  static constexpr int kSmemJoin = kSmemLand + (MODE == kE4m3 ? 2 * kLandBytes + 256 : 0);
+  // 8-bit tiles on their way in: one of K and V each, more where there is room (a
+  // widened tile's buffer is filled again only after it, a latency of about 2 us)
+  static constexpr int kLand = MODE != kE4m3 ? 0 : (D == 128 ? (SPLIT ? 2 : 1) : 3);
+  static constexpr int kSmemScales = kSmemLand + kLand * 2 * kLandBytes;  // [kLand][K, V][128]
+  static constexpr int kSmemJoin = kSmemScales + kLand * 256;
   static constexpr int kSmemBar = kSmemJoin + 128 * 8;  // [128] (m, l) of stream 1
   static constexpr int B_QFULL = 0, B_QFREE = 1, B_KFULL = 2, B_VFULL = B_KFULL + kStages,
                        B_KEMPTY = B_VFULL + kStages, B_VEMPTY = B_KEMPTY + kStages,
                        B_SFULL = B_VEMPTY + kStages, B_PHALF = B_SFULL + 2, B_PFULL = B_PHALF + 2,
                        B_OFINAL = B_PFULL + 2, B_OFREE = B_OFINAL + 2, B_VREADY = B_OFREE + 2,
-                       B_LFULL = B_VREADY + kStages, B_LEMPTY = B_LFULL + 2, kNumBars = B_LEMPTY + 2;
+                       B_LFULL = B_VREADY + kStages, B_LEMPTY = B_LFULL + 2 * kLand, kNumBars = B_LEMPTY + 2 * kLand;
   static constexpr int kSmemBytes = kSmemBar + kNumBars * 8 + 32 + 1024;  // + alignment slack
   static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 };
@@ -187,9 +191,14 @@ __device__ void producer(const CUtensorMap* tm_q, const CUtensorMap* tm_k, const
       for (int kv = 0; kv < 2; ++kv) {
         uint64_t* full;
         bool ok = true;
-        if (MODE == kE4m3) {  // one landing buffer each
-          full = &bars[C::B_LFULL + kv];
-          if (lane == 0 && kt > 0) ok = mbar_wait(&bars[C::B_LEMPTY + kv], (kt - 1) & 1, abort);
+        uint8_t* land = nullptr;
+        uint8_t* scales = nullptr;
+        if constexpr (MODE == kE4m3) {
+          const uint32_t ls = kt % C::kLand, lu = kt / C::kLand;
+          full = &bars[C::B_LFULL + 2 * ls + kv];
+          land = smem + C::kSmemLand + (2 * ls + kv) * C::kLandBytes;
+          scales = smem + C::kSmemScales + (2 * ls + kv) * 128;
+          if (lane == 0 && lu > 0) ok = mbar_wait(&bars[C::B_LEMPTY + 2 * ls + kv], (lu - 1) & 1, abort);
         } else {
           full = &bars[(kv ? C::B_VFULL : C::B_KFULL) + st];
           if (lane == 0 && use > 0)
@@ -210,7 +219,7 @@ __device__ void producer(const CUtensorMap* tm_q, const CUtensorMap* tm_k, const
           }
         } else {
           constexpr int kBlock = 16 * D * (MODE == kE4m3 ? 1 : 2);  // a page of one head
-          uint8_t* dst = MODE == kE4m3 ? smem + C::kSmemLand + kv * C::kLandBytes
+          uint8_t* dst = MODE == kE4m3 ? land
                                        : smem + (kv ? C::kSmemV : C::kSmemK) + st * C::kTileBytes;
           if (lane == 0) mbar_arrive_expect_tx(full, 8 * (kBlock + (MODE == kE4m3 ? 16 : 0)));
           __syncwarp();
@@ -219,7 +228,7 @@ __device__ void producer(const CUtensorMap* tm_q, const CUtensorMap* tm_k, const
             bulk_load(dst + lane * kBlock, (kv ? a.v_pool : a.k_pool) + p * a.g.stride_page + I.head * a.g.stride_head,
                       kBlock, full);
             if (MODE == kE4m3)
-              bulk_load(smem + C::kSmemLand + 2 * C::kLandBytes + kv * 128 + lane * 16,
+              bulk_load(scales + lane * 16,
                         (kv ? a.v_scale : a.k_scale) + p * a.g.scale_page + I.head * a.g.scale_head, 16, full);
           }
         }
@@ -388,10 +397,11 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
       const int key = I.key0 + t * kTileKeys;
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
-        if (!warp_wait(&bars[C::B_LFULL + kv], kt & 1, abort)) return;
+        const uint32_t ls = kt % C::kLand;
+        if (!warp_wait(&bars[C::B_LFULL + 2 * ls + kv], (kt / C::kLand) & 1, abort)) return;
         if (use > 0 && !warp_wait(&bars[(kv ? C::B_VEMPTY : C::B_KEMPTY) + st], (use - 1) & 1, abort)) return;
-        const uint8_t* src = smem + C::kSmemLand + kv * C::kLandBytes + tid * 16;
-        const uint8_t* scales = smem + C::kSmemLand + 2 * C::kLandBytes + kv * 128 + row0;
+        const uint8_t* src = smem + C::kSmemLand + (2 * ls + kv) * C::kLandBytes + tid * 16;
+        const uint8_t* scales = smem + C::kSmemScales + (2 * ls + kv) * 128 + row0;
         uint8_t* dst = smem + (kv ? C::kSmemV : C::kSmemK) + st * C::kTileBytes + dst0;
         const bool fix = kv == 1 && (key + kTileKeys > hi || key < lo);
 #pragma unroll 2
@@ -433,7 +443,7 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&bars[C::B_LEMPTY + kv]);
+          mbar_arrive(&bars[C::B_LEMPTY + 2 * ls + kv]);
           mbar_arrive(&bars[(kv ? C::B_VFULL : C::B_KFULL) + st]);
         }
       }
@@ -796,6 +806,8 @@ __global__ void __launch_bounds__(Cfg<D, MODE, SPLIT>::kThreads, 1)
       mbar_init(&bars[C::B_PFULL + i], 4);
       mbar_init(&bars[C::B_OFINAL + i], 1);
       mbar_init(&bars[C::B_OFREE + i], 4);
+    }
+    for (int i = 0; i < 2 * C::kLand; ++i) {
       mbar_init(&bars[C::B_LFULL + i], 1);
       mbar_init(&bars[C::B_LEMPTY + i], 4);
     }

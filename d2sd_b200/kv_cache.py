@@ -316,7 +316,7 @@ class PagedKVPool(PagedKVCache):
         if len(q_lens) != self.num_seqs:
             raise ValueError("q_lens must have an entry for each sequence")
         return PagedAttentionPlan(q_lens, self.lengths, num_qo_heads, self.num_kv_heads, self.head_dim,
-                                  self.device, page_offsets=self.page_offsets_host, **kw)
+                                  self.device, page_offsets=self.page_offsets_host, cache_dtype=self.dtype, **kw)
 
     def write_seq(self, l: int, s: int, k: torch.Tensor, v: torch.Tensor, start: int = 0) -> None:
         """Write k, v [n, Hk, D] at positions start.. of sequence s, layer l."""

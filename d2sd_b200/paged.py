@@ -27,7 +27,8 @@ class PagedAttentionPlan:
     ones included (the new tokens are the last of them). page_offsets: each
     request's first entry in the page table (default: one request from entry 0, or
     ``PagedKVPool.page_offsets_host``); a longer list (page bounds) is cut.
-    window: a row sees only the last ``window`` positions up to its own.
+    window: a row sees only the last ``window`` positions up to its own. cache_dtype:
+    float8_e4m3fn chooses the kernels for an 8-bit cache (any plan works with any).
 
     The plan owns the workspace of its calls: two calls that overlap on the GPU
     need a plan each. ``update`` re-plans in place, on the current stream. With
@@ -39,7 +40,8 @@ class PagedAttentionPlan:
 
     def __init__(self, q_lens, kv_lens, num_qo_heads: int, num_kv_heads: int, head_dim: int,
                  device: torch.device | str, *, causal: bool = True, window: int | None = None,
-                 page_offsets=None, reserve: tuple[int, int] | None = None):
+                 page_offsets=None, cache_dtype: torch.dtype | None = None,
+                 reserve: tuple[int, int] | None = None):
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("PagedAttentionPlan needs a CUDA device")
@@ -47,6 +49,7 @@ class PagedAttentionPlan:
             raise ValueError("window must be positive")
         self.num_qo_heads, self.num_kv_heads, self.head_dim = num_qo_heads, num_kv_heads, head_dim
         self.causal, self.window = causal, window
+        self.eight_bit = cache_dtype == torch.float8_e4m3fn
         self.num_ctas = ops.num_sms(device)
         self.fixed_grid = reserve is not None
         self.reserve = reserve
@@ -94,7 +97,8 @@ class PagedAttentionPlan:
         sections = np.zeros(20, dtype=np.int32)
         check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, R,
                                   self.num_qo_heads, self.num_kv_heads, 1 if self.causal else 0,
-                                  self.window or 0, self.num_ctas, plan.ctypes.data, cap,
+                                  self.window or 0, 1 if self.eight_bit else 0,
+                                  self.num_ctas, plan.ctypes.data, cap,
                                   used.ctypes.data, sections.ctypes.data), "d2sd_paged_plan")
         return plan[:int(used[0])], sections, int(q.sum())
 

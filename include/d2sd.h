@@ -601,14 +601,16 @@ int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_requests,
  * q_lens[r] new tokens, the last of its kv_lens[r] cached positions (causal:
  * token i sees positions up to kv_lens[r] - q_lens[r] + i, and with window > 0
  * only the last `window` of them; not causal: every position), and its pages
- * start at page_table[page_offsets[r]]. num_ctas is the grid (the SM count).
+ * start at page_table[page_offsets[r]]. eight_bit: choose the kernels for an
+ * 8-bit cache (either choice is right for both). num_ctas is the SM count.
  * plan[0 .. capacity) is written on the HOST (*used entries): copy it to the
  * device. sections [20] is the host's copy of what the launch needs. */
 int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
                     const int32_t* page_offsets, int32_t num_requests,
                     int32_t num_qo_heads, int32_t num_kv_heads, int32_t causal,
-                    int32_t window, int32_t num_ctas, int32_t* plan,
-                    int64_t capacity, int64_t* used, int32_t* sections);
+                    int32_t window, int32_t eight_bit, int32_t num_ctas,
+                    int32_t* plan, int64_t capacity, int64_t* used,
+                    int32_t* sections);
 
 /* Workspace bytes of d2sd_paged_attention for a grid of num_ctas; it holds
  * nothing from one call to the next. Calls that overlap on the GPU need a

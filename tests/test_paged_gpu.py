@@ -137,7 +137,8 @@ def test_attention(cuda_device, i, garbage):
     q = torch.randn(n + 2, Hq + 3, D, generator=g).to(dtype).to(cuda_device)[:, 1:Hq + 1]
     sinks = torch.randn(Hq, generator=g).to(cuda_device) if with_sinks else None
     plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, window=window,
-                                page_offsets=c["bounds"])
+                                page_offsets=c["bounds"],
+                                cache_dtype=c["k"].dtype if garbage else None)
     out = torch.full((n + 2, Hq + 1, D), 7.0, dtype=dtype, device=cuda_device)[:, :Hq]
     lse = torch.full((n + 2, Hq), 7.0, device=cuda_device)
     for _ in range(2):  # the second call finds the workspace as the first left it

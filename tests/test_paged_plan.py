@@ -13,17 +13,18 @@ def lib():
     return _lib.load()
 
 
-def make(lib, q, kv, off, Hq, Hk, causal, window, ctas):
+def make(lib, q, kv, off, Hq, Hk, causal, window, ctas, eight_bit=0):
     from d2sd_b200._lib import check
     q, kv, off = (np.ascontiguousarray(x, dtype=np.int32) for x in (q, kv, off))
     cap = lib.d2sd_paged_plan_capacity(q.ctypes.data, len(q), Hq, Hk, ctas)
     plan, used, sec = np.zeros(cap, np.int32), np.zeros(1, np.int64), np.zeros(20, np.int32)
     check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, len(q), Hq, Hk, causal,
-                              window, ctas, plan.ctypes.data, cap, used.ctypes.data,
+                              window, eight_bit, ctas, plan.ctypes.data, cap, used.ctypes.data,
                               sec.ctypes.data), "plan")
     return plan[:int(used[0])], sec
 
 
+@pytest.mark.parametrize("eight_bit", [0, 1])
 @pytest.mark.parametrize("q,kv,Hq,Hk,causal,window,ctas", [
     ([1] * 64, list(range(512, 8193, 120))[:64], 32, 8, 1, 0, 148),
     ([1], [1000], 32, 8, 1, 0, 148),
@@ -36,9 +37,9 @@ def make(lib, q, kv, off, Hq, Hk, causal, window, ctas):
     ([100], [40], 4, 2, 1, 0, 5),
     ([3] * 300, [77] * 300, 8, 1, 1, 0, 3),
 ])
-def test_plan_covers_every_tile_once(lib, q, kv, Hq, Hk, causal, window, ctas):
+def test_plan_covers_every_tile_once(lib, eight_bit, q, kv, Hq, Hk, causal, window, ctas):
     off = np.cumsum([0] + [-(-n // 16) for n in kv])[:-1]
-    plan, sec = make(lib, q, kv, off, Hq, Hk, causal, window, ctas)
+    plan, sec = make(lib, q, kv, off, Hq, Hk, causal, window, ctas, eight_bit)
     G = Hq // Hk
     starts = np.cumsum([0] + list(q))
     seen = {}
@@ -127,7 +128,7 @@ def test_plan_refusals(lib):
     n = np.ones(1, np.int32)
     buf, used, sec = np.zeros(4, np.int32), np.zeros(1, np.int64), np.zeros(20, np.int32)
     rc = lib.d2sd_paged_plan(n.ctypes.data, n.ctypes.data, ctypes.c_void_p(np.zeros(1, np.int32).ctypes.data),
-                             1, 4, 2, 1, 0, 8, buf.ctypes.data, 4, used.ctypes.data, sec.ctypes.data)
+                             1, 4, 2, 1, 0, 0, 8, buf.ctypes.data, 4, used.ctypes.data, sec.ctypes.data)
     assert rc == 3 and "small" in lib.d2sd_last_error().decode()
     assert lib.d2sd_paged_plan_capacity(n.ctypes.data, 1, 5, 2, 8) == -1
     assert lib.d2sd_paged_workspace_bytes(148, 96) == -1
