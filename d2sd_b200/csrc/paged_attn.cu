@@ -15,8 +15,8 @@
 // are m16n8k16 matrix instructions: one 16-row tile is all the rows there are,
 // and a 128-row tensor-core tile would be mostly padding. A page is stored as
 // 8-row x 16-byte core matrices, exactly what ldmatrix fetches, without bank
-// conflicts and without a swizzle; pages of plain rows are put into that order by
-// the copy. At the end the warps' states are joined in shared memory, and for a
+// conflicts and without a swizzle; pages of plain rows are fetched as TMA boxes with a
+// 128-byte swizzle, which serves ldmatrix as well. At the end the warps' states are joined in shared memory, and for a
 // unit of several spans join_kernel joins the spans.
 //
 // e4m3 pages: their values are widened to f16 in registers (one conversion for two,
@@ -33,6 +33,7 @@
 // product; maximum, sum and output stay in fp32.
 #include <atomic>
 #include <string>
+#include <type_traits>
 
 #include "paged_attn.cuh"
 
@@ -59,7 +60,7 @@ struct RowsCfg {
   static constexpr int kSmemQ = kSmemMl + 2 * kWarps * 16 * 4;  // [D / 16][32 lanes][16 bytes] (8-bit)
   static constexpr int kSmemBars = kSmemQ + (ELEM == 1 ? 16 * D * 2 : 0);
   static constexpr int kSmemFlags = kSmemBars + kWarps * 8 * 8;
-  static constexpr int kSmemBytes = kSmemFlags + 16 + 128;
+  static constexpr int kSmemBytes = kSmemFlags + 16 + 1024;
   static_assert(kState <= kRing, "the state fits the ring");
   static_assert(kRowsCtas * (kSmemBytes + 1024) <= 227 * 1024 + 1024, "the CTAs of an SM");
 };
@@ -112,16 +113,37 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+// Byte offset of (row, 16-byte chunk) of a page in shared memory: core matrices, or
+// (rows fetched as TMA boxes) 128-byte-swizzled panels of 64 values. ldmatrix reads
+// eight rows of a chunk without bank conflicts in both.
+template <int CHUNKS, bool UMMA>
+__device__ __forceinline__ uint32_t page_at(int row, int chunk) {
+  return UMMA ? static_cast<uint32_t>(((row >> 3) * CHUNKS + chunk) * 128 + (row & 7) * 16)
+              : static_cast<uint32_t>((chunk >> 3) * 2048 + row * 128 + (((chunk ^ row) & 7) << 4));
+}
+
+// Zeroes rows [r0, r1) of a page in shared memory (the whole warp).
+template <int D, int ELEM, bool UMMA>
+__device__ __forceinline__ void zero_rows(uint8_t* page, int r0, int r1) {
+  constexpr int C = D * ELEM / 16;
+  const int lane = threadIdx.x & 31;
+  for (int i = lane; i < 16 * C; i += 32) {
+    const int r = i & 15, c = i >> 4;
+    if (r >= r0 && r < r1) *reinterpret_cast<uint4*>(page + page_at<C, UMMA>(r, c)) = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // ELEM: bytes of a cached value (2: T, 1: e4m3); UMMA: pages in core-matrix order,
-// fetched with one bulk copy each (else rows, 16-byte cp.async).
+// fetched with one bulk copy each (else rows, TMA boxes).
 template <typename T, int D, int ELEM, bool UMMA>
-__global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_kernel(
+    const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnArgs a) {
   using C = RowsCfg<D, ELEM>;
   constexpr int kWarps = C::kWarps, kThreads = C::kThreads;
   constexpr int kChunks = D * ELEM / 16;  // 16-byte chunks of a row
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) &
-                                             ~static_cast<uintptr_t>(127));
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));  // of the swizzle
   float* sm_m = reinterpret_cast<float*>(smem + C::kSmemMl);
   float* sm_l = sm_m + kWarps * 16;
   uint4* sm_q = reinterpret_cast<uint4*>(smem + C::kSmemQ);
@@ -259,26 +281,18 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
         }
       } else {
-        const int slot0 = (b0 + warp + j * kWarps) * 16 % a.g.page_size;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint8_t* src = (kv ? a.v_pool : a.k_pool) + off;
-          const uint32_t d = smem_u32(dst + kv * C::kPageBytes);
-#pragma unroll
-          for (int i = 0; i < kChunks / 2; ++i) {  // 8 rows x 4 chunks at a time
-            const int r = (lane & 7) + 8 * (i & 1), c = (i >> 1) * 4 + (lane >> 3);
-            cp_async16(d + ((r >> 3) * kChunks + c) * 128 + (r & 7) * 16,
-                       src + static_cast<int64_t>(slot0 + r) * a.g.stride_slot + c * 16);
-          }
+        if (lane < 2 * (D / 64)) {  // a box of 16 rows by 64 values each
+          const int slot0 = (b0 + warp + j * kWarps) * 16 % a.g.page_size;
+          const int kv = lane & 1, pn = lane >> 1;
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * C::kPageBytes);
+          __syncwarp((1u << (2 * (D / 64))) - 1u);
+          tma_load_4d(dst + kv * C::kPageBytes + pn * 2048, kv ? &tm_v : &tm_k, &full[st], pn * 64, slot0, head,
+                      static_cast<int>(page));
         }
       }
     };
-    auto commit = [&] {
-      if (!UMMA) asm volatile("cp.async.commit_group;" ::: "memory");
-    };
     for (int j = 0; j < C::kStages - 1; ++j) {
       if (j < mine) issue(j);
-      commit();
     }
     if (ELEM == 1) __syncthreads();  // q is in shared memory
     bool alive = true;
@@ -286,17 +300,11 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
     for (; j < mine; ++j) {
       // the stage freed by block j - 1 takes block j + kStages - 1
       if (j + C::kStages - 1 < mine) issue(j + C::kStages - 1);
-      commit();
       const uint32_t st = read;
-      if (UMMA) {
-        const bool ok = mbar_wait(&full[st], parity, flags);
-        if (!__all_sync(0xffffffffu, ok)) {
-          alive = false;
-          break;
-        }
-      } else {
-        asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
-        __syncwarp();
+      const bool ok = mbar_wait(&full[st], parity, flags);
+      if (!__all_sync(0xffffffffu, ok)) {
+        alive = false;
+        break;
       }
       uint8_t* kp = ring + st * C::kStageBytes;
       uint8_t* vp = kp + C::kPageBytes;
@@ -305,20 +313,20 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       if (edge && (key + 16 > hi_max || key < lo_min)) {
         // values no row of the unit sees may be anything; a weight of 0 would
         // still turn a NaN or an infinity there into NaN
-        zero_rows<D, ELEM>(vp, max(0, hi_max - key), 16);
-        zero_rows<D, ELEM>(vp, 0, min(16, lo_min - key));
-        if (UMMA) fence_proxy_async_smem();  // before the next bulk copy into this stage
+        zero_rows<D, ELEM, UMMA>(vp, max(0, hi_max - key), 16);
+        zero_rows<D, ELEM, UMMA>(vp, 0, min(16, lo_min - key));
+        fence_proxy_async_smem();  // before the next copy into this stage
         __syncwarp();
       }
       // ---- scores ----
       float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-      const uint32_t ka = smem_u32(kp) + (lane & 7) * 16;
-      const int mt = lane >> 3;  // matrix of an x4 this lane addresses
+      const uint32_t ka = smem_u32(kp);
+      const int mt = lane >> 3, r8 = lane & 7;  // matrix of an x4 this lane addresses, and its row
       if (ELEM == 2) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           uint32_t b[4];  // (keys 0-7, d lo), (0-7, hi), (8-15, lo), (8-15, hi)
-          ldsm4(ka + ((mt >> 1) * kChunks + ks * 2 + (mt & 1)) * 128, b);
+          ldsm4(ka + page_at<kChunks, UMMA>((mt >> 1) * 8 + r8, ks * 2 + (mt & 1)), b);
           mma16816<T>(c[0], qf[ks], b[0], b[1]);
           mma16816<T>(c[1], qf[ks], b[2], b[3]);
         }
@@ -326,7 +334,7 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
 #pragma unroll
         for (int ks = 0; ks < D / 16; ks += 2) {
           uint32_t b[4];  // (keys 0-7, chunk ks), (8-15, ks), (0-7, ks + 1), (8-15, ks + 1)
-          ldsm4(ka + ((mt & 1) * kChunks + ks + (mt >> 1)) * 128, b);
+          ldsm4(ka + page_at<kChunks, UMMA>((mt & 1) * 8 + r8, ks + (mt >> 1)), b);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint4 q = sm_q[(ks + h) * 32 + lane];
@@ -434,12 +442,12 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
         }
       }
       // ---- o += p v ----
-      const uint32_t va = smem_u32(vp) + (lane & 7) * 16;
+      const uint32_t va = smem_u32(vp);
       if (ELEM == 2) {
 #pragma unroll
         for (int i = 0; i < D / 8; i += 2) {
           uint32_t b[4];  // (keys 0-7, chunk i), (8-15, i), (0-7, i + 1), (8-15, i + 1), transposed
-          ldsm4_t(va + ((mt & 1) * kChunks + i + (mt >> 1)) * 128, b);
+          ldsm4_t(va + page_at<kChunks, UMMA>((mt & 1) * 8 + r8, i + (mt >> 1)), b);
           mma16816<T>(o[i], p, b[0], b[1]);
           mma16816<T>(o[i + 1], p, b[2], b[3]);
         }
@@ -447,7 +455,7 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
 #pragma unroll
         for (int i = 0; i < D / 16; i += 2) {
           uint32_t b[4];  // pairs of neighbouring d, transposed
-          ldsm4_t(va + ((mt & 1) * kChunks + i + (mt >> 1)) * 128, b);
+          ldsm4_t(va + page_at<kChunks, UMMA>((mt & 1) * 8 + r8, i + (mt >> 1)), b);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             // (key, d): bytes (0, 0) (0, 1) (1, 0) (1, 1) -> even d's pair of keys, odd d's
@@ -508,7 +516,7 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       sm_l[warp * 16 + qr] = l0;
       sm_l[warp * 16 + qr + 8] = l1;
     }
-    if (UMMA) fence_proxy_async_smem();  // before the next item's bulk copies into the ring
+    fence_proxy_async_smem();  // before the next item's copies into the ring
     __syncthreads();
     constexpr int kPer = 16 * D / kThreads;  // outputs of a thread, neighbours in a row
     const int row = threadIdx.x / (kThreads / 16), dcol = (threadIdx.x % (kThreads / 16)) * kPer;
@@ -662,7 +670,7 @@ int run_join(const AttnArgs& a, int32_t dtype, int32_t head_dim, const int32_t* 
 }
 
 template <typename T, int D, int ELEM, bool UMMA>
-int launch_rows(const AttnArgs& a, int ctas, cudaStream_t stream) {
+int launch_rows(const AttnArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, int ctas, cudaStream_t stream) {
   using C = RowsCfg<D, ELEM>;
   static std::atomic<uint64_t> configured{0};  // bit per device
   int dev = 0;
@@ -675,18 +683,29 @@ int launch_rows(const AttnArgs& a, int ctas, cudaStream_t stream) {
     if (dev < 64) configured.fetch_or(1ull << dev);
   }
   return launch_pdl(rows_kernel<T, D, ELEM, UMMA>, dim3(ctas), dim3(C::kThreads), C::kSmemBytes, stream,
-                    "rows_kernel", a);
+                    "rows_kernel", tk, tv, a);
 }
 
-int run_rows(const AttnArgs& a, int32_t dtype, int32_t head_dim, bool scaled, int ctas, cudaStream_t st) {
-  const bool d128 = head_dim == 128, umma = a.g.umma != 0;
-  if (scaled) return d128 ? launch_rows<__nv_bfloat16, 128, 1, true>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 1, true>(a, ctas, st);
-  if (dtype == D2SD_DTYPE_BF16) {
-    if (umma) return d128 ? launch_rows<__nv_bfloat16, 128, 2, true>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 2, true>(a, ctas, st);
-    return d128 ? launch_rows<__nv_bfloat16, 128, 2, false>(a, ctas, st) : launch_rows<__nv_bfloat16, 64, 2, false>(a, ctas, st);
+int run_rows(const AttnArgs& a, int32_t dtype, int32_t head_dim, int32_t num_kv_heads, bool scaled, int ctas,
+             cudaStream_t st) {
+  CUtensorMap tk = {}, tv = {};  // of pages of rows only
+  if (!a.g.umma) {
+    int rc = encode_pages(&tk, &tv, a, dtype, head_dim, num_kv_heads);
+    if (rc) return rc;
   }
-  if (umma) return d128 ? launch_rows<__half, 128, 2, true>(a, ctas, st) : launch_rows<__half, 64, 2, true>(a, ctas, st);
-  return d128 ? launch_rows<__half, 128, 2, false>(a, ctas, st) : launch_rows<__half, 64, 2, false>(a, ctas, st);
+  auto go = [&](auto t, auto elem, auto umma) {
+    using T = decltype(t);
+    constexpr int E = decltype(elem)::value;
+    constexpr bool U = decltype(umma)::value;
+    return head_dim == 128 ? launch_rows<T, 128, E, U>(a, tk, tv, ctas, st)
+                           : launch_rows<T, 64, E, U>(a, tk, tv, ctas, st);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (scaled) return go(__nv_bfloat16(), One(), std::true_type());
+  if (dtype == D2SD_DTYPE_BF16)
+    return a.g.umma ? go(__nv_bfloat16(), Two(), std::true_type()) : go(__nv_bfloat16(), Two(), std::false_type());
+  return a.g.umma ? go(__half(), Two(), std::true_type()) : go(__half(), Two(), std::false_type());
 }
 
 }  // namespace
@@ -768,7 +787,7 @@ extern "C" int d2sd_paged_attention(
   AttnArgs t = a;  // the tiles kernel's half of the workspace
   t.slots += tile_slots_at(num_ctas, head_dim);
   if (sections[S_ITEMS] > 0 || fixed_grid) {
-    rc = run_rows(a, dtype, head_dim, scaled, fixed_grid ? section_ctas(0, num_ctas) : sections[S_CTAS], st);
+    rc = run_rows(a, dtype, head_dim, num_kv_heads, scaled, fixed_grid ? section_ctas(0, num_ctas) : sections[S_CTAS], st);
     if (rc) return rc;
   }
   if (tiles[S_ITEMS] > 0 || fixed_grid) {

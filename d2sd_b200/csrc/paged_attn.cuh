@@ -43,17 +43,10 @@ __device__ __forceinline__ float sink_factor(float lse2, float sink, int mode) {
   return 1.f / (1.f + expf(-x));
 }
 
-// One 16-byte chunk of zeros is written over rows [r0, r1) of a page in smem.
-template <int D, int ELEM>
-__device__ __forceinline__ void zero_rows(uint8_t* page, int r0, int r1) {
-  constexpr int C = D * ELEM / 16;
-  const int lane = threadIdx.x & 31;
-  for (int i = lane; i < 16 * C; i += 32) {
-    const int r = i & 15, c = i >> 4;
-    if (r >= r0 && r < r1)
-      *reinterpret_cast<uint4*>(page + ((r >> 3) * C + c) * 128 + (r & 7) * 16) = make_uint4(0, 0, 0, 0);
-  }
-}
+// Tensor maps of K and V pools of row pages: boxes of 16 rows by 64 values, 128-byte
+// swizzled, at (value, slot, head, page) (paged_tiles.cu).
+int encode_pages(CUtensorMap* tk, CUtensorMap* tv, const AttnArgs& a, int32_t dtype, int32_t head_dim,
+                 int32_t num_kv_heads);
 
 // Units of more than 16 query rows (paged_tiles.cu); num_tokens of q for its copies;
 // split: no unit of the plan has more rows than one q tile.

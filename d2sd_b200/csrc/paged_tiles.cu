@@ -896,6 +896,19 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
 
 }  // namespace
 
+int encode_pages(CUtensorMap* tk, CUtensorMap* tv, const AttnArgs& a, int32_t dtype, int32_t head_dim,
+                 int32_t num_kv_heads) {
+  const CUtensorMapDataType type =
+      dtype == D2SD_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(a.g.page_size),
+                            static_cast<uint64_t>(num_kv_heads), static_cast<uint64_t>(a.g.num_pages)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(a.g.stride_slot), static_cast<uint64_t>(a.g.stride_head),
+                               static_cast<uint64_t>(a.g.stride_page)};
+  const uint32_t box[4] = {64, 16, 1, 1};
+  int rc = encode_tensor_map(tk, type, a.k_pool, 4, dims, strides, box, "k");
+  return rc ? rc : encode_tensor_map(tv, type, a.v_pool, 4, dims, strides, box, "v");
+}
+
 int launch_tiles(const AttnArgs& a, int32_t dtype, int32_t head_dim, bool scaled, int64_t num_tokens,
                  int32_t num_qo_heads, int32_t num_kv_heads, bool split, int ctas, void* stream) {
   const int G = num_qo_heads / num_kv_heads;
@@ -913,14 +926,7 @@ int launch_tiles(const AttnArgs& a, int32_t dtype, int32_t head_dim, bool scaled
   constexpr int rpb = 16;  // rows of a box: a span starts at any multiple of 16 keys
   tk = tv = tq;  // unused with UMMA pages
   if (!a.g.umma) {
-    const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(a.g.page_size),
-                              static_cast<uint64_t>(num_kv_heads), static_cast<uint64_t>(a.g.num_pages)};
-    const uint64_t strides[3] = {static_cast<uint64_t>(a.g.stride_slot), static_cast<uint64_t>(a.g.stride_head),
-                                 static_cast<uint64_t>(a.g.stride_page)};
-    const uint32_t box[4] = {64, static_cast<uint32_t>(rpb), 1, 1};
-    int rc = encode_tensor_map(&tk, type, a.k_pool, 4, dims, strides, box, "k");
-    if (rc) return rc;
-    rc = encode_tensor_map(&tv, type, a.v_pool, 4, dims, strides, box, "v");
+    int rc = encode_pages(&tk, &tv, a, dtype, head_dim, num_kv_heads);
     if (rc) return rc;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
