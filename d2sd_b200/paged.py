@@ -100,7 +100,17 @@ class PagedAttentionPlan:
                                   self.window or 0, 1 if self.eight_bit else 0,
                                   self.num_ctas, plan.ctypes.data, cap,
                                   used.ctypes.data, sections.ctypes.data), "d2sd_paged_plan")
+        self._requests, self._entries = (kv, off), {}
         return plan[:int(used[0])], sections, int(q.sum())
+
+    def entries(self, page_size: int) -> int:
+        """Entries that a page table must have for pages of this size."""
+        n = self._entries.get(page_size)
+        if n is None:
+            kv, off = self._requests
+            n = int((off.astype(np.int64) + -(-kv.astype(np.int64) // page_size)).max(initial=0))
+            self._entries[page_size] = n
+        return n
 
     def _set(self, host, sections, tokens):
         self.plan[:len(host)].copy_(torch.from_numpy(host))
@@ -147,7 +157,7 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     Hq, Hk, D = plan.num_qo_heads, plan.num_kv_heads, plan.head_dim
     dtype, n = q.dtype, q.shape[0]
     tokens = plan.reserve[1] if plan.reserve else plan.tokens
-    if n < tokens or n < 1:
+    if n < tokens:
         raise ValueError(f"q must hold the plan's {tokens} tokens")
     pool, heads, dim = ops._pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale)
     if heads != Hk or dim != D:
@@ -159,6 +169,8 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     if sinks is not None and (sinks.dtype != torch.float32 or not sinks.is_contiguous()
                               or sinks.numel() != Hq):
         raise ValueError("sinks must be a contiguous fp32 tensor [num_qo_heads]")
+    if page_table.numel() < plan.entries(pool[3]):
+        raise ValueError(f"the page table must have {plan.entries(pool[3])} entries for this plan")
     q_args = ops._rows("q", q, n, Hq, D, dtype)
     if out is None:
         out = torch.empty((n, Hq, D), dtype=dtype, device=plan.device)

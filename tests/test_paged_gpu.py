@@ -208,6 +208,32 @@ def test_attention_large_scores(cuda_device):
     check_attention(out, lse, q, c, ql, D, torch.bfloat16)
 
 
+@pytest.mark.parametrize("n", [1, 70])
+def test_attention_reference_sink_mode(cuda_device, n):
+    import d2sd_b200 as d
+    Hq, Hk, D, kl = 8, 2, 64, [300]
+    g = torch.Generator().manual_seed(30 + n)
+    c = make_cache(g, kl, Hk, D, torch.bfloat16, "paged_umma", cuda_device)
+    q = torch.randn(n, Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    sinks = (4 + torch.randn(Hq, generator=g)).to(cuda_device)
+    plan = d.PagedAttentionPlan([n], kl, Hq, Hk, D, cuda_device)
+    out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, sinks=sinks,
+                                 sink_mode="reference")
+    check_attention(out, lse, q, c, [n], D, torch.bfloat16, sinks=sinks.cpu(), sink_mode="reference")
+
+
+def test_attention_of_no_tokens(cuda_device):
+    import d2sd_b200 as d
+    kp = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device=cuda_device)
+    table = torch.arange(4, dtype=torch.int32, device=cuda_device)
+    plan = d.PagedAttentionPlan([0, 0], [7, 0], 4, 2, 64, cuda_device, page_offsets=[0, 1])
+    for n in (0, 3):
+        q = torch.zeros(n, 4, 64, dtype=torch.bfloat16, device=cuda_device)
+        out = torch.full_like(q, 2.0)
+        d.paged_attention(q, kp, kp, "paged_umma", table, plan, out=out)
+        assert (out == 2).all()
+
+
 def test_attention_bad_page_ids(cuda_device):
     """Ids outside the pool are read as its first or last page: no fault, and the
     other requests' rows are right."""
@@ -496,7 +522,7 @@ def test_refusals(cuda_device):
     with pytest.raises(NotImplementedError):
         P([1], [1], 129, 1, 64, dev)
     plan = P([3], [3], 4, 2, 64, dev)
-    q = z(3, 4, 64)
+    q, e8 = z(3, 4, 64), z(4, 2, 16, 64, t=torch.uint8).view(E4M3)
     for err, a, kw in [
             (ValueError, (q[:2], kp, kp, "paged_umma", one[0], plan), {}),
             (ValueError, (q.half(), kp, kp, "paged_umma", one[0], plan), {}),
@@ -504,6 +530,10 @@ def test_refusals(cuda_device):
             (ValueError, (q, kp, kp, "paged_umma", one[0], plan), {"sinks": z(3, t=torch.float32)}),
             (ValueError, (q, kp[:, :1], kp[:, :1], "paged_hnd", one[0], plan), {}),
             (ValueError, (q, kp, kp, "paged_umma", one[0], plan), {"out": z(2, 4, 64)}),
+            (ValueError, (q, kp, kp, "paged_umma", one[0][:0], plan), {}),     # a short page table
+            (ValueError, (q, kp, kp, "paged_umma", one[0], plan), {"sm_scale": 0.0}),
+            (NotImplementedError, (q.half(), e8, e8, "paged_umma", one[0], plan),
+             {"k_scale": z(4, 2, 16, t=torch.uint8), "v_scale": z(4, 2, 16, t=torch.uint8)}),
             (NotImplementedError, (q, z(4, 2, 8, 64), z(4, 2, 8, 64), "paged_hnd", one[0], plan), {})]:
         with pytest.raises(err):
             d.paged_attention(*a, **kw)
