@@ -26,9 +26,10 @@
 // bytes are two keys by two neighbouring columns. f16's range is met by powers of
 // two, which cost no precision: q's rows are scaled to 2^14 .. 2^15, and with e_j
 // the exponent of value row j the weights are
-//   w_j = 2^(s_j + e_j - M), M the running maximum of s_j + e_j,
-// at most 1 whatever the rows' sizes are; the sum of plain weights keeps its own
-// maximum m. The key's scale multiplies the score in fp32.
+//   w_j = 2^(s_j - m) 2^(e_j), m the running maximum of s_j + max(e_j, -60),
+// at most 1 whatever the rows' sizes are, and the sum takes 2^(s_j - m) <= 2^60 (a
+// value row under 2^-60 is below what f16 weights resolve). The key's scale
+// multiplies the score in fp32.
 // Weights are rounded to 16 bits (bf16: 2^-8 relative, f16: 2^-11) for the second
 // product; maximum, sum and output stay in fp32.
 #include <atomic>
@@ -95,11 +96,11 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// 2^e of a scale byte. A row marked NaN (255, here 2^128) has NaN values too, so the
-// product is NaN; e of byte 0 (factor 0) is only a reference for the weights.
+// 2^e of a scale byte (a row marked NaN, 255, here 2^128, has NaN values too, so the
+// product is NaN), and e from -60 on, the weights' reference.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
-__device__ __forceinline__ float exponent_of(uint32_t byte) {  // byte - 127
-  return __uint_as_float(0x4b000000u | byte) - (8388608.f + 127.f);
+__device__ __forceinline__ float exponent_of(uint32_t byte) {
+  return __uint_as_float(0x4b000000u | max(byte, 67u)) - (8388608.f + 127.f);
 }
 
 // The four e4m3 values of x as two pairs of f16 (bytes 0 and 1, bytes 2 and 3).
@@ -247,7 +248,6 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    float M0 = -INFINITY, M1 = -INFINITY, g0 = 0.f, g1 = 0.f;  // e4m3: of s_j + e_j, 2^(m - M)
 
     // ---- this warp's pages of 16 keys: b0 + warp, b0 + warp + 8, ... ----
     const int b0 = key0 / 16, nb = (key1 - key0 + 15) / 16;
@@ -376,15 +376,13 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
             if (ELEM == 1 && (x >= hi_max || x < lo_min)) vb[n] &= e ? 0x00ffu : 0xff00u;
           }
       }
-      // ---- running maxima and sum; o is rescaled only when its maximum grew ----
+      // ---- running maximum and sum; o is rescaled only when the maximum grew ----
       auto row_max = [](float x) {  // over the four lanes of a row
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
         return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
       };
-      const float x0 = row_max(fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1])));
-      const float x1 = row_max(fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3])));
-      float vs[2][2];           // 2^e_j
-      float y0 = x0, y1 = x1;   // maxima of s_j + e_j
+      float vs[2][2];  // 2^e_j
+      float x0, x1;    // the rows' maxima of s_j (e4m3: s_j + e_j)
       if (ELEM == 1) {
         float ve[2][2];
 #pragma unroll
@@ -395,28 +393,21 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
             vs[n][e] = scale_of(byte);
             ve[n][e] = exponent_of(byte);
           }
-        y0 = row_max(fmaxf(fmaxf(c[0][0] + ve[0][0], c[0][1] + ve[0][1]),
-                           fmaxf(c[1][0] + ve[1][0], c[1][1] + ve[1][1])));
-        y1 = row_max(fmaxf(fmaxf(c[0][2] + ve[0][0], c[0][3] + ve[0][1]),
-                           fmaxf(c[1][2] + ve[1][0], c[1][3] + ve[1][1])));
+        x0 = fmaxf(fmaxf(c[0][0] + ve[0][0], c[0][1] + ve[0][1]), fmaxf(c[1][0] + ve[1][0], c[1][1] + ve[1][1]));
+        x1 = fmaxf(fmaxf(c[0][2] + ve[0][0], c[0][3] + ve[0][1]), fmaxf(c[1][2] + ve[1][0], c[1][3] + ve[1][1]));
+      } else {
+        x0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
+        x1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
       }
-      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1 || (ELEM == 1 && (y0 > M0 || y1 > M1)))) {
+      x0 = row_max(x0);
+      x1 = row_max(x1);
+      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
         const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-        float f0 = m0 == n0 ? 1.f : fast_exp2(m0 - n0), f1 = m1 == n1 ? 1.f : fast_exp2(m1 - n1);
+        const float f0 = m0 == n0 ? 1.f : fast_exp2(m0 - n0), f1 = m1 == n1 ? 1.f : fast_exp2(m1 - n1);
         m0 = n0;
         m1 = n1;
         l0 *= f0;
         l1 *= f1;
-        if (ELEM == 1) {
-          const float N0 = fmaxf(M0, y0), N1 = fmaxf(M1, y1);
-          f0 = M0 == N0 ? 1.f : fast_exp2(M0 - N0);
-          f1 = M1 == N1 ? 1.f : fast_exp2(M1 - N1);
-          M0 = N0;
-          M1 = N1;
-          // 2^(m - M), 0 while the row has seen no value
-          g0 = M0 == -INFINITY ? 0.f : fast_exp2(m0 - M0);
-          g1 = M1 == -INFINITY ? 0.f : fast_exp2(m1 - M1);
-        }
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           o[i][0] *= f0;
@@ -434,8 +425,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
         l0 += p0 + p1;
         l1 += p2 + p3;
         if (ELEM == 1) {
-          p[2 * n] = pack2(p0 * g0 * vs[n][0], p1 * g0 * vs[n][1], __half());
-          p[2 * n + 1] = pack2(p2 * g1 * vs[n][0], p3 * g1 * vs[n][1], __half());
+          p[2 * n] = pack2(p0 * vs[n][0], p1 * vs[n][1], __half());
+          p[2 * n + 1] = pack2(p2 * vs[n][0], p3 * vs[n][1], __half());
         } else {
           p[2 * n] = pack2(p0, p1, T());
           p[2 * n + 1] = pack2(p2, p3, T());
@@ -489,16 +480,6 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
     // ---- join the warps: O over the warp's own ring, m and l beside it ----
     __syncwarp();
     float* os = reinterpret_cast<float*>(ring);
-    if (ELEM == 1) {  // back from the reference M to m
-      const float f0 = M0 == -INFINITY ? 0.f : fast_exp2(M0 - m0), f1 = M1 == -INFINITY ? 0.f : fast_exp2(M1 - m1);
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][0] *= f0;
-        o[i][1] *= f0;
-        o[i][2] *= f1;
-        o[i][3] *= f1;
-      }
-    }
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) {
       // 16-bit: columns of tile i are d = 8 i + n. 8-bit: tiles 2 j, 2 j + 1 hold
