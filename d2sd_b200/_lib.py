@@ -83,11 +83,11 @@ SIGNATURES = {
                                 i32, i32, i32, vp, vp, f32, vp, vp, i64, i32, vp, vp]),
     "d2sd_append_kv": (i32, [vp, i64, i64, vp, i64, i64, i32, vp, i64, i64, vp, i64, i64, i32, i64,
                              i32, i32, vp, vp, f32, vp, vp, i64, i64, i32, i32, vp, vp, i32, vp, vp,
-                             i64, i64, i64, i32, i64, i32, vp, vp, i64, i64, vp, vp, vp, vp]),
-    "d2sd_read_kv": (i32, [vp, vp, i64, i64, i64, i32, i64, i32, vp, vp, i64, i64, vp, vp, vp, vp,
+                             i64, i64, i64, i32, i64, i32, vp, vp, i64, i64, vp, i64, vp, vp, vp]),
+    "d2sd_read_kv": (i32, [vp, vp, i64, i64, i64, i32, i64, i32, vp, vp, i64, i64, vp, i64, vp, vp, vp,
                            i32, i64, i32, i32, i32, vp, i64, i64, vp, i64, i64, vp, vp]),
     "d2sd_commit_kv_e4m3": (i32, [vp, i32, i32, i32, i32, i32, i32, i64, i64, i64, i64, i64, i64,
-                                  i64, i64, i64, vp, vp, vp, vp, vp, vp]),
+                                  i64, i64, i64, vp, i64, vp, vp, vp, vp, vp]),
     "d2sd_paged_plan_capacity": (i64, [vp, i32, i32, i32, i32]),
     "d2sd_paged_plan": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, i64, vp, vp]),
     "d2sd_paged_workspace_bytes": (i64, [i32, i32]),

@@ -164,7 +164,9 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
 
   const int32_t* sec = a.plan + H_SECTION;
   const int G = a.plan[H_GROUP];
-  grid_dep_launch();  // the join's blocks wait beside this kernel
+  // the join's blocks wait beside this kernel (without one, the next kernel may be
+  // any, and one that reads this kernel's output before it waits must not start early)
+  if (sec[S_JOINS] > 0) grid_dep_launch();
   if (static_cast<int>(blockIdx.x) >= sec[S_CTAS]) return;  // a fixed grid's spare CTA
   const int item0 = a.plan[sec[S_OFF_CTA] + blockIdx.x], item1 = a.plan[sec[S_OFF_CTA] + blockIdx.x + 1];
   const int qr = lane >> 2, qc = lane & 3;

@@ -73,6 +73,16 @@ __device__ __forceinline__ float group_max(float x) {
   return x;
 }
 
+// 1 / sqrt(x) with a Newton step, e = 1 - x r^2 from the exact product x r: to about
+// half a last place (rsqrtf alone: 2). 0 and infinity keep rsqrtf's answers.
+__device__ __forceinline__ float exact_rsqrt(float x) {
+  const float r = rsqrtf(x);
+  if (!(x > 0.f && x <= 3.402823466e38f)) return r;
+  const float h = x * r, l = fmaf(x, r, -h);
+  const float e = fmaf(-l, r, fmaf(-h, r, 1.f));
+  return fmaf(0.5f * r, e, r);
+}
+
 // Lane `part` of a row's group holds elements 8 part .. 8 part + 7. Writes them to
 // `at` (this lane's 8 bytes of the page) and the row's scale byte. The whole group
 // calls it; rows with store == false only take part in the shuffles.
@@ -108,6 +118,7 @@ struct AppendArgs {
   int64_t table_stride, table_rows;
   const int32_t *token_start, *first_pos;
   const int32_t *page_table, *page_bounds;
+  int64_t page_table_len;
   uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
   int32_t* status;
   int64_t tokens;
@@ -127,7 +138,8 @@ struct Place {
 template <int W>
 __device__ __forceinline__ Place find_place(int64_t t, int64_t tokens, const int32_t* token_start,
                                             const int32_t* first_pos, int R, const int32_t* page_table,
-                                            const int32_t* page_bounds, const PageGeom& g) {
+                                            int64_t page_table_len, const int32_t* page_bounds,
+                                            const PageGeom& g) {
   int r = R;
 #pragma unroll
   for (int k = 0; k < 32 / W; ++k) {
@@ -142,8 +154,9 @@ __device__ __forceinline__ Place find_place(int64_t t, int64_t tokens, const int
   const int64_t lo = page_bounds[r], n = page_bounds[r + 1] - lo;
   p.pos = static_cast<int64_t>(first_pos[r]) + (t - start);
   p.err = kStatusPosition;
-  if (p.pos < 0 || p.pos / g.page_size >= n) return p;
-  p.page = page_table[lo + p.pos / g.page_size];
+  const int64_t index = p.pos / g.page_size;
+  if (p.pos < 0 || index >= n || lo < 0 || lo + index >= page_table_len) return p;
+  p.page = page_table[lo + index];
   p.slot = static_cast<int>(p.pos % g.page_size);
   p.err = p.page < 0 || p.page >= g.num_pages ? kStatusPage : 0;
   return p;
@@ -158,7 +171,8 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a,
   const int rows = a.Hq + 2 * a.Hk;
   const int row0 = blockIdx.y * rows_per_block, row1 = min(rows, row0 + rows_per_block);
   grid_dep_wait();
-  Place p = find_place<W>(t, a.tokens, a.token_start, a.first_pos, a.R, a.page_table, a.page_bounds, a.g);
+  Place p = find_place<W>(t, a.tokens, a.token_start, a.first_pos, a.R, a.page_table, a.page_table_len,
+                            a.page_bounds, a.g);
   if (p.err == 0 && a.half && p.pos >= a.table_rows) p.err = kStatusTable;
   if (p.err > 0 && part == 0 && row0 == 0) report(a.status, p.err);
   const bool ok = p.err == 0;  // else the token's rows are not written at all
@@ -214,13 +228,14 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a,
         if (h + u >= h1) break;
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (ok) in[u].get(f);
+        float inv = 1.f;
         if (kKind != 2 && weight) {
           float ss = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
-          const float inv = rsqrtf(group_sum<W>(ss) * (1.f / D) + a.eps);
+          inv = exact_rsqrt(group_sum<W>(ss) * (1.f / D) + a.eps);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
+          for (int i = 0; i < 8; ++i) f[i] *= w[i];
         }
         if (kKind != 2 && a.half) {
           float x[8];  // the partners
@@ -235,6 +250,12 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a,
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + x[i] * s[i];
           }
+        }
+        // last, as one rounding (x w is exact in fp32 for 16-bit types): fewer values
+        // land on the wrong side of a border of e4m3
+        if (kKind != 2 && weight) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] *= inv;
         }
         if (Q8 && kKind != 0) {
           store_e4m3<D>(f, part, dst + u * dst_sh, scale + u * a.g.scale_head, ok);
@@ -276,6 +297,7 @@ struct ReadArgs {
   void *k_out, *v_out;
   int64_t ko_st, ko_sh, vo_st, vo_sh;  // element strides
   const int32_t *token_start, *first_pos, *page_table, *page_bounds;
+  int64_t page_table_len;
   int32_t* status;
   int64_t tokens;
   PageGeom g;
@@ -292,7 +314,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a, const 
   const int row0 = blockIdx.y * rows_per_block, row1 = min(2 * a.Hk, row0 + rows_per_block);
   grid_dep_wait();
   const Place p =
-      find_place<W>(t, a.tokens, a.token_start, a.first_pos, a.R, a.page_table, a.page_bounds, a.g);
+      find_place<W>(t, a.tokens, a.token_start, a.first_pos, a.R, a.page_table, a.page_table_len,
+                            a.page_bounds, a.g);
   if (p.err > 0 && part == 0 && row0 == 0) report(a.status, p.err);
   if (p.err != 0) return;
   for (int r0 = row0; r0 < row1; r0 += kAhead) {
@@ -384,6 +407,7 @@ struct CommitArgs8 {
   const void* const* layer_ptrs;  // [L][6] {new_k, new_v, cache_k, cache_v, k_scale, v_scale}
   int64_t n_sr, n_sb, n_sh, n_st;
   const int32_t *page_table, *page_bounds, *accept_results, *cache_lens;
+  int64_t page_table_len;
   int32_t* status;
   PageGeom g;
   int32_t R, L, Hk, TB;
@@ -425,7 +449,7 @@ __global__ void __launch_bounds__(kThreads) commit_e4m3_kernel(const CommitArgs8
       const int64_t pos = len + t;
       if (ok) {
         int err = 0;
-        if (pos < 0 || pos / 16 >= n) {
+        if (pos < 0 || pos / 16 >= n || lo < 0 || lo + pos / 16 >= a.page_table_len) {
           err = kStatusPosition;
         } else {
           page = a.page_table[lo + pos / 16];
@@ -474,11 +498,12 @@ extern "C" int d2sd_append_kv(
     void* k_pool, void* v_pool, int64_t cache_stride_page, int64_t cache_stride_slot,
     int64_t cache_stride_head, int32_t page_size, int64_t num_pages, int32_t cache_format,
     void* k_scale, void* v_scale, int64_t scale_stride_page, int64_t scale_stride_head,
-    const int32_t* page_table, const int32_t* page_bounds, int32_t* status, void* stream) {
+    const int32_t* page_table, int64_t page_table_len, const int32_t* page_bounds, int32_t* status,
+    void* stream) {
   using namespace d2sd;
   const char* const w = "d2sd_append_kv";
   if (num_tokens < 0 || num_requests < 0 || num_kv_heads <= 0 || num_qo_heads < 0 || !token_start ||
-      !first_pos || !k_pool || !v_pool || !page_table || !page_bounds ||
+      !first_pos || !k_pool || !v_pool || !page_table || page_table_len < 0 || !page_bounds ||
       (num_tokens > 0 && (!k || !v || (num_qo_heads > 0 && (!q || !q_out)))))
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
   if (num_tokens == 0 || num_requests == 0) return D2SD_OK;
@@ -519,7 +544,7 @@ extern "C" int d2sd_append_kv(
   a.q_weight = q_weight, a.k_weight = k_weight;
   a.cos = cos_table, a.sin = sin_table, a.table_stride = table_stride, a.table_rows = table_rows;
   a.token_start = token_start, a.first_pos = first_pos;
-  a.page_table = page_table, a.page_bounds = page_bounds;
+  a.page_table = page_table, a.page_table_len = page_table_len, a.page_bounds = page_bounds;
   a.k_pool = static_cast<uint8_t*>(k_pool), a.v_pool = static_cast<uint8_t*>(v_pool);
   a.k_scale = static_cast<uint8_t*>(k_scale), a.v_scale = static_cast<uint8_t*>(v_scale);
   a.status = status;
@@ -547,8 +572,8 @@ extern "C" int d2sd_read_kv(const void* k_pool, const void* v_pool, int64_t cach
                             int64_t cache_stride_slot, int64_t cache_stride_head, int32_t page_size,
                             int64_t num_pages, int32_t cache_format, const void* k_scale,
                             const void* v_scale, int64_t scale_stride_page, int64_t scale_stride_head,
-                            const int32_t* page_table, const int32_t* page_bounds,
-                            const int32_t* token_start, const int32_t* first_pos, int32_t num_requests,
+                            const int32_t* page_table, int64_t page_table_len,
+                            const int32_t* page_bounds, const int32_t* token_start, const int32_t* first_pos, int32_t num_requests,
                             int64_t num_tokens, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
                             void* k_out, int64_t k_out_stride_token, int64_t k_out_stride_head,
                             void* v_out, int64_t v_out_stride_token, int64_t v_out_stride_head,
@@ -556,7 +581,7 @@ extern "C" int d2sd_read_kv(const void* k_pool, const void* v_pool, int64_t cach
   using namespace d2sd;
   const char* const w = "d2sd_read_kv";
   if (num_tokens < 0 || num_requests < 0 || num_kv_heads <= 0 || !token_start || !first_pos || !k_pool ||
-      !v_pool || !page_table || !page_bounds || (num_tokens > 0 && (!k_out || !v_out)))
+      !v_pool || !page_table || page_table_len < 0 || !page_bounds || (num_tokens > 0 && (!k_out || !v_out)))
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
   if (num_tokens == 0 || num_requests == 0) return D2SD_OK;
   if (head_dim != 64 && head_dim != 128)
@@ -585,7 +610,7 @@ extern "C" int d2sd_read_kv(const void* k_pool, const void* v_pool, int64_t cach
   a.ko_st = k_out_stride_token, a.ko_sh = k_out_stride_head, a.vo_st = v_out_stride_token,
   a.vo_sh = v_out_stride_head;
   a.token_start = token_start, a.first_pos = first_pos, a.page_table = page_table,
-  a.page_bounds = page_bounds;
+  a.page_table_len = page_table_len, a.page_bounds = page_bounds;
   a.status = status;
   a.tokens = num_tokens;
   a.R = num_requests, a.Hk = num_kv_heads;
@@ -612,13 +637,14 @@ extern "C" int d2sd_commit_kv_e4m3(const void* const* layer_ptrs, int32_t num_la
                                    int64_t new_stride_token, int64_t cache_stride_page,
                                    int64_t cache_stride_head, int64_t num_pages,
                                    int64_t scale_stride_page, int64_t scale_stride_head,
-                                   const int32_t* page_table, const int32_t* page_bounds,
-                                   const int32_t* accept_results, const int32_t* cache_lens,
+                                   const int32_t* page_table, int64_t page_table_len,
+                                   const int32_t* page_bounds, const int32_t* accept_results,
+                                   const int32_t* cache_lens,
                                    int32_t* status, void* stream) {
   using namespace d2sd;
   const char* const w = "d2sd_commit_kv_e4m3";
   if (!layer_ptrs || num_layers <= 0 || num_requests <= 0 || num_kv_heads <= 0 || block_len <= 0 ||
-      !page_table || !page_bounds || !accept_results || !cache_lens)
+      !page_table || page_table_len < 0 || !page_bounds || !accept_results || !cache_lens)
     return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": invalid argument");
   if (head_dim != 64 && head_dim != 128)
     return fail(D2SD_ERR_UNSUPPORTED, std::string(w) + ": head_dim must be 64 or 128");
@@ -634,7 +660,8 @@ extern "C" int d2sd_commit_kv_e4m3(const void* const* layer_ptrs, int32_t num_la
   a.layer_ptrs = layer_ptrs;
   a.n_sr = new_stride_request, a.n_sb = new_stride_branch, a.n_sh = new_stride_head,
   a.n_st = new_stride_token;
-  a.page_table = page_table, a.page_bounds = page_bounds, a.accept_results = accept_results,
+  a.page_table = page_table, a.page_table_len = page_table_len, a.page_bounds = page_bounds,
+  a.accept_results = accept_results,
   a.cache_lens = cache_lens, a.status = status;
   a.R = num_requests, a.L = num_layers, a.Hk = num_kv_heads, a.TB = block_len;
   const int64_t groups = static_cast<int64_t>(num_requests) * num_layers * 2 * num_kv_heads;

@@ -129,6 +129,7 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
     return plan_fail(D2SD_ERR_INVALID_ARGUMENT, "query heads must be a multiple of kv heads");
   if (window > 0 && !causal)
     return plan_fail(D2SD_ERR_UNSUPPORTED, "a window needs a causal mask");
+  window = std::min(window, kNoLimit);  // positions are below it
   const int G = num_qo_heads / num_kv_heads;
   try {
     if (G > 128) return plan_fail(D2SD_ERR_UNSUPPORTED, "more than 128 query heads per kv head");

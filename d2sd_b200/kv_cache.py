@@ -190,6 +190,11 @@ class PagedKVCache:
 
     def _commit_e4m3(self, new_k, new_v, new_strides, sequences, accept_results, cache_lens):
         kl, sl = self.k[0], self.k_scale[0]
+        for t in list(new_k) + list(new_v):
+            if t.shape != new_k[0].shape or t.shape[1] != self.num_kv_heads \
+                    or t.shape[3] != self.head_dim or t.data_ptr() % 16:
+                raise ValueError("new K/V tensors must share a shape, have the cache's heads and "
+                                 "head_dim and start on 16 bytes")
         ops.commit_kv_e4m3(self._layer_ptrs(new_k, new_v), num_layers=self.num_layers,
                            num_requests=sequences, num_kv_heads=new_k[0].shape[1],
                            head_dim=new_k[0].shape[3], dtype=new_k[0].dtype,

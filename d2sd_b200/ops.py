@@ -618,8 +618,8 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: to
             Hk, n, D, dtype_code(k), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
             stride, rows, rot, 1 if interleaved else 0, _int32("token_start", token_start, R + 1),
             _int32("first_pos", first_pos), R, k_pool.data_ptr(), v_pool.data_ptr(), *pool,
-            _int32("page_table", page_table), _int32("page_bounds", page_bounds, R + 1),
-            _ptr(status))
+            _int32("page_table", page_table), page_table.numel(),
+            _int32("page_bounds", page_bounds, R + 1), _ptr(status))
     _call(dev, load().d2sd_append_kv, args, "d2sd_append_kv")
     return q_out
 
@@ -640,7 +640,7 @@ def read_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, kv_layout: str, page_tab
     if k_pool.dtype != dtype and k_pool.dtype != _E4M3:
         raise ValueError(f"a {k_pool.dtype} cache is not read into {dtype} rows")
     args = (k_pool.data_ptr(), v_pool.data_ptr(), *pool, _int32("page_table", page_table),
-            _int32("page_bounds", page_bounds, R + 1), _int32("token_start", token_start, R + 1),
+            page_table.numel(), _int32("page_bounds", page_bounds, R + 1), _int32("token_start", token_start, R + 1),
             _int32("first_pos", first_pos), R, n, Hk, D, dtype_code(k_out),
             *_rows("k_out", k_out, n, Hk, D, dtype), *_rows("v_out", v_out, n, Hk, D, dtype),
             _ptr(status))
@@ -660,7 +660,7 @@ def commit_kv_e4m3(layer_ptrs: torch.Tensor, *, num_layers: int, num_requests: i
     _same_device(dev, page_table, page_bounds, accept_results, cache_lens, status)
     args = (layer_ptrs.data_ptr(), num_layers, num_requests, num_kv_heads, head_dim,
             _DTYPES.get(dtype, -1), block_len, *new_strides, *cache_strides, num_pages,
-            *scale_strides, _int32("page_table", page_table),
+            *scale_strides, _int32("page_table", page_table), page_table.numel(),
             _int32("page_bounds", page_bounds, num_requests + 1),
             _int32("accept_results", accept_results), _int32("cache_lens", cache_lens),
             _ptr(status))

@@ -17,6 +17,7 @@ import torch
 from . import _lib, ops
 from ._lib import check, load
 
+_WIDE_BYTES = 4 << 30  # scratch of widened pages: a million positions of 8 heads of 128
 _SINKS = {"reference": _lib.SINK_REFERENCE, "exact": _lib.SINK_EXACT}
 
 
@@ -97,7 +98,7 @@ class PagedAttentionPlan:
         sections = np.zeros(20, dtype=np.int32)
         check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, R,
                                   self.num_qo_heads, self.num_kv_heads, 1 if self.causal else 0,
-                                  self.window or 0, 1 if self.eight_bit else 0,
+                                  min(self.window or 0, 1 << 30), 1 if self.eight_bit else 0,
                                   self.num_ctas, plan.ctypes.data, cap,
                                   used.ctypes.data, sections.ctypes.data), "d2sd_paged_plan")
         self._requests, self._entries = (kv, off), {}
@@ -118,9 +119,10 @@ class PagedAttentionPlan:
         # an 8-bit cache is widened first where its keys are gone over three times or
         # more (32 query heads over 16k tokens: 128 new tokens 76 us either way, 256
         # 106 against 117, 2048 over 32k 1060 against 1330), not where the launch has
-        # to fit any batch
-        self.widen = int(sections[16]) >= 3 and not self.fixed_grid
+        # to fit any batch or the scratch would be a cache of its own
         self.wide_pages = int(sections[18] - sections[17])
+        wide_bytes = self.wide_pages * self.num_kv_heads * 16 * self.head_dim * 4
+        self.widen = int(sections[16]) >= 3 and not self.fixed_grid and wide_bytes <= _WIDE_BYTES
         # what every call passes on
         self._args = (self.plan.data_ptr(), sections.ctypes.data, self.num_ctas,
                       1 if self.fixed_grid else 0, self.workspace.data_ptr(),
@@ -149,7 +151,8 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     Returns (out [tokens, Hq, D], lse [tokens, Hq] fp32, base 2), written into
     ``out`` / ``lse`` when given; rows behind the plan's tokens are left alone. A
     row that sees no key has out 0 and lse -inf. Prompt chunks over an e4m3 cache
-    take scratch of 4 * Hk * D bytes for each of their positions. Cache slots past a request's last
+    take scratch of 4 * Hk * D bytes for each of their positions (up to 4 GiB; above
+    it the pages are widened tile by tile). Cache slots past a request's last
     position may hold anything. A NaN or an infinity in the value of a position that
     some row of a tile sees may reach rows of that tile that do not see it."""
     dev = q.get_device()

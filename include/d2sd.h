@@ -513,8 +513,8 @@ int d2sd_commit_kv_hidden(const void* const* layer_ptrs, int32_t num_layers,
  * num_requests requests: request r's new tokens are rows token_start[r] ..
  * token_start[r+1]-1 (device int32 [num_requests+1], ascending), its token i is
  * at position first_pos[r] + i (device int32), and its positions live in pages
- * page_table[page_bounds[r] + p / page_size] (device int32; page_bounds has
- * num_requests+1 entries). Rows behind the last request are not touched.
+ * page_table[page_bounds[r] + p / page_size] (device int32 [page_table_len];
+ * page_bounds has num_requests+1 entries). Rows behind the last request are not touched.
  *
  * 8-bit caches (k_scale, v_scale != NULL): UMMA pages of e4m3 values, element
  * (page, slot r, head h, d) at page*stride_page + h*stride_head + ((r/8)*
@@ -525,7 +525,7 @@ int d2sd_commit_kv_hidden(const void* const* layer_ptrs, int32_t num_layers,
  * A row with a NaN or an infinity reads back as NaN; a byte of 0 reads as 0.
  *
  * status (device int32, may be NULL) receives 4 when a position lies outside
- * its request's pages, 5 for a page id outside the pool, 6 for a position
+ * its request's pages or the table, 5 for a page id outside the pool, 6 for a position
  * outside the rotary tables (the smallest of them, if several); that token's
  * rows are then not written. */
 
@@ -557,7 +557,8 @@ int d2sd_append_kv(const void* q, int64_t q_stride_token, int64_t q_stride_head,
                    int32_t page_size, int64_t num_pages, int32_t cache_format,
                    void* k_scale, void* v_scale, int64_t scale_stride_page,
                    int64_t scale_stride_head, const int32_t* page_table,
-                   const int32_t* page_bounds, int32_t* status, void* stream);
+                   int64_t page_table_len, const int32_t* page_bounds,
+                   int32_t* status, void* stream);
 
 /* Rows out of the cache: k_out/v_out [num_tokens, num_kv_heads, head_dim] in
  * dtype (the cache's type; BF16 or F16 for an e4m3 cache, exact in BF16),
@@ -568,7 +569,8 @@ int d2sd_read_kv(const void* k_pool, const void* v_pool,
                  int64_t num_pages, int32_t cache_format, const void* k_scale,
                  const void* v_scale, int64_t scale_stride_page,
                  int64_t scale_stride_head, const int32_t* page_table,
-                 const int32_t* page_bounds, const int32_t* token_start,
+                 int64_t page_table_len, const int32_t* page_bounds,
+                 const int32_t* token_start,
                  const int32_t* first_pos, int32_t num_requests,
                  int64_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
                  int32_t dtype, void* k_out, int64_t k_out_stride_token,
@@ -587,7 +589,7 @@ int d2sd_commit_kv_e4m3(const void* const* layer_ptrs, int32_t num_layers,
                         int64_t cache_stride_page, int64_t cache_stride_head,
                         int64_t num_pages, int64_t scale_stride_page,
                         int64_t scale_stride_head, const int32_t* page_table,
-                        const int32_t* page_bounds,
+                        int64_t page_table_len, const int32_t* page_bounds,
                         const int32_t* accept_results,
                         const int32_t* cache_lens, int32_t* status,
                         void* stream);

@@ -679,3 +679,100 @@ def test_verify_forward_over_an_8bit_cache(cuda_device):
     a = d.cascade_verify_forward(model, ids, pos, c8)[0]
     b = d.cascade_verify_forward(model, ids, pos, c16)[0]
     assert torch.equal(a, b)
+
+
+def test_page_bounds_behind_the_table_are_reported(cuda_device):
+    """Bounds that give a request more pages than the table has: the positions behind
+    its end are skipped with status 4, the others are written and read."""
+    from d2sd_b200 import ops
+    dev, Hk, D = cuda_device, 2, 128
+    g = torch.Generator().manual_seed(31)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for dtype in (torch.bfloat16, E4M3):
+        kp, ks = new_pool(6, Hk, D, dtype, "paged_umma", dev, g)
+        vp, vs = kp.clone(), None if ks is None else ks.clone()
+        rows = torch.randn(40, Hk, D, generator=g).to(torch.bfloat16).to(dev)
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
+        args = ("paged_umma", ints([4, 2]), ints([0, 3]), ints([0, 40]), ints([0]))
+        kw = dict(k_scale=ks, v_scale=vs, status=status)
+        ops.append_kv(rows, rows, kp, vp, *args, **kw)
+        assert int(status) == 4
+        status.zero_()
+        out = torch.full_like(rows, 9.0), torch.full_like(rows, 9.0)
+        ops.read_kv(kp, vp, *args, *out, **kw)
+        assert int(status) == 4
+        want = rows[:32].double().cpu()
+        if dtype == E4M3:
+            want = OP.e4m3_rows(want)[0]
+        for o in out:
+            assert torch.equal(o[:32].double().cpu(), want) and (o[32:] == 9).all()
+
+
+def test_commit_e4m3_skips_bad_positions_and_pages(cuda_device):
+    from d2sd_b200 import ops
+    dev, Hk, D, T = cuda_device, 2, 64, 8
+    g = torch.Generator().manual_seed(33)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    new = torch.randn(1, Hk, T, D, generator=g).to(torch.bfloat16).to(dev)
+    # (status, page table, bounds, cached length, rows written)
+    for code, table, bounds, length, written in ((4, [1], [0, 1], 12, 4), (4, [1], [0, 2], 12, 4),
+                                                 (5, [1, 9], [0, 2], 12, 4), (0, [2, 0], [0, 2], 12, 8)):
+        kp, ks = new_pool(3, Hk, D, E4M3, "paged_umma", dev, g)
+        kp.view(torch.uint8).zero_()
+        ks.zero_()
+        vp, vs = kp.clone(), ks.clone()
+        ptrs = torch.tensor([t.data_ptr() for t in (new, new, kp, vp, ks, vs)],
+                            dtype=torch.int64, device=dev)
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
+        ops.commit_kv_e4m3(ptrs, num_layers=1, num_requests=1, num_kv_heads=Hk, head_dim=D,
+                           dtype=torch.bfloat16, block_len=T, new_strides=(0, *new.stride()[:3]),
+                           cache_strides=kp.stride()[:2], num_pages=3, scale_strides=ks.stride()[:2],
+                           page_table=ints(table), page_bounds=ints(bounds),
+                           accept_results=ints([T, 0]), cache_lens=ints([length]), status=status)
+        assert int(status) == code
+        for s in (ks, vs):
+            assert int((s != 0).sum()) == written * Hk
+
+
+def test_commit_refuses_other_shapes(cuda_device):
+    import d2sd_b200 as d
+    cache = d.PagedKVCache(1, 2, 64, 64, dtype=E4M3, device=cuda_device)
+    res = torch.tensor([1, 0], dtype=torch.int32, device=cuda_device)
+    for shape in ((1, 3, 4, 64), (1, 2, 4, 128)):
+        x = torch.zeros(shape, dtype=torch.bfloat16, device=cuda_device)
+        with pytest.raises(ValueError):
+            cache.commit([x], [x], res)
+    x = torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16, device=cuda_device)
+    with pytest.raises(ValueError):
+        cache.commit([x], [x[:, :, :3]], res)
+
+
+def test_widened_pages_stay_within_a_bound(cuda_device, monkeypatch):
+    """Above the bound of the scratch the pages are widened tile by tile instead."""
+    import d2sd_b200 as d
+    from d2sd_b200 import paged
+    Hq, Hk, D, ql, kl = 16, 2, 128, [300], [1000]
+    g = torch.Generator().manual_seed(35)
+    c = make_cache(g, kl, Hk, D, E4M3, "paged_umma", cuda_device)
+    q = torch.randn(300, Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    for limit, widen in ((None, True), (63 * 16 * Hk * D * 4, True), (63 * 16 * Hk * D * 4 - 1, False)):
+        if limit is not None:
+            monkeypatch.setattr(paged, "_WIDE_BYTES", limit)
+        plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device)
+        assert plan.widen == widen and plan.wide_pages == 63
+        out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan,
+                                     k_scale=c["ks"], v_scale=c["vs"])
+        check_attention(out, lse, q, c, ql, D, torch.bfloat16)
+
+
+def test_window_larger_than_any_length(cuda_device):
+    import d2sd_b200 as d
+    Hq, Hk, D, ql, kl = 8, 2, 64, [3, 40, 2], [3, 100, 0]
+    g = torch.Generator().manual_seed(37)
+    c = make_cache(g, kl, Hk, D, torch.float16, "paged_hnd", cuda_device)
+    q = torch.randn(sum(ql), Hq, D, generator=g).half().to(cuda_device)
+    for window in (2 ** 31 - 1, 2 ** 31 + 5, 2 ** 32 + 5):
+        plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, window=window,
+                                    page_offsets=c["bounds"])
+        out, lse = d.paged_attention(q, c["k"], c["v"], "paged_hnd", c["table"], plan)
+        check_attention(out, lse, q, c, ql, D, torch.float16)

@@ -154,3 +154,12 @@ def test_e4m3_oracle_against_the_type():
     assert (top <= 448 * 2.0 ** e).all() and ((top > 448 * 2.0 ** (e - 1)) | (e == -126)).all()
     y = x.double() / (2.0 ** e)[:, None]
     assert torch.equal(y.float().to(torch.float8_e4m3fn).double() * (2.0 ** e)[:, None], vals)
+
+
+def test_window_above_every_position(lib):
+    """The largest window an int32 holds is the plan of no position left out, rows
+    without a key (fewer cached positions than new tokens) included."""
+    args = ([1, 40, 7], [5, 900, 2], [0, 1, 58], 8, 2, 1)
+    plan, _ = make(lib, *args, 2 ** 31 - 1, 16)
+    free, _ = make(lib, *args, 1 << 30, 16)
+    assert np.array_equal(plan, free)
