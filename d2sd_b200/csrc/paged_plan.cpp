@@ -4,7 +4,9 @@
 
 #include <algorithm>
 #include <exception>
+#include <functional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/d2sd.h"
@@ -27,6 +29,47 @@ struct Unit {
   int32_t tiles() const { return key1 > key0 ? (key1 - key0 + kTileKeys - 1) / kTileKeys : 0; }
 };
 
+// Whole units on the CTAs, the costliest first and each on the CTA with the least so
+// far, if that leaves no CTA with more than its share and the cost of a cut: then
+// nothing has to be joined. first: the first item of each CTA.
+bool place_whole(const std::vector<Unit>& units, int ctas, int extra, int32_t group, int32_t window,
+                 std::vector<int32_t>& items, std::vector<int32_t>& first) {
+  const size_t n = static_cast<size_t>(ctas);
+  if (units.size() < n) return false;
+  int64_t total = 0, fixed = 0;
+  for (const Unit& u : units) {
+    total += static_cast<int64_t>(u.tiles() + extra) * u.weight;
+    fixed = std::max(fixed, static_cast<int64_t>(extra) * u.weight);
+  }
+  std::vector<int32_t> order(units.size());
+  for (size_t i = 0; i < order.size(); ++i) order[i] = static_cast<int32_t>(i);
+  auto cost = [&](int32_t i) { return static_cast<int64_t>(units[i].tiles() + extra) * units[i].weight; };
+  std::stable_sort(order.begin(), order.end(), [&](int32_t a, int32_t b) { return cost(a) > cost(b); });
+  std::vector<std::pair<int64_t, int32_t>> heap;  // (load, CTA), least load first
+  for (size_t c = 0; c < n; ++c) heap.push_back({0, static_cast<int32_t>(c)});
+  const auto later = std::greater<std::pair<int64_t, int32_t>>();
+  std::vector<std::vector<int32_t>> of(n);
+  for (int32_t i : order) {
+    std::pop_heap(heap.begin(), heap.end(), later);
+    auto& least = heap.back();
+    least.first += cost(i);
+    if (least.first > total / static_cast<int64_t>(n) + fixed) return false;
+    of[least.second].push_back(i);
+    std::push_heap(heap.begin(), heap.end(), later);
+  }
+  first.assign(1, 0);
+  for (const auto& list : of) {
+    for (int32_t i : list) {
+      const Unit& u = units[i];
+      const int32_t it[kItemInts] = {u.req,  u.head,     u.tok0,   u.row0, u.nrows, u.key0, u.key1, u.pos0,
+                                     window, u.page_off, u.kv_len, -1,     1,       u.row0 / group, 0, 0};
+      items.insert(items.end(), it, it + kItemInts);
+    }
+    first.push_back(static_cast<int32_t>(items.size() / kItemInts));
+  }
+  return true;
+}
+
 // The units in order, cut where a CTA's share of the cost ends. An item costs its
 // tiles and `extra` more (its start, its end and, for a split unit, the joining),
 // each of the unit's weight, so a CTA of many small items gets fewer tiles.
@@ -42,6 +85,7 @@ void cut(const std::vector<Unit>& units, int ctas, int section, int32_t group, i
   const int64_t n = std::max<int64_t>(1, std::min<int64_t>(ctas, tiles));
   *slots = 0;
   *most = 1;
+  if (place_whole(units, ctas, extra, group, window, items, first)) return;
   first.assign(1, 0);
   int64_t done = 0;  // cost handed out so far
   int32_t count = 0;

@@ -163,3 +163,26 @@ def test_window_above_every_position(lib):
     plan, _ = make(lib, *args, 2 ** 31 - 1, 16)
     free, _ = make(lib, *args, 1 << 30, 16)
     assert np.array_equal(plan, free)
+
+
+@pytest.mark.parametrize("q,kv,Hq,Hk,window,ctas", [
+    ([4000], [4000], 32, 8, 0, 148),            # a prompt: row tiles of rising cost
+    ([700, 301, 999], [700, 4000, 999], 64, 8, 128, 148),
+    ([1] * 200, [50 + 7 * i for i in range(200)], 8, 8, 0, 100),
+])
+def test_many_units_stay_whole(lib, q, kv, Hq, Hk, window, ctas):
+    """Where whole units balance, none is cut, and no CTA has more than its share and
+    the cost of a cut."""
+    off = np.cumsum([0] + [-(-n // 16) for n in kv])[:-1]
+    plan, sec = make(lib, q, kv, off, Hq, Hk, 1, window, ctas)
+    s = 0 if sec[1] else 1
+    n, items, slots, joins, oc, oi, _, parts = sec[8 * s:8 * s + 8]
+    extra = 1 if s == 0 else 4
+    assert n == (4 * ctas if s == 0 else ctas) and slots == 0 and joins == 0 and parts == 1
+    it = plan[oi:oi + 16 * items].reshape(items, 16)
+    pair = 2 * (128 // (Hq // Hk)) * (Hq // Hk)
+    weight = np.where((it[:, 4] > pair // 2) & (s == 1), 2, 1)
+    cost = (-(-(it[:, 6] - it[:, 5]) // 128) + extra) * weight
+    load = [cost[plan[oc + c]:plan[oc + c + 1]].sum() for c in range(n)]
+    assert plan[oc] == 0 and plan[oc + n] == items and min(load) > 0
+    assert max(load) <= cost.sum() // n + extra * weight.max()
