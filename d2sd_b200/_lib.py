@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from ctypes import POINTER, c_float, c_int32, c_int64, c_uint64, c_void_p, c_char_p
 from pathlib import Path
@@ -94,6 +95,7 @@ SIGNATURES = {
     "d2sd_paged_attention": (i32, [vp, i64, i64, i64, i32, vp, vp, i64, i64, i64, i32, i64, i32, vp, vp,
                                    i64, i64, vp, i64, i32, i32, i32, f32, vp, vp, i32, i32, vp, i64,
                                    vp, vp, vp, i32, vp, i64, i64, vp, i64, vp, vp]),
+    "d2sd_call": (i32, [i32, c_char_p, i32]),
     "d2sd_commit_kv_hidden": (i32, [vp, i32, i32, i32, i32, i32, i64, i64, i64, i64, i64, i64, i32,
                                     i32, vp, vp, vp, i64, vp, i32, i32, i32, i64, i64, vp, i64,
                                     vp]),
@@ -125,6 +127,19 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def packed(entry: int, name: str):
+    """Entry point `name` as a callable of the same arguments (integers and floats, 0
+    for a null pointer), handed over in one piece (d2sd_call)."""
+    args = SIGNATURES[name][1]
+    pack = struct.Struct("=" + "".join("d" if a is f32 else "q" for a in args)).pack
+    n = len(args)
+
+    def call(*values) -> int:
+        return load().d2sd_call(entry, pack(*values), n)
+
+    return call
 
 
 def last_error() -> str:

@@ -484,7 +484,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
 # ---------------------------------------------------------------------------
 # These calls are made for every layer of every step, single tokens included, so
 # the checks below read each tensor's shape and strides once and build nothing.
-_E4M3 = torch.float8_e4m3fn
+_E4M3, _F32, _I32, _U8 = torch.float8_e4m3fn, torch.float32, torch.int32, torch.uint8
+_append_kv = _lib.packed(0, "d2sd_append_kv")
+_read_kv = _lib.packed(1, "d2sd_read_kv")
+paged_attention_call = _lib.packed(2, "d2sd_paged_attention")
+
+
+def _at(t) -> int:
+    """Address of a tensor, 0 for None."""
+    return 0 if t is None else t.data_ptr()
 
 
 def _same_device(dev: int, *ts) -> None:
@@ -497,7 +505,7 @@ def _same_device(dev: int, *ts) -> None:
 
 
 def _int32(name: str, t: torch.Tensor, n: int | None = None) -> int:
-    if t.dtype != torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
+    if t.dtype != _I32 or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise ValueError(f"{name} must be a contiguous int32 tensor"
                          + (f" with {n} entries" if n is not None else ""))
     return t.data_ptr()
@@ -531,13 +539,13 @@ def _pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale):
             raise NotImplementedError("8-bit rows are kept in the paged_umma layout")
         ss = k_scale.stride()
         for s in (k_scale, v_scale):
-            if s.dtype != torch.uint8 or s.shape != shape[:3] or s.stride() != ss or ss[2] != 1:
+            if s.dtype != _U8 or s.shape != shape[:3] or s.stride() != ss or ss[2] != 1:
                 raise ValueError("scales must be uint8 [pages, Hk, 16], slots contiguous")
         return (st[0], slot, head, page, pages, fmt, k_scale.data_ptr(), v_scale.data_ptr(), ss[0],
                 ss[1]), heads, dim
     if k_scale is not None or v_scale is not None:
         raise ValueError("only e4m3 pools have scales")
-    return (st[0], slot, head, page, pages, fmt, None, None, 0, 0), heads, dim
+    return (st[0], slot, head, page, pages, fmt, 0, 0, 0, 0), heads, dim
 
 
 def _rows(name: str, t: torch.Tensor, tokens: int, heads: int, dim: int, dtype):
@@ -590,7 +598,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     if k_pool.dtype != dtype and k_pool.dtype != _E4M3:
         raise ValueError(f"a {k_pool.dtype} cache does not take {dtype} rows")
     R = first_pos.numel()
-    q_args = o_args = (None, 0, 0)
+    q_args = o_args = (0, 0, 0)
     Hq = 0
     if q is not None:
         Hq = q.shape[1]
@@ -609,18 +617,18 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: to
         raise ValueError("cos and sin go together")
     if cos is not None:
         shape, st = cos.shape, cos.stride()
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or sin.shape != shape \
+        if cos.dtype != _F32 or sin.dtype != _F32 or sin.shape != shape \
                 or len(shape) != 2 or sin.stride() != st or st[1] != 1:
             raise ValueError("cos and sin must be fp32 [positions, rotary_dim / 2] with the same "
                              "strides, columns contiguous")
         rows, rot, stride = shape[0], 2 * shape[1], st[0]
     args = (*q_args, *o_args, Hq, *_rows("k", k, n, Hk, D, dtype), *_rows("v", v, n, Hk, D, dtype),
-            Hk, n, D, dtype_code(k), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
+            Hk, n, D, dtype_code(k), _at(q_weight), _at(k_weight), float(eps), _at(cos), _at(sin),
             stride, rows, rot, 1 if interleaved else 0, _int32("token_start", token_start, R + 1),
             _int32("first_pos", first_pos), R, k_pool.data_ptr(), v_pool.data_ptr(), *pool,
             _int32("page_table", page_table), page_table.numel(),
-            _int32("page_bounds", page_bounds, R + 1), _ptr(status))
-    _call(dev, load().d2sd_append_kv, args, "d2sd_append_kv")
+            _int32("page_bounds", page_bounds, R + 1), _at(status))
+    _call(dev, _append_kv, args, "d2sd_append_kv")
     return q_out
 
 
@@ -643,8 +651,8 @@ def read_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, kv_layout: str, page_tab
             page_table.numel(), _int32("page_bounds", page_bounds, R + 1), _int32("token_start", token_start, R + 1),
             _int32("first_pos", first_pos), R, n, Hk, D, dtype_code(k_out),
             *_rows("k_out", k_out, n, Hk, D, dtype), *_rows("v_out", v_out, n, Hk, D, dtype),
-            _ptr(status))
-    _call(dev, load().d2sd_read_kv, args, "d2sd_read_kv")
+            _at(status))
+    _call(dev, _read_kv, args, "d2sd_read_kv")
 
 
 def commit_kv_e4m3(layer_ptrs: torch.Tensor, *, num_layers: int, num_requests: int,

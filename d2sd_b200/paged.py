@@ -190,16 +190,16 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         if lse.dtype != torch.float32 or lse.dim() != 2 or lse.stride(1) != 1 \
                 or lse.shape[0] < tokens or lse.shape[1] != Hq:
             raise ValueError("lse must be fp32 [tokens, num_qo_heads] with a contiguous head axis")
-    wide = (None, None)
+    wide = (0, 0)
     if k_scale is not None and plan.widen:
         scratch = torch.empty((2, plan.wide_pages, Hk, 16, D), dtype=dtype, device=plan.device)
         wide = (scratch.data_ptr(), scratch.data_ptr() + scratch.numel())
     args = (*q_args, n, ops.dtype_code(q), k_pool.data_ptr(), v_pool.data_ptr(), *pool,
             ops._int32("page_table", page_table), page_table.numel(), Hq, Hk, D,
-            D ** -0.5 if sm_scale is None else float(sm_scale), *plan._args, *wide, ops._ptr(sinks),
+            D ** -0.5 if sm_scale is None else float(sm_scale), *plan._args, *wide, ops._at(sinks),
             _SINKS[sink_mode] if sinks is not None else 0, *o_args, lse.data_ptr(), l_stride,
             plan.status.data_ptr())
-    ops._call(dev, load().d2sd_paged_attention, args, "d2sd_paged_attention")
+    ops._call(dev, ops.paged_attention_call, args, "d2sd_paged_attention")
     return out, lse
 
 

@@ -186,3 +186,11 @@ def test_many_units_stay_whole(lib, q, kv, Hq, Hk, window, ctas):
     load = [cost[plan[oc + c]:plan[oc + c + 1]].sum() for c in range(n)]
     assert plan[oc] == 0 and plan[oc + n] == items and min(load) > 0
     assert max(load) <= cost.sum() // n + extra * weight.max()
+
+
+def test_packed_calls_are_checked(lib):
+    """d2sd_call: an unknown entry and a wrong number of words."""
+    words = b"\0" * 8 * 64
+    for entry, n in ((-1, 44), (3, 44), (0, 43), (1, 44), (2, 64)):
+        assert lib.d2sd_call(entry, words, n) == 1 and "d2sd_call" in lib.d2sd_last_error().decode()
+    assert lib.d2sd_call(0, None, 45) == 1
