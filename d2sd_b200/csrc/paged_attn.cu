@@ -62,7 +62,7 @@ struct RowsCfg {
   static constexpr int kSmemBars = kSmemQ + (ELEM == 1 ? 16 * D * 2 : 0);
   static constexpr int kSmemFlags = kSmemBars + kWarps * 8 * 8;
   static constexpr int kSmemBytes = kSmemFlags + 16 + 1024;
-  static_assert(kState <= kRing, "the state fits the ring");
+  static_assert(kState + 128 <= kRing, "the state fits the ring");
   static_assert(kRowsCtas * (kSmemBytes + 1024) <= 227 * 1024 + 1024, "the CTAs of an SM");
 };
 
@@ -121,6 +121,30 @@ template <int CHUNKS, bool UMMA>
 __device__ __forceinline__ uint32_t page_at(int row, int chunk) {
   return UMMA ? static_cast<uint32_t>(((row >> 3) * CHUNKS + chunk) * 128 + (row & 7) * 16)
               : static_cast<uint32_t>((chunk >> 3) * 2048 + row * 128 + (((chunk ^ row) & 7) << 4));
+}
+
+// Shared memory of the cluster's CTA `rank` at this CTA's address, and the barrier of
+// all its threads.
+__device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float peer_float(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 peer_float4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Zeroes rows [r0, r1) of a page in shared memory (the whole warp).
@@ -517,7 +541,60 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
 #pragma unroll
       for (int e = 0; e < kPer; ++e) acc[e] = fmaf(ow[e], f, acc[e]);
     }
-    if (I[P_PARTS] > 1) {  // a span of a unit: leave the state in its slot (join_kernel)
+    if (I[P_PARTS] > 1 && sec[S_JOINS] == 0) {
+      // a unit of one cluster: every CTA leaves its state in its shared memory, and
+      // takes its share of the columns from all of them, in order
+      __syncthreads();  // the rings are read
+      float* state = reinterpret_cast<float*>(smem);
+#pragma unroll
+      for (int e = 0; e < kPer; e += 4)
+        *reinterpret_cast<float4*>(state + row * D + dcol + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+      if (dcol == 0) {
+        state[16 * D + row] = M;
+        state[16 * D + 16 + row] = L;
+      }
+      cluster_sync();
+      auto join = [&](auto n) {
+        constexpr int kSize = decltype(n)::value, kVecs = D / kSize / 4;  // kVecs of a row
+        const int rank = blockIdx.x % kSize;
+        for (int x = threadIdx.x; x < 16 * kVecs; x += kThreads) {
+          const int r = x / kVecs, c = rank * (D / kSize) + x % kVecs * 4;
+          if (r >= nrows) break;
+          float m[kSize], top = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int p = 0; p < kSize; ++p) {
+            m[p] = peer_float(peer_addr(state + 16 * D + r, p));
+            top = fmaxf(top, m[p]);
+          }
+          const float ref = top == -INFINITY ? 0.f : top;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int p = 0; p < kSize; ++p) {
+            const float w = fast_exp2(m[p] - ref);
+            const float4 v = peer_float4(peer_addr(state + r * D + c, p));
+            sum = fmaf(peer_float(peer_addr(state + 16 * D + 16 + r, p)), w, sum);
+            o.x = fmaf(v.x, w, o.x);
+            o.y = fmaf(v.y, w, o.y);
+            o.z = fmaf(v.z, w, o.z);
+            o.w = fmaf(v.w, w, o.w);
+          }
+          const int64_t tok = tok0 + static_cast<int64_t>((row0 + r) / G);
+          const int hq = head * G + (row0 + r) % G;
+          float lse2;
+          float f = row_factor(top, sum, lse2);
+          if (a.sinks) f *= sink_factor(lse2, a.sinks[hq], a.sink_mode);
+          uint2 v;
+          v.x = pack2(o.x * f, o.y * f, T());
+          v.y = pack2(o.z * f, o.w * f, T());
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + tok * a.o_st + hq * a.o_sh + c) = v;
+          if (a.lse && c == 0) a.lse[tok * a.lse_st + hq] = lse2;
+        }
+      };
+      if (I[P_PARTS] == 8) join(std::integral_constant<int, 8>());
+      else if (I[P_PARTS] == 4) join(std::integral_constant<int, 4>());
+      else join(std::integral_constant<int, 2>());
+      cluster_sync();  // the states are read
+    } else if (I[P_PARTS] > 1) {  // a span of a unit: leave the state in its slot (join_kernel)
       float* own = a.slots + static_cast<int64_t>(I[P_SLOT]) * rows_slot_floats(D);
       if (row < nrows) {
 #pragma unroll
@@ -653,7 +730,8 @@ int run_join(const AttnArgs& a, int32_t dtype, int32_t head_dim, const int32_t* 
 }
 
 template <typename T, int D, int ELEM, bool UMMA>
-int launch_rows(const AttnArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, int ctas, cudaStream_t stream) {
+int launch_rows(const AttnArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, int ctas, int cluster,
+                cudaStream_t stream) {
   using C = RowsCfg<D, ELEM>;
   static std::atomic<uint64_t> configured{0};  // bit per device
   int dev = 0;
@@ -665,12 +743,12 @@ int launch_rows(const AttnArgs& a, const CUtensorMap& tk, const CUtensorMap& tv,
       return fail(D2SD_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
     if (dev < 64) configured.fetch_or(1ull << dev);
   }
-  return launch_pdl(rows_kernel<T, D, ELEM, UMMA>, dim3(ctas), dim3(C::kThreads), C::kSmemBytes, stream,
-                    "rows_kernel", tk, tv, a);
+  return launch_pdl_clusters(cluster, rows_kernel<T, D, ELEM, UMMA>, dim3(ctas), dim3(C::kThreads),
+                             C::kSmemBytes, stream, "rows_kernel", tk, tv, a);
 }
 
 int run_rows(const AttnArgs& a, int32_t dtype, int32_t head_dim, int32_t num_kv_heads, bool scaled, int ctas,
-             cudaStream_t st) {
+             int cluster, cudaStream_t st) {
   CUtensorMap tk = {}, tv = {};  // of pages of rows only
   if (!a.g.umma) {
     int rc = encode_pages(&tk, &tv, a, dtype, head_dim, num_kv_heads);
@@ -680,8 +758,8 @@ int run_rows(const AttnArgs& a, int32_t dtype, int32_t head_dim, int32_t num_kv_
     using T = decltype(t);
     constexpr int E = decltype(elem)::value;
     constexpr bool U = decltype(umma)::value;
-    return head_dim == 128 ? launch_rows<T, 128, E, U>(a, tk, tv, ctas, st)
-                           : launch_rows<T, 64, E, U>(a, tk, tv, ctas, st);
+    return head_dim == 128 ? launch_rows<T, 128, E, U>(a, tk, tv, ctas, cluster, st)
+                           : launch_rows<T, 64, E, U>(a, tk, tv, ctas, cluster, st);
   };
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
@@ -738,6 +816,9 @@ extern "C" int d2sd_paged_attention(
       out_stride_token % 8 || out_stride_head % 8 || scale_stride_page % 16 || scale_stride_head % 16)
     return fail(D2SD_ERR_INVALID_ARGUMENT,
                 std::string(w) + ": rows must be 16-byte aligned, strides multiples of 8");
+  const int cluster = sections[S_PARTS] > 1 && sections[S_JOINS] == 0 ? sections[S_PARTS] : 1;
+  if (cluster > 1 && (fixed_grid || cluster > kCluster || sections[S_CTAS] % cluster))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": a plan of clusters does not take a fixed grid");
   bool fits = num_ctas > 0;
   for (int s = 0; s < kSections; ++s) {
     const int32_t* sec = sections + s * kSectionInts;
@@ -770,7 +851,8 @@ extern "C" int d2sd_paged_attention(
   AttnArgs t = a;  // the tiles kernel's half of the workspace
   t.slots += tile_slots_at(num_ctas, head_dim);
   if (sections[S_ITEMS] > 0 || fixed_grid) {
-    rc = run_rows(a, dtype, head_dim, num_kv_heads, scaled, fixed_grid ? section_ctas(0, num_ctas) : sections[S_CTAS], st);
+    rc = run_rows(a, dtype, head_dim, num_kv_heads, scaled, fixed_grid ? section_ctas(0, num_ctas) : sections[S_CTAS],
+                  cluster, st);
     if (rc) return rc;
   }
   if (tiles[S_ITEMS] > 0 || fixed_grid) {

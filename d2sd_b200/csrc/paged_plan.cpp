@@ -70,10 +70,44 @@ bool place_whole(const std::vector<Unit>& units, int ctas, int extra, int32_t gr
   return true;
 }
 
+// Few units of the rows kernel: a cluster of 8, 4 or 2 CTAs for each, its pages shared
+// out evenly, if that ends before the same units cut over all CTAs and joined by a second
+// kernel would. Both estimates in units of a CTA's time for 128 keys with the memory to
+// itself (2.5 us in 16 bits, 1.9 us in 8): all CTAs at once take 2.4 (1.9) times that, and
+// the join costs 4 (5) of them. Measured, clusters against the cut, 8 kv heads of 128, one
+// new token each in 16 bits: 1 request of 1000 keys 8.5 us and 14.7, of 8000 27 and 24; 9
+// of 1000 16 and 27; 18 of 2000 32 and 42; 37 of 500 23.5 and 26.7.
+bool place_clusters(const std::vector<Unit>& units, int ctas, int32_t group, int32_t window, bool eight_bit,
+                    std::vector<int32_t>& items, std::vector<int32_t>& first, int32_t* parts) {
+  int32_t most = 0, size = kCluster;
+  int64_t tiles = 0;
+  for (const Unit& u : units) most = std::max(most, u.key1 - u.key0), tiles += u.tiles();
+  // up to half of the CTAs, or pairs on all of them
+  while (size > 2 && units.size() * size * 2 > static_cast<size_t>(ctas)) size /= 2;
+  if (units.size() * size > static_cast<size_t>(ctas) || most <= kTileKeys) return false;
+  const double full = eight_bit ? 1.9 : 2.4, join = eight_bit ? 5 : 4;
+  const double span = (most + size - 1) / size / static_cast<double>(kTileKeys) * (eight_bit ? 1.25 : 1);
+  const double load = static_cast<double>(tiles) / ctas, used = units.size() * size / static_cast<double>(ctas);
+  if (span * std::max(1., full * used) > std::max(1., load) * std::max(1., full * std::min(1., load)) + join) return false;
+  *parts = size;
+  first.assign(1, 0);
+  for (const Unit& u : units) {
+    const int32_t pages = (u.key1 - u.key0 + 15) / 16, per = (pages + size - 1) / size * 16;
+    for (int32_t p = 0; p < size; ++p) {
+      const int32_t k0 = std::min(u.key0 + p * per, u.key1), k1 = std::min(k0 + per, u.key1);
+      const int32_t it[kItemInts] = {u.req,  u.head,     u.tok0,   u.row0, u.nrows,  k0, k1, u.pos0,
+                                     window, u.page_off, u.kv_len, -1,     size,     u.row0 / group, 0, 0};
+      items.insert(items.end(), it, it + kItemInts);
+      first.push_back(static_cast<int32_t>(items.size() / kItemInts));
+    }
+  }
+  return true;
+}
+
 // The units in order, cut where a CTA's share of the cost ends. An item costs its
 // tiles and `extra` more (its start, its end and, for a split unit, the joining),
 // each of the unit's weight, so a CTA of many small items gets fewer tiles.
-void cut(const std::vector<Unit>& units, int ctas, int section, int32_t group, int32_t window,
+void cut(const std::vector<Unit>& units, int ctas, int section, int32_t group, int32_t window, int32_t flags,
          std::vector<int32_t>& items, std::vector<int32_t>& first, std::vector<int32_t>& joins, int32_t* slots, int32_t* most) {
   const int extra = section == 0 ? 1 : 4;
   const int q_tile = section == 0 ? kRowsTile : 128 / group * group, per = section == 0 ? 1 : 2;
@@ -86,6 +120,9 @@ void cut(const std::vector<Unit>& units, int ctas, int section, int32_t group, i
   *slots = 0;
   *most = 1;
   if (place_whole(units, ctas, extra, group, window, items, first)) return;
+  if (section == 0 && (flags & D2SD_PLAN_CLUSTERS) &&
+      place_clusters(units, ctas, group, window, (flags & D2SD_PLAN_EIGHT_BIT) != 0, items, first, most))
+    return;
   first.assign(1, 0);
   int64_t done = 0;  // cost handed out so far
   int32_t count = 0;
@@ -162,7 +199,7 @@ extern "C" int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_r
 
 extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
                                const int32_t* page_offsets, int32_t num_requests, int32_t num_qo_heads,
-                               int32_t num_kv_heads, int32_t causal, int32_t window, int32_t eight_bit,
+                               int32_t num_kv_heads, int32_t causal, int32_t window, int32_t flags,
                                int32_t num_ctas, int32_t* plan, int64_t capacity, int64_t* used, int32_t* sections) {
   using namespace d2sd;
   using namespace d2sd::paged;
@@ -188,7 +225,7 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
       const int64_t rows = n * G;
       // few rows: tiles of 16 rows; else pairs of q tiles of whole tokens, where a
       // unit of one q tile works on two key tiles at a time
-      const int section = rows <= (eight_bit ? kRowsLimit8 : kRowsLimit) ? 0 : 1;
+      const int section = rows <= (flags & D2SD_PLAN_EIGHT_BIT ? kRowsLimit8 : kRowsLimit) ? 0 : 1;
       const int64_t q_tile = static_cast<int64_t>(128 / G) * G;
       const int64_t tile = section == 0 ? kRowsTile : 2 * q_tile;
       const int32_t pos0 = causal ? static_cast<int32_t>(kv - n) : kNoLimit;
@@ -222,7 +259,7 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
       int32_t sec[kSectionInts] = {0};
       if (!units[s].empty()) {
         std::vector<int32_t> items, first, joins;
-        cut(units[s], section_ctas(s, num_ctas), s, G, window, items, first, joins, &sec[S_SLOTS], &sec[S_PARTS]);
+        cut(units[s], section_ctas(s, num_ctas), s, G, window, flags, items, first, joins, &sec[S_SLOTS], &sec[S_PARTS]);
         sec[S_CTAS] = static_cast<int32_t>(first.size()) - 1;
         sec[S_ITEMS] = static_cast<int32_t>(items.size() / kItemInts);
         sec[S_OFF_CTA] = static_cast<int32_t>(out.size());

@@ -6,7 +6,9 @@
 // cut into spans of whole 128-key tiles; an item is one span. A unit of one item is written out directly; the
 // items of a split unit leave partial states in consecutive slots, which a second
 // kernel joins in slot order (kept apart so that all SMs join, and no state stays
-// behind in the workspace), 4 or 8 rows to an entry of the join list.
+// behind in the workspace), 4 or 8 rows to an entry of the join list. Where every unit
+// can have a cluster of CTAs of its own (few units, not too many keys), its spans are
+// joined inside the cluster instead: parts > 1 and no join list.
 #pragma once
 
 #include <stdint.h>
@@ -22,6 +24,7 @@ constexpr int kRowsCtas = 4;     // CTAs of the rows kernel on an SM
 // tiles of the rows kernel; 8-bit, 20 rows 213 and 142, 32 rows 200 and 136, 64 rows
 // 217 and 264.
 constexpr int kRowsLimit = 16, kRowsLimit8 = 32;
+constexpr int kCluster = 8;  // CTAs of a cluster at most
 constexpr int kMagic = 0x50474131;
 
 // header: magic, then one section per kernel (S_*), kSectionInts ints each

@@ -50,7 +50,7 @@ class PagedAttentionPlan:
             raise ValueError("window must be positive")
         self.num_qo_heads, self.num_kv_heads, self.head_dim = num_qo_heads, num_kv_heads, head_dim
         self.causal, self.window = causal, window
-        self.eight_bit = cache_dtype == torch.float8_e4m3fn
+        self.eight_bit = int(cache_dtype == torch.float8_e4m3fn)
         self.num_ctas = ops.num_sms(device)
         self.fixed_grid = reserve is not None
         self.reserve = reserve
@@ -98,7 +98,7 @@ class PagedAttentionPlan:
         sections = np.zeros(20, dtype=np.int32)
         check(lib.d2sd_paged_plan(q.ctypes.data, kv.ctypes.data, off.ctypes.data, R,
                                   self.num_qo_heads, self.num_kv_heads, 1 if self.causal else 0,
-                                  min(self.window or 0, 1 << 30), 1 if self.eight_bit else 0,
+                                  min(self.window or 0, 1 << 30), self.eight_bit + (0 if self.fixed_grid else 2),
                                   self.num_ctas, plan.ctypes.data, cap,
                                   used.ctypes.data, sections.ctypes.data), "d2sd_paged_plan")
         self._requests, self._entries = (kv, off), {}

@@ -594,6 +594,9 @@ int d2sd_commit_kv_e4m3(const void* const* layer_ptrs, int32_t num_layers,
                         const int32_t* cache_lens, int32_t* status,
                         void* stream);
 
+#define D2SD_PLAN_EIGHT_BIT 1
+#define D2SD_PLAN_CLUSTERS 2
+
 /* Number of int32 entries a d2sd_paged_plan needs (upper bound), -1 if invalid. */
 int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_requests,
                                  int32_t num_qo_heads, int32_t num_kv_heads,
@@ -603,14 +606,16 @@ int64_t d2sd_paged_plan_capacity(const int32_t* q_lens, int32_t num_requests,
  * q_lens[r] new tokens, the last of its kv_lens[r] cached positions (causal:
  * token i sees positions up to kv_lens[r] - q_lens[r] + i, and with window > 0
  * only the last `window` of them; not causal: every position), and its pages
- * start at page_table[page_offsets[r]]. eight_bit: choose the kernels for an
- * 8-bit cache (either choice is right for both). num_ctas is the SM count.
+ * start at page_table[page_offsets[r]]. flags: D2SD_PLAN_EIGHT_BIT chooses the
+ * kernels for an 8-bit cache (either choice is right for both),
+ * D2SD_PLAN_CLUSTERS allows plans of CTA clusters (not with fixed_grid).
+ * num_ctas is the SM count.
  * plan[0 .. capacity) is written on the HOST (*used entries): copy it to the
  * device. sections [20] is the host's copy of what the launch needs. */
 int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
                     const int32_t* page_offsets, int32_t num_requests,
                     int32_t num_qo_heads, int32_t num_kv_heads, int32_t causal,
-                    int32_t window, int32_t eight_bit, int32_t num_ctas,
+                    int32_t window, int32_t flags, int32_t num_ctas,
                     int32_t* plan, int64_t capacity, int64_t* used,
                     int32_t* sections);
 

@@ -776,3 +776,38 @@ def test_window_larger_than_any_length(cuda_device):
                                     page_offsets=c["bounds"])
         out, lse = d.paged_attention(q, c["k"], c["v"], "paged_hnd", c["table"], plan)
         check_attention(out, lse, q, c, ql, D, torch.float16)
+
+
+@pytest.mark.parametrize("D,dtype,layout", [(128, torch.bfloat16, "paged_umma"), (64, torch.float16, "paged_hnd"),
+                                            (64, E4M3, "paged_umma"), (128, E4M3, "paged_umma")])
+@pytest.mark.parametrize("R", [1, 9, 18])
+def test_attention_in_clusters(cuda_device, D, dtype, layout, R):
+    """Plans of clusters of 8, 4 and 2 CTAs: ragged lengths, a request without a key,
+    windows and sinks; and the same plan through an update to one without clusters."""
+    import d2sd_b200 as d
+    Hq, Hk = 16, 8
+    qt = torch.bfloat16 if dtype == E4M3 else dtype
+    g = torch.Generator().manual_seed(41 + R)
+    ql = [1 + i % 8 for i in range(R)]
+    kl = [400] + [(137 * i) % 401 for i in range(1, R)]
+    if R > 1:
+        kl[3], kl[4] = 0, ql[4] - 2
+    c = make_cache(g, kl, Hk, D, dtype, layout, cuda_device, garbage=True)
+    q = torch.randn(sum(ql), Hq, D, generator=g).to(qt).to(cuda_device)
+    sinks = torch.randn(Hq, generator=g).to(cuda_device)
+    kw = dict(cache_dtype=dtype, page_offsets=c["bounds"])
+    for window, s in ((None, None), (150, sinks)):
+        plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, window=window, **kw)
+        if window is None:
+            assert plan.sections[7] == {1: 8, 9: 4, 18: 2}[R] and plan.sections[3] == 0
+        run = lambda: d.paged_attention(q, c["k"], c["v"], layout, c["table"], plan, k_scale=c["ks"],  # noqa: E731
+                                        v_scale=c["vs"], sinks=s)
+        out, lse = run()
+        check_attention(out, lse, q, c, ql, D, qt, window=window, sinks=None if s is None else s.cpu())
+        again, _ = run()
+        assert torch.equal(out, again)
+        plan.update([1] * R, [min(n, 100) for n in kl], c["bounds"])
+        assert plan.sections[7] <= 1 or plan.sections[3] > 0
+        plan.update(ql, kl, c["bounds"])
+        again, _ = run()
+        assert torch.equal(out, again)

@@ -194,3 +194,32 @@ def test_packed_calls_are_checked(lib):
     for entry, n in ((-1, 44), (3, 44), (0, 43), (1, 44), (2, 64)):
         assert lib.d2sd_call(entry, words, n) == 1 and "d2sd_call" in lib.d2sd_last_error().decode()
     assert lib.d2sd_call(0, None, 45) == 1
+
+
+@pytest.mark.parametrize("q,kv,Hq,Hk,window", [([1], [1000], 32, 8, 0), ([4], [130], 32, 8, 0),
+                                               ([1, 0, 3, 2], [2001, 7, 0, 129], 8, 2, 300),
+                                               ([1], [4096], 64, 8, 0), ([3], [4000], 40, 8, 17 + 512)])
+def test_plan_of_clusters(lib, q, kv, Hq, Hk, window):
+    """Few units: eight consecutive CTAs of one item each for every unit, their spans of
+    whole pages in order and without a gap, and nothing to join."""
+    off = np.cumsum([0] + [-(-n // 16) for n in kv])[:-1]
+    plan, sec = make(lib, q, kv, off, Hq, Hk, 1, window, 148, 2)
+    n, items, slots, joins, oc, oi, _, parts = sec[:8]
+    assert parts in (4, 8) and slots == 0 and joins == 0 and n == items and n % parts == 0 and n <= 592
+    assert list(plan[oc:oc + n + 1]) == list(range(n + 1))
+    it = plan[oi:oi + 16 * items].reshape(-1, parts, 16)
+    G, seen = Hq // Hk, set()
+    for unit in it:
+        r, head, row0, rows = unit[0, 0], unit[0, 1], unit[0, 3], unit[0, 4]
+        assert (unit[:, [0, 1, 2, 3, 4, 7, 8, 9, 10]] == unit[0, [0, 1, 2, 3, 4, 7, 8, 9, 10]]).all()
+        assert (unit[1:, 5] == unit[:-1, 6]).all() and (unit[:, 5] <= unit[:, 6]).all()
+        last = kv[r] - q[r] + (row0 + rows - 1) // G
+        lo = max(0, kv[r] - q[r] + row0 // G + 1 - window) if window else 0
+        assert unit[0, 5] <= lo or last < 0
+        assert unit[-1, 6] == max(last + 1, 0)
+        inner = unit[:, 5][unit[:, 5] < unit[:, 6]]
+        assert (inner % 16 == 0).all()
+        seen |= {(r, head, x) for x in range(row0, row0 + rows)}
+    assert seen == {(r, h, x) for r in range(len(q)) for h in range(Hk) for x in range(q[r] * G)}
+    # longer prefixes and many units are cut over all CTAs
+    assert make(lib, [1], [9000], [0], Hq, Hk, 1, 0, 148, 2)[1][3] > 0
