@@ -110,6 +110,13 @@ __device__ __forceinline__ void e4m3x4_f16(uint32_t x, uint32_t& lo, uint32_t& h
       : "r"(x));
 }
 
+// The 8 x 8 matrix of 16-bit values of the warp (lane: row lane / 4, two columns), transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -159,8 +166,11 @@ __device__ __forceinline__ void zero_rows(uint8_t* page, int r0, int r1) {
 }
 
 // ELEM: bytes of a cached value (2: T, 1: e4m3); UMMA: pages in core-matrix order,
-// fetched with one bulk copy each (else rows, TMA boxes).
-template <typename T, int D, int ELEM, bool UMMA>
+// fetched with one bulk copy each (else rows, TMA boxes); R8 (8-bit pages): no unit has
+// more than 8 rows, and the products are transposed, keys and columns of v in the
+// instruction's 16 rows and the query rows in its 8 columns: half the products, half the
+// accumulators (64 tokens over e4m3 123 us without).
+template <typename T, int D, int ELEM, bool UMMA, bool R8>
 __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_kernel(
     const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnArgs a) {
   using C = RowsCfg<D, ELEM>;
@@ -207,7 +217,9 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
     // keys a row sees: [lo, hi)
     auto row_hi = [&](int r) { return r < nrows ? max(0, min(kv_len, pos0 + (row0 + r) / G + 1)) : 0; };
     auto row_lo = [&](int r) { return window ? max(0, pos0 + (row0 + r) / G + 1 - window) : 0; };
-    const int hi0 = row_hi(qr), hi1 = row_hi(qr + 8), lo0 = row_lo(qr), lo1 = row_lo(qr + 8);
+    // the two rows whose scores this lane has
+    const int row_a = R8 ? 2 * qc : qr, row_b = R8 ? 2 * qc + 1 : qr + 8;
+    const int hi0 = row_hi(row_a), hi1 = row_hi(row_b), lo0 = row_lo(row_a), lo1 = row_lo(row_b);
     const int hi_min = row_hi(0), hi_max = row_hi(nrows - 1);
     const int lo_min = row_lo(0), lo_max = row_lo(nrows - 1);
 
@@ -234,7 +246,31 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       }
     }
     float row_scale[2] = {a.scale_log2, a.scale_log2};
-    if constexpr (ELEM == 1) {
+    uint32_t qt[R8 ? D / 16 : 1][2];  // row qr, as the second operand
+    if constexpr (R8) {
+      float m = 0.f;
+      uint2 x[D / 16];
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        x[ks] = q0 ? *reinterpret_cast<const uint2*>(q0 + ks * 16 + qc * 4) : make_uint2(0u, 0u);
+        const T* e = reinterpret_cast<const T*>(&x[ks]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(Num<T>::to_f(e[i])));
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const int k = min(141 - static_cast<int>(__float_as_uint(m) >> 23), 126);
+      const float sc = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+      const float inv = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+      row_scale[0] = __shfl_sync(0xffffffffu, inv, 8 * qc);
+      row_scale[1] = __shfl_sync(0xffffffffu, inv, 8 * qc + 4);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const T* e = reinterpret_cast<const T*>(&x[ks]);
+        qt[ks][0] = pack2(Num<T>::to_f(e[0]) * sc, Num<T>::to_f(e[1]) * sc, __half());
+        qt[ks][1] = pack2(Num<T>::to_f(e[2]) * sc, Num<T>::to_f(e[3]) * sc, __half());
+      }
+    } else if constexpr (ELEM == 1) {
       // rows scaled by 2^k to 2^14 <= max|q| < 2^15 and their scores by 2^-k
       float q_scale[2];
 #pragma unroll
@@ -270,9 +306,10 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
         sm_q[ks * 32 + lane] = f;
       }
     }
-    float o[D / 8][4];
+    constexpr int kO = R8 ? D / 16 : D / 8;
+    float o[kO][4];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int i = 0; i < kO; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
     // ---- this warp's pages of 16 keys: b0 + warp, b0 + warp + 8, ... ----
@@ -320,7 +357,7 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
     for (int j = 0; j < C::kStages - 1; ++j) {
       if (j < mine) issue(j);
     }
-    if (ELEM == 1) __syncthreads();  // q is in shared memory
+    if (ELEM == 1 && !R8) __syncthreads();  // q is in shared memory
     bool alive = true;
     int j = 0;
     for (; j < mine; ++j) {
@@ -348,7 +385,23 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       const uint32_t ka = smem_u32(kp);
       const int mt = lane >> 3, r8 = lane & 7;  // matrix of an x4 this lane addresses, and its row
-      if (ELEM == 2) {
+      if constexpr (R8) {
+        // c[0][...]: keys qr (0, 1) and qr + 8 (2, 3) by rows a and b
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ks += 2) {
+          uint32_t b[4];  // (keys 0-7, chunk ks), (8-15, ks), (0-7, ks + 1), (8-15, ks + 1)
+          ldsm4(ka + page_at<kChunks, UMMA>((mt & 1) * 8 + r8, ks + (mt >> 1)), b);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t k[4];
+            e4m3x4_f16(b[2 * h], k[0], k[2]);
+            e4m3x4_f16(b[2 * h + 1], k[1], k[3]);
+            mma16816<__half>(c[h], k, qt[ks + h][0], qt[ks + h][1]);  // two chains
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[0][e] += c[1][e];
+      } else if (ELEM == 2) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           uint32_t b[4];  // (keys 0-7, d lo), (0-7, hi), (8-15, lo), (8-15, hi)
@@ -374,59 +427,86 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
           }
         }
       }
-      uint32_t vb[2] = {0u, 0u};  // value scale bytes of this lane's four keys
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        float k0 = 1.f, k1 = 1.f;
-        if (ELEM == 1) {
-          const uint8_t* sp = kp + 2 * C::kPageBytes + n * 8 + qc * 2;
-          const uint32_t kb = *reinterpret_cast<const uint16_t*>(sp);
-          vb[n] = *reinterpret_cast<const uint16_t*>(sp + 16);
-          k0 = scale_of(kb & 255u);
-          k1 = scale_of(kb >> 8);
-        }
-        c[n][0] *= row_scale[0] * k0;
-        c[n][1] *= row_scale[0] * k1;
-        c[n][2] *= row_scale[1] * k0;
-        c[n][3] *= row_scale[1] * k1;
-      }
-      if (edge) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int x = key + n * 8 + qc * 2 + e;
-            if (x >= hi0 || x < lo0) c[n][e] = -INFINITY;
-            if (x >= hi1 || x < lo1) c[n][2 + e] = -INFINITY;
-            // a scale byte no row sees
-            if (ELEM == 1 && (x >= hi_max || x < lo_min)) vb[n] &= e ? 0x00ffu : 0xff00u;
-          }
-      }
-      // ---- running maximum and sum; o is rescaled only when the maximum grew ----
-      auto row_max = [](float x) {  // over the four lanes of a row
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-      };
-      float vs[2][2];  // 2^e_j
       float x0, x1;    // the rows' maxima of s_j (e4m3: s_j + e_j)
-      if (ELEM == 1) {
-        float ve[2][2];
+      float vs[2][2];  // 2^e_j
+      if constexpr (R8) {
+        const uint8_t* sp = kp + 2 * C::kPageBytes + qr;
+        float ve[2];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t byte = (vb[n] >> (8 * e)) & 255u;
-            vs[n][e] = scale_of(byte);
-            ve[n][e] = exponent_of(byte);
+        for (int n = 0; n < 2; ++n) {
+          const float ks = scale_of(sp[n * 8]);
+          uint32_t vb = sp[16 + n * 8];
+          c[0][2 * n] *= row_scale[0] * ks;
+          c[0][2 * n + 1] *= row_scale[1] * ks;
+          if (edge) {
+            const int x = key + n * 8 + qr;
+            if (x >= hi0 || x < lo0) c[0][2 * n] = -INFINITY;
+            if (x >= hi1 || x < lo1) c[0][2 * n + 1] = -INFINITY;
+            if (x >= hi_max || x < lo_min) vb = 0u;  // a scale byte no row sees
           }
-        x0 = fmaxf(fmaxf(c[0][0] + ve[0][0], c[0][1] + ve[0][1]), fmaxf(c[1][0] + ve[1][0], c[1][1] + ve[1][1]));
-        x1 = fmaxf(fmaxf(c[0][2] + ve[0][0], c[0][3] + ve[0][1]), fmaxf(c[1][2] + ve[1][0], c[1][3] + ve[1][1]));
+          vs[n][0] = scale_of(vb);
+          ve[n] = exponent_of(vb);
+        }
+        x0 = fmaxf(c[0][0] + ve[0], c[0][2] + ve[1]);
+        x1 = fmaxf(c[0][1] + ve[0], c[0][3] + ve[1]);
+#pragma unroll
+        for (int step = 4; step < 32; step *= 2) {  // over the eight lanes of a row
+          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, step));
+          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, step));
+        }
       } else {
-        x0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
-        x1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
+        uint32_t vb[2] = {0u, 0u};  // value scale bytes of this lane's four keys
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          float k0 = 1.f, k1 = 1.f;
+          if (ELEM == 1) {
+            const uint8_t* sp = kp + 2 * C::kPageBytes + n * 8 + qc * 2;
+            const uint32_t kb = *reinterpret_cast<const uint16_t*>(sp);
+            vb[n] = *reinterpret_cast<const uint16_t*>(sp + 16);
+            k0 = scale_of(kb & 255u);
+            k1 = scale_of(kb >> 8);
+          }
+          c[n][0] *= row_scale[0] * k0;
+          c[n][1] *= row_scale[0] * k1;
+          c[n][2] *= row_scale[1] * k0;
+          c[n][3] *= row_scale[1] * k1;
+        }
+        if (edge) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int x = key + n * 8 + qc * 2 + e;
+              if (x >= hi0 || x < lo0) c[n][e] = -INFINITY;
+              if (x >= hi1 || x < lo1) c[n][2 + e] = -INFINITY;
+              // a scale byte no row sees
+              if (ELEM == 1 && (x >= hi_max || x < lo_min)) vb[n] &= e ? 0x00ffu : 0xff00u;
+            }
+        }
+        // ---- running maximum and sum; o is rescaled only when the maximum grew ----
+        auto row_max = [](float x) {  // over the four lanes of a row
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        };
+        if (ELEM == 1) {
+          float ve[2][2];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t byte = (vb[n] >> (8 * e)) & 255u;
+              vs[n][e] = scale_of(byte);
+              ve[n][e] = exponent_of(byte);
+            }
+          x0 = fmaxf(fmaxf(c[0][0] + ve[0][0], c[0][1] + ve[0][1]), fmaxf(c[1][0] + ve[1][0], c[1][1] + ve[1][1]));
+          x1 = fmaxf(fmaxf(c[0][2] + ve[0][0], c[0][3] + ve[0][1]), fmaxf(c[1][2] + ve[1][0], c[1][3] + ve[1][1]));
+        } else {
+          x0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
+          x1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
+        }
+        x0 = row_max(x0);
+        x1 = row_max(x1);
       }
-      x0 = row_max(x0);
-      x1 = row_max(x1);
       if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
         const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
         const float f0 = m0 == n0 ? 1.f : fast_exp2(m0 - n0), f1 = m1 == n1 ? 1.f : fast_exp2(m1 - n1);
@@ -435,32 +515,55 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
         l0 *= f0;
         l1 *= f1;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
+        for (int i = 0; i < kO; ++i) {
           o[i][0] *= f0;
-          o[i][1] *= f0;
-          o[i][2] *= f1;
+          o[i][R8 ? 2 : 1] *= f0;
+          o[i][R8 ? 1 : 2] *= f1;
           o[i][3] *= f1;
         }
       }
       const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
       uint32_t p[4];
+      if constexpr (R8) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float p0 = fast_exp2(c[n][0] - r0), p1 = fast_exp2(c[n][1] - r0);
-        const float p2 = fast_exp2(c[n][2] - r1), p3 = fast_exp2(c[n][3] - r1);
-        l0 += p0 + p1;
-        l1 += p2 + p3;
-        if (ELEM == 1) {
-          p[2 * n] = pack2(p0 * vs[n][0], p1 * vs[n][1], __half());
-          p[2 * n + 1] = pack2(p2 * vs[n][0], p3 * vs[n][1], __half());
-        } else {
-          p[2 * n] = pack2(p0, p1, T());
-          p[2 * n + 1] = pack2(p2, p3, T());
+        for (int n = 0; n < 2; ++n) {
+          const float p0 = fast_exp2(c[0][2 * n] - r0), p1 = fast_exp2(c[0][2 * n + 1] - r1);
+          l0 += p0;
+          l1 += p1;
+          p[n] = transpose8(pack2(p0 * vs[n][0], p1 * vs[n][0], __half()));  // row qr, keys 2 qc, 2 qc + 1
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float p0 = fast_exp2(c[n][0] - r0), p1 = fast_exp2(c[n][1] - r0);
+          const float p2 = fast_exp2(c[n][2] - r1), p3 = fast_exp2(c[n][3] - r1);
+          l0 += p0 + p1;
+          l1 += p2 + p3;
+          if (ELEM == 1) {
+            p[2 * n] = pack2(p0 * vs[n][0], p1 * vs[n][1], __half());
+            p[2 * n + 1] = pack2(p2 * vs[n][0], p3 * vs[n][1], __half());
+          } else {
+            p[2 * n] = pack2(p0, p1, T());
+            p[2 * n + 1] = pack2(p2, p3, T());
+          }
         }
       }
       // ---- o += p v ----
       const uint32_t va = smem_u32(vp);
-      if (ELEM == 2) {
+      if constexpr (R8) {
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 2) {
+          uint32_t b[4];  // pairs of neighbouring d, transposed
+          ldsm4_t(va + page_at<kChunks, UMMA>((mt & 1) * 8 + r8, i + (mt >> 1)), b);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[4];  // even d's pairs of keys, odd d's; keys 0-7, 8-15
+            e4m3x4_f16(__byte_perm(b[2 * h], 0u, 0x3120), v[0], v[1]);
+            e4m3x4_f16(__byte_perm(b[2 * h + 1], 0u, 0x3120), v[2], v[3]);
+            mma16816<__half>(o[i + h], v, p[0], p[1]);
+          }
+        }
+      } else if (ELEM == 2) {
 #pragma unroll
         for (int i = 0; i < D / 8; i += 2) {
           uint32_t b[4];  // (keys 0-7, chunk i), (8-15, i), (0-7, i + 1), (8-15, i + 1), transposed
@@ -498,30 +601,39 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
         if (++read == C::kStages) read = 0, parity ^= 1;
       }
     }
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+#pragma unroll
+    for (int step = R8 ? 4 : 1; step < (R8 ? 32 : 4); step *= 2) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, step);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, step);
+    }
 
     // ---- join the warps: O over the warp's own ring, m and l beside it ----
     __syncwarp();
     float* os = reinterpret_cast<float*>(ring);
+    if constexpr (R8) {
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      // 16-bit: columns of tile i are d = 8 i + n. 8-bit: tiles 2 j, 2 j + 1 hold
-      // the even and the odd d of chunk j
-      const int d0 = ELEM == 2 ? i * 8 + qc * 2 : (i >> 1) * 16 + qc * 4 + (i & 1);
-      const int d1 = ELEM == 2 ? d0 + 1 : d0 + 2;
-      os[qr * D + d0] = o[i][0];
-      os[qr * D + d1] = o[i][1];
-      os[(qr + 8) * D + d0] = o[i][2];
-      os[(qr + 8) * D + d1] = o[i][3];
+      for (int i = 0; i < kO; ++i) {  // columns 16 i + 2 qr and the next, rows a and b
+        *reinterpret_cast<float2*>(os + row_a * D + i * 16 + qr * 2) = make_float2(o[i][0], o[i][2]);
+        *reinterpret_cast<float2*>(os + row_b * D + i * 16 + qr * 2) = make_float2(o[i][1], o[i][3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        // 16-bit: columns of tile i are d = 8 i + n. 8-bit: tiles 2 j, 2 j + 1 hold
+        // the even and the odd d of chunk j
+        const int d0 = ELEM == 2 ? i * 8 + qc * 2 : (i >> 1) * 16 + qc * 4 + (i & 1);
+        const int d1 = ELEM == 2 ? d0 + 1 : d0 + 2;
+        os[qr * D + d0] = o[i][0];
+        os[qr * D + d1] = o[i][1];
+        os[(qr + 8) * D + d0] = o[i][2];
+        os[(qr + 8) * D + d1] = o[i][3];
+      }
     }
-    if (qc == 0) {
-      sm_m[warp * 16 + qr] = m0;
-      sm_m[warp * 16 + qr + 8] = m1;
-      sm_l[warp * 16 + qr] = l0;
-      sm_l[warp * 16 + qr + 8] = l1;
+    if (R8 ? qr == 0 : qc == 0) {
+      sm_m[warp * 16 + row_a] = m0;
+      sm_m[warp * 16 + row_b] = m1;
+      sm_l[warp * 16 + row_a] = l0;
+      sm_l[warp * 16 + row_b] = l1;
     }
     fence_proxy_async_smem();  // before the next item's copies into the ring
     __syncthreads();
@@ -729,7 +841,7 @@ int run_join(const AttnArgs& a, int32_t dtype, int32_t head_dim, const int32_t* 
   return launch_join<SECTION, 1>(a, dtype, head_dim, blocks, st);
 }
 
-template <typename T, int D, int ELEM, bool UMMA>
+template <typename T, int D, int ELEM, bool UMMA, bool R8>
 int launch_rows(const AttnArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, int ctas, int cluster,
                 cudaStream_t stream) {
   using C = RowsCfg<D, ELEM>;
@@ -737,36 +849,38 @@ int launch_rows(const AttnArgs& a, const CUtensorMap& tk, const CUtensorMap& tv,
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 64 || !((configured.load() >> dev) & 1)) {
-    cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, D, ELEM, UMMA>,
+    cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, D, ELEM, UMMA, R8>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
     if (e != cudaSuccess)
       return fail(D2SD_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
     if (dev < 64) configured.fetch_or(1ull << dev);
   }
-  return launch_pdl_clusters(cluster, rows_kernel<T, D, ELEM, UMMA>, dim3(ctas), dim3(C::kThreads),
+  return launch_pdl_clusters(cluster, rows_kernel<T, D, ELEM, UMMA, R8>, dim3(ctas), dim3(C::kThreads),
                              C::kSmemBytes, stream, "rows_kernel", tk, tv, a);
 }
 
 int run_rows(const AttnArgs& a, int32_t dtype, int32_t head_dim, int32_t num_kv_heads, bool scaled, int ctas,
-             int cluster, cudaStream_t st) {
+             int cluster, bool r8, cudaStream_t st) {
   CUtensorMap tk = {}, tv = {};  // of pages of rows only
   if (!a.g.umma) {
     int rc = encode_pages(&tk, &tv, a, dtype, head_dim, num_kv_heads);
     if (rc) return rc;
   }
-  auto go = [&](auto t, auto elem, auto umma) {
+  auto go = [&](auto t, auto elem, auto umma, auto few) {
     using T = decltype(t);
     constexpr int E = decltype(elem)::value;
-    constexpr bool U = decltype(umma)::value;
-    return head_dim == 128 ? launch_rows<T, 128, E, U>(a, tk, tv, ctas, cluster, st)
-                           : launch_rows<T, 64, E, U>(a, tk, tv, ctas, cluster, st);
+    constexpr bool U = decltype(umma)::value, F = decltype(few)::value;
+    return head_dim == 128 ? launch_rows<T, 128, E, U, F>(a, tk, tv, ctas, cluster, st)
+                           : launch_rows<T, 64, E, U, F>(a, tk, tv, ctas, cluster, st);
   };
+  const auto no = std::false_type();
+  const auto yes = std::true_type();
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
-  if (scaled) return go(__nv_bfloat16(), One(), std::true_type());
+  if (scaled) return r8 ? go(__nv_bfloat16(), One(), yes, yes) : go(__nv_bfloat16(), One(), yes, no);
   if (dtype == D2SD_DTYPE_BF16)
-    return a.g.umma ? go(__nv_bfloat16(), Two(), std::true_type()) : go(__nv_bfloat16(), Two(), std::false_type());
-  return a.g.umma ? go(__half(), Two(), std::true_type()) : go(__half(), Two(), std::false_type());
+    return a.g.umma ? go(__nv_bfloat16(), Two(), yes, no) : go(__nv_bfloat16(), Two(), no, no);
+  return a.g.umma ? go(__half(), Two(), yes, no) : go(__half(), Two(), no, no);
 }
 
 }  // namespace
@@ -848,11 +962,12 @@ extern "C" int d2sd_paged_attention(
   a.status = status;
   a.scale_log2 = sm_scale * kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int32_t kinds = sections[kSections * kSectionInts + 3];  // of units (paged_plan.cpp)
   AttnArgs t = a;  // the tiles kernel's half of the workspace
   t.slots += tile_slots_at(num_ctas, head_dim);
   if (sections[S_ITEMS] > 0 || fixed_grid) {
     rc = run_rows(a, dtype, head_dim, num_kv_heads, scaled, fixed_grid ? section_ctas(0, num_ctas) : sections[S_CTAS],
-                  cluster, st);
+                  cluster, !fixed_grid && !(kinds & 2), st);
     if (rc) return rc;
   }
   if (tiles[S_ITEMS] > 0 || fixed_grid) {
@@ -872,7 +987,7 @@ extern "C" int d2sd_paged_attention(
       t.g.num_pages = hi - lo;
     }
     rc = launch_tiles(t, dtype, head_dim, scaled && !wide_k, num_tokens, num_qo_heads, num_kv_heads,
-                      !fixed_grid && sections[kSections * kSectionInts + 3] == 0,
+                      !fixed_grid && !(kinds & 1),
                       fixed_grid ? num_ctas : tiles[S_CTAS], stream);
     if (rc) return rc;
   }

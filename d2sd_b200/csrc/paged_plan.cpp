@@ -284,7 +284,8 @@ extern "C" int d2sd_paged_plan(const int32_t* q_lens, const int32_t* kv_lens,
     }
     int32_t* host = sections + kSections * kSectionInts;
     host[0] = host[1] = host[2] = host[3] = 0;
-    for (const Unit& u : units[1]) host[3] |= u.weight > 1;  // a unit of two q tiles
+    for (const Unit& u : units[1]) host[3] |= u.weight > 1 ? 1 : 0;  // a unit of two q tiles
+    for (const Unit& u : units[0]) host[3] |= u.nrows > 8 ? 2 : 0;   // of more than 8 rows
     if (hi > lo && hi < kNoLimit) {
       host[0] = static_cast<int32_t>(std::min<int64_t>(visits / ((hi - lo) * num_kv_heads), kNoLimit));
       host[1] = static_cast<int32_t>(lo);

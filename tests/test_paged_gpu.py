@@ -811,3 +811,30 @@ def test_attention_in_clusters(cuda_device, D, dtype, layout, R):
         plan.update(ql, kl, c["bounds"])
         again, _ = run()
         assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("Hq,Hk,D,ql,kl,window", [
+    (32, 8, 128, [1, 2, 0, 1, 2, 1], [1, 2, 40, 17, 3001, 1500], None),
+    (64, 8, 64, [1] * 5, [0, 15, 16, 700, 2100], None),
+    (6, 2, 128, [2, 1, 2], [333, 90, 1], 50),
+    (8, 8, 64, [8, 3, 5], [1100, 2, 129], 300),
+    (8, 1, 128, [1], [60000], None),
+    (32, 8, 128, [1] * 80, [37 * i for i in range(80)], None),
+])
+def test_eight_bit_units_of_up_to_eight_rows(cuda_device, Hq, Hk, D, ql, kl, window):
+    import d2sd_b200 as d
+    g = torch.Generator().manual_seed(51)
+    c = make_cache(g, kl, Hk, D, E4M3, "paged_umma", cuda_device, garbage=True)
+    n = sum(ql)
+    # rows of very different sizes: each is scaled by a power of two of its own
+    q = torch.randn(n, Hq, D, generator=g) * 2.0 ** torch.randint(-9, 3, (n, Hq, 1), generator=g)
+    q = q.to(torch.bfloat16).to(cuda_device)
+    sinks = torch.randn(Hq, generator=g).to(cuda_device)
+    plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, window=window, page_offsets=c["bounds"],
+                                cache_dtype=E4M3)
+    assert plan.sections[19] == 0 and plan.sections[9] == 0  # the form of few rows alone
+    for s in (None, sinks):
+        out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, k_scale=c["ks"],
+                                     v_scale=c["vs"], sinks=s)
+        check_attention(out, lse, q, c, ql, D, torch.bfloat16, window=window, sinks=None if s is None else s.cpu())
+    assert int(plan.status) == 0
