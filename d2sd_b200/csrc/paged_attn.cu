@@ -166,10 +166,10 @@ __device__ __forceinline__ void zero_rows(uint8_t* page, int r0, int r1) {
 }
 
 // ELEM: bytes of a cached value (2: T, 1: e4m3); UMMA: pages in core-matrix order,
-// fetched with one bulk copy each (else rows, TMA boxes); R8 (8-bit pages): no unit has
-// more than 8 rows, and the products are transposed, keys and columns of v in the
-// instruction's 16 rows and the query rows in its 8 columns: half the products, half the
-// accumulators (64 tokens over e4m3 123 us without).
+// fetched with one bulk copy each (else rows, TMA boxes); R8: no unit has more than 8
+// rows, and the products are transposed, keys and columns of v in the instruction's 16
+// rows and the query rows in its 8 columns: half the products, exponentials and
+// accumulators (64 tokens over e4m3 pages 111 us, 123 without).
 template <typename T, int D, int ELEM, bool UMMA, bool R8>
 __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_kernel(
     const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const AttnArgs a) {
@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
         q1 = qb + (tok0 + static_cast<int64_t>((row0 + qr + 8) / G)) * a.q_st +
              (head * G + (row0 + qr + 8) % G) * a.q_sh;
     }
-    uint32_t qf[ELEM == 2 ? D / 16 : 1][4];
-    if constexpr (ELEM == 2) {
+    uint32_t qf[ELEM == 2 && !R8 ? D / 16 : 1][4];
+    if constexpr (ELEM == 2 && !R8) {
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         const int d = ks * 16 + qc * 2;
@@ -247,7 +247,13 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
     }
     float row_scale[2] = {a.scale_log2, a.scale_log2};
     uint32_t qt[R8 ? D / 16 : 1][2];  // row qr, as the second operand
-    if constexpr (R8) {
+    if constexpr (R8 && ELEM == 2) {
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qt[ks][0] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + ks * 16 + qc * 2) : 0u;
+        qt[ks][1] = q0 ? *reinterpret_cast<const uint32_t*>(q0 + ks * 16 + qc * 2 + 8) : 0u;
+      }
+    } else if constexpr (R8) {
       float m = 0.f;
       uint2 x[D / 16];
 #pragma unroll
@@ -385,8 +391,15 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       const uint32_t ka = smem_u32(kp);
       const int mt = lane >> 3, r8 = lane & 7;  // matrix of an x4 this lane addresses, and its row
-      if constexpr (R8) {
-        // c[0][...]: keys qr (0, 1) and qr + 8 (2, 3) by rows a and b
+      // R8: c[0] has keys qr (0, 1) and qr + 8 (2, 3) by rows a and b
+      if constexpr (R8 && ELEM == 2) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t k[4];  // (keys 0-7, d lo), (8-15, lo), (0-7, hi), (8-15, hi)
+          ldsm4(ka + page_at<kChunks, UMMA>((mt & 1) * 8 + r8, ks * 2 + (mt >> 1)), k);
+          mma16816<T>(c[ks & 1], k, qt[ks][0], qt[ks][1]);  // two chains
+        }
+      } else if constexpr (R8) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ks += 2) {
           uint32_t b[4];  // (keys 0-7, chunk ks), (8-15, ks), (0-7, ks + 1), (8-15, ks + 1)
@@ -399,8 +412,6 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
             mma16816<__half>(c[h], k, qt[ks + h][0], qt[ks + h][1]);  // two chains
           }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[0][e] += c[1][e];
       } else if (ELEM == 2) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
@@ -434,18 +445,18 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
         float ve[2];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const float ks = scale_of(sp[n * 8]);
-          uint32_t vb = sp[16 + n * 8];
-          c[0][2 * n] *= row_scale[0] * ks;
-          c[0][2 * n + 1] *= row_scale[1] * ks;
+          const float ks = ELEM == 1 ? scale_of(sp[n * 8]) : 1.f;
+          uint32_t vb = ELEM == 1 ? sp[16 + n * 8] : 127u;
+          c[0][2 * n] = (c[0][2 * n] + c[1][2 * n]) * (row_scale[0] * ks);
+          c[0][2 * n + 1] = (c[0][2 * n + 1] + c[1][2 * n + 1]) * (row_scale[1] * ks);
           if (edge) {
             const int x = key + n * 8 + qr;
             if (x >= hi0 || x < lo0) c[0][2 * n] = -INFINITY;
             if (x >= hi1 || x < lo1) c[0][2 * n + 1] = -INFINITY;
-            if (x >= hi_max || x < lo_min) vb = 0u;  // a scale byte no row sees
+            if (ELEM == 1 && (x >= hi_max || x < lo_min)) vb = 0u;  // a scale byte no row sees
           }
           vs[n][0] = scale_of(vb);
-          ve[n] = exponent_of(vb);
+          ve[n] = ELEM == 1 ? exponent_of(vb) : 0.f;
         }
         x0 = fmaxf(c[0][0] + ve[0], c[0][2] + ve[1]);
         x1 = fmaxf(c[0][1] + ve[0], c[0][3] + ve[1]);
@@ -530,7 +541,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
           const float p0 = fast_exp2(c[0][2 * n] - r0), p1 = fast_exp2(c[0][2 * n + 1] - r1);
           l0 += p0;
           l1 += p1;
-          p[n] = transpose8(pack2(p0 * vs[n][0], p1 * vs[n][0], __half()));  // row qr, keys 2 qc, 2 qc + 1
+          // row qr, keys 2 qc and 2 qc + 1
+          p[n] = transpose8(ELEM == 1 ? pack2(p0 * vs[n][0], p1 * vs[n][0], __half()) : pack2(p0, p1, T()));
         }
       } else {
 #pragma unroll
@@ -550,7 +562,14 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       }
       // ---- o += p v ----
       const uint32_t va = smem_u32(vp);
-      if constexpr (R8) {
+      if constexpr (R8 && ELEM == 2) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t v[4];  // (chunk 2 i, keys 0-7), (2 i + 1, 0-7), (2 i, 8-15), (2 i + 1, 8-15), transposed
+          ldsm4_t(va + page_at<kChunks, UMMA>((mt >> 1) * 8 + r8, 2 * i + (mt & 1)), v);
+          mma16816<T>(o[i], v, p[0], p[1]);
+        }
+      } else if constexpr (R8) {
 #pragma unroll
         for (int i = 0; i < D / 16; i += 2) {
           uint32_t b[4];  // pairs of neighbouring d, transposed
@@ -612,7 +631,15 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
     float* os = reinterpret_cast<float*>(ring);
     if constexpr (R8) {
 #pragma unroll
-      for (int i = 0; i < kO; ++i) {  // columns 16 i + 2 qr and the next, rows a and b
+      for (int i = 0; i < kO; ++i) {  // rows a and b
+        if (ELEM == 2) {  // columns 16 i + qr and 16 i + 8 + qr
+          os[row_a * D + i * 16 + qr] = o[i][0];
+          os[row_b * D + i * 16 + qr] = o[i][1];
+          os[row_a * D + i * 16 + 8 + qr] = o[i][2];
+          os[row_b * D + i * 16 + 8 + qr] = o[i][3];
+          continue;
+        }
+        // columns 16 i + 2 qr and the next
         *reinterpret_cast<float2*>(os + row_a * D + i * 16 + qr * 2) = make_float2(o[i][0], o[i][2]);
         *reinterpret_cast<float2*>(os + row_b * D + i * 16 + qr * 2) = make_float2(o[i][1], o[i][3]);
       }
@@ -877,10 +904,11 @@ int run_rows(const AttnArgs& a, int32_t dtype, int32_t head_dim, int32_t num_kv_
   const auto yes = std::true_type();
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
-  if (scaled) return r8 ? go(__nv_bfloat16(), One(), yes, yes) : go(__nv_bfloat16(), One(), yes, no);
+  auto rows = [&](auto t, auto elem, auto umma) { return r8 ? go(t, elem, umma, yes) : go(t, elem, umma, no); };
+  if (scaled) return rows(__nv_bfloat16(), One(), yes);
   if (dtype == D2SD_DTYPE_BF16)
-    return a.g.umma ? go(__nv_bfloat16(), Two(), yes, no) : go(__nv_bfloat16(), Two(), no, no);
-  return a.g.umma ? go(__half(), Two(), yes, no) : go(__half(), Two(), no, no);
+    return a.g.umma ? rows(__nv_bfloat16(), Two(), yes) : rows(__nv_bfloat16(), Two(), no);
+  return a.g.umma ? rows(__half(), Two(), yes) : rows(__half(), Two(), no);
 }
 
 }  // namespace

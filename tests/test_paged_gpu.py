@@ -838,3 +838,24 @@ def test_eight_bit_units_of_up_to_eight_rows(cuda_device, Hq, Hk, D, ql, kl, win
                                      v_scale=c["vs"], sinks=s)
         check_attention(out, lse, q, c, ql, D, torch.bfloat16, window=window, sinks=None if s is None else s.cpu())
     assert int(plan.status) == 0
+
+
+@pytest.mark.parametrize("Hq,Hk,D,dtype,layout,ql,kl,window", [
+    (32, 8, 128, torch.bfloat16, "paged_umma", [1, 2, 0, 1, 2, 1], [1, 2, 40, 17, 3001, 1500], None),
+    (10, 2, 64, torch.float16, "paged_umma", [1] * 5, [0, 15, 16, 700, 2100], None),
+    (6, 2, 128, torch.float16, "paged_hnd", [2, 1, 2], [333, 90, 1], 50),
+    (8, 8, 64, torch.bfloat16, "paged_nhd", [8, 3, 5], [1100, 2, 129], 300),
+    (32, 8, 64, torch.float16, "paged_hnd", [1] * 80, [37 * i for i in range(80)], None),
+])
+def test_units_of_up_to_eight_rows(cuda_device, Hq, Hk, D, dtype, layout, ql, kl, window):
+    import d2sd_b200 as d
+    g = torch.Generator().manual_seed(53)
+    c = make_cache(g, kl, Hk, D, dtype, layout, cuda_device, garbage=True)
+    q = torch.randn(sum(ql), Hq, D, generator=g).to(dtype).to(cuda_device)
+    sinks = torch.randn(Hq, generator=g).to(cuda_device)
+    plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, window=window, page_offsets=c["bounds"])
+    assert plan.sections[19] == 0 and plan.sections[9] == 0  # the form of few rows alone
+    for s in (None, sinks):
+        out, lse = d.paged_attention(q, c["k"], c["v"], layout, c["table"], plan, sinks=s)
+        check_attention(out, lse, q, c, ql, D, dtype, window=window, sinks=None if s is None else s.cpu())
+    assert int(plan.status) == 0
