@@ -9,7 +9,8 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w
 //   (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s)
 // with pairs (i, i + rotary/2) or (2i, 2i + 1), i < rotary/2; the rest of the head
-// stays. All of it in fp32 and rounded once, into q_out and into the cache.
+// stays. All of it in fp32 and rounded once, into q_out and into the cache; an 8-bit k
+// value next to a border between two of them is decided in 64 bits (exact_row).
 // read_kernel: rows back out of the pages, 8-bit values times their scale.
 // commit_e4m3_kernel: the accepted branch's rows (commit.cu) into an 8-bit cache.
 //
@@ -21,6 +22,14 @@
 // table) and its cos and sin are paid once for all its heads, and a warp's
 // neighbouring tokens fill whole 32-byte sectors of the pages, whose rows of eight
 // values lie 16 bytes apart. Few tokens spread their heads over several blocks.
+//
+// Bound: HBM, each row read once and written once. Measured (GPU time; of 6.54 TB/s of a
+// plain copy): 9 prompts of 7 to 3001 tokens, 64 / 8 heads of 64, f16, 389 MB, 74 us =
+// 0.80; about 13,000 tokens of 32 / 8 heads of 128 into e4m3 pages 77 us = 0.59 (rows of 128
+// bytes written as 8-byte pieces), and their rows back 16 us; 32,768 rows of 8 e4m3
+// heads of 128 read into bf16, 202 MB, 37 us = 0.83; one new token of 64 requests 4.2 us.
+// One group per row (the head inside the row index) took 84 us for that read: the chain
+// of loads for each row, and sectors filled by half.
 #include <string>
 #include <type_traits>
 
@@ -84,10 +93,13 @@ __device__ __forceinline__ float exact_rsqrt(float x) {
 }
 
 // Lane `part` of a row's group holds elements 8 part .. 8 part + 7. Writes them to
-// `at` (this lane's 8 bytes of the page) and the row's scale byte. The whole group
-// calls it; rows with store == false only take part in the shuffles.
-template <int D>
-__device__ __forceinline__ void store_e4m3(const float (&f)[8], int part, uint8_t* at, uint8_t* scale,
+// `at` (this lane's 8 bytes of the page) and the row's scale byte. The whole warp
+// calls it; rows with store == false only take part in the shuffles. Returns (with
+// kNear) whether a value lies so near a border between two e4m3 values that the fp32 f
+// may have it on the wrong side: within 16 last places, which covers what cancels in a
+// rotation.
+template <int D, bool kNear>
+__device__ __forceinline__ bool store_e4m3(const float (&f)[8], int part, uint8_t* at, uint8_t* scale,
                                            bool store) {
   float m = 0.f;
   bool bad = false;
@@ -100,13 +112,24 @@ __device__ __forceinline__ void store_e4m3(const float (&f)[8], int part, uint8_
   const bool finite = m <= 3.402823466e38f;
   const uint32_t byte = finite ? e4m3_scale_byte(m) : 255u;
   const float inv = finite ? e4m3_inv_scale(byte) : 0.f;
+  float u[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = f[i] * inv;
+  bool near = false;
+  if (kNear) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)  // the 20 bits behind e4m3's three, against one half
+      near |= ((__float_as_uint(u[i]) - 0x80000u + 16u) & 0xfffffu) < 32u;
+    near = near && finite && store;
+  }
   uint2 q;
-  q.x = e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
-  q.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
+  q.x = e4m3x2(u[0], u[1]) | (e4m3x2(u[2], u[3]) << 16);
+  q.y = e4m3x2(u[4], u[5]) | (e4m3x2(u[6], u[7]) << 16);
   if (!finite) q.x = q.y = 0x7f7f7f7fu;
-  if (!store) return;
+  if (!store) return false;
   *reinterpret_cast<uint2*>(at) = q;
   if (part == 0) *scale = static_cast<uint8_t>(byte);
+  return near;
 }
 
 struct AppendArgs {
@@ -162,8 +185,68 @@ __device__ __forceinline__ Place find_place(int64_t t, int64_t tokens, const int
   return p;
 }
 
+__device__ __forceinline__ uint64_t warp_or(uint64_t x) {
+  const uint32_t lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(x));
+  const uint32_t hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(x >> 32));
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// A lane's eight elements of a k row once more, in 64 bits, rounded to e4m3 with the
+// scale that is there already. The whole warp calls it, after the other rows: about one
+// row in 250 needs it, and in their loop its registers cost all of them (the 13,000
+// tokens named above, written and read back: 90 us without it, 93 so, 116 in the loop).
+template <typename T, int D>
+__device__ __forceinline__ void exact_row(bool ok, const T* row, const T* weight, const float* cos, const float* sin,
+                                       int half, int interleaved, float eps, uint8_t* at, const uint8_t* scale) {
+  constexpr int W = D / 8;
+  const int lane = threadIdx.x & 31, part = lane % W, rot_lanes = half / 4;
+  const bool rotated = part < rot_lanes, first = part < rot_lanes / 2;
+  const int from = rotated ? (first ? lane + rot_lanes / 2 : lane - rot_lanes / 2) : lane;
+  float g[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  Vec8<T> in;
+  __syncwarp();
+  const uint32_t byte = ok ? *scale : 255u;
+  if (ok) {
+    in.load(row);
+    in.get(g);
+  }
+  double r = e4m3_inv_scale(min(byte, 253u));
+  if (weight) {
+    double ss = 0.;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fma(static_cast<double>(g[i]), static_cast<double>(g[i]), ss);
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    ss = ss * (1. / D) + static_cast<double>(eps);
+    const double y = rsqrtf(static_cast<float>(ss));  // to 2^-22, and 2^-43 after a step
+    r *= y * fma(-0.5 * ss * y, y, 1.5);
+    float w[8];
+    in.load(weight);
+    in.get(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] *= w[i];  // exact
+  }
+  uint32_t q[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = interleaved ? g[i ^ 1] : __shfl_sync(0xffffffffu, g[i], from);
+    double y = g[i];
+    if (cos) {
+      const int col = interleaved ? part * 4 + i / 2 : part * 8 - (first ? 0 : half) + i;
+      const double s = sin[col];
+      y = y * cos[col] + static_cast<double>(x) * ((interleaved ? i % 2 == 0 : first) ? -s : s);
+    }
+    y *= r;
+    float u = static_cast<float>(y);  // not onto a border from beside it
+    const uint32_t bits = __float_as_uint(u);
+    if ((bits & 0xfffffu) == 0x80000u && y != u) u = __uint_as_float((y > u) == (u > 0.f) ? bits + 1u : bits - 1u);
+    q[i / 4] |= (e4m3x2(u, 0.f) & 255u) << (i % 4 * 8);
+  }
+  if (byte != 255u) *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
+}
+
 template <typename T, int D, bool Q8>
-__global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a, const int rows_per_block) {
+__global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendArgs a, const int rows_per_block) {
   constexpr int W = D / 8;               // lanes of a row
   constexpr int kGroups = kThreads / W;  // tokens of a block
   const int part = threadIdx.x % W;
@@ -205,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a,
   }
   // heads h0 .. h1 - 1 of q (0), k (1) or v (2): four rows' loads, then their work
   constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+  uint64_t redo = 0;  // (8-bit) k heads with a value of this lane near a border; bit 63: 63 on
   auto heads = [&](auto kind, int h0, int h1, const void* src_p, int64_t st, int64_t sh, const void* weight,
                    uint8_t* dst, int64_t dst_sh, uint8_t* scale) {
     constexpr int kKind = decltype(kind)::value;
@@ -251,14 +335,14 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a,
             for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + x[i] * s[i];
           }
         }
-        // last, as one rounding (x w is exact in fp32 for 16-bit types): fewer values
-        // land on the wrong side of a border of e4m3
+        // last, as one rounding (x w is exact in fp32 for 16-bit types)
         if (kKind != 2 && weight) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] *= inv;
         }
         if (Q8 && kKind != 0) {
-          store_e4m3<D>(f, part, dst + u * dst_sh, scale + u * a.g.scale_head, ok);
+          if (store_e4m3<D, kKind == 1>(f, part, dst + u * dst_sh, scale + u * a.g.scale_head, ok))
+            redo |= 1ull << min(h + u, 63);
         } else if (ok) {
           Vec8<T> v;
           v.set(f);
@@ -277,10 +361,23 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a,
   heads(std::integral_constant<int, 0>(), row0, min(row1, a.Hq), a.q, a.q_st, a.q_sh, a.q_weight,
         static_cast<uint8_t*>(a.q_out) + (t * a.o_st + part * 8) * static_cast<int64_t>(sizeof(T)),
         a.o_sh * static_cast<int64_t>(sizeof(T)), nullptr);
-  heads(std::integral_constant<int, 1>(), max(row0, a.Hq) - a.Hq, min(row1, a.Hq + a.Hk) - a.Hq, a.k, a.k_st,
-        a.k_sh, a.k_weight, a.k_pool + at, a.g.stride_head, a.k_scale + sat);
+  const int k0 = max(row0, a.Hq) - a.Hq, k1 = min(row1, a.Hq + a.Hk) - a.Hq;
+  heads(std::integral_constant<int, 1>(), k0, k1, a.k, a.k_st, a.k_sh, a.k_weight, a.k_pool + at, a.g.stride_head,
+        a.k_scale + sat);
   heads(std::integral_constant<int, 2>(), max(row0, a.Hq + a.Hk) - a.Hq - a.Hk, row1 - a.Hq - a.Hk, a.v, a.v_st,
         a.v_sh, nullptr, a.v_pool + at, a.g.stride_head, a.v_scale + sat);
+  if constexpr (Q8) {
+    if (!a.half && !a.k_weight) return;  // k itself, exact
+    redo = warp_or(redo);
+    for (int h = k0; h < k1; ++h) {
+      if (!(redo >> min(h, 63) & 1)) continue;
+      exact_row<T, D>(ok, static_cast<const T*>(a.k) + t * a.k_st + h * a.k_sh + part * 8,
+                      a.k_weight ? static_cast<const T*>(a.k_weight) + part * 8 : nullptr,
+                      rotated && ok ? a.cos + p.pos * a.table_stride : nullptr,
+                      rotated && ok ? a.sin + p.pos * a.table_stride : nullptr, a.half, a.interleaved, a.eps,
+                      a.k_pool + at + h * a.g.stride_head, a.k_scale + sat + h * a.g.scale_head);
+    }
+  }
 }
 
 // Heads of a token that one block takes: all of them when there are tokens enough
@@ -363,7 +460,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a, const 
 
 // The 8-bit pages of page-table entries [0, entries) as bf16 UMMA pages, entry e at
 // page e: a 16-byte core-matrix row becomes two (exact, see paged.cuh). For attention
-// that goes over the same keys many times.
+// that goes over the same keys many times. 32k positions of 8 heads of 128, 201 MB moved,
+// 30 us = 1.0 of a plain copy's rate (the write stays in L2).
 __global__ void __launch_bounds__(kThreads)
     widen_kernel(const uint8_t* k_pool, const uint8_t* v_pool, const uint8_t* k_scale, const uint8_t* v_scale,
                  const PageGeom g, const int32_t* __restrict__ page_table, int64_t entries, int Hk, int D,
@@ -413,7 +511,8 @@ struct CommitArgs8 {
   int32_t R, L, Hk, TB;
 };
 
-// One group per (request, layer, K | V, head): the accepted rows one after another.
+// One group per (request, layer, K | V, head): the accepted rows one after another. A few
+// rows for each layer; bound by latency.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) commit_e4m3_kernel(const CommitArgs8 a) {
   constexpr int W = D / 8;
@@ -465,7 +564,7 @@ __global__ void __launch_bounds__(kThreads) commit_e4m3_kernel(const CommitArgs8
         }
       }
       const int slot = static_cast<int>(pos & 15);
-      store_e4m3<D>(f, part, pool + page_chunk(a.g, page, h, slot, part >> 1, D / 16) + (part & 1) * 8,
+      store_e4m3<D, false>(f, part, pool + page_chunk(a.g, page, h, slot, part >> 1, D / 16) + (part & 1) * 8,
                     scale + page * a.g.scale_page + h * a.g.scale_head + slot, ok);
     }
   }

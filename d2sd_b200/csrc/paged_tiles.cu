@@ -26,8 +26,17 @@
 // Online softmax in the log2 domain with a lazy maximum: O is rescaled in TMEM
 // only when the running maximum grows by more than 8 (weights stay below 2^8,
 // inside f16). Weights are rounded to nearest for the second product; their fp32
-// values go into the sum. Tiles that every row sees whole skip
-// the mask; the others compare each key with the row's [lo, hi).
+// values go into the sum. Tiles that every row sees whole skip the mask; the others take
+// each score's minimum with an infinity of the sign that the row's [lo, hi) gives it.
+//
+// Measured (32 / 8 heads of 128, bf16; of 1657 TFLOP/s of a library product at full
+// clock): a prompt of 8192 tokens 490 us = 1122 TFLOP/s = 0.68; 2048 tokens over 16k
+// keys 440 to 480 us = 0.65 to 0.70. The chain of one q tile -- softmax, P V, the next
+// Q K^T and two hand-offs -- is as long as the other tile's, which it passes under, so
+// the tensor pipe is active for 53% of the time and the exponential unit for 54%.
+// Heads of 64 have half the product per tile and the same softmax. 16 blocks of 16
+// tokens over 2k to 16k keys 134 us = 0.75 of the copy rate. Chunks under a window of
+// 128 are two tiles each: the start and end of a unit are most of its 10 us.
 #include <atomic>
 #include <string>
 #include <type_traits>
@@ -64,7 +73,8 @@ struct Cfg {
   static constexpr int kSmemLand = kSmemV + kStages * kTileBytes;  // 8-bit K, V tiles, their scales
   static constexpr int kLandBytes = 128 * D;
   // 8-bit tiles on their way in: one of K and V each, more where there is room (a
-  // widened tile's buffer is filled again only after it, a latency of about 2 us)
+  // widened tile's buffer is filled again only after it, a latency of about 2 us; 16
+  // blocks of 16 tokens over e4m3 223 us with one)
   static constexpr int kLand = MODE != kE4m3 ? 0 : (D == 128 ? (SPLIT ? 2 : 1) : 3);
   static constexpr int kSmemScales = kSmemLand + kLand * 2 * kLandBytes;  // [kLand][K, V][128]
   static constexpr int kSmemJoin = kSmemScales + kLand * 256;

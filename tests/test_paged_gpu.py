@@ -859,3 +859,40 @@ def test_units_of_up_to_eight_rows(cuda_device, Hq, Hk, D, dtype, layout, ql, kl
         out, lse = d.paged_attention(q, c["k"], c["v"], layout, c["table"], plan, sinks=s)
         check_attention(out, lse, q, c, ql, D, dtype, window=window, sinks=None if s is None else s.cpu())
     assert int(plan.status) == 0
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_quantised_keys_are_the_nearest(cuda_device, interleaved):
+    """8-bit keys after norm and rotation are the e4m3 values nearest to the 64-bit ones.
+    fp32 is off by at most 4 last places of the rotation's larger operand (inverse root,
+    product by it, two products, their sum), and values within 16 of their own of a border
+    are decided in 64 bits; so only a value under a quarter of its operands may differ."""
+    from d2sd_b200 import ops, rope_tables
+    dev, n, Hk, D = cuda_device, 8192, 8, 128
+    g = torch.Generator(device=dev).manual_seed(61)
+    k = (torch.randn(n, Hk, D, generator=g, device=dev) * 1.7).to(torch.bfloat16)
+    w = (1 + 0.2 * torch.randn(D, generator=g, device=dev)).to(torch.bfloat16)
+    cos, sin = rope_tables(n, D, 1e6, dev)
+    kp = torch.zeros(n // 16, Hk, 16, D, dtype=torch.uint8, device=dev).view(E4M3)
+    vp, ks = kp.clone(), torch.zeros(n // 16, Hk, 16, dtype=torch.uint8, device=dev)
+    vs = ks.clone()
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    args = ("paged_umma", torch.arange(n // 16, dtype=torch.int32, device=dev), ints([0, n // 16]),
+            ints([0, n]), ints([0]))
+    ops.append_kv(k, k, kp, vp, *args, k_scale=ks, v_scale=vs, k_weight=w, cos=cos, sin=sin,
+                  interleaved=interleaved)
+    got, v = torch.empty_like(k), torch.empty_like(k)
+    ops.read_kv(kp, vp, *args, got, v, k_scale=ks, v_scale=vs)
+    x = k.double()
+    y = x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+    c, s = cos.double()[:, None], sin.double()[:, None]
+    a, b = (y[..., 0::2], y[..., 1::2]) if interleaved else (y[..., :D // 2], y[..., D // 2:])
+    pair = (a * c - b * s, b * c + a * s), (a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs()
+    join = (lambda p: torch.stack(p, -1).flatten(-2)) if interleaved else (lambda p: torch.cat(p, -1))
+    f, size = join(pair[0]), join(pair[1:])
+    unit = torch.exp2(ks.view(n // 16, Hk, 16).transpose(1, 2).reshape(n, Hk, 1).double() - 127)
+    # the border test in 64 bits: |f - got| against the distance to the neighbours
+    step = torch.exp2(torch.floor(torch.log2((f.abs() / unit).clamp(min=2.0 ** -6))) - 3) * unit
+    off = (got.double() - f).abs() > step / 2
+    assert int((off & (f.abs() >= size / 4)).sum()) == 0
+    assert int(off.sum()) < 64  # of 8.4 million
