@@ -70,6 +70,7 @@ class PagedAttentionPlan:
                 raise NotImplementedError("paged attention: head_dim must be 64 or 128")
             self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
             self.status = torch.zeros(1, dtype=torch.int32, device=device)
+            self._f32 = torch.empty(0, dtype=torch.float32, device=device)  # new_empty: less host time
             self._set(host, sections, tokens)
             torch.cuda.current_stream(device).synchronize()  # usable on any stream from here
 
@@ -176,14 +177,14 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError(f"the page table must have {plan.entries(pool[3])} entries for this plan")
     q_args = ops._rows("q", q, n, Hq, D, dtype)
     if out is None:
-        out = torch.empty((n, Hq, D), dtype=dtype, device=plan.device)
+        out = q.new_empty(n, Hq, D)
         o_args = (out.data_ptr(), Hq * D, D)
     else:
         if out.shape[0] < tokens:
             raise ValueError(f"out must hold the plan's {tokens} tokens")
         o_args = ops._rows("out", out, out.shape[0], Hq, D, dtype)
     if lse is None:
-        lse = torch.empty((n, Hq), dtype=torch.float32, device=plan.device)
+        lse = plan._f32.new_empty(n, Hq)
         l_stride = Hq
     else:
         l_stride = lse.stride(0)
