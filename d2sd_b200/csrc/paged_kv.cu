@@ -27,7 +27,8 @@
 // plain copy): 9 prompts of 7 to 3001 tokens, 64 / 8 heads of 64, f16, 389 MB, 74 us =
 // 0.80; about 13,000 tokens of 32 / 8 heads of 128 into e4m3 pages 77 us = 0.59 (rows of 128
 // bytes written as 8-byte pieces), and their rows back 16 us; 32,768 rows of 8 e4m3
-// heads of 128 read into bf16, 202 MB, 37 us = 0.83; one new token of 64 requests 4.2 us.
+// heads of 128 read into bf16, 202 MB, 36.6 us = 0.84 (37.2 with four rows in flight);
+// one new token of 64 requests 4.2 us.
 // One group per row (the head inside the row index) took 84 us for that read: the chain
 // of loads for each row, and sectors filled by half.
 #include <string>
@@ -405,7 +406,7 @@ template <typename T, int D, bool Q8>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a, const int rows_per_block) {
   constexpr int W = D / 8;
   constexpr int kGroups = kThreads / W;
-  constexpr int kAhead = 4;  // rows in flight
+  constexpr int kAhead = 8;  // rows in flight
   const int part = threadIdx.x % W;
   const int64_t t = blockIdx.x * static_cast<int64_t>(kGroups) + threadIdx.x / W;
   const int row0 = blockIdx.y * rows_per_block, row1 = min(2 * a.Hk, row0 + rows_per_block);
