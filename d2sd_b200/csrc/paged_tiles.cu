@@ -30,13 +30,13 @@
 // each score's minimum with an infinity of the sign that the row's [lo, hi) gives it.
 //
 // Measured (32 / 8 heads of 128, bf16; of 1657 TFLOP/s of a library product at full
-// clock): a prompt of 8192 tokens 490 us = 1122 TFLOP/s = 0.68; 2048 tokens over 16k
+// clock): a prompt of 8192 tokens 480 us = 1146 TFLOP/s = 0.69; 2048 tokens over 16k
 // keys 440 to 480 us = 0.65 to 0.70. The chain of one q tile -- softmax, P V, the next
 // Q K^T and two hand-offs -- is as long as the other tile's, which it passes under, so
 // the tensor pipe is active for 53% of the time and the exponential unit for 54%.
 // Heads of 64 have half the product per tile and the same softmax. 16 blocks of 16
 // tokens over 2k to 16k keys 134 us = 0.75 of the copy rate. Chunks under a window of
-// 128 are two tiles each: the start and end of a unit are most of its 10 us.
+// 128 are two tiles each: the start and end of a unit are most of its 7 us.
 #include <atomic>
 #include <string>
 #include <type_traits>
