@@ -112,9 +112,10 @@ class PagedKVCache:
         """int32 [0, n] on the device, without a copy from the host (n > 0)."""
         return torch.arange(0, n + 1, n, dtype=torch.int32, device=self.device)
 
-    def _rows_of(self, l: int, s: int, n: int, dtype=torch.bfloat16):
-        """The first n rows of sequence s of an 8-bit layer, [n, Hk, D]."""
-        out = torch.empty(2, n, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
+    def _rows_of(self, l: int, s: int, n: int):
+        """The first n rows of sequence s of an 8-bit layer, bf16 [n, Hk, D]."""
+        out = torch.empty(2, n, self.num_kv_heads, self.head_dim, dtype=torch.bfloat16,
+                          device=self.device)
         if n > 0:
             ks, vs = self.scales(l)
             ops.read_kv(self.k[l], self.v[l], self.kv_layout, self.page_table,
