@@ -34,6 +34,10 @@ MASK_NONE = 0
 MASK_CAUSAL = 1
 MASK_CUSTOM = 2
 
+GRID_FIXED = 1
+GRID_FEW_ROWS = 2
+GRID_EIGHT_ROWS = 4
+
 SINK_NONE = 0
 SINK_REFERENCE = 1
 SINK_EXACT = 2

@@ -869,7 +869,8 @@ template <int SECTION>
 int run_join(const AttnArgs& a, int32_t dtype, int32_t head_dim, const int32_t* sec, int num_ctas,
              bool fixed_grid, cudaStream_t st) {
   const int most = 16 * num_ctas;
-  const int blocks = fixed_grid ? 8 * num_ctas : (sec[S_JOINS] < most ? sec[S_JOINS] : most);
+  // a fixed grid takes what fits the SMs at once (blocks of 1024 threads) and goes on from there
+  const int blocks = fixed_grid ? 2 * num_ctas : (sec[S_JOINS] < most ? sec[S_JOINS] : most);
   if (fixed_grid || sec[S_PARTS] > 8) return launch_join<SECTION, SECTION == 0 ? 8 : 4>(a, dtype, head_dim, blocks, st);
   return launch_join<SECTION, 1>(a, dtype, head_dim, blocks, st);
 }
@@ -997,14 +998,18 @@ extern "C" int d2sd_paged_attention(
   a.scale_log2 = sm_scale * kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int32_t kinds = sections[kSections * kSectionInts + 3];  // of units (paged_plan.cpp)
+  const bool few_rows = (fixed_grid & (D2SD_GRID_FEW_ROWS | D2SD_GRID_EIGHT_ROWS)) != 0;
+  if ((few_rows && tiles[S_ITEMS] > 0) || ((fixed_grid & D2SD_GRID_EIGHT_ROWS) && (kinds & 2)))
+    return fail(D2SD_ERR_INVALID_ARGUMENT, std::string(w) + ": the plan has more rows than fixed_grid says");
   AttnArgs t = a;  // the tiles kernel's half of the workspace
   t.slots += tile_slots_at(num_ctas, head_dim);
   if (sections[S_ITEMS] > 0 || fixed_grid) {
     rc = run_rows(a, dtype, head_dim, num_kv_heads, scaled, fixed_grid ? section_ctas(0, num_ctas) : sections[S_CTAS],
-                  cluster, !fixed_grid && !(kinds & 2), st);
+                  cluster, fixed_grid ? (fixed_grid & D2SD_GRID_EIGHT_ROWS) != 0 : !(kinds & 2), st);
     if (rc) return rc;
   }
-  if (tiles[S_ITEMS] > 0 || fixed_grid) {
+  const bool any_tiles = fixed_grid ? !few_rows : tiles[S_ITEMS] > 0;
+  if (any_tiles) {
     if (wide_k) {  // 8-bit pages that many row tiles go over: widened once
       const int32_t lo = sections[kSections * kSectionInts + 1], hi = sections[kSections * kSectionInts + 2];
       if (lo < 0 || hi <= lo || hi > page_table_len)
@@ -1029,6 +1034,6 @@ extern "C" int d2sd_paged_attention(
     rc = run_join<0>(a, dtype, head_dim, sections, num_ctas, fixed_grid != 0, st);
     if (rc) return rc;
   }
-  if (tiles[S_JOINS] > 0 || fixed_grid) rc = run_join<1>(t, dtype, head_dim, tiles, num_ctas, fixed_grid != 0, st);
+  if (any_tiles && (tiles[S_JOINS] > 0 || fixed_grid)) rc = run_join<1>(t, dtype, head_dim, tiles, num_ctas, fixed_grid != 0, st);
   return rc;
 }

@@ -36,13 +36,15 @@ class PagedAttentionPlan:
     ``reserve=(requests, tokens)`` the device buffers have room for that many, the
     tensors of a call must hold that many tokens, and the launch does not depend on
     the lengths: a captured ``paged_attention`` replays with the updated ones (of a
-    plan without a reserve it must not be replayed after an update).
+    plan without a reserve it must not be replayed after an update). A third number,
+    the most new tokens of one request, saves the launches that only longer ones need
+    (1 for a decode step; up to 16 query rows per kv head).
     """
 
     def __init__(self, q_lens, kv_lens, num_qo_heads: int, num_kv_heads: int, head_dim: int,
                  device: torch.device | str, *, causal: bool = True, window: int | None = None,
                  page_offsets=None, cache_dtype: torch.dtype | None = None,
-                 reserve: tuple[int, int] | None = None):
+                 reserve: tuple[int, ...] | None = None):
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("PagedAttentionPlan needs a CUDA device")
@@ -52,8 +54,16 @@ class PagedAttentionPlan:
         self.causal, self.window = causal, window
         self.eight_bit = int(cache_dtype == torch.float8_e4m3fn)
         self.num_ctas = ops.num_sms(device)
-        self.fixed_grid = reserve is not None
         self.reserve = reserve
+        self.fixed_grid = 0
+        if reserve is not None:
+            self.longest = reserve[2] if len(reserve) > 2 else reserve[1]
+            rows = self.longest * num_qo_heads // num_kv_heads
+            self.fixed_grid = _lib.GRID_FIXED
+            if rows <= (32 if self.eight_bit else 16):
+                self.fixed_grid |= _lib.GRID_FEW_ROWS
+            if rows <= 8:
+                self.fixed_grid |= _lib.GRID_EIGHT_ROWS
         host, sections, tokens = self._plan(q_lens, kv_lens, page_offsets)
         need = len(host)
         if reserve is not None:
@@ -84,7 +94,8 @@ class PagedAttentionPlan:
             if R > 1:
                 raise ValueError("page_offsets are required for several requests")
             page_offsets = [0] * R
-        if self.reserve is not None and (R > self.reserve[0] or int(q.sum()) > self.reserve[1]):
+        if self.reserve is not None and (R > self.reserve[0] or int(q.sum()) > self.reserve[1]
+                                         or int(q.max(initial=0)) > self.longest):
             raise ValueError(f"the batch is larger than the plan's reserve {self.reserve}")
         off = np.ascontiguousarray(page_offsets, dtype=np.int32)[:R]
         if len(off) != R:
@@ -126,7 +137,7 @@ class PagedAttentionPlan:
         self.widen = int(sections[16]) >= 3 and not self.fixed_grid and wide_bytes <= _WIDE_BYTES
         # what every call passes on
         self._args = (self.plan.data_ptr(), sections.ctypes.data, self.num_ctas,
-                      1 if self.fixed_grid else 0, self.workspace.data_ptr(),
+                      self.fixed_grid, self.workspace.data_ptr(),
                       self.workspace.numel())
 
     def update(self, q_lens, kv_lens, page_offsets=None) -> None:

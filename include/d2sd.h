@@ -594,6 +594,9 @@ int d2sd_commit_kv_e4m3(const void* const* layer_ptrs, int32_t num_layers,
                         const int32_t* cache_lens, int32_t* status,
                         void* stream);
 
+#define D2SD_GRID_FIXED 1
+#define D2SD_GRID_FEW_ROWS 2
+#define D2SD_GRID_EIGHT_ROWS 4
 #define D2SD_PLAN_EIGHT_BIT 1
 #define D2SD_PLAN_CLUSTERS 2
 
@@ -633,7 +636,10 @@ int64_t d2sd_paged_workspace_bytes(int32_t num_ctas, int32_t head_dim);
  * Slots past a request's last position may hold anything, NaN included; page
  * ids outside the pool are read as its first or last page. fixed_grid: launch
  * num_ctas CTAs whatever the plan says, so that a captured call stays valid
- * when the plan's device buffer is rewritten. wide_k, wide_v (8-bit caches, or
+ * when the plan's device buffer is rewritten: 0, or D2SD_GRID_FIXED with what
+ * holds for every plan that the buffer will have -- D2SD_GRID_FEW_ROWS: no request
+ * has more rows (new tokens * query heads per kv head) than 16, or 32 in plans with
+ * D2SD_PLAN_EIGHT_BIT; D2SD_GRID_EIGHT_ROWS: none has more than 8. wide_k, wide_v (8-bit caches, or
  * NULL): scratch of (sections[18] - sections[17]) * num_kv_heads * 16 * head_dim
  * bf16 values each, into which the pages of those page-table entries, the span of
  * the requests of many rows, are widened first; sections[16] says how often their

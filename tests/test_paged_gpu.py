@@ -896,3 +896,40 @@ def test_quantised_keys_are_the_nearest(cuda_device, interleaved):
     off = (got.double() - f).abs() > step / 2
     assert int((off & (f.abs() >= size / 4)).sum()) == 0
     assert int(off.sum()) < 64  # of 8.4 million
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("longest", [1, 2, 5])
+def test_captured_decode_steps(cuda_device, dtype, longest):
+    """Reserved plans that say how many new tokens a request has at most: the captured call
+    of up to 8, 16 and 32 query rows replays, and longer requests are refused."""
+    import d2sd_b200 as d
+    Hq, Hk, D, R = 32, 8, 64, 3
+    g = torch.Generator().manual_seed(71)
+    full = [1100, 300, 2500]
+    c = make_cache(g, full, Hk, D, dtype, "paged_umma", cuda_device)
+    q = torch.randn(R * longest, Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    plan = d.PagedAttentionPlan([1] * R, [9] * R, Hq, Hk, D, cuda_device, page_offsets=c["bounds"],
+                                cache_dtype=dtype, reserve=(R, R * longest, longest))
+    out, lse = torch.zeros_like(q), torch.zeros(len(q), Hq, device=cuda_device)
+    call = lambda: d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, k_scale=c["ks"],  # noqa: E731
+                                     v_scale=c["vs"], out=out, lse=lse)
+    call()
+    s = torch.cuda.Stream(cuda_device)
+    s.wait_stream(torch.cuda.current_stream(cuda_device))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s), torch.cuda.graph(graph, stream=s):
+        call()
+    torch.cuda.current_stream(cuda_device).wait_stream(s)
+    for ql, kl in (([1] * R, [9] * R), ([longest, 1, longest], [1100, 16, 2500]), ([0, longest, 0], [7, 300, 9]),
+                   ([longest] * R, [longest - 1, longest, 2000])):
+        plan.update(ql, kl, c["bounds"])
+        graph.replay()
+        torch.cuda.synchronize(cuda_device)
+        cut = dict(c, k_rows=[x[:n] for x, n in zip(c["k_rows"], kl)],
+                   v_rows=[x[:n] for x, n in zip(c["v_rows"], kl)])
+        check_attention(out, lse, q, cut, ql, D, torch.bfloat16)
+    with pytest.raises(ValueError):
+        plan.update([longest + 1, 0, 0], [50] * 3, c["bounds"])
+    assert int(plan.status) == 0
+    del graph
