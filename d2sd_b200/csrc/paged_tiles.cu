@@ -423,13 +423,17 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
           uint32_t f0 = min(byte + 120u, 254u) << 7;
           if (byte == 0u) f0 = 0u;
           if (byte == 255u) f0 = 0x7fc0u;  // NaN
-          if (fix) {
-            const int k = key + row0 + x * kPagesPer * 16;
-            if (k >= hi || k < lo) f0 = 0u;  // a value no row sees
-          }
+          const int k = key + row0 + x * kPagesPer * 16;
+          const bool unseen = fix && (k >= hi || k < lo);  // a value no row sees
+          if (unseen) f0 = 0u;
           f0 |= f0 << 16;
           uint32_t o[8];
           const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+          // e4m3's NaN (all ones but the sign) is no number of the bits moved below:
+          // a byte's carry into its sign bit finds it
+          uint32_t nan = 0u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) nan |= (in[i] & 0x7f7f7f7fu) + 0x01010101u;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -445,6 +449,11 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
             f1 |= f1 << 16;
 #pragma unroll
             for (int i = 0; i < 8; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[i]) : "r"(f1));
+          }
+          if ((nan & 0x80808080u) && !unseen) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if ((in[e / 4] >> (e % 4 * 8) & 0x7fu) == 0x7fu) o[e / 2] |= 0x7fffu << (e % 2 * 16);
           }
           uint8_t* at = dst + x * kPagesPer * (32 * D);
           *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);

@@ -522,7 +522,8 @@ int d2sd_commit_kv_hidden(const void* const* layer_ptrs, int32_t num_layers,
  * row at page*scale_stride_page + h*scale_stride_head + r. The row's values are
  * e4m3 * 2^(byte - 127); the byte is that of the smallest power of two from
  * 2^-126 on with max|row| <= 448 * 2^e, the values are rounded to nearest even.
- * A row with a NaN or an infinity reads back as NaN; a byte of 0 reads as 0.
+ * A row with a NaN or an infinity reads back as NaN; a byte of 0 reads as 0. A
+ * NaN code of e4m3 is NaN whatever its row's byte is.
  *
  * status (device int32, may be NULL) receives 4 when a position lies outside
  * its request's pages or the table, 5 for a page id outside the pool, 6 for a position
