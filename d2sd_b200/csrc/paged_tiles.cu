@@ -10,9 +10,10 @@
 //                as one bulk copy each, row pages as TMA boxes (128-byte swizzle)
 //   warp 9       MMA issuer (one thread): S = Q K^T and O += P V, 128 x 128 x 16
 //                steps, S and O in TMEM, P written over S as 16-bit A operand
-//   warp 10      zeroes the value rows of a span's first and last tile that no row
-//                sees: a weight of 0 would still turn a NaN there into NaN
+//   warp 10      (16-bit pages) zeroes the value rows of a span's first and last tile
+//                that no row sees: a weight of 0 would still turn a NaN there into NaN
 //   warps 0-7    two softmax warpgroups, thread = row = TMEM lane
+//   warps 10, 11 (e4m3 pages) look for NaN codes in the landed tiles
 //   warps 12-15  (e4m3 pages) widen the landed 8-bit tiles, scale included, into the
 //                bf16 tiles the products read; exact, see paged.cuh
 // The two warpgroups ("streams") alternate on the tensor core: while one turns S
@@ -76,6 +77,7 @@ struct Cfg {
   // widened tile's buffer is filled again only after it, a latency of about 2 us; 16
   // blocks of 16 tokens over e4m3 223 us with one)
   static constexpr int kLand = MODE != kE4m3 ? 0 : (D == 128 ? (SPLIT ? 2 : 1) : 3);
+  static_assert(kLand <= kStages, "a tile lands only when the stage's last tile has been counted (nan_finder)");
   static constexpr int kSmemScales = kSmemLand + kLand * 2 * kLandBytes;  // [kLand][K, V][128]
   static constexpr int kSmemJoin = kSmemScales + kLand * 256;
   static constexpr int kSmemBar = kSmemJoin + 128 * 8;  // [128] (m, l) of stream 1
@@ -83,7 +85,8 @@ struct Cfg {
                        B_KEMPTY = B_VFULL + kStages, B_VEMPTY = B_KEMPTY + kStages,
                        B_SFULL = B_VEMPTY + kStages, B_PHALF = B_SFULL + 2, B_PFULL = B_PHALF + 2,
                        B_OFINAL = B_PFULL + 2, B_OFREE = B_OFINAL + 2, B_VREADY = B_OFREE + 2,
-                       B_LFULL = B_VREADY + kStages, B_LEMPTY = B_LFULL + 2 * kLand, kNumBars = B_LEMPTY + 2 * kLand;
+                       B_LFULL = B_VREADY + kStages, B_LEMPTY = B_LFULL + 2 * kLand, B_WIDE = B_LEMPTY + 2 * kLand,
+                       kNumBars = B_WIDE + 2 * kLand;
   static constexpr int kSmemBytes = kSmemBar + kNumBars * 8 + 32 + 1024;  // + alignment slack
   static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 };
@@ -423,17 +426,13 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
           uint32_t f0 = min(byte + 120u, 254u) << 7;
           if (byte == 0u) f0 = 0u;
           if (byte == 255u) f0 = 0x7fc0u;  // NaN
-          const int k = key + row0 + x * kPagesPer * 16;
-          const bool unseen = fix && (k >= hi || k < lo);  // a value no row sees
-          if (unseen) f0 = 0u;
+          if (fix) {
+            const int k = key + row0 + x * kPagesPer * 16;
+            if (k >= hi || k < lo) f0 = 0u;  // a value no row sees
+          }
           f0 |= f0 << 16;
           uint32_t o[8];
           const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-          // e4m3's NaN (all ones but the sign) is no number of the bits moved below:
-          // a byte's carry into its sign bit finds it
-          uint32_t nan = 0u;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) nan |= (in[i] & 0x7f7f7f7fu) + 0x01010101u;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -450,11 +449,6 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
 #pragma unroll
             for (int i = 0; i < 8; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[i]) : "r"(f1));
           }
-          if ((nan & 0x80808080u) && !unseen) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if ((in[e / 4] >> (e % 4 * 8) & 0x7fu) == 0x7fu) o[e / 2] |= 0x7fffu << (e % 2 * 16);
-          }
           uint8_t* at = dst + x * kPagesPer * (32 * D);
           *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
           *reinterpret_cast<uint4*>(at + 128) = make_uint4(o[4], o[5], o[6], o[7]);
@@ -462,8 +456,63 @@ __device__ void widener(uint8_t* smem, uint64_t* bars, volatile int* abort, cons
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&bars[C::B_LEMPTY + 2 * ls + kv]);
+          // the landing buffer last: its next tile is what lets any role go on, which then
+          // finds the other barriers' phases of this tile counted
+          mbar_arrive(&bars[C::B_WIDE + 2 * ls + kv]);
           mbar_arrive(&bars[(kv ? C::B_VFULL : C::B_KFULL) + st]);
+          mbar_arrive(&bars[C::B_LEMPTY + 2 * ls + kv]);
+        }
+      }
+    }
+  }
+}
+
+// e4m3's NaN (all ones but the sign) is no number of the bits that the widener moves.
+// These two warps, idle otherwise, look for it in the landed tiles and put NaN over what
+// the widener has written in its place (in the widener's own loop the search cost 17%: 16
+// blocks of 16 tokens 274 us against 235).
+template <int D, bool SPLIT>
+__device__ void nan_finder(uint8_t* smem, uint64_t* bars, volatile int* abort, const int32_t* items, int item0,
+                           int item1, float rG, int TT) {
+  using C = Cfg<D, kE4m3, SPLIT>;
+  const int tid = threadIdx.x - kFixWarp * 32, lane = threadIdx.x & 31;
+  constexpr int kChunks = 128 * D / 16 / 64;  // of a thread
+  uint32_t kt = 0;
+  for (int it = item0; it < item1; ++it) {
+    const Item I(items, it, rG, TT);
+    const int hi = I.hi_max(), lo = I.lo_min();
+    for (int t = 0; t < I.tiles; ++t, ++kt) {
+      const uint32_t st = kt % C::kStages, ls = kt % C::kLand;
+      const int key = I.key0 + t * kTileKeys;
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        if (!warp_wait(&bars[C::B_LFULL + 2 * ls + kv], (kt / C::kLand) & 1, abort)) return;
+        const uint8_t* src = smem + C::kSmemLand + (2 * ls + kv) * C::kLandBytes;
+        uint32_t found = 0u;  // a byte's carry into its sign bit
+#pragma unroll 4
+        for (int x = 0; x < kChunks; ++x) {
+          const uint4 w = *reinterpret_cast<const uint4*>(src + (x * 64 + tid) * 16);
+          found |= (w.x ^ (w.x + 0x01010101u)) | (w.y ^ (w.y + 0x01010101u));
+          found |= (w.z ^ (w.z + 0x01010101u)) | (w.w ^ (w.w + 0x01010101u));
+        }
+        if (__any_sync(0xffffffffu, (found & 0x80808080u) != 0u)) {
+          if (!warp_wait(&bars[C::B_WIDE + 2 * ls + kv], (kt / C::kLand) & 1, abort)) return;
+          uint8_t* dst = smem + (kv ? C::kSmemV : C::kSmemK) + st * C::kTileBytes;
+          for (int x = 0; x < kChunks; ++x) {
+            // page, row group, chunk and row of the 16 bytes (as in the widener)
+            const int i = x * 64 + tid, y = i % D, g = y / (D / 2), c = (y / 8) % (D / 16), r = y % 8;
+            const int k = key + i / D * 16 + g * 8 + r;
+            if (kv == 1 && (k >= hi || k < lo)) continue;  // zeroed
+            uint16_t* row = reinterpret_cast<uint16_t*>(dst + i / D * (32 * D) + (g * (D / 8) + 2 * c) * 128 + r * 16);
+            for (int e = 0; e < 16; ++e)
+              if ((src[i * 16 + e] & 0x7f) == 0x7f) row[e / 8 * 64 + e % 8] = 0x7fff;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) {
+          mbar_arrive(&bars[(kv ? C::B_VFULL : C::B_KFULL) + st]);
+          mbar_arrive(&bars[C::B_LEMPTY + 2 * ls + kv]);  // last, as there
         }
       }
     }
@@ -812,9 +861,10 @@ __global__ void __launch_bounds__(Cfg<D, MODE, SPLIT>::kThreads, 1)
     mbar_init(&bars[C::B_QFULL], 1);
     mbar_init(&bars[C::B_QFREE], 1);
     for (int s = 0; s < C::kStages; ++s) {
-      // e4m3: full when the widener's four warps have written the tile
-      mbar_init(&bars[C::B_KFULL + s], MODE == kE4m3 ? 4 : 1);
-      mbar_init(&bars[C::B_VFULL + s], MODE == kE4m3 ? 4 : 1);
+      // e4m3: full when the widener's four warps have written the tile and the two
+      // that look for NaN have looked at it
+      mbar_init(&bars[C::B_KFULL + s], MODE == kE4m3 ? 6 : 1);
+      mbar_init(&bars[C::B_VFULL + s], MODE == kE4m3 ? 6 : 1);
       mbar_init(&bars[C::B_KEMPTY + s], 1);
       mbar_init(&bars[C::B_VEMPTY + s], 1);
       mbar_init(&bars[C::B_VREADY + s], 1);
@@ -828,7 +878,8 @@ __global__ void __launch_bounds__(Cfg<D, MODE, SPLIT>::kThreads, 1)
     }
     for (int i = 0; i < 2 * C::kLand; ++i) {
       mbar_init(&bars[C::B_LFULL + i], 1);
-      mbar_init(&bars[C::B_LEMPTY + i], 4);
+      mbar_init(&bars[C::B_LEMPTY + i], 6);
+      mbar_init(&bars[C::B_WIDE + i], 4);
     }
     *abort = 0;
     fence_mbar_init();
@@ -868,7 +919,10 @@ __global__ void __launch_bounds__(Cfg<D, MODE, SPLIT>::kThreads, 1)
     } else if (warp == kMmaWarp) {
       if (elect_one()) mma_issuer<T, D, MODE, SPLIT>(smem, bars, tmem, abort, items, item0, item1, rG, TT);
       __syncwarp();
-    } else if (warp == kFixWarp && MODE != kE4m3) {
+    } else if (MODE == kE4m3 && (warp == kFixWarp || warp == kFixWarp + 1)) {
+      if constexpr (MODE == kE4m3) nan_finder<D, SPLIT>(smem, bars, abort, items, item0, item1, rG, TT);
+      __syncwarp();
+    } else if (warp == kFixWarp) {
       fixer<D, MODE, SPLIT>(smem, bars, abort, items, item0, item1, rG, TT);
       __syncwarp();
     } else if (warp >= 12) {
