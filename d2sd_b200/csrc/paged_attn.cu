@@ -34,8 +34,10 @@
 // at most 1 whatever the rows' sizes are, and the sum takes 2^(s_j - m) <= 2^60 (a
 // value row under 2^-60 is below what f16 weights resolve). The key's scale
 // multiplies the score in fp32.
-// Weights are rounded to 16 bits (bf16: 2^-8 relative, f16: 2^-11) for the second
-// product; maximum, sum and output stay in fp32.
+// Weights are rounded to 16 bits for the second product: bf16 2^-8 relative, f16
+// 2^-11. An f16 below 2^-14 is subnormal, so f16 weights are taken 2^15 times as large
+// (m is 15 less than the maximum): relative down to 2^-29 of the row's largest, and off
+// by at most 2^-40 of it below that. Maximum, sum and output stay in fp32.
 #include <atomic>
 #include <string>
 #include <type_traits>
@@ -180,6 +182,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
   using C = RowsCfg<D, ELEM>;
   constexpr int kWarps = C::kWarps, kThreads = C::kThreads;
   constexpr int kChunks = D * ELEM / 16;  // 16-byte chunks of a row
+  // log2 of the largest weight: 15 in f16, which holds up to 2^16
+  constexpr float kTop = ELEM == 1 || std::is_same<T, __half>::value ? 15.f : 0.f;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));  // of the swizzle
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
           o[i][3] *= f1;
         }
       }
-      const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+      const float r0 = m0 == -INFINITY ? 0.f : m0 - kTop, r1 = m1 == -INFINITY ? 0.f : m1 - kTop;
       uint32_t p[4];
       if constexpr (R8) {
 #pragma unroll
@@ -661,8 +665,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       }
     }
     if (R8 ? qr == 0 : qc == 0) {
-      sm_m[warp * 16 + row_a] = m0;
-      sm_m[warp * 16 + row_b] = m1;
+      sm_m[warp * 16 + row_a] = m0 - kTop;  // what the weights are relative to
+      sm_m[warp * 16 + row_b] = m1 - kTop;
       sm_l[warp * 16 + row_a] = l0;
       sm_l[warp * 16 + row_b] = l1;
     }

@@ -43,3 +43,48 @@ def test_nan_code_of_e4m3_is_nan_in_every_form(cuda_device, D, n, widen, code):
     assert torch.equal(out[~nan], base[~nan])
     out = run(dict(c, k=planted(c["k"])))
     assert out[:, Hq // 2:].isnan().all() and torch.equal(out[:, :Hq // 2], base[:, :Hq // 2])
+
+
+# ---------------------------------------------------------------------------
+# one key far above all others
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("type,layout", [("f16", "paged_umma"), ("f16", "paged_hnd"), ("bf16", "paged_umma"),
+                                         ("e4m3", "paged_umma")])
+@pytest.mark.parametrize("n,kl", [(1, 2000), (4, 2000), (1, 20000), (160, 2000), (40, 9000)])
+@pytest.mark.parametrize("at", [0, 900])
+def test_weights_far_below_the_largest(cuda_device, type, layout, n, kl, at):
+    """A key 16.26 nats (23.5 binades) above all others, whose value row has one column:
+    the other columns are the sum of the others' weights, each of the same relative
+    error as any."""
+    import d2sd_b200 as d
+    Hq, Hk, D = 8, 2, 64
+    dt = torch.float16 if type == "f16" else torch.bfloat16
+    g = torch.Generator().manual_seed(95)
+    c = make_cache(g, [kl], Hk, D, E4M3 if type == "e4m3" else dt, layout, cuda_device)
+    k, v = torch.zeros(kl, Hk, D), torch.ones(kl, Hk, D)
+    k[at, :, 0] = 1.0
+    v[at] = 0.0
+    v[at, :, 5] = 1.0
+    q = torch.zeros(n, Hq, D)
+    q[:, :, 0] = 16.25
+    page_rows = {"k": k, "v": v}
+    for x, rows in page_rows.items():  # as plain rows or core matrices, scales of one
+        blocks = torch.zeros(-(-kl // 16) * 16, Hk, D)
+        blocks[:kl] = rows
+        blocks = blocks.view(-1, 16, Hk, D).transpose(1, 2)
+        store = E4M3 if type == "e4m3" else dt
+        val, byte = OP.e4m3_rows(blocks.double())
+        if type == "e4m3":
+            blocks = (val / 2.0 ** (byte.double() - 127)[..., None]).float()
+            c[x + "s"][c["table"].long()] = byte.to(cuda_device)
+        flat = torch.empty(len(blocks), Hk, 16 * D)
+        flat[..., OP.page_index(layout, D, store.itemsize).flatten()] = blocks.flatten(2)
+        new = flat.view(-1, Hk, 16, D).to(store).to(cuda_device)
+        bits = torch.uint8 if type == "e4m3" else store
+        c[x].view(bits)[c["table"].long()] = new.view(bits)
+    c["k_rows"], c["v_rows"] = [k.double()], [v.double()]
+    q = q.to(dt).to(cuda_device)
+    plan = d.PagedAttentionPlan([n], [kl], Hq, Hk, D, cuda_device, cache_dtype=c["k"].dtype)
+    out, lse = d.paged_attention(q, c["k"], c["v"], layout, c["table"], plan, sm_scale=1.0,
+                                 k_scale=c["ks"], v_scale=c["vs"])
+    check_attention(out, lse, q, c, [n], D, dt, scale=1.0)
