@@ -37,8 +37,10 @@ __device__ __forceinline__ float row_factor(float m, float l, float& lse2) {
   lse2 = l > 0.f ? m + log2f(l) : (l == 0.f ? -INFINITY : l);
   return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 }
-// Factor of the attention sink: o *= sigmoid(lse - sink) (include/d2sd.h).
+// Factor of the attention sink: o *= sigmoid(lse - sink) (include/d2sd.h). A row
+// without a key keeps its 0, with a sink of -inf too.
 __device__ __forceinline__ float sink_factor(float lse2, float sink, int mode) {
+  if (lse2 == -INFINITY) return 0.f;
   const float x = (mode == D2SD_SINK_EXACT ? lse2 * kLn2 : lse2) - sink;
   return 1.f / (1.f + expf(-x));
 }

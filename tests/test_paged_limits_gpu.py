@@ -88,3 +88,32 @@ def test_weights_far_below_the_largest(cuda_device, type, layout, n, kl, at):
     out, lse = d.paged_attention(q, c["k"], c["v"], layout, c["table"], plan, sm_scale=1.0,
                                  k_scale=c["ks"], v_scale=c["vs"])
     check_attention(out, lse, q, c, [n], D, dt, scale=1.0)
+
+
+# ---------------------------------------------------------------------------
+# sinks of -inf
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("Hq,Hk,D,store,ql,kl,kind", [
+    (8, 2, 128, "bf16", [1, 3, 2], [5, 1, 0], "whole"),
+    (16, 8, 64, "bf16", [8], [400], "cluster"), (16, 8, 64, "e4m3", [8, 5], [400, 3], "cluster"),
+    (8, 1, 128, "bf16", [2], [20000], "join"), (8, 8, 64, "bf16", [300, 20], [130, 0], "tiles"),
+    (4, 1, 128, "e4m3", [700], [690], "tiles"),
+])
+def test_sinks_of_minus_infinity(cuda_device, Hq, Hk, D, store, ql, kl, kind):
+    """A head with a sink of -inf has none: nothing is taken from its rows, and a row
+    without a key still gets 0."""
+    import d2sd_b200 as d
+    g = torch.Generator().manual_seed(99)
+    dt = E4M3 if store == "e4m3" else torch.bfloat16
+    c = make_cache(g, kl, Hk, D, dt, "paged_umma", cuda_device, garbage=True)
+    q = torch.randn(sum(ql), Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    sinks = torch.randn(Hq, generator=g).to(cuda_device)
+    sinks[::2] = float("-inf")
+    plan = d.PagedAttentionPlan(ql, kl, Hq, Hk, D, cuda_device, page_offsets=c["bounds"], cache_dtype=dt)
+    s = plan.sections
+    assert {"whole": s[1] > 0 and s[7] <= 1, "cluster": s[7] > 1 and s[3] == 0, "join": s[3] > 0,
+            "tiles": s[9] > 0}[kind]
+    for mode in ("exact", "reference"):
+        out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, k_scale=c["ks"],
+                                     v_scale=c["vs"], sinks=sinks, sink_mode=mode)
+        check_attention(out, lse, q, c, ql, D, torch.bfloat16, sinks=sinks.cpu(), sink_mode=mode)
