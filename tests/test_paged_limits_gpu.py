@@ -117,3 +117,33 @@ def test_sinks_of_minus_infinity(cuda_device, Hq, Hk, D, store, ql, kl, kind):
         out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, k_scale=c["ks"],
                                      v_scale=c["vs"], sinks=sinks, sink_mode=mode)
         check_attention(out, lse, q, c, ql, D, torch.bfloat16, sinks=sinks.cpu(), sink_mode=mode)
+
+
+@pytest.mark.parametrize("n", [1, 4])
+def test_weights_of_large_8bit_values(cuda_device, n):
+    """Values near the top of fp32's range, whose exponent the weights' reference holds:
+    one key 17 binades above the others keeps them."""
+    import d2sd_b200 as d
+    Hq, Hk, D, kl = 8, 2, 64, 300
+    g = torch.Generator().manual_seed(97)
+    c = make_cache(g, [kl], Hk, D, E4M3, "paged_umma", cuda_device)
+    one = torch.zeros(16, D, dtype=torch.float64)
+    one[:, 0] = 1.0
+    for x, rows, byte in (("k", one, 127), ("v", one * 0 + 256, 127 + 112)):
+        flat = torch.empty(16 * D, dtype=torch.uint8)
+        flat[OP.page_index("paged_umma", D, 1).flatten()] = rows.float().to(E4M3).view(torch.uint8).flatten()
+        c[x].view(torch.uint8).flatten(2)[:] = flat.to(cuda_device)
+        c[x + "s"].fill_(byte)
+    # scores by the key's scale: 2^(byte - 127) q_0; position 20 above all others
+    c["ks"].fill_(100)
+    c["ks"][c["table"][1].long(), :, 4] = 127
+    pages = c["table"].long().cpu()
+    c["k_rows"] = [OP.cached_rows(c["k"], "paged_umma", pages, kl, c["ks"])]
+    c["v_rows"] = [OP.cached_rows(c["v"], "paged_umma", pages, kl, c["vs"])]
+    q = torch.zeros(n, Hq, D)
+    q[..., 0] = 12.0
+    q = q.to(torch.bfloat16).to(cuda_device)
+    plan = d.PagedAttentionPlan([n], [kl], Hq, Hk, D, cuda_device, cache_dtype=E4M3)
+    out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, sm_scale=1.0,
+                                 k_scale=c["ks"], v_scale=c["vs"])
+    check_attention(out, lse, q, c, [n], D, torch.bfloat16, scale=1.0)
