@@ -38,7 +38,7 @@
 // 2^-11. An f16 below 2^-14 is subnormal, so f16 weights are taken 2^15 times as large
 // (m is 15 less than the maximum): relative down to 2^-29 of the row's largest, and off
 // by at most 2^-40 of it below that (fp32's own end, 2^-126, is met before that only
-// where value rows are above 2^105: with e = 119 at 2^-22 of the largest). Maximum, sum
+// where value rows are above 2^108: with e = 119 at 2^-22 of the largest). Maximum, sum
 // and output stay in fp32.
 #include <atomic>
 #include <string>

@@ -96,12 +96,16 @@ __device__ __forceinline__ float exact_rsqrt(float x) {
 // Lane `part` of a row's group holds elements 8 part .. 8 part + 7. Writes them to
 // `at` (this lane's 8 bytes of the page) and the row's scale byte. The whole warp
 // calls it; rows with store == false only take part in the shuffles. Returns (with
-// kNear) whether a value lies so near a border between two e4m3 values that the fp32 f
-// may have it on the wrong side: within 16 last places, which covers what cancels in a
-// rotation.
+// kNear) whether a value lies so near a border between two e4m3 values, or the row's
+// largest so near the scale's, that the fp32 f may have it on the wrong side. What f can
+// be off: 10 * 2^-24 relative from the norm's factor and the last products, and from a
+// rotation 2^-24 of the product that is rounded before the sum, of which `product` is
+// the lane's largest. Values are taken 12 * 2^-24 of themselves and 1.25 * 2^-24 of the
+// product up and down (inexact; rows as they came are not); where both round alike the
+// exact value does too.
 template <int D, bool kNear>
 __device__ __forceinline__ bool store_e4m3(const float (&f)[8], int part, uint8_t* at, uint8_t* scale,
-                                           bool store) {
+                                           bool store, bool inexact = false, float product = 0.f) {
   float m = 0.f;
   bool bad = false;
 #pragma unroll
@@ -113,19 +117,29 @@ __device__ __forceinline__ bool store_e4m3(const float (&f)[8], int part, uint8_
   const bool finite = m <= 3.402823466e38f;
   const uint32_t byte = finite ? e4m3_scale_byte(m) : 255u;
   const float inv = finite ? e4m3_inv_scale(byte) : 0.f;
-  float u[8];
+  float u[8], d[8];
+  const float rel = inexact ? 0x1.8p-21f : 0.f;
+  // (2^-23 of the scale for rows whose f are subnormal)
+  const float least = inexact ? fmaf(product * inv, 0x1.4p-24f, 0x1p-23f) : 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = f[i] * inv;
+  for (int i = 0; i < 8; ++i) {
+    u[i] = f[i] * inv;
+    d[i] = kNear ? fmaf(fabsf(u[i]), rel, least) : 0.f;
+  }
+  auto pack = [&](float sign) {
+    auto x = [&](int i) { return fmaf(d[i], sign, u[i]); };
+    return make_uint2(e4m3x2(x(0), x(1)) | (e4m3x2(x(2), x(3)) << 16),
+                      e4m3x2(x(4), x(5)) | (e4m3x2(x(6), x(7)) << 16));
+  };
+  uint2 q = pack(kNear ? 1.f : 0.f);
   bool near = false;
   if (kNear) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)  // the 20 bits behind e4m3's three, against one half
-      near |= ((__float_as_uint(u[i]) - 0x80000u + 16u) & 0xfffffu) < 32u;
-    near = near && finite && store;
+    const uint2 down = pack(-1.f);
+    const float top = m * inv;  // 224 to 448
+    near = (((q.x ^ down.x) | (q.y ^ down.y)) & 0x7f7f7f7fu) != 0u  // (a zero's sign aside)
+           || top > 448.f - 0x1p-10f || (top < 224.f + 0x1p-10f && byte > 1u);
+    near = near && inexact && finite && store;
   }
-  uint2 q;
-  q.x = e4m3x2(u[0], u[1]) | (e4m3x2(u[2], u[3]) << 16);
-  q.y = e4m3x2(u[4], u[5]) | (e4m3x2(u[6], u[7]) << 16);
   if (!finite) q.x = q.y = 0x7f7f7f7fu;
   if (!store) return false;
   *reinterpret_cast<uint2*>(at) = q;
@@ -192,26 +206,25 @@ __device__ __forceinline__ uint64_t warp_or(uint64_t x) {
   return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-// A lane's eight elements of a k row once more, in 64 bits, rounded to e4m3 with the
-// scale that is there already. The whole warp calls it, after the other rows: about one
-// row in 250 needs it, and in their loop its registers cost all of them (the 13,000
-// tokens named above, written and read back: 90 us without it, 93 so, 116 in the loop).
+// A lane's eight elements of a k row once more, in 64 bits, with the scale. The whole
+// warp calls it, after the other rows, and only rows with ok are written: what a token's
+// rows become is theirs alone. About one row in 230 needs it, which costs 1 us of the 77
+// of 13,000 tokens; in the rows' own loop its registers would cost all of them (116 us
+// for the same tokens written and read back, 93 so).
 template <typename T, int D>
 __device__ __forceinline__ void exact_row(bool ok, const T* row, const T* weight, const float* cos, const float* sin,
-                                       int half, int interleaved, float eps, uint8_t* at, const uint8_t* scale) {
+                                          int half, int interleaved, float eps, uint8_t* at, uint8_t* scale) {
   constexpr int W = D / 8;
   const int lane = threadIdx.x & 31, part = lane % W, rot_lanes = half / 4;
   const bool rotated = part < rot_lanes, first = part < rot_lanes / 2;
   const int from = rotated ? (first ? lane + rot_lanes / 2 : lane - rot_lanes / 2) : lane;
   float g[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   Vec8<T> in;
-  __syncwarp();
-  const uint32_t byte = ok ? *scale : 255u;
   if (ok) {
     in.load(row);
     in.get(g);
   }
-  double r = e4m3_inv_scale(min(byte, 253u));
+  double root = 1.;
   if (weight) {
     double ss = 0.;
 #pragma unroll
@@ -219,31 +232,43 @@ __device__ __forceinline__ void exact_row(bool ok, const T* row, const T* weight
 #pragma unroll
     for (int o = W / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     ss = ss * (1. / D) + static_cast<double>(eps);
-    const double y = rsqrtf(static_cast<float>(ss));  // to 2^-22, and 2^-43 after a step
-    r *= y * fma(-0.5 * ss * y, y, 1.5);
+    root = rsqrtf(static_cast<float>(ss));  // to 2^-22, and 2^-43 and 2^-52 after a step
+    root *= fma(-0.5 * ss * root, root, 1.5);
+    root *= fma(-0.5 * ss * root, root, 1.5);
     float w[8];
     in.load(weight);
     in.get(w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) g[i] *= w[i];  // exact
   }
-  uint32_t q[2] = {0u, 0u};
+  double y[8], top = 0.;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float x = interleaved ? g[i ^ 1] : __shfl_sync(0xffffffffu, g[i], from);
-    double y = g[i];
+    y[i] = g[i];
     if (cos) {
       const int col = interleaved ? part * 4 + i / 2 : part * 8 - (first ? 0 : half) + i;
       const double s = sin[col];
-      y = y * cos[col] + static_cast<double>(x) * ((interleaved ? i % 2 == 0 : first) ? -s : s);
+      y[i] = y[i] * cos[col] + static_cast<double>(x) * ((interleaved ? i % 2 == 0 : first) ? -s : s);
     }
-    y *= r;
-    float u = static_cast<float>(y);  // not onto a border from beside it
-    const uint32_t bits = __float_as_uint(u);
-    if ((bits & 0xfffffu) == 0x80000u && y != u) u = __uint_as_float((y > u) == (u > 0.f) ? bits + 1u : bits - 1u);
+    y[i] *= root;
+    top = fmax(top, fabs(y[i]));
+  }
+  // rounded up to fp32: above the scale's border, an fp32 value, where the exact one is
+  const uint32_t byte = e4m3_scale_byte(group_max<W>(__double2float_ru(top)));
+  uint32_t q[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    y[i] *= e4m3_inv_scale(byte);
+    float u = static_cast<float>(y[i]);
+    // not onto a border from beside it: borders have four bits at most behind the first
+    if ((__float_as_uint(u) & 0x7ffffu) == 0u && y[i] != u && u != 0.f)
+      u = __uint_as_float(__float_as_uint(u) + ((y[i] > u) == (u > 0.f) ? 1u : -1u));
     q[i / 4] |= (e4m3x2(u, 0.f) & 255u) << (i % 4 * 8);
   }
-  if (byte != 255u) *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
+  if (!ok) return;
+  *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
+  if (part == 0) *scale = static_cast<uint8_t>(byte);
 }
 
 template <typename T, int D, bool Q8>
@@ -313,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendArgs a,
         if (h + u >= h1) break;
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (ok) in[u].get(f);
-        float inv = 1.f;
+        float inv = 1.f, product = 0.f;
         if (kKind != 2 && weight) {
           float ss = 0.f;
 #pragma unroll
@@ -333,7 +358,11 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendArgs a,
           }
           if (rotated) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = f[i] * c[i] + x[i] * s[i];
+            for (int i = 0; i < 8; ++i) {
+              const float xs = x[i] * s[i];
+              f[i] = fmaf(f[i], c[i], xs);
+              if (Q8 && kKind == 1) product = fmaxf(product, fabsf(xs));
+            }
           }
         }
         // last, as one rounding (x w is exact in fp32 for 16-bit types)
@@ -342,7 +371,8 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendArgs a,
           for (int i = 0; i < 8; ++i) f[i] *= inv;
         }
         if (Q8 && kKind != 0) {
-          if (store_e4m3<D, kKind == 1>(f, part, dst + u * dst_sh, scale + u * a.g.scale_head, ok))
+          if (store_e4m3<D, kKind == 1>(f, part, dst + u * dst_sh, scale + u * a.g.scale_head, ok,
+                                            a.half || a.k_weight, product * inv))
             redo |= 1ull << min(h + u, 63);
         } else if (ok) {
           Vec8<T> v;
@@ -369,10 +399,12 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendArgs a,
         a.v_sh, nullptr, a.v_pool + at, a.g.stride_head, a.v_scale + sat);
   if constexpr (Q8) {
     if (!a.half && !a.k_weight) return;  // k itself, exact
-    redo = warp_or(redo);
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) redo |= __shfl_xor_sync(0xffffffffu, redo, o);  // the row's
+    const uint64_t any = warp_or(redo);
     for (int h = k0; h < k1; ++h) {
-      if (!(redo >> min(h, 63) & 1)) continue;
-      exact_row<T, D>(ok, static_cast<const T*>(a.k) + t * a.k_st + h * a.k_sh + part * 8,
+      if (!(any >> min(h, 63) & 1)) continue;
+      exact_row<T, D>(redo >> min(h, 63) & 1, static_cast<const T*>(a.k) + t * a.k_st + h * a.k_sh + part * 8,
                       a.k_weight ? static_cast<const T*>(a.k_weight) + part * 8 : nullptr,
                       rotated && ok ? a.cos + p.pos * a.table_stride : nullptr,
                       rotated && ok ? a.sin + p.pos * a.table_stride : nullptr, a.half, a.interleaved, a.eps,

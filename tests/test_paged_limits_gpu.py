@@ -147,3 +147,121 @@ def test_weights_of_large_8bit_values(cuda_device, n):
     out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, sm_scale=1.0,
                                  k_scale=c["ks"], v_scale=c["vs"])
     check_attention(out, lse, q, c, [n], D, torch.bfloat16, scale=1.0)
+
+
+# ---------------------------------------------------------------------------
+# 8-bit keys next to a border
+# ---------------------------------------------------------------------------
+def quantise(k, w, cos, sin, interleaved, eps=1e-6):
+    """append_kv of k as one request's rows from position 0: (what they read as, scale bytes)."""
+    from d2sd_b200 import ops
+    n, Hk, D = k.shape
+    dev = k.device
+    pages = -(-n // 16)
+    kp = torch.zeros(pages, Hk, 16, D, dtype=torch.uint8, device=dev).view(E4M3)
+    vp, ks = kp.clone(), torch.zeros(pages, Hk, 16, dtype=torch.uint8, device=dev)
+    vs = ks.clone()
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    args = ("paged_umma", torch.arange(pages, dtype=torch.int32, device=dev), ints([0, pages]), ints([0, n]),
+            ints([0]))
+    ops.append_kv(k, k, kp, vp, *args, k_scale=ks, v_scale=vs, k_weight=w, cos=cos, sin=sin,
+                  interleaved=interleaved, eps=eps)
+    got, v = torch.empty_like(k), torch.empty_like(k)
+    ops.read_kv(kp, vp, *args, got, v, k_scale=ks, v_scale=vs)
+    return got, ks.transpose(1, 2).reshape(-1, Hk)[:n]
+
+
+def keys_64(k, w, cos, sin, interleaved, eps=1e-6):
+    """Norm and rotation of rows 0.. in 64 bits."""
+    y = k.double()
+    if w is not None:
+        y = y / (y.square().mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    if cos is None:
+        return y
+    c, s = cos[:len(k)].double()[:, None], sin[:len(k)].double()[:, None]
+    h = cos.shape[1]
+    a, b = (y[..., 0:2 * h:2], y[..., 1:2 * h:2]) if interleaved else (y[..., :h], y[..., h:2 * h])
+    p = a * c - b * s, b * c + a * s
+    turned = torch.stack(p, -1).flatten(-2) if interleaved else torch.cat(p, -1)
+    return torch.cat([turned, y[..., 2 * h:]], -1)
+
+
+def check_nearest(got, byte, f):
+    """The scale is that of the definition and every value the nearest e4m3 one: off by at
+    most half of the step at the exact value (2^-9 of the scale at the least; 2^-40 of it
+    for what 64 bits themselves round)."""
+    top = f.abs().amax(-1)
+    unit = torch.exp2(byte.double() - 127)
+    assert bool((top <= 448 * unit).all())
+    assert bool(((top > 224 * unit) | (byte == 1)).all())
+    step = torch.exp2(torch.floor(torch.log2((f.abs() / unit[..., None]).clamp(min=2.0 ** -6))) - 3) * unit[..., None]
+    off = (got.double() - f).abs() > step / 2 * (1 + 2.0 ** -40)
+    assert int(off.sum()) == 0, int(off.sum())
+
+
+def cancelling_tables(n, half, device):
+    """cos = 1 and sin = 1 - d, d of 2^-16 to 2^-8: equal pairs nearly cancel."""
+    g = torch.Generator(device=device).manual_seed(109)
+    d = 2.0 ** -(8 + 8 * torch.rand(n, half, generator=g, device=device))
+    return torch.ones(n, half, device=device), 1 - d
+
+
+@pytest.mark.parametrize("type", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,rot,interleaved,norm", [(128, 128, False, True), (128, 128, True, True),
+                                                    (64, 32, False, True), (128, 96, True, False),
+                                                    (64, 0, False, True)])
+@pytest.mark.parametrize("spread", [0, 8, "cancel"])
+def test_quantised_keys_are_the_nearest_ones(cuda_device, type, D, rot, interleaved, norm, spread):
+    """8.4 million values: none rounded past a border, however small it is beside its row
+    (spread: columns of different sizes, down to 2^-spread) or its rotation's operands."""
+    from d2sd_b200 import rope_tables
+    dev, n, Hk = cuda_device, 8192, 1024 // D
+    g = torch.Generator(device=dev).manual_seed(101)
+    k = torch.randn(n, Hk, D, generator=g, device=dev) * 1.7
+    if spread == "cancel":
+        k = 1.5 + torch.rand(n, Hk, 1, generator=g, device=dev).expand(n, Hk, D)
+    elif spread:
+        k *= 2.0 ** -(spread * torch.rand(D, generator=g, device=dev)).round()
+    k = k.to(type)
+    w = (1 + 0.2 * torch.randn(D, generator=g, device=dev)).to(type) if norm else None
+    cos, sin = rope_tables(n, rot, 1e6, dev) if rot else (None, None)
+    if spread == "cancel" and rot:
+        w = torch.full_like(w, 1.25) if norm else None
+        cos, sin = cancelling_tables(n, rot // 2, dev)
+    got, byte = quantise(k, w, cos, sin, interleaved)
+    f = keys_64(k, w, cos, sin, interleaved)
+    if type == torch.float16:  # read into fp16, whose own step is coarser under 2^-14
+        got = torch.where(f.abs() >= 2.0 ** -13, got.double(), f)
+    check_nearest(got, byte, f)
+
+
+def test_scale_of_a_row_next_to_its_border(cuda_device):
+    """Rows whose largest value is 448 * 2^e to within a last place of fp32: each has the
+    scale of its exact value. The norm's eps is what puts it there."""
+    dev, D = cuda_device, 64
+    g = torch.Generator(device=dev).manual_seed(103)
+    w = torch.ones(D, dtype=torch.bfloat16, device=dev)
+    for i in range(200):
+        k = torch.randn(1, 1, D, generator=g, device=dev).to(torch.bfloat16)
+        x = k.double().flatten()
+        top, mean = float(x.abs().max()), float(x.square().mean())
+        target = 1.75 * 2.0 ** -2  # the border under most rows' normalised maximum
+        assert (top / target) ** 2 > mean
+        eps = float(torch.tensor((top / target) ** 2 - mean, dtype=torch.float32))
+        got, byte = quantise(k, w, None, None, False, eps=eps)
+        check_nearest(got, byte, keys_64(k, w, None, None, False, eps=eps))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_tokens_keys_do_not_depend_on_its_batch(cuda_device, D):
+    """The same token beside 4096 others (even rows; one table row for all) has the same
+    bytes every time, values next to a border included."""
+    dev, n, Hk = cuda_device, 8192, 8
+    g = torch.Generator(device=dev).manual_seed(107)
+    w = torch.full((D,), 1.25, dtype=torch.bfloat16, device=dev)
+    for i in range(12):
+        cos, sin = (t[i:i + 1].expand(n, -1).contiguous() for t in cancelling_tables(12, D // 2, dev))
+        k = torch.randn(n, Hk, D, generator=g, device=dev)
+        k[::2] = 1.5 + torch.rand(1, Hk, 1, generator=g, device=dev)
+        got, byte = quantise(k.to(torch.bfloat16), w, cos, sin, False)
+        assert bool((got[::2] == got[0]).all()) and bool((byte[::2] == byte[0]).all()), i
