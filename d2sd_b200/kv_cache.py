@@ -311,18 +311,30 @@ class PagedKVPool(PagedKVCache):
         return len(self.capacities)
 
     def set_lengths(self, lengths) -> None:
+        """Every sequence's cached positions, at most its capacity."""
+        self._check_lengths(lengths)
         self.lengths = [int(x) for x in lengths]
         self.lengths_dev.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+
+    def _check_lengths(self, lengths) -> None:
+        if len(lengths) != self.num_seqs:
+            raise ValueError("lengths must have an entry for each sequence")
+        for s, (n, cap) in enumerate(zip(lengths, self.capacities)):
+            if not 0 <= int(n) <= cap:
+                raise ValueError(f"sequence {s} holds up to {cap} positions, not {int(n)}")
 
     def plan(self, q_lens, num_qo_heads: int, **kw):
         """A ``PagedAttentionPlan`` of every sequence's q_lens[s] newest tokens, which
         ``append`` has written and ``lengths`` counts (its keyword arguments: causal,
-        window, reserve)."""
+        window, reserve). Lengths above a sequence's capacity are refused, by the plan's
+        ``update`` too."""
         from .paged import PagedAttentionPlan
         if len(q_lens) != self.num_seqs:
             raise ValueError("q_lens must have an entry for each sequence")
+        self._check_lengths(self.lengths)
         return PagedAttentionPlan(q_lens, self.lengths, num_qo_heads, self.num_kv_heads, self.head_dim,
-                                  self.device, page_offsets=self.page_offsets_host, cache_dtype=self.dtype, **kw)
+                                  self.device, page_offsets=self.page_offsets_host,
+                                  capacities=self.capacities, cache_dtype=self.dtype, **kw)
 
     def write_seq(self, l: int, s: int, k: torch.Tensor, v: torch.Tensor, start: int = 0) -> None:
         """Write k, v [n, Hk, D] at positions start.. of sequence s, layer l."""

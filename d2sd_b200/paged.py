@@ -27,7 +27,11 @@ class PagedAttentionPlan:
     q_lens / kv_lens: new tokens of each request and its cached positions, the new
     ones included (the new tokens are the last of them). page_offsets: each
     request's first entry in the page table (default: one request from entry 0, or
-    ``PagedKVPool.page_offsets_host``); a longer list (page bounds) is cut.
+    ``PagedKVPool.page_offsets_host``). With an entry more (page bounds, ascending) a
+    request with more cached positions than its pages hold is refused by the call; with
+    capacities, the positions that each request has room for, by the plan and ``update``
+    (``PagedKVPool.plan`` gives them). Without either, such a request reads on in the
+    page table.
     window: a row sees only the last ``window`` positions up to its own. cache_dtype:
     float8_e4m3fn chooses the kernels for an 8-bit cache (any plan works with any).
 
@@ -43,7 +47,7 @@ class PagedAttentionPlan:
 
     def __init__(self, q_lens, kv_lens, num_qo_heads: int, num_kv_heads: int, head_dim: int,
                  device: torch.device | str, *, causal: bool = True, window: int | None = None,
-                 page_offsets=None, cache_dtype: torch.dtype | None = None,
+                 page_offsets=None, capacities=None, cache_dtype: torch.dtype | None = None,
                  reserve: tuple[int, ...] | None = None):
         device = torch.device(device)
         if device.type != "cuda":
@@ -52,6 +56,8 @@ class PagedAttentionPlan:
             raise ValueError("window must be positive")
         self.num_qo_heads, self.num_kv_heads, self.head_dim = num_qo_heads, num_kv_heads, head_dim
         self.causal, self.window = causal, window
+        self.capacities = None if capacities is None else np.asarray(capacities, dtype=np.int64)
+        self._captured = set()  # (page size, entries of the page table) of captured calls
         self.eight_bit = int(cache_dtype == torch.float8_e4m3fn)
         self.num_ctas = ops.num_sms(device)
         self.reserve = reserve
@@ -97,9 +103,18 @@ class PagedAttentionPlan:
         if self.reserve is not None and (R > self.reserve[0] or int(q.sum()) > self.reserve[1]
                                          or int(q.max(initial=0)) > self.longest):
             raise ValueError(f"the batch is larger than the plan's reserve {self.reserve}")
-        off = np.ascontiguousarray(page_offsets, dtype=np.int32)[:R]
+        bounds = np.ascontiguousarray(page_offsets, dtype=np.int32)
+        off = bounds[:R]
         if len(off) != R:
             raise ValueError("page_offsets must have an entry for each request")
+        if self.capacities is not None and (len(self.capacities) < R
+                                            or (kv > self.capacities[:R]).any()):
+            raise ValueError("kv_lens are above the requests' capacities")
+        ends = bounds[1:R + 1] if len(bounds) > R and (bounds[1:R + 1] >= off).all() else None
+        requests = (kv, off, ends)
+        for page_size, entries in self._captured:
+            if self._pages(requests, page_size) > entries:
+                raise ValueError("the page table of a captured call is too short for these lengths")
         lib = load()
         cap = lib.d2sd_paged_plan_capacity(q.ctypes.data, R, self.num_qo_heads, self.num_kv_heads,
                                            self.num_ctas)
@@ -113,16 +128,23 @@ class PagedAttentionPlan:
                                   min(self.window or 0, 1 << 30), self.eight_bit + (0 if self.fixed_grid else 2),
                                   self.num_ctas, plan.ctypes.data, cap,
                                   used.ctypes.data, sections.ctypes.data), "d2sd_paged_plan")
-        self._requests, self._entries = (kv, off), {}
+        self._requests, self._entries = requests, {}
         return plan[:int(used[0])], sections, int(q.sum())
+
+    @staticmethod
+    def _pages(requests, page_size: int) -> int:
+        kv, off, ends = requests
+        last = off.astype(np.int64) + -(-kv.astype(np.int64) // page_size)
+        if ends is not None and (last > ends).any():
+            r = int((last > ends).argmax())
+            raise ValueError(f"request {r} has {kv[r]} cached positions, more than its pages hold")
+        return int(last.max(initial=0))
 
     def entries(self, page_size: int) -> int:
         """Entries that a page table must have for pages of this size."""
         n = self._entries.get(page_size)
         if n is None:
-            kv, off = self._requests
-            n = int((off.astype(np.int64) + -(-kv.astype(np.int64) // page_size)).max(initial=0))
-            self._entries[page_size] = n
+            n = self._entries[page_size] = self._pages(self._requests, page_size)
         return n
 
     def _set(self, host, sections, tokens):
@@ -186,6 +208,8 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("sinks must be a contiguous fp32 tensor [num_qo_heads]")
     if page_table.numel() < plan.entries(pool[3]):
         raise ValueError(f"the page table must have {plan.entries(pool[3])} entries for this plan")
+    if plan.fixed_grid and torch.cuda.is_current_stream_capturing():
+        plan._captured.add((pool[3], page_table.numel()))  # what updates have to fit
     q_args = ops._rows("q", q, n, Hq, D, dtype)
     if out is None:
         out = q.new_empty(n, Hq, D)

@@ -265,3 +265,85 @@ def test_a_tokens_keys_do_not_depend_on_its_batch(cuda_device, D):
         k[::2] = 1.5 + torch.rand(1, Hk, 1, generator=g, device=dev)
         got, byte = quantise(k.to(torch.bfloat16), w, cos, sin, False)
         assert bool((got[::2] == got[0]).all()) and bool((byte[::2] == byte[0]).all()), i
+
+
+# ---------------------------------------------------------------------------
+# lengths above a sequence's pages
+# ---------------------------------------------------------------------------
+def test_pool_refuses_lengths_above_capacity(cuda_device):
+    """Positions behind a sequence's capacity would be the next sequence's rows."""
+    import d2sd_b200 as d
+    pool = d.PagedKVPool(1, 2, 64, [40, 100, 33], device=cuda_device)
+    for bad in ([41, 0, 0], [0, 101, 0], [0, 0, 34], [-1, 0, 0], [1, 1]):
+        with pytest.raises(ValueError):
+            pool.set_lengths(bad)
+    assert pool.lengths == [0, 0, 0]
+    pool.set_lengths([40, 100, 33])
+    plan = pool.plan([1, 2, 3], 4)
+    with pytest.raises(ValueError):
+        plan.update([1, 2, 3], [41, 100, 33], pool.page_offsets_host)
+    with pytest.raises(ValueError):
+        pool.plan([1, 2, 3], 4, reserve=(3, 6)).update([1, 2, 3], [40, 100, 48], pool.page_offsets_host)
+    plan.update([1, 2, 3], [40, 99, 33], pool.page_offsets_host)
+    pool.lengths[0] += 1
+    with pytest.raises(ValueError):
+        pool.plan([1, 2, 3], 4)
+
+
+@pytest.mark.parametrize("layout,page_size", [("paged_umma", 16), ("paged_hnd", 32)])
+def test_page_bounds_limit_every_request(cuda_device, layout, page_size):
+    """Plans with page bounds: a request longer than its own pages is refused, though the
+    page table goes on."""
+    import d2sd_b200 as d
+    Hq, Hk, D = 4, 2, 64
+    g = torch.Generator().manual_seed(111)
+    kl = [3 * page_size, 2 * page_size]
+    c = make_cache(g, kl, Hk, D, torch.bfloat16, layout, cuda_device, page_size=page_size)
+    q = torch.randn(2, Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    run = lambda plan: d.paged_attention(q, c["k"], c["v"], layout, c["table"], plan)  # noqa: E731
+    plan = d.PagedAttentionPlan([1, 1], kl, Hq, Hk, D, cuda_device, page_offsets=c["bounds"])
+    out, lse = run(plan)
+    check_attention(out, lse, q, c, [1, 1], D, torch.bfloat16)
+    plan.update([1, 1], [3 * page_size + 1, 5], c["bounds"])
+    with pytest.raises(ValueError):
+        run(plan)
+    plan.update([1, 1], kl, c["bounds"])
+    again, _ = run(plan)
+    assert torch.equal(out, again)
+
+
+def test_updates_fit_the_page_table_of_a_captured_call(cuda_device):
+    """A replay reads the page table that its call was captured with: an update to
+    lengths that go on behind it is refused, and the plan stays as it was."""
+    import d2sd_b200 as d
+    Hq, Hk, D = 8, 2, 64
+    g = torch.Generator().manual_seed(113)
+    c = make_cache(g, [200, 90], Hk, D, torch.bfloat16, "paged_umma", cuda_device)
+    q = torch.randn(2, Hq, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    plan = d.PagedAttentionPlan([1, 1], [20, 30], Hq, Hk, D, cuda_device, page_offsets=c["bounds"][:2],
+                                reserve=(2, 2, 1))
+    out, lse = torch.zeros_like(q), torch.zeros(2, Hq, device=cuda_device)
+    call = lambda: d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, out=out, lse=lse)  # noqa
+    call()
+    plan.update([1, 1], [200, 90 + 17], c["bounds"][:2])  # a longer table may come with the next call
+    plan.update([1, 1], [20, 30], c["bounds"][:2])
+    s = torch.cuda.Stream(cuda_device)
+    s.wait_stream(torch.cuda.current_stream(cuda_device))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s), torch.cuda.graph(graph, stream=s):
+        call()
+    torch.cuda.current_stream(cuda_device).wait_stream(s)
+    for kl in ([200, 90], [200, 90 + 17], [5, 90]):
+        if kl[1] > 96:
+            with pytest.raises(ValueError):
+                plan.update([1, 1], kl, c["bounds"][:2])
+            kl = [200, 90]
+        else:
+            plan.update([1, 1], kl, c["bounds"][:2])
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize(cuda_device)
+        cut = dict(c, k_rows=[x[:n] for x, n in zip(c["k_rows"], kl)],
+                   v_rows=[x[:n] for x, n in zip(c["v_rows"], kl)])
+        check_attention(out, lse, q, cut, [1, 1], D, torch.bfloat16)
+    del graph
