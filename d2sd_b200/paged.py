@@ -242,31 +242,42 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
 def rope_tables(num_positions: int, rotary_dim: int, theta: float, device, *,
                 scaling: dict | None = None):
     """cos and sin tables for ``ops.append_kv``: fp32 [num_positions, rotary_dim / 2],
-    angles in 64 bits. scaling: None; {"type": "linear", "factor": f} (positions
-    divided by f); {"type": "yarn", "factor": f, "original": L, "beta_fast": 32,
-    "beta_slow": 1} (wavelengths far below L keep their frequency, those far above
-    are divided by f, with a linear ramp between, and both tables are multiplied by
-    0.1 ln f + 1, as YaRN's paper defines them)."""
+    angles in 64 bits, frequencies theta^(-2 i / rotary_dim). scaling: None;
+    {"type": "linear", "factor": f}: frequencies divided by f;
+    {"type": "yarn", "factor": f, "original": L, "beta_fast": 32, "beta_slow": 1,
+    "truncate": True}: columns whose waves turn more than beta_fast times over L
+    positions keep their frequency, those of fewer than beta_slow turns are divided by
+    f, with a ramp between that is linear in the column, from the column of beta_fast
+    turns to that of beta_slow (rounded down and up to whole ones unless ``truncate`` is
+    False, as in GPT-OSS), and both tables are multiplied by 0.1 ln f + 1. Other keys are
+    refused."""
     if rotary_dim <= 0 or rotary_dim % 2 or num_positions <= 0:
         raise ValueError("rope_tables: positive sizes, an even rotary_dim")
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
     freq = theta ** (-i / rotary_dim)
     gain = 1.0
     if scaling is not None:
+        kind, known = scaling.get("type"), {"type", "factor"}
+        if kind == "yarn":
+            known |= {"original", "beta_fast", "beta_slow", "truncate"}
+        elif kind != "linear":
+            raise NotImplementedError(f"rope_tables: scaling {kind!r}")
+        if not set(scaling) <= known:
+            raise ValueError(f"rope_tables: {sorted(set(scaling) - known)} with scaling {kind!r}")
         f = float(scaling["factor"])
-        if scaling["type"] == "linear":
+        if kind == "linear":
             freq = freq / f
-        elif scaling["type"] == "yarn":
+        else:
             L = float(scaling["original"])
 
             def column(turns):  # the (real) column whose wave makes `turns` turns over L
                 return rotary_dim * math.log(L / (turns * 2 * math.pi)) / (2 * math.log(theta))
-            lo = max(math.floor(column(scaling.get("beta_fast", 32))), 0)
-            hi = min(math.ceil(column(scaling.get("beta_slow", 1))), rotary_dim - 1)
+            lo, hi = column(scaling.get("beta_fast", 32)), column(scaling.get("beta_slow", 1))
+            if scaling.get("truncate", True):
+                lo, hi = math.floor(lo), math.ceil(hi)
+            lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
             ramp = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
             freq = freq * (1 - ramp) + freq / f * ramp
             gain = 0.1 * math.log(f) + 1.0 if f > 1 else 1.0
-        else:
-            raise NotImplementedError(f"rope_tables: scaling {scaling['type']!r}")
     angle = torch.arange(num_positions, dtype=torch.float64)[:, None] * freq[None]
     return ((angle.cos() * gain).float().to(device), (angle.sin() * gain).float().to(device))
