@@ -20,6 +20,11 @@ are zero-initialised so every slot past a sequence's length holds finite values.
 for each (layer, page, head, slot) in ``k_scale`` / ``v_scale`` (a power of two; see
 include/d2sd.h), half of a bf16 cache's bytes. ``append`` and ``commit`` quantise as
 they write, ``ops.read_kv`` (``read``, ``gather``) and ``paged_attention`` read it.
+
+``status`` (int32 on the device) is what ``append``, ``read`` and the 8-bit forms of
+``write`` and the commits report to: 0, or the smallest code since it was last zeroed of
+a token that was skipped (4: a position outside its sequence's pages, 5: a page outside
+the pool, 6: a position outside the rotary tables).
 """
 from __future__ import annotations
 
@@ -61,6 +66,7 @@ class PagedKVCache:
         self.page_table = page_order.to(torch.int32).to(self.device)
         # first page-table entry of each sequence, and the end (one sequence here)
         self.page_bounds = torch.tensor([0, self.num_pages], dtype=torch.int32, device=self.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.length = 0
         self._ptr_cache: dict = {}
 
@@ -94,9 +100,11 @@ class PagedKVCache:
         """``ops.append_kv`` into layer l: sequence r's new rows are token_start[r] ..
         token_start[r + 1] - 1 of k, v (int32 [sequences + 1], device) and go to its
         positions first_pos[r] onward (int32, device). Takes its keyword arguments
-        (q, q_out, q_weight, k_weight, eps, cos, sin, interleaved, status) and returns
-        the rotated q. The caller advances the lengths, once all layers are written."""
+        (q, q_out, q_weight, k_weight, eps, cos, sin, interleaved; status, by default the
+        cache's own) and returns the rotated q. The caller advances the lengths, once all layers are written."""
         ks, vs = self.scales(l)
+        if kw.get("status") is None:
+            kw["status"] = self.status
         return ops.append_kv(k, v, self.k[l], self.v[l], self.kv_layout, self.page_table,
                              self.page_bounds, token_start, first_pos, k_scale=ks, v_scale=vs, **kw)
 
@@ -106,22 +114,24 @@ class PagedKVCache:
         [tokens, Hk, D] from sequence r's positions first_pos[r] on."""
         ks, vs = self.scales(l)
         ops.read_kv(self.k[l], self.v[l], self.kv_layout, self.page_table, self.page_bounds,
-                    token_start, first_pos, k_out, v_out, k_scale=ks, v_scale=vs, status=status)
+                    token_start, first_pos, k_out, v_out, k_scale=ks, v_scale=vs,
+                    status=self.status if status is None else status)
 
     def _span(self, n: int) -> torch.Tensor:
         """int32 [0, n] on the device, without a copy from the host (n > 0)."""
         return torch.arange(0, n + 1, n, dtype=torch.int32, device=self.device)
 
-    def _rows_of(self, l: int, s: int, n: int):
-        """The first n rows of sequence s of an 8-bit layer, bf16 [n, Hk, D]."""
+    def _rows_of(self, l: int, bounds: torch.Tensor, n: int, capacity: int):
+        """The first n rows of an 8-bit layer's pages bounds[0] .. bounds[1], bf16 [n, Hk, D]."""
+        if not 0 <= n <= capacity:
+            raise ValueError(f"{n} rows of a cache of {capacity}")
         out = torch.empty(2, n, self.num_kv_heads, self.head_dim, dtype=torch.bfloat16,
                           device=self.device)
         if n > 0:
             ks, vs = self.scales(l)
-            ops.read_kv(self.k[l], self.v[l], self.kv_layout, self.page_table,
-                        self.page_bounds[s:s + 2], self._span(n),
+            ops.read_kv(self.k[l], self.v[l], self.kv_layout, self.page_table, bounds, self._span(n),
                         torch.zeros(1, dtype=torch.int32, device=self.device), out[0], out[1],
-                        k_scale=ks, v_scale=vs)
+                        k_scale=ks, v_scale=vs, status=self.status)
         return out[0], out[1]
 
     # -- host-side set-up (not on the hot path) ------------------------------
@@ -130,14 +140,14 @@ class PagedKVCache:
         n = k.shape[0]
         if self.quantised:
             pages = self.page_table.numel()
-            if start + n > pages * self.page_size:
+            if start < 0 or start + n > pages * self.page_size:
                 raise ValueError("cache capacity exceeded")
             if n > 0:
                 ks, vs = self.scales(l)
                 ops.append_kv(k, v, self.k[l], self.v[l], self.kv_layout, self.page_table,
                               self._span(pages), self._span(n),
                               torch.full((1,), start, dtype=torch.int32, device=self.device),
-                              k_scale=ks, v_scale=vs)
+                              k_scale=ks, v_scale=vs, status=self.status)
             return
         pos = torch.arange(start, start + n, device=self.device)
         page, slot = self.positions_to_slots(pos)
@@ -154,7 +164,8 @@ class PagedKVCache:
         """Layer l as contiguous [length, Hk, D] tensors (for checks)."""
         n = self.length if length is None else length
         if self.quantised:
-            return self._rows_of(l, 0, n)
+            pages = self.page_table.numel()
+            return self._rows_of(l, self._span(pages), n, pages * self.page_size)
         pos = torch.arange(n, device=self.device)
         page, slot = self.positions_to_slots(pos)
         if self.layout == "hnd":
@@ -203,7 +214,7 @@ class PagedKVCache:
                            cache_strides=(kl.stride(0), kl.stride(1)), num_pages=kl.shape[0],
                            scale_strides=(sl.stride(0), sl.stride(1)), page_table=self.page_table,
                            page_bounds=self.page_bounds, accept_results=accept_results,
-                           cache_lens=cache_lens)
+                           cache_lens=cache_lens, status=self.status)
 
     def commit(self, new_k, new_v, accept_result: torch.Tensor, advance_by: int | None = None,
                cache_len: int | None = None, target_hidden=None) -> None:
@@ -345,7 +356,7 @@ class PagedKVPool(PagedKVCache):
     def gather_seq(self, l: int, s: int, length: int):
         """Sequence s of layer l as contiguous [length, Hk, D] tensors (for checks)."""
         if self.quantised:
-            return self._rows_of(l, s, length)
+            return self._rows_of(l, self.page_bounds[s:s + 2], length, self.capacities[s])
         base = self.page_offsets_host[s] * self.page_size
         pos = torch.arange(base, base + length, device=self.device)
         page, slot = self.positions_to_slots(pos)
@@ -365,7 +376,8 @@ class PagedKVPool(PagedKVCache):
         branch b at row s * num_branches + b; a list or a stacked [L, ...]
         tensor) with identical strides; accept_results: int32 [S, 2] from
         ``BatchVerifier``. Rows land at each sequence's ``lengths_dev`` onward;
-        the lengths are not advanced (the caller reads acc when it needs it)."""
+        the lengths are not advanced (the caller reads acc when it needs it). An 8-bit
+        cache's rows behind a sequence's pages are left out, and ``status`` reads 4."""
         if isinstance(new_k, torch.Tensor):
             new_k = [new_k[l] for l in range(new_k.shape[0])]
             new_v = [new_v[l] for l in range(new_v.shape[0])]

@@ -347,3 +347,76 @@ def test_updates_fit_the_page_table_of_a_captured_call(cuda_device):
                    v_rows=[x[:n] for x, n in zip(c["v_rows"], kl)])
         check_attention(out, lse, q, cut, [1, 1], D, torch.bfloat16)
     del graph
+
+
+# ---------------------------------------------------------------------------
+# rows that are not there, through the caches
+# ---------------------------------------------------------------------------
+def test_8bit_rows_behind_the_cache_are_refused(cuda_device):
+    """gather and gather_seq of more rows than there are raise, instead of returning
+    memory that nothing wrote; a negative start is refused."""
+    import d2sd_b200 as d
+    cache = d.PagedKVCache(1, 2, 64, 32, dtype=E4M3, device=cuda_device)
+    pool = d.PagedKVPool(1, 2, 64, [20, 40], dtype=E4M3, device=cuda_device)
+    x = torch.ones(16, 2, 64, dtype=torch.bfloat16, device=cuda_device)
+    for call in (lambda: cache.gather(0, 33), lambda: cache.gather(0, -1), lambda: pool.gather_seq(0, 0, 21),
+                 lambda: pool.gather_seq(0, 1, 41), lambda: pool.gather(0, 81),
+                 lambda: cache.write(0, x, x, start=-1), lambda: cache.write(0, x, x, start=17)):
+        with pytest.raises(ValueError):
+            call()
+    for got, n in ((cache.gather(0, 32), 32), (pool.gather_seq(0, 0, 20), 20), (pool.gather(0, 80), 80)):
+        assert got[0].shape == (n, 2, 64) and not got[0].any() and not got[1].any()
+    assert int(cache.status) == 0 and int(pool.status) == 0
+
+
+def test_gather_of_a_pool_is_the_same_in_both_types(cuda_device):
+    """The pool's gather goes over the whole page table, whatever the cache's type."""
+    import d2sd_b200 as d
+    g = torch.Generator().manual_seed(117)
+    pools = [d.PagedKVPool(1, 2, 64, [20, 40, 5], dtype=t, device=cuda_device, shuffle_seed=2)
+             for t in (torch.bfloat16, E4M3)]
+    for s, n in enumerate([20, 40, 5]):
+        x = torch.randint(-8, 9, (n, 2, 64), generator=g).to(torch.bfloat16).to(cuda_device)
+        for p in pools:
+            p.write_seq(0, s, x, -x)
+    for n in (7, 20, 33, 96):
+        a, b = (p.gather(0, n) for p in pools)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_status_of_the_caches(cuda_device):
+    """A commit past a sequence's pages, an append past them and a bad page are reported
+    by the cache's own status; a tensor that is passed is used instead."""
+    import d2sd_b200 as d
+    dev = cuda_device
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    new = torch.ones(2, 2, 8, 64, dtype=torch.bfloat16, device=dev)
+    pool = d.PagedKVPool(1, 2, 64, [16, 40], dtype=E4M3, device=dev)
+    pool.set_lengths([10, 20])
+    pool.commit_batch([new], [new], ints([[6, 0], [8, 0]]), 1)
+    assert int(pool.status) == 0
+    pool.commit_batch([new], [new], ints([[7, 0], [8, 0]]), 1)  # position 16 of a page of 16
+    assert int(pool.status) == 4
+    for dtype in (torch.bfloat16, E4M3):
+        pool = d.PagedKVPool(1, 2, 64, [16, 40], dtype=dtype, device=dev)
+        rows = torch.ones(5, 2, 64, dtype=torch.bfloat16, device=dev)
+        starts, first = ints([0, 3, 5]), ints([14, 0])
+        own = ints([0])
+        pool.append(0, rows, rows, starts, first, status=own)
+        assert int(own) == 4 and int(pool.status) == 0
+        pool.append(0, rows, rows, starts, first)
+        assert int(pool.status) == 4
+        pool.status.zero_()
+        out = torch.zeros_like(rows)
+        pool.read(0, starts, first, out, out.clone())
+        assert int(pool.status) == 4
+        pool.status.zero_()
+        pool.page_table[2] = 99
+        pool.append(0, rows, rows, starts, ints([3, 10]))
+        assert int(pool.status) == 0
+        pool.append(0, rows, rows, starts, ints([3, 16]))
+        assert int(pool.status) == 5
+    cache = d.PagedKVCache(1, 2, 64, 32, dtype=E4M3, device=dev, page_order=torch.tensor([0, 1]))
+    cache.page_table[1] = -1
+    cache.commit([new[:1]], [new[:1]], ints([8, 0]), cache_len=12)
+    assert int(cache.status) == 5
