@@ -511,6 +511,15 @@ def _int32(name: str, t: torch.Tensor, n: int | None = None) -> int:
     return t.data_ptr()
 
 
+def _status(t) -> int:
+    """Address of a status word, 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype != _I32 or t.numel() < 1:
+        raise ValueError("status must be an int32 tensor")
+    return t.data_ptr()
+
+
 def _pool_args(k_pool, v_pool, kv_layout, k_scale, v_scale):
     """The C arguments (strides, page size, pages, format, scales) of a K and V
     pool, and its (heads, head_dim)."""
@@ -627,7 +636,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: to
             stride, rows, rot, 1 if interleaved else 0, _int32("token_start", token_start, R + 1),
             _int32("first_pos", first_pos), R, k_pool.data_ptr(), v_pool.data_ptr(), *pool,
             _int32("page_table", page_table), page_table.numel(),
-            _int32("page_bounds", page_bounds, R + 1), _at(status))
+            _int32("page_bounds", page_bounds, R + 1), _status(status))
     _call(dev, _append_kv, args, "d2sd_append_kv")
     return q_out
 
@@ -651,7 +660,7 @@ def read_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, kv_layout: str, page_tab
             page_table.numel(), _int32("page_bounds", page_bounds, R + 1), _int32("token_start", token_start, R + 1),
             _int32("first_pos", first_pos), R, n, Hk, D, dtype_code(k_out),
             *_rows("k_out", k_out, n, Hk, D, dtype), *_rows("v_out", v_out, n, Hk, D, dtype),
-            _at(status))
+            _status(status))
     _call(dev, _read_kv, args, "d2sd_read_kv")
 
 
@@ -666,10 +675,13 @@ def commit_kv_e4m3(layer_ptrs: torch.Tensor, *, num_layers: int, num_requests: i
     pointers; cache and scale strides are (page, head)."""
     dev = layer_ptrs.get_device()
     _same_device(dev, page_table, page_bounds, accept_results, cache_lens, status)
+    if layer_ptrs.dtype != torch.int64 or not layer_ptrs.is_contiguous() \
+            or layer_ptrs.numel() != 6 * num_layers:
+        raise ValueError(f"layer_ptrs must be a contiguous int64 tensor with {6 * num_layers} entries")
     args = (layer_ptrs.data_ptr(), num_layers, num_requests, num_kv_heads, head_dim,
             _DTYPES.get(dtype, -1), block_len, *new_strides, *cache_strides, num_pages,
             *scale_strides, _int32("page_table", page_table), page_table.numel(),
             _int32("page_bounds", page_bounds, num_requests + 1),
-            _int32("accept_results", accept_results), _int32("cache_lens", cache_lens),
-            _ptr(status))
+            _int32("accept_results", accept_results, 2 * num_requests),
+            _int32("cache_lens", cache_lens, num_requests), _status(status))
     _call(dev, load().d2sd_commit_kv_e4m3, args, "d2sd_commit_kv_e4m3")

@@ -420,3 +420,41 @@ def test_status_of_the_caches(cuda_device):
     cache.page_table[1] = -1
     cache.commit([new[:1]], [new[:1]], ints([8, 0]), cache_len=12)
     assert int(cache.status) == 5
+
+
+# ---------------------------------------------------------------------------
+# arguments of the wrong size or type
+# ---------------------------------------------------------------------------
+def test_sizes_of_device_arguments(cuda_device):
+    """What a kernel reads or writes by the number of requests is checked against it."""
+    import d2sd_b200 as d
+    from d2sd_b200 import ops
+    dev = cuda_device
+    ints = lambda x, t=torch.int32: torch.tensor(x, dtype=t, device=dev)  # noqa: E731
+    pool = d.PagedKVPool(1, 2, 64, [40, 40], dtype=E4M3, device=dev)
+    new = torch.zeros(2, 2, 8, 64, dtype=torch.bfloat16, device=dev)
+    for res in (ints([1, 0]), ints([[1, 0]] * 3), ints([[1, 0], [1, 0]], torch.int64)):
+        with pytest.raises(ValueError):
+            pool.commit_batch([new], [new], res, 1)
+    pool.lengths_dev = ints([0])
+    with pytest.raises(ValueError):
+        pool.commit_batch([new], [new], ints([[1, 0], [1, 0]]), 1)
+    kw = dict(num_layers=1, num_requests=1, num_kv_heads=2, head_dim=64, dtype=torch.bfloat16, block_len=8,
+              new_strides=(0, *new.stride()[:3]), cache_strides=pool.k[0].stride()[:2], num_pages=6,
+              scale_strides=pool.k_scale[0].stride()[:2], page_table=pool.page_table, page_bounds=ints([0, 3]),
+              accept_results=ints([0, 0]), cache_lens=ints([0]))
+    ptrs = [t.data_ptr() for t in (new, new, pool.k, pool.v, pool.k_scale, pool.v_scale)]
+    ops.commit_kv_e4m3(ints(ptrs, torch.int64), **kw)
+    for bad in (ints(ptrs[:4], torch.int64), torch.zeros(6, dtype=torch.float64, device=dev)):
+        with pytest.raises(ValueError):
+            ops.commit_kv_e4m3(bad, **kw)
+    rows = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device=dev)
+    args = (ints([0, 2]), ints([0]))
+    cache = d.PagedKVCache(1, 2, 64, 32, device=dev)
+    for status in (ints([0], torch.uint8), ints([0], torch.int64), ints([])):
+        with pytest.raises(ValueError):
+            cache.append(0, rows, rows, *args, status=status)
+        with pytest.raises(ValueError):
+            cache.read(0, *args, rows, rows.clone(), status=status)
+        with pytest.raises(ValueError):
+            ops.commit_kv_e4m3(ints(ptrs, torch.int64), status=status, **kw)
