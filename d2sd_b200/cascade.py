@@ -136,14 +136,15 @@ def cascade_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
         ptok = None
     if plan is None:
         plan = CascadePlan([Request(n_u, 0, kv_start, kv_len)], Hq, Hk, D, q.device)
+    # copies, if any, before kernel (a): kernel (b) reads them while the launch before it ends
+    q, k_new, v_new = (t.reshape(B * T, t.shape[2], D) for t in (q, k_new, v_new))
     plan.run_prefix(q_pref, k_cache, v_cache, kv_layout, scale, page_table=page_table)
     if out is None:
         out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=q.device)
     if lse is None:
         lse = torch.empty(B, T, Hq, dtype=torch.float32, device=q.device)
     mode = _MASKS["custom" if custom_mask is not None else ("causal" if causal else "none")]
-    ops.suffix_merge(q.reshape(B * T, Hq, D), k_new.reshape(B * T, Hk, D),
-                     v_new.reshape(B * T, Hk, D), out.view(B * T, Hq, D), lse.view(B * T, Hq),
+    ops.suffix_merge(q, k_new, v_new, out.view(B * T, Hq, D), lse.view(B * T, Hq),
                      num_blocks=B, block_len=T, num_qo_heads=Hq, num_kv_heads=Hk, sm_scale=scale,
                      mask_mode=mode, custom_mask=custom_mask,
                      partial=plan.partial if plan.num_ctas else None, plan_dev=plan.plan,

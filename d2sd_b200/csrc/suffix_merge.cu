@@ -242,6 +242,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     tc_fence_after();
     tmem = *tmem_slot;
+    // Behind kernel (a), q and the block's K/V (and the custom mask) were written before
+    // it, and it has waited for them. Without its partial states the kernel before this
+    // one may be any, the one that writes them too.
+    if (!p.partial) grid_dep_wait();
     if (threadIdx.x == 0) {
       mbar_arrive_expect_tx(&bars[0], C::kQBytes + 2 * C::kKVBytes);
 #pragma unroll
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   // with up to 8 slot rows and all their LSEs in flight before any use; the
   // row's groups then add their partial sums with shuffles.
   // The partial slots come from the previous kernel (kernel (a)): wait for it.
-  // Phase 1 read only q and the block's K/V, which precede kernel (a).
+  // Phase 1 read only q and the block's K/V, which precede kernel (a) (above).
   grid_dep_wait();
   constexpr int CPL = D / 8;          // columns per lane
   constexpr int VEC = CPL * 2 / 16;   // 16-byte vectors per lane and slot row

@@ -181,6 +181,10 @@ int d2sd_prefix_attention(const void* q, int64_t q_stride_token,
  *     in the q dtype, lse [tokens, Hq] fp32 base-2) as produced by
  *     single_prefill_with_kv_cache; the CascadeGraphRunner.run in-place form.
  *   - neither: no prefix (level 2 alone).
+ * Order: with partial, q, k_local, v_local and custom_mask are read while the
+ * launch before this one in the stream ends, so they have to be written before
+ * the d2sd_prefix_attention that fills partial is launched. Without partial they
+ * may be what the launch before this one writes.
  * out/lse receive the merged output (q dtype) and base-2 LSE; they may alias
  * prefix_out/prefix_lse. mask_mode is a D2SD_MASK_*, custom_mask is
  * uint64 [num_blocks*block_len] (bit j = token may see block token j).

@@ -458,3 +458,50 @@ def test_sizes_of_device_arguments(cuda_device):
             cache.read(0, *args, rows, rows.clone(), status=status)
         with pytest.raises(ValueError):
             ops.commit_kv_e4m3(ints(ptrs, torch.int64), status=status, **kw)
+
+
+# ---------------------------------------------------------------------------
+# verify blocks right behind the launch that writes them
+# ---------------------------------------------------------------------------
+def test_verify_block_behind_append_and_read(cuda_device):
+    """q rotated in place by append, k and v read out of the cache, and at once the block's
+    attention (no prefix; a dense one; an empty paged one): as with a wait between."""
+    import d2sd_b200 as d
+    from d2sd_b200 import CascadeGraphRunner, single_prefill_with_kv_cache
+    dev, Hq, Hk, D, n, T = cuda_device, 32, 8, 128, 4096, 16
+    g = torch.Generator(device=dev).manual_seed(121)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    cache = d.PagedKVCache(1, Hk, D, n, device=dev)
+    cos, sin = d.rope_tables(n, D, 1e6, dev)
+    starts, first = ints([0, n]), ints([0])
+    runner = CascadeGraphRunner(T, Hq, Hk, D, torch.bfloat16, dev, D ** -0.5, True)
+    plan = d.CascadePlan([d.Request(2 * T, 0, 0, 0)], Hq, Hk, D, dev)
+    dense = (torch.randn(2, T, Hq, D, generator=g, device=dev).to(torch.bfloat16),
+             torch.randn(2, T, Hq, generator=g, device=dev))
+
+    def step(qkv, form, wait):
+        q, kr, vr = qkv[:, :Hq].clone(), torch.zeros(n, Hk, D, dtype=torch.bfloat16, device=dev), None
+        vr, out = kr.clone(), tuple(t.clone() for t in dense)
+        torch.cuda.synchronize(dev)
+        cache.append(0, qkv[:, Hq:Hq + Hk], qkv[:, Hq + Hk:], starts, first, q=q, cos=cos, sin=sin)
+        cache.read(0, starts, first, kr, vr)
+        if form == "append":  # q last: rotated once more, in place
+            cache.append(0, kr, vr, starts, first, q=q, cos=cos, sin=sin)
+        if wait:
+            torch.cuda.synchronize(dev)
+        b = lambda t: t[-2 * T:].view(2, T, *t.shape[1:])  # noqa: E731
+        if form == "runner":
+            runner.run(b(q), b(kr), b(vr), *out)
+            return out
+        if form == "cascade":
+            return d.cascade_attention(b(q), b(kr), b(vr), cache.k[0], cache.v[0], cache.kv_layout, 0,
+                                       page_table=cache.page_table, plan=plan)
+        return single_prefill_with_kv_cache(q[-T:], kr[-T:], vr[-T:], causal=True, return_lse=True)
+
+    runner.run(*(torch.zeros(2, T, h, D, dtype=torch.bfloat16, device=dev) for h in (Hq, Hk, Hk)),
+               *(t.clone() for t in dense))
+    for i in range(6):
+        qkv = torch.randn(n, Hq + 2 * Hk, D, generator=g, device=dev).to(torch.bfloat16)
+        for form in ("append", "read", "runner", "cascade"):
+            for a, b in zip(step(qkv, form, False), step(qkv, form, True)):
+                assert torch.equal(a, b), (i, form)
