@@ -36,7 +36,7 @@
 // multiplies the score in fp32.
 // Weights are rounded to 16 bits for the second product: bf16 2^-8 relative, f16
 // 2^-11. An f16 below 2^-14 is subnormal, so f16 weights are taken 2^15 times as large
-// (m is 15 less than the maximum): relative down to 2^-29 of the row's largest, and off
+// (and the state is taken back): relative down to 2^-29 of the row's largest, and off
 // by at most 2^-40 of it below that (fp32's own end, 2^-126, is met before that only
 // where value rows are above 2^108: with e = 119 at 2^-22 of the largest). Maximum, sum
 // and output stay in fp32.
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
   using C = RowsCfg<D, ELEM>;
   constexpr int kWarps = C::kWarps, kThreads = C::kThreads;
   constexpr int kChunks = D * ELEM / 16;  // 16-byte chunks of a row
-  // log2 of the largest weight: 15 in f16, which holds up to 2^16
+  // log2 of the largest weight (2^-15 takes it back): 15 in f16, which holds up to 2^16
   constexpr float kTop = ELEM == 1 || std::is_same<T, __half>::value ? 15.f : 0.f;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -543,12 +543,15 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
           o[i][3] *= f1;
         }
       }
-      const float r0 = m0 == -INFINITY ? 0.f : m0 - kTop, r1 = m1 == -INFINITY ? 0.f : m1 - kTop;
+      const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+      // the headroom is added last: x is exact for the largest weight (for 8-bit values a
+      // whole number, -e), where m - 15 and what is relative to it would round by more
+      auto weight = [](float x) { return fast_exp2(kTop > 0.f ? x + kTop : x); };
       uint32_t p[4];
       if constexpr (R8) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const float p0 = fast_exp2(c[0][2 * n] - r0), p1 = fast_exp2(c[0][2 * n + 1] - r1);
+          const float p0 = weight(c[0][2 * n] - r0), p1 = weight(c[0][2 * n + 1] - r1);
           l0 += p0;
           l1 += p1;
           // row qr, keys 2 qc and 2 qc + 1
@@ -557,8 +560,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       } else {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const float p0 = fast_exp2(c[n][0] - r0), p1 = fast_exp2(c[n][1] - r0);
-          const float p2 = fast_exp2(c[n][2] - r1), p3 = fast_exp2(c[n][3] - r1);
+          const float p0 = weight(c[n][0] - r0), p1 = weight(c[n][1] - r0);
+          const float p2 = weight(c[n][2] - r1), p3 = weight(c[n][3] - r1);
           l0 += p0 + p1;
           l1 += p2 + p3;
           if (ELEM == 1) {
@@ -630,6 +633,14 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
         if (++read == C::kStages) read = 0, parity ^= 1;
       }
     }
+    if constexpr (kTop > 0.f) {
+      l0 *= 0x1p-15f;
+      l1 *= 0x1p-15f;
+#pragma unroll
+      for (int i = 0; i < kO; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] *= 0x1p-15f;
+    }
 #pragma unroll
     for (int step = R8 ? 4 : 1; step < (R8 ? 32 : 4); step *= 2) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, step);
@@ -667,8 +678,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
       }
     }
     if (R8 ? qr == 0 : qc == 0) {
-      sm_m[warp * 16 + row_a] = m0 - kTop;  // what the weights are relative to
-      sm_m[warp * 16 + row_b] = m1 - kTop;
+      sm_m[warp * 16 + row_a] = m0;
+      sm_m[warp * 16 + row_b] = m1;
       sm_l[warp * 16 + row_a] = l0;
       sm_l[warp * 16 + row_b] = l1;
     }

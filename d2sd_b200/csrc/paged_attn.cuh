@@ -31,9 +31,16 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// 1 / sum and log-sum-exp (base 2) of a row with maximum m and sum l: 0 and -inf for
-// a row that saw no key, NaN for one with a NaN.
+// 1 / sum and log-sum-exp (base 2) of a row with weights relative to m and their sum l:
+// 0 and -inf for a row that saw no key, NaN for one with a NaN. m and log2 l are both
+// large where they nearly cancel (8-bit values' exponents and f16's headroom are in m),
+// so l's exponent, whole, goes to m before its mantissa's logarithm is added.
 __device__ __forceinline__ float row_factor(float m, float l, float& lse2) {
+  const uint32_t bits = __float_as_uint(l), x = bits >> 23;
+  if (x - 1u < 254u) {  // positive and normal
+    lse2 = m + (static_cast<int>(x) - 127) + log2f(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u));
+    return 1.f / l;
+  }
   lse2 = l > 0.f ? m + log2f(l) : (l == 0.f ? -INFINITY : l);
   return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 }

@@ -505,3 +505,36 @@ def test_verify_block_behind_append_and_read(cuda_device):
         for form in ("append", "read", "runner", "cascade"):
             for a, b in zip(step(qkv, form, False), step(qkv, form, True)):
                 assert torch.equal(a, b), (i, form)
+
+
+# ---------------------------------------------------------------------------
+# the log-sum-exp of few keys
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["bf16", "f16", "e4m3"])
+@pytest.mark.parametrize("kl", [1, 2, 40, 300])
+@pytest.mark.parametrize("n", [1, 70])
+def test_lse_of_small_scores(cuda_device, type, kl, n):
+    """Scores near zero: the log-sum-exp is as exact as its own size, whatever the values'
+    exponents are (8-bit rows from 2^-17 to 1 here). The score's error, 2^-22 for the
+    exponentials, (kl + 8) 2^-24 for their sum, and two steps of the result at its size
+    or 1."""
+    import d2sd_b200 as d
+    Hq, Hk, D = 8, 2, 64
+    dt = torch.float16 if type == "f16" else torch.bfloat16
+    g = torch.Generator().manual_seed(131)
+    c = make_cache(g, [kl], Hk, D, E4M3 if type == "e4m3" else dt, "paged_umma", cuda_device)
+    if type == "e4m3":
+        byte = torch.randint(102, 120, c["vs"].shape, generator=g).to(torch.uint8)
+        c["vs"].copy_(byte)
+    q = torch.randn(n, Hq, D, generator=g).to(dt).to(cuda_device)
+    plan = d.PagedAttentionPlan([n], [kl], Hq, Hk, D, cuda_device, cache_dtype=c["k"].dtype)
+    out, lse = d.paged_attention(q, c["k"], c["v"], "paged_umma", c["table"], plan, sm_scale=1e-3,
+                                 k_scale=c["ks"], v_scale=c["vs"])
+    v = OP.cached_rows(c["v"], "paged_umma", c["table"].cpu().long(), kl, None if type != "e4m3" else c["vs"])
+    _, want, _, big = OP.attention(q.double().cpu(), c["k_rows"][0], v, scale=1e-3)
+    got = lse.double().cpu()
+    empty = want == float("-inf")
+    assert torch.equal(got == float("-inf"), empty)
+    tol = ((D + 4) * 2.0 ** -24 * big + 2.0 ** -22 + (min(kl, 300) + 8) * 2.0 ** -24) * 1.4427 \
+        + 2 * 2.0 ** -23 * want.abs().clamp(min=1.0)
+    assert ((got - want).abs() <= tol)[~empty].all(), float((got - want).abs()[~empty].max())
