@@ -63,6 +63,9 @@ class PagedAttentionPlan:
         self.reserve = reserve
         self.fixed_grid = 0
         if reserve is not None:
+            if len(reserve) not in (2, 3) or min(reserve) <= 0:
+                raise ValueError("reserve is (requests, tokens) or (requests, tokens, most of a "
+                                 "request), all positive")
             self.longest = reserve[2] if len(reserve) > 2 else reserve[1]
             rows = self.longest * num_qo_heads // num_kv_heads
             self.fixed_grid = _lib.GRID_FIXED

@@ -538,3 +538,14 @@ def test_lse_of_small_scores(cuda_device, type, kl, n):
     tol = ((D + 4) * 2.0 ** -24 * big + 2.0 ** -22 + (min(kl, 300) + 8) * 2.0 ** -24) * 1.4427 \
         + 2 * 2.0 ** -23 * want.abs().clamp(min=1.0)
     assert ((got - want).abs() <= tol)[~empty].all(), float((got - want).abs()[~empty].max())
+
+
+def test_reserves_of_no_size_are_refused(cuda_device):
+    import d2sd_b200 as d
+    for reserve in ((0, 4), (1, 0), (1, 4, 0), (1,), (1, 4, 1, 1), (-1, 4)):
+        with pytest.raises(ValueError):
+            d.PagedAttentionPlan([], [], 4, 2, 64, cuda_device, reserve=reserve)
+    plan = d.PagedAttentionPlan([], [], 4, 2, 64, cuda_device, reserve=(1, 4, 4))
+    plan.update([4], [9])
+    with pytest.raises(ValueError):
+        plan.update([5], [9])
