@@ -19,9 +19,10 @@
 // well. At the end the warps' states are joined in shared memory; a unit of several spans
 // is joined inside its cluster of CTAs, or by join_kernel.
 // Measured (32 / 8 heads of 128, bf16; of 6.54 TB/s of a plain copy): 64 requests of 512
-// to 8191 keys, one token each, 1133 MB, 187 us = 0.93; over e4m3 pages, 571 MB, 111 us =
-// 0.79 (instruction issue and the chain of one page share the rest); one request of 1000
-// keys 8.3 us, the latency of one launch.
+// to 8191 keys, one token each, 1133 MB, 187 us = 0.92; over e4m3 pages, 571 MB, 113 us =
+// 0.77 (instruction issue and the chain of one page share the rest); one request of 1000
+// keys 8.3 us on the GPU, the latency of one launch (a call from Python is 12.7 us, its
+// host time).
 //
 // e4m3 pages: their values are widened to f16 in registers (one conversion for two,
 // exact) and both products are f16. A 16-byte row of a core matrix holds 16 elements
@@ -791,7 +792,8 @@ __global__ void __launch_bounds__(RowsCfg<D, ELEM>::kThreads, kRowsCtas) rows_ke
 // GROUPS groups of threads share the spans (joined in shared memory, in order), so
 // that a unit of many spans has many loads in flight (32 tokens over 32k keys: 63 us for
 // the whole attention with one group, 48 with them). Bound by the states' way through L2,
-// 66 KB a span and q tile, and by its own start, which passes under the first kernel's end.
+// 66 KB a span and q tile, and by its own start, which passes under the end of the rows
+// kernel; the tiles kernel does not let it start early.
 template <typename T, int D, int SECTION, int GROUPS>
 __global__ void __launch_bounds__(kJoinRows[SECTION] * D / 4 * GROUPS) join_kernel(const AttnArgs a) {
   constexpr int RB = kJoinRows[SECTION], kThreads = RB * D / 4;  // of a group

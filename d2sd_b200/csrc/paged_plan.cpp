@@ -88,8 +88,11 @@ bool place_whole(const std::vector<Unit>& units, int ctas, int extra, int32_t gr
 // kernel would. Both estimates in units of a CTA's time for 128 keys with the memory to
 // itself (2.5 us in 16 bits, 1.9 us in 8): all CTAs at once take 2.4 (1.9) times that, and
 // the join costs 4 (5) of them. Measured, clusters against the cut, 8 kv heads of 128, one
-// new token each in 16 bits: 1 request of 1000 keys 8.5 us and 14.7, of 8000 27 and 24; 9
-// of 1000 16 and 27; 18 of 2000 32 and 42; 37 of 500 23.5 and 26.7.
+// new token each in 16 bits: 1 request of 1000 keys 9.2 us and 15.4, of 8000 25 and 20; 9
+// of 1000 14.3 and 21.5; 18 of 2000 32 and 40; 37 of 500 18.2 and 23.3. The choice was
+// within 1 us of the better one in all of 48 such pairs at heads of 128 and of 64, 16- and
+// 8-bit (heads of 64, 16-bit: 8.7 and 14.3, 23 and 17, 11.5 and 17.9, 23.6 and 24.1, 12.8
+// and 18.4).
 bool place_clusters(const std::vector<Unit>& units, int ctas, int32_t group, int32_t window, bool eight_bit,
                     std::vector<int32_t>& items, std::vector<int32_t>& first, int32_t* parts) {
   int32_t most = 0, size = kCluster;

@@ -20,9 +20,12 @@ constexpr int kTileKeys = 128;
 constexpr int kRowsTile = 16;    // query rows of a unit of the rows kernel
 constexpr int kRowsCtas = 4;     // CTAs of the rows kernel on an SM
 // Requests of more rows per kv head go to the tiles kernel. Measured with 16 requests
-// of 2k to 16k keys, 32 / 8 heads of 128: 16-bit, 20 rows 130 us there and 187 in two
-// tiles of the rows kernel; 8-bit, 20 rows 213 and 142, 32 rows 200 and 136, 64 rows
-// 217 and 264.
+// of 2k to 16k keys, there and in tiles of 16 rows of the rows kernel. 32 / 8 heads of
+// 128: 16-bit, 20 rows 122 us and 194; 8-bit, 20 rows 199 and 131, 32 rows 198 and 132, 64
+// rows 198 and 240. Heads of 64 (32 or 64 query heads): 16-bit, 24 to 32 rows 115 and 100,
+// 40 rows 117 and 133; 8-bit, 32 rows 160 and 98, 40 rows 163 and 136, 64 rows 163 and 178.
+// One limit for both head sizes, so heads of 64 give away 15 us at 17 to 32 rows of 16-bit
+// pages.
 constexpr int kRowsLimit = 16, kRowsLimit8 = 32;
 constexpr int kCluster = 8;  // CTAs of a cluster at most
 constexpr int kMagic = 0x50474131;

@@ -33,14 +33,17 @@
 // up to 2^8, and 509 with rescaling from 2 on and a factor of 2^13). Tiles that every row sees whole skip the mask; the others take
 // each score's minimum with an infinity of the sign that the row's [lo, hi) gives it.
 //
-// Measured (32 / 8 heads of 128, bf16; of 1657 TFLOP/s of a library product at full
-// clock): a prompt of 8192 tokens 480 us = 1146 TFLOP/s = 0.69; 2048 tokens over 16k
-// keys 440 to 480 us = 0.65 to 0.70. The chain of one q tile -- softmax, P V, the next
+// Measured, as calls among others (32 / 8 heads of 128, bf16; of 1657 TFLOP/s of a
+// library product in a burst, 1395 under the power cap): a prompt of 8192 tokens 540 us =
+// 1019 TFLOP/s = 0.61 (0.73). The chain of one q tile -- softmax, P V, the next
 // Q K^T and two hand-offs -- is as long as the other tile's, which it passes under, so
 // the tensor pipe is active for 53% of the time and the exponential unit for 54%.
 // Heads of 64 have half the product per tile and the same softmax. 16 blocks of 16
-// tokens over 2k to 16k keys 134 us = 0.75 of the copy rate. Chunks under a window of
-// 128 are two tiles each: the start and end of a unit are most of its 7 us.
+// tokens over 2k to 16k keys 150 us = 0.67 of the copy rate, 9 us of it the joining
+// kernel (134 us a call where calls follow at once and the next one starts under it); over
+// e4m3 pages, half of the bytes, 234 us: the widening is the chain. Chunks under a window
+// of 128 are two tiles each: the start and end of a unit are most of its 7 us (six
+// chunks 79 us a call).
 #include <atomic>
 #include <string>
 #include <type_traits>
@@ -58,7 +61,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr int kPanelBytes = 128 * 128;  // 128 rows x 64 16-bit values
 
 // SPLIT: no unit of the launch has a second q tile, and its room goes to more stages
-// (16 blocks of 16 tokens against 2k to 16k keys: 134 us against 146).
+// (16 blocks of 16 tokens against 2k to 16k keys, back to back: 134 us against 146).
 template <int D, int MODE, bool SPLIT>
 struct Cfg {
   static constexpr int kThreads = MODE == kE4m3 ? 512 : 384;
