@@ -678,10 +678,12 @@ def commit_kv_e4m3(layer_ptrs: torch.Tensor, *, num_layers: int, num_requests: i
     if layer_ptrs.dtype != torch.int64 or not layer_ptrs.is_contiguous() \
             or layer_ptrs.numel() != 6 * num_layers:
         raise ValueError(f"layer_ptrs must be a contiguous int64 tensor with {6 * num_layers} entries")
+    if accept_results.numel() < 2 * num_requests or cache_lens.numel() < num_requests:
+        raise ValueError(f"accept_results and cache_lens must hold {num_requests} requests")
     args = (layer_ptrs.data_ptr(), num_layers, num_requests, num_kv_heads, head_dim,
             _DTYPES.get(dtype, -1), block_len, *new_strides, *cache_strides, num_pages,
             *scale_strides, _int32("page_table", page_table), page_table.numel(),
             _int32("page_bounds", page_bounds, num_requests + 1),
-            _int32("accept_results", accept_results, 2 * num_requests),
-            _int32("cache_lens", cache_lens, num_requests), _status(status))
+            _int32("accept_results", accept_results), _int32("cache_lens", cache_lens),
+            _status(status))
     _call(dev, load().d2sd_commit_kv_e4m3, args, "d2sd_commit_kv_e4m3")

@@ -433,9 +433,10 @@ def test_sizes_of_device_arguments(cuda_device):
     ints = lambda x, t=torch.int32: torch.tensor(x, dtype=t, device=dev)  # noqa: E731
     pool = d.PagedKVPool(1, 2, 64, [40, 40], dtype=E4M3, device=dev)
     new = torch.zeros(2, 2, 8, 64, dtype=torch.bfloat16, device=dev)
-    for res in (ints([1, 0]), ints([[1, 0]] * 3), ints([[1, 0], [1, 0]], torch.int64)):
+    for res in (ints([1, 0]), ints([[1, 0], [1, 0]], torch.int64)):
         with pytest.raises(ValueError):
             pool.commit_batch([new], [new], res, 1)
+    pool.commit_batch([new], [new], ints([[1, 0]] * 3), 1)  # of a verifier of more requests
     pool.lengths_dev = ints([0])
     with pytest.raises(ValueError):
         pool.commit_batch([new], [new], ints([[1, 0], [1, 0]]), 1)
