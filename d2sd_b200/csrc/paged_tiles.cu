@@ -30,7 +30,8 @@
 // taken 2^11 times as large, up to 2^15: what lies below 2^-14 is subnormal, so they
 // are off by 2^-11 relative down to 2^-25 of the row's largest, and below that by at
 // most 2^-36 of it (a prompt of 8192 tokens in f16 takes 482 us so, 483 with weights of
-// up to 2^8, and 509 with rescaling from 2 on and a factor of 2^13). Tiles that every row sees whole skip the mask; the others take
+// up to 2^8, and 509 with rescaling from 2 on and a factor of 2^13). Tiles that every
+// row sees whole skip the mask; the others take
 // each score's minimum with an infinity of the sign that the row's [lo, hi) gives it.
 //
 // Measured, as calls among others (32 / 8 heads of 128, bf16; of 1657 TFLOP/s of a
